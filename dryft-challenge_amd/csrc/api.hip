@@ -786,6 +786,117 @@ int qdec_spec_accept(const qdec_accept_args *a, qdec_stream_t stream) {
                        "qdec_spec_accept");
 }
 
+// ------------------------------------------------------ tree speculation
+static int tree_shape(const char *fn, int batch, int t_rows, int cap) {
+  if (batch < 1 || batch > 65535) return set_error(QDEC_EINVAL, "%s: batch %d", fn, batch);
+  if (t_rows < 1 || t_rows > kTreeMaxT)
+    return set_error(QDEC_EINVAL, "%s: t_rows %d not in [1, %d]", fn, t_rows, kTreeMaxT);
+  if (cap < 1) return set_error(QDEC_EINVAL, "%s: cap %d", fn, cap);
+  return QDEC_OK;
+}
+
+int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream) {
+  if (!a || !a->hist || !a->lens || !a->ids || !a->parents) return set_error(QDEC_EINVAL, "qdec_tree_draft: null pointer");
+  const int rc = tree_shape("qdec_tree_draft", a->batch, a->t_rows, a->cap);
+  if (rc != QDEC_OK) return rc;
+  if (a->primary < 1 || a->primary > 64 || a->backoff < 1 || a->backoff > 64)
+    return set_error(QDEC_EINVAL, "qdec_tree_draft: primary %d / backoff %d not in [1, 64]", a->primary, a->backoff);
+  if (a->depth < 1 || a->depth >= kTreeMaxT)
+    return set_error(QDEC_EINVAL, "qdec_tree_draft: depth %d not in [1, %d]", a->depth, kTreeMaxT - 1);
+  if (a->matches < 1 || a->matches > kTreeMaxMatches)
+    return set_error(QDEC_EINVAL, "qdec_tree_draft: matches %d not in [1, %d]", a->matches, kTreeMaxMatches);
+  return launch_status(launch_tree_draft(*a, (hipStream_t)stream), "qdec_tree_draft");
+}
+
+static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool need_scratch) {
+  if (!a) return set_error(QDEC_EINVAL, "qdec_tree_attn: null args");
+  if (a->head_dim != 128 && a->head_dim != 64)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_tree_attn: head_dim %d (128 or 64)", a->head_dim);
+  if (a->nkv < 1 || a->nkv > 65535 || a->nq < a->nkv || a->nq % a->nkv || a->nq / a->nkv > 16)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_tree_attn: nq %d / nkv %d (1 to 16 whole query heads per kv head)", a->nq,
+                     a->nkv);
+  const int rc = tree_shape("qdec_tree_attn", a->batch, a->t_rows, a->cap);
+  if (rc != QDEC_OK) return rc;
+  if (a->cap < 32 || a->cap % 32)
+    return set_error(QDEC_EINVAL, "qdec_tree_attn: cap %d not a positive multiple of 32", a->cap);
+  if (a->splits < 0 || a->splits > 256) return set_error(QDEC_EINVAL, "qdec_tree_attn: splits %d not in [0, 256]", a->splits);
+  if (a->out_frag != 0 && a->out_frag != 1)
+    return set_error(QDEC_EINVAL, "qdec_tree_attn: out_frag %d not 0 or 1", a->out_frag);
+  *p = TreeAttnParams{};
+  p->eps = a->eps;
+  p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p->batch = a->batch; p->t_rows = a->t_rows; p->nq = a->nq; p->nkv = a->nkv;
+  p->head_dim = a->head_dim; p->cap = a->cap;
+  p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
+  tree_attn_plan(p, a->splits);
+  // workgroups of the launch, numbered in 31 bits
+  if ((int64_t)p->batch * p->nkv * p->groups * p->splits > 0x7fffffff)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_tree_attn: batch %d x nkv %d x %d row groups x %d splits", p->batch,
+                     p->nkv, p->groups, p->splits);
+  if (!need_scratch) return QDEC_OK;
+  if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->parents ||
+      !a->k_cache || !a->v_cache || !a->k_nodes || !a->v_nodes || !a->out)
+    return set_error(QDEC_EINVAL, "qdec_tree_attn: null pointer argument");
+  if (p->splits > 1 && (!a->partial || !a->counters))
+    return set_error(QDEC_EINVAL, "qdec_tree_attn: more than one split needs partial and counters");
+  if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
+      !aligned16(a->sin_tab) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->k_nodes) ||
+      !aligned16(a->v_nodes) || !aligned16(a->out) || !aligned16(a->partial))
+    return set_error(QDEC_EALIGN, "qdec_tree_attn: tensor pointers must be 16-byte aligned");
+  auto u16 = [](const void *x) { return reinterpret_cast<const uint16_t *>(x); };
+  p->qkv = u16(a->qkv); p->q_norm_w = u16(a->q_norm_w); p->k_norm_w = u16(a->k_norm_w);
+  p->cos_tab = u16(a->cos_tab); p->sin_tab = u16(a->sin_tab);
+  p->lens = a->lens; p->parents = a->parents;
+  p->k_cache = u16(a->k_cache); p->v_cache = u16(a->v_cache);
+  p->k_nodes = reinterpret_cast<uint16_t *>(a->k_nodes);
+  p->v_nodes = reinterpret_cast<uint16_t *>(a->v_nodes);
+  p->out = reinterpret_cast<uint16_t *>(a->out);
+  p->partial = a->partial; p->counters = a->counters;
+  return QDEC_OK;
+}
+
+int qdec_tree_attn_workspace(const qdec_tree_attn_args *a, size_t *partial_bytes, size_t *counter_bytes) {
+  TreeAttnParams p;
+  const int rc = plan_tree_attn(a, &p, false);
+  if (rc != QDEC_OK) return rc;
+  const size_t cells = (size_t)p.batch * p.nkv * p.groups;
+  if (partial_bytes)
+    *partial_bytes = p.splits > 1 ? sizeof(float) * cells * p.splits * (16 * p.mtq) * (p.head_dim + 2) : 0;
+  if (counter_bytes) *counter_bytes = p.splits > 1 ? sizeof(uint32_t) * cells : 0;
+  return QDEC_OK;
+}
+
+int qdec_tree_attn(const qdec_tree_attn_args *a, qdec_stream_t stream) {
+  TreeAttnParams p;
+  const int rc = plan_tree_attn(a, &p, true);
+  if (rc != QDEC_OK) return rc;
+  return launch_status(launch_tree_attn(p, (hipStream_t)stream), "qdec_tree_attn");
+}
+
+int qdec_tree_accept(const qdec_tree_accept_args *a, qdec_stream_t stream) {
+  if (!a || !a->out_tok || !a->ids || !a->parents || !a->hist || !a->lens || !a->lens_out || !a->naccept || !a->path)
+    return set_error(QDEC_EINVAL, "qdec_tree_accept: null pointer");
+  const int rc = tree_shape("qdec_tree_accept", a->batch, a->t_rows, a->cap);
+  if (rc != QDEC_OK) return rc;
+  return launch_status(launch_tree_accept(*a, (hipStream_t)stream), "qdec_tree_accept");
+}
+
+int qdec_tree_commit(const qdec_tree_commit_args *a, qdec_stream_t stream) {
+  if (!a || !a->k_nodes || !a->v_nodes || !a->k_cache || !a->v_cache || !a->path || !a->naccept || !a->lens)
+    return set_error(QDEC_EINVAL, "qdec_tree_commit: null pointer");
+  const int rc = tree_shape("qdec_tree_commit", a->batch, a->t_rows, a->cap);
+  if (rc != QDEC_OK) return rc;
+  if (a->head_dim != 128 && a->head_dim != 64)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_tree_commit: head_dim %d (128 or 64)", a->head_dim);
+  if (a->n_layers < 1 || a->n_layers > 65535 || a->nkv < 1 || a->nkv > 65535)
+    return set_error(QDEC_EINVAL, "qdec_tree_commit: n_layers %d nkv %d", a->n_layers, a->nkv);
+  if (a->cap < 32 || a->cap % 32)
+    return set_error(QDEC_EINVAL, "qdec_tree_commit: cap %d not a positive multiple of 32", a->cap);
+  if (!aligned16(a->k_nodes) || !aligned16(a->v_nodes) || !aligned16(a->k_cache) || !aligned16(a->v_cache))
+    return set_error(QDEC_EALIGN, "qdec_tree_commit: nodes and caches must be 16-byte aligned");
+  return launch_status(launch_tree_commit(*a, (hipStream_t)stream), "qdec_tree_commit");
+}
+
 // ------------------------------------------------------------- prefill
 static int rownorm(const qdec_rownorm_args *a, const float *parts, int nparts, void *merged, qdec_stream_t stream) {
   if (!a || !a->x || !a->out) return set_error(QDEC_EINVAL, "qdec_rownorm: null pointer");

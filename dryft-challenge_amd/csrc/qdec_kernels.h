@@ -265,4 +265,31 @@ hipError_t launch_accept(const int64_t *out_tok, const int64_t *draft, int64_t *
                          int32_t *lens, int32_t *naccept, int batch, int cap, int k,
                          int stop_len, hipStream_t s);
 
+// ---- tree speculation (tree.hip, tree_attn.hip)
+constexpr int kTreeMaxT = QDEC_TREE_MAX_T;
+constexpr int kTreeMaxMatches = QDEC_TREE_MAX_MATCHES;
+// Query rows of a (sequence, kv head) one tree attention workgroup takes.
+constexpr int kTreeGroupRows = 64;
+struct TreeAttnParams {
+  const uint16_t *qkv, *q_norm_w, *k_norm_w, *cos_tab, *sin_tab;
+  const int32_t *lens, *parents;
+  const uint16_t *k_cache, *v_cache;
+  uint16_t *k_nodes, *v_nodes, *out;
+  float *partial;
+  uint32_t *counters;
+  float eps;
+  float scale_log2;  // log2(e) / sqrt(head_dim)
+  int batch, t_rows, nq, nkv, head_dim, cap;
+  int splits;      // workgroups per (sequence, kv head, row group)
+  int min_blocks;  // 32-row blocks a workgroup gets before another one is used
+  int groups;      // row groups: ceil(t_rows * nq / nkv / kTreeGroupRows)
+  int mtq;         // 16-row M tiles per row group
+  int ofrag;       // > 0: out is written in fragment order with this many M tiles
+};
+void tree_attn_plan(TreeAttnParams *p, int splits);
+hipError_t launch_tree_attn(const TreeAttnParams &p, hipStream_t s);
+hipError_t launch_tree_draft(const qdec_tree_draft_args &a, hipStream_t s);
+hipError_t launch_tree_accept(const qdec_tree_accept_args &a, hipStream_t s);
+hipError_t launch_tree_commit(const qdec_tree_commit_args &a, hipStream_t s);
+
 }  // namespace qdec

@@ -24,6 +24,9 @@ NOALLOC_COUNTER_BYTES = 64 << 10
 # Device memory of a qdec_layer call (QDEC_LAYER_PLAN_BYTES, QDEC_LAYER_CTL_BYTES).
 LAYER_PLAN_BYTES = 4096
 LAYER_CTL_BYTES = 1152
+# Nodes of a drafted tree and candidates per pattern (QDEC_TREE_MAX_*).
+TREE_MAX_T = 64
+TREE_MAX_MATCHES = 32
 
 P = ctypes.c_void_p
 I32 = ctypes.c_int32
@@ -99,6 +102,31 @@ class PrefillAttnArgs(ctypes.Structure):
                 ("head_dim", I32), ("cap", I32), ("tiles", I32)]
 
 
+class TreeDraftArgs(ctypes.Structure):
+    _fields_ = [("hist", P), ("lens", P), ("ids", P), ("parents", P), ("batch", I32), ("cap", I32),
+                ("t_rows", I32), ("primary", I32), ("backoff", I32), ("depth", I32), ("matches", I32)]
+
+
+class TreeAttnArgs(ctypes.Structure):
+    _fields_ = [("qkv", P), ("q_norm_w", P), ("k_norm_w", P), ("cos_tab", P), ("sin_tab", P), ("lens", P),
+                ("parents", P), ("k_cache", P), ("v_cache", P), ("k_nodes", P), ("v_nodes", P), ("out", P),
+                ("partial", P), ("counters", P), ("eps", F32), ("sm_scale", F32), ("batch", I32),
+                ("t_rows", I32), ("nq", I32), ("nkv", I32), ("head_dim", I32), ("cap", I32), ("splits", I32),
+                ("out_frag", I32)]
+
+
+class TreeAcceptArgs(ctypes.Structure):
+    _fields_ = [("out_tok", P), ("ids", P), ("parents", P), ("hist", P), ("lens", P), ("lens_out", P),
+                ("naccept", P), ("path", P), ("emit", P), ("batch", I32), ("cap", I32), ("t_rows", I32),
+                ("stop_len", I32)]
+
+
+class TreeCommitArgs(ctypes.Structure):
+    _fields_ = [("k_nodes", P), ("v_nodes", P), ("k_cache", P), ("v_cache", P), ("path", P), ("naccept", P),
+                ("lens", P), ("n_layers", I32), ("batch", I32), ("t_rows", I32), ("nkv", I32),
+                ("head_dim", I32), ("cap", I32)]
+
+
 def declared_functions(header=HEADER):
     """Names of every function declared in include/qdec.h."""
     with open(header) as f:
@@ -129,6 +157,8 @@ class Lib:
         for name, st in (("qdec_embed", EmbedArgs), ("qdec_gemm", GemmArgs), ("qdec_gemm_wide", GemmArgs), ("qdec_attn", AttnArgs),
                          ("qdec_attn_noalloc", AttnArgs),
                          ("qdec_ngram_draft", DraftArgs), ("qdec_spec_accept", AcceptArgs),
+                         ("qdec_tree_draft", TreeDraftArgs), ("qdec_tree_attn", TreeAttnArgs),
+                         ("qdec_tree_accept", TreeAcceptArgs), ("qdec_tree_commit", TreeCommitArgs),
                          ("qdec_rownorm", RownormArgs), ("qdec_prefill_gemm", PgemmArgs),
                          ("qdec_prefill_qk", PrefillQkArgs), ("qdec_prefill_attn", PrefillAttnArgs)):
             fn = getattr(so, name)
@@ -138,7 +168,8 @@ class Lib:
         so.qdec_layer_prepare.restype = ctypes.c_int
         so.qdec_layer.argtypes = [ctypes.POINTER(LayerArgs), P]
         so.qdec_layer.restype = ctypes.c_int
-        for name, st in (("qdec_gemm_workspace", GemmArgs), ("qdec_attn_workspace", AttnArgs)):
+        for name, st in (("qdec_gemm_workspace", GemmArgs), ("qdec_attn_workspace", AttnArgs),
+                         ("qdec_tree_attn_workspace", TreeAttnArgs)):
             fn = getattr(so, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.POINTER(ctypes.c_size_t),
                            ctypes.POINTER(ctypes.c_size_t)]
@@ -206,6 +237,18 @@ class Lib:
     def spec_accept(self, args, stream):
         self._check("qdec_spec_accept", self.so.qdec_spec_accept(ctypes.byref(args), stream))
 
+    def tree_draft(self, args, stream):
+        self._check("qdec_tree_draft", self.so.qdec_tree_draft(ctypes.byref(args), stream))
+
+    def tree_attn(self, args, stream):
+        self._check("qdec_tree_attn", self.so.qdec_tree_attn(ctypes.byref(args), stream))
+
+    def tree_accept(self, args, stream):
+        self._check("qdec_tree_accept", self.so.qdec_tree_accept(ctypes.byref(args), stream))
+
+    def tree_commit(self, args, stream):
+        self._check("qdec_tree_commit", self.so.qdec_tree_commit(ctypes.byref(args), stream))
+
     def rownorm(self, args, stream):
         self._check("qdec_rownorm", self.so.qdec_rownorm(ctypes.byref(args), stream))
 
@@ -244,6 +287,12 @@ class Lib:
         pb, cb = ctypes.c_size_t(), ctypes.c_size_t()
         self._check("qdec_attn_workspace",
                     self.so.qdec_attn_workspace(ctypes.byref(args), ctypes.byref(pb), ctypes.byref(cb)))
+        return pb.value, cb.value
+
+    def tree_attn_workspace(self, args):
+        pb, cb = ctypes.c_size_t(), ctypes.c_size_t()
+        self._check("qdec_tree_attn_workspace",
+                    self.so.qdec_tree_attn_workspace(ctypes.byref(args), ctypes.byref(pb), ctypes.byref(cb)))
         return pb.value, cb.value
 
 

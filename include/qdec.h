@@ -450,6 +450,148 @@ typedef struct {
 } qdec_accept_args;
 int qdec_spec_accept(const qdec_accept_args *a, qdec_stream_t stream);
 
+/* ------------------------------------------------------ tree speculation */
+
+/* Speculation on a tree of drafted tokens instead of one chain of them: one
+ * pass verifies several continuations.  An iteration is qdec_tree_draft, a
+ * forward over batch * t_rows rows whose attention is qdec_tree_attn,
+ * qdec_tree_accept on the greedy picks, qdec_tree_commit.  No counterpart in
+ * the reference, which verifies one chain (notes/v10/spec.py:36-224).
+ *
+ * A tree of t_rows nodes (1..64) is parents[b*t_rows + t], row b*t_rows + t
+ * of the forward being node t of sequence b.  Node 0 is the root, the current
+ * token (its entry is not read).  Node t > 0 hangs on node parents[t] when
+ * 0 <= parents[t] < t; any other value (-1 by convention), and any parent
+ * that is no node itself, means that row t holds no node: a tree smaller than
+ * t_rows.  A node's depth is its number of edges to the root, its position
+ * lens[b] + depth. */
+#define QDEC_TREE_MAX_T 64
+#define QDEC_TREE_MAX_MATCHES 32
+
+/* Suffix-match drafter of a tree over each sequence's own history
+ * hist[b, 0..lens[b]] (hist[b, lens[b]] is the token not yet fed).  The
+ * candidates are the `matches` most recent earlier occurrences of the last
+ * `primary` tokens, most recent first, then those of the last `backoff`
+ * tokens; a candidate's draft is what followed it, at most `depth` tokens and
+ * not past hist[b, lens[b]].  The drafts enter a tree in that order: tokens
+ * that repeat an existing path follow it, the rest become new nodes, numbered
+ * in order of entry, until t_rows are used.  ids[b*t_rows] = hist[b,
+ * lens[b]]; a row that holds no node gets id 0, parent -1 (the root's entry is
+ * -1 too).  t_rows = 1 only feeds the current token.  A length outside
+ * [0, cap) is clamped into it, as qdec_ngram_draft clamps it. */
+typedef struct {
+  const int64_t *hist; /* [batch, cap] */
+  const int32_t *lens; /* [batch] */
+  int64_t *ids;        /* [batch*t_rows] out */
+  int32_t *parents;    /* [batch*t_rows] out */
+  int32_t batch;
+  int32_t cap;
+  int32_t t_rows;      /* 1..64 */
+  int32_t primary;     /* 1..64 */
+  int32_t backoff;     /* 1..64 */
+  int32_t depth;       /* 1..63 */
+  int32_t matches;     /* 1..32 */
+} qdec_tree_draft_args;
+int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
+
+/* For every sequence b and node t (see above), from the raw projection row
+ * qkv[b*t_rows + t]:
+ *   q, k = per-head RMSNorm and RoPE at position lens[b] + depth(t), with the
+ *          arithmetic and rounding points of qdec_attn;
+ *   out  = softmax(q . K^T / sqrt(D)) . V over cache slots 0 .. lens[b] - 1,
+ *          node t's ancestors and node t itself: fp32 scores, statistics and
+ *          accumulation, probabilities rounded to bf16 before the P.V product
+ *          (the operand type of the matrix instruction), one rounding to bf16;
+ *   k and the raw v go to k_nodes / v_nodes ([batch][nkv][t_rows][head_dim]).
+ * The cache is only read: qdec_tree_commit appends what was accepted.  What a
+ * row does not see (other branches, slots from lens[b] on) does not reach it,
+ * whatever it holds, NaN and infinities included.
+ * A row that holds no node: out is zero, its k_nodes / v_nodes are left as
+ * they were.  A length with lens[b] < 0 or lens[b] + t_rows > cap reads and
+ * writes no cache or node memory; the rows of sequence b become NaN.
+ * The cached slots and the nodes are dealt in 32-row blocks, evenly, to
+ * `splits` workgroups per 64 query rows of a (sequence, kv head), fewer for a
+ * short cache; the last one to finish merges their partials in order.  So a
+ * result depends on splits, lens[b] and t_rows, never on timing. */
+typedef struct {
+  const void *qkv;        /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
+  const void *q_norm_w;   /* [head_dim] bf16 */
+  const void *k_norm_w;   /* [head_dim] bf16 */
+  const void *cos_tab;    /* [cap, head_dim] bf16 */
+  const void *sin_tab;    /* [cap, head_dim] bf16 */
+  const int32_t *lens;    /* [batch] slots in the cache per sequence */
+  const int32_t *parents; /* [batch*t_rows] */
+  const void *k_cache;    /* K slab of this layer */
+  const void *v_cache;    /* V slab of this layer */
+  void *k_nodes;          /* [batch][nkv][t_rows][head_dim] bf16 out */
+  void *v_nodes;          /* the same */
+  void *out;              /* [batch*t_rows, nq*head_dim] bf16 */
+  float *partial;         /* split partials (qdec_tree_attn_workspace) */
+  uint32_t *counters;     /* zeroed arrival counters (qdec_tree_attn_workspace) */
+  float eps;
+  float sm_scale;         /* 1/sqrt(head_dim) */
+  int32_t batch;
+  int32_t t_rows;         /* 1..64 */
+  int32_t nq;             /* a multiple of nkv, at most 16 per kv head */
+  int32_t nkv;
+  int32_t head_dim;       /* 128 or 64 */
+  int32_t cap;            /* slots per sequence, multiple of 32 */
+  int32_t splits;         /* 1..256, or 0: chosen from the shape */
+  int32_t out_frag;       /* 1: out in the fragment order of qdec_gemm_args */
+} qdec_tree_attn_args;
+int qdec_tree_attn(const qdec_tree_attn_args *a, qdec_stream_t stream);
+int qdec_tree_attn_workspace(const qdec_tree_attn_args *a, size_t *partial_bytes, size_t *counter_bytes);
+
+/* Greedy acceptance on a tree: from the root, as long as some child of the
+ * current node holds the model's pick at that node (ids == out_tok; the lowest
+ * such child), step to it.  path[b*t_rows + i] is the i-th node of the walk
+ * (path[..0] = 0, the root), emit[b*t_rows + i] = out_tok at that node, -1 both
+ * past the walk; naccept[b] = steps taken a.  The a + 1 emitted tokens are
+ * appended to the history at lens[b] + 1 .. (entries past cap are dropped);
+ * lens_out[b] = lens[b] + a + 1 (lens_out may be lens).  A sequence with
+ * lens[b] >= stop_len is frozen: naccept 0, path and emit all -1, history and
+ * length kept. */
+typedef struct {
+  const int64_t *out_tok;  /* [batch*t_rows] greedy pick of every row */
+  const int64_t *ids;      /* [batch*t_rows] the rows' tokens */
+  const int32_t *parents;  /* [batch*t_rows] */
+  int64_t *hist;           /* [batch, cap] */
+  const int32_t *lens;     /* [batch] */
+  int32_t *lens_out;       /* [batch] out */
+  int32_t *naccept;        /* [batch] out */
+  int32_t *path;           /* [batch*t_rows] out */
+  int64_t *emit;           /* [batch*t_rows] out, or NULL */
+  int32_t batch;
+  int32_t cap;
+  int32_t t_rows;          /* 1..64 */
+  int32_t stop_len;
+} qdec_tree_accept_args;
+int qdec_tree_accept(const qdec_tree_accept_args *a, qdec_stream_t stream);
+
+/* The accepted path's keys and values into the cache, in every layer: with n =
+ * naccept[b] + 1 and base = lens[b] - n, cache slot base + i of layer l takes
+ * node path[b*t_rows + i] of k_nodes / v_nodes, i < n.  lens are the lengths
+ * after qdec_tree_accept.  The slabs of the layers follow one another in every
+ * buffer (k_nodes: [n_layers][batch][nkv][t_rows][head_dim]).  A sequence
+ * whose path[..0] is not 0 (frozen), with a path entry outside [0, t_rows), n
+ * outside [1, t_rows], base < 0 or lens[b] > cap is left as it was. */
+typedef struct {
+  const void *k_nodes;
+  const void *v_nodes;
+  void *k_cache;          /* K slab of layer 0 */
+  void *v_cache;          /* V slab of layer 0 */
+  const int32_t *path;    /* [batch*t_rows] */
+  const int32_t *naccept; /* [batch] */
+  const int32_t *lens;    /* [batch] */
+  int32_t n_layers;
+  int32_t batch;
+  int32_t t_rows;         /* 1..64 */
+  int32_t nkv;
+  int32_t head_dim;       /* 128 or 64 */
+  int32_t cap;            /* multiple of 32 */
+} qdec_tree_commit_args;
+int qdec_tree_commit(const qdec_tree_commit_args *a, qdec_stream_t stream);
+
 /* ------------------------------------------------------------ prefill */
 
 /* Prompt processing: every prompt position of every sequence in one forward
