@@ -861,7 +861,7 @@ int qdec_tree_attn_workspace(const qdec_tree_attn_args *a, size_t *partial_bytes
   if (rc != QDEC_OK) return rc;
   const size_t cells = (size_t)p.batch * p.nkv * p.groups;
   if (partial_bytes)
-    *partial_bytes = p.splits > 1 ? sizeof(float) * cells * p.splits * (16 * p.mtq) * (p.head_dim + 2) : 0;
+    *partial_bytes = p.splits > 1 ? sizeof(float) * cells * p.splits * p.group_rows * (p.head_dim + 2) : 0;
   if (counter_bytes) *counter_bytes = p.splits > 1 ? sizeof(uint32_t) * cells : 0;
   return QDEC_OK;
 }

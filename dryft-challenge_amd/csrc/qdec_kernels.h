@@ -268,8 +268,6 @@ hipError_t launch_accept(const int64_t *out_tok, const int64_t *draft, int64_t *
 // ---- tree speculation (tree.hip, tree_attn.hip)
 constexpr int kTreeMaxT = QDEC_TREE_MAX_T;
 constexpr int kTreeMaxMatches = QDEC_TREE_MAX_MATCHES;
-// Query rows of a (sequence, kv head) one tree attention workgroup takes.
-constexpr int kTreeGroupRows = 64;
 struct TreeAttnParams {
   const uint16_t *qkv, *q_norm_w, *k_norm_w, *cos_tab, *sin_tab;
   const int32_t *lens, *parents;
@@ -282,8 +280,8 @@ struct TreeAttnParams {
   int batch, t_rows, nq, nkv, head_dim, cap;
   int splits;      // workgroups per (sequence, kv head, row group)
   int min_blocks;  // 32-row blocks a workgroup gets before another one is used
-  int groups;      // row groups: ceil(t_rows * nq / nkv / kTreeGroupRows)
-  int mtq;         // 16-row M tiles per row group
+  int group_rows;  // query rows a workgroup takes: 16, 32, 64, 128 or 256
+  int groups;      // row groups: ceil(t_rows * nq / nkv / group_rows)
   int ofrag;       // > 0: out is written in fragment order with this many M tiles
 };
 void tree_attn_plan(TreeAttnParams *p, int splits);

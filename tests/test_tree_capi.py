@@ -118,13 +118,13 @@ def test_null_args(qlib, name):
 
 def test_workspace(qlib):
     assert qlib.tree_attn_workspace(attn(splits=1)) == (0, 0)
-    # 8 x 4 = 32 query rows: one group of two M tiles
+    # a partial is 16, 32, 64, 128 or 256 rows (a group of them from 257) of D + 2 floats
     assert qlib.tree_attn_workspace(attn(splits=3)) == (4 * 16 * 3 * 32 * 130, 4 * 16)
-    # 64 x 5 = 320 rows: five groups of 64
-    assert qlib.tree_attn_workspace(attn(splits=2, nq=40, t_rows=64)) == (4 * 16 * 5 * 2 * 64 * 130, 4 * 16 * 5)
-    # 9 x 8 = 72 rows: two groups of three M tiles
-    assert qlib.tree_attn_workspace(attn(splits=2, nq=64, t_rows=9)) == (4 * 16 * 2 * 2 * 48 * 130, 4 * 16 * 2)
     assert qlib.tree_attn_workspace(attn(splits=2, head_dim=64, t_rows=1)) == (4 * 16 * 2 * 16 * 66, 4 * 16)
+    for nq, t in ((64, 9), (40, 64), (8, 64), (128, 64)):
+        pb, cb = qlib.tree_attn_workspace(attn(splits=2, nq=nq, t_rows=t))
+        groups = cb // (4 * 16)
+        assert pb % (4 * 16 * 2 * 130 * groups) == 0 and pb >= 4 * 16 * 2 * 130 * t * (nq // 8)
     # splits = 0: the shape decides, and no more than one per four blocks of the cache
     pb, cb = qlib.tree_attn_workspace(attn(batch=1, cap=128))
     assert (pb, cb) == (0, 0)
