@@ -829,8 +829,8 @@ static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool 
   p->head_dim = a->head_dim; p->cap = a->cap;
   p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
   tree_attn_plan(p, a->splits);
-  // workgroups of the launch, numbered in 31 bits
-  if ((int64_t)p->batch * p->nkv * p->groups * p->splits > 0x7fffffff)
+  // workgroups of the launches (at most 128 per cell in the merge), numbered in 31 bits
+  if ((int64_t)p->batch * p->nkv * std::max(p->groups * p->splits, 128) > 0x7fffffff)
     return set_error(QDEC_EUNSUPPORTED, "qdec_tree_attn: batch %d x nkv %d x %d row groups x %d splits", p->batch,
                      p->nkv, p->groups, p->splits);
   if (!need_scratch) return QDEC_OK;

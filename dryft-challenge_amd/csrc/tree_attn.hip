@@ -6,9 +6,10 @@
 // is node t's query head h.  A workgroup takes a group of rows of one
 // (sequence, kv head) and a contiguous run of the 32-row key/value blocks, of
 // which there are ceil(L / 32) in the cache and ceil(T / 32) of nodes behind
-// them; runs are equal to within a block whatever L is.  Up to 32 rows go to
-// tree_attn_kernel, whose waves split the run's blocks; more go to
-// tree_wide_kernel, whose waves split the rows.
+// them; runs are equal to within a block whatever L is, the node blocks
+// counting for kTailWeight each (their rows are prepared first).  Two kernels:
+// tree_narrow_kernel, 16 rows per workgroup, whose waves split the run's
+// blocks, and tree_wide_kernel, 64 to 256 rows, whose waves split the rows.
 //
 // Common to both:
 //   * Ancestor sets: lane t of a wave holds node t's set as 64 bits and a
@@ -19,9 +20,15 @@
 //     base 2 on fp32 scores, O^T += V^T . P^T (P rounded to bf16, the operand
 //     type).  The running maximum is only moved, and the sums rescaled, in
 //     blocks where some row's maximum grows.
+//   * A lane's query rows are prepared in registers, in the place where the
+//     MFMA's B operand wants them: lane (c, g) holds channels 32s + 8g .. +8 of
+//     row c for every k step s, so the rotation's partner channel is the
+//     lane's own and only the sum of squares crosses lanes.  The node blocks'
+//     keys are prepared the same way as A operands.
 //   * With more than one workgroup per row group the partials go to memory and
-//     the last workgroup to arrive merges them in order.  A part whose rows saw
-//     nothing has maximum -inf and sum 0.
+//     are merged in order: by the last workgroup to arrive (narrow), or by
+//     tree_merge_kernel (wide, whose partials are too much for one CU).  A part
+//     whose rows saw nothing has maximum -inf and sum 0.
 #include "dma_dev.h"
 #include "qdec_common.h"
 #include "qdec_kernels.h"
@@ -30,496 +37,15 @@ namespace qdec {
 
 namespace {
 
-constexpr int kTW = 4;  // waves per workgroup
-
-template <int D>
-struct TreeLds {
-  static constexpr int RS = D + 8;  // bf16 per LDS row of queries or keys (bank spread)
-  static constexpr int q = 0;       // queries [32][RS], then the waves' partials
-  static constexpr int part_bytes = kTW * (D / 16) * 64 * 16;
-  static constexpr int q_bytes = 32 * RS * 2 > part_bytes ? 32 * RS * 2 : part_bytes;
-  static constexpr int k = q + q_bytes;                 // new keys [64][RS]
-  static constexpr int v = k + kTreeMaxT * RS * 2;      // new values [8][D][8]
-  static constexpr int m = v + kTreeMaxT * D * 2;       // wave row maxima [kTW][16]
-  static constexpr int l = m + kTW * 16 * 4;            // wave row sums [kTW][16]
-  static constexpr int bad = l + kTW * 16 * 4;          // nodes with a value that is not finite
-  static constexpr int flag = bad + kTreeMaxT * 4;
-  static constexpr int bytes = flag + 16;
-};
+constexpr int kTW = 4;  // waves of a narrow workgroup
+// Blocks that a node block counts for when a sequence's blocks are dealt.
+constexpr int kTailWeight = 3;
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t v, int l) {
   const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, l, 64);
   const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(v >> 32), l, 64);
   return ((uint64_t)hi << 32) | lo;
 }
-
-// Head RMSNorm and RoPE of one head row held by D/8 consecutive lanes, 8
-// channels each (raw, w, cos and sin as bf16).  The sum of squares is the
-// balanced tree over the channels that head_norm_rope builds and the products
-// of bf16 squares are exact, so both give the same bits.
-template <int D>
-__device__ __forceinline__ uint4 head_row(const uint4 &raw, const uint4 &w, const uint4 &cw, const uint4 &sw, float eps) {
-  constexpr int LPR = D / 8;
-  float x[8], g[8], c[8], s[8], y[8];
-  unpack8(raw, x);
-  unpack8(w, g);
-  unpack8(cw, c);
-  unpack8(sw, s);
-  float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
-             ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
-  ss += dpp_f<0xB1>(ss);                           // lane ^ 1
-  ss += dpp_f<0x4E>(ss);                           // lane ^ 2
-  ss += dpp_f<0x141>(ss);                          // the other quad of 8
-  if constexpr (LPR == 16) ss += dpp_f<0x140>(ss); // the other 8 of 16
-  const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = rbf(g[e] * rbf(x[e] * rstd));
-  const uint4 mine = pack8(y);
-  uint4 other;  // channels i +- D/2: bf16 values, so four words
-  other.x = (uint32_t)__shfl_xor((int)mine.x, LPR / 2, 64);
-  other.y = (uint32_t)__shfl_xor((int)mine.y, LPR / 2, 64);
-  other.z = (uint32_t)__shfl_xor((int)mine.z, LPR / 2, 64);
-  other.w = (uint32_t)__shfl_xor((int)mine.w, LPR / 2, 64);
-  float r[8];
-  unpack8(other, r);
-  const bool first = (threadIdx.x & (LPR - 1)) < LPR / 2;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = rbf(y[e] * c[e]) + rbf((first ? -r[e] : r[e]) * s[e]);
-  return pack8(y);
-}
-
-__device__ __forceinline__ bool finite8(const uint4 &v) {
-  auto two = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
-  return two(v.x) && two(v.y) && two(v.z) && two(v.w);
-}
-
-// A workgroup's place: split c of row group g of cell = b * nkv + kvh.  The row
-// groups of one (cell, split) read the same keys and values: they get numbers
-// that are equal modulo 8, the number of XCDs, and close together, so that
-// they share an L2.
-struct TreeUnit {
-  int c, cell, g, kvh, b;
-};
-__device__ __forceinline__ TreeUnit tree_unit(const TreeAttnParams &p) {
-  const int ng = p.groups, units = p.batch * p.nkv * p.splits, whole = units & ~7;
-  TreeUnit r;
-  int unit;
-  if ((int)blockIdx.x < whole * ng) {
-    const int q = blockIdx.x >> 3;
-    r.g = q % ng;
-    unit = (q / ng) * 8 + (blockIdx.x & 7);
-  } else {
-    const int y = blockIdx.x - whole * ng;
-    r.g = y % ng;
-    unit = whole + y / ng;
-  }
-  r.c = unit % p.splits;
-  r.cell = unit / p.splits;
-  r.kvh = r.cell % p.nkv;
-  r.b = r.cell / p.nkv;
-  return r;
-}
-
-// The blocks j0 .. j1 - 1 of split c of a sequence of L cached slots, the first
-// nb of all from the cache; n_active splits hold any (c >= n_active: -1).
-struct TreeRun {
-  int nb, n_active, j0, j1;
-};
-__device__ __forceinline__ TreeRun tree_run(const TreeAttnParams &p, int L, int c) {
-  TreeRun r;
-  r.nb = (L + 31) >> 5;
-  const int ntot = r.nb + ((p.t_rows + 31) >> 5);
-  r.n_active = max(1, min(p.splits, (ntot + p.min_blocks - 1) / p.min_blocks));
-  r.j0 = (int)((int64_t)ntot * c / r.n_active);
-  r.j1 = (int)((int64_t)ntot * (c + 1) / r.n_active);
-  if (c >= r.n_active) r.n_active = -1;
-  return r;
-}
-
-// Lane t: the nodes from the root to node t as bits, 0 where row t holds none.
-// up: parents[t] as loaded (anything on lanes from T on).
-__device__ __forceinline__ uint64_t tree_ancestors(int up, int T, int lane) {
-  if (lane == 0) up = 0;
-  if (lane >= T || up < 0 || up > lane || (up == lane && lane > 0)) up = lane;  // no node: a root of its own
-  uint64_t anc = 1ull << lane;
-  for (int i = 0; i < 6; ++i) {
-    const int up2 = __shfl(up, up, 64);
-    anc |= shfl64(anc, up);
-    if (!__any(up2 != up)) break;
-    up = up2;
-  }
-  return (anc & 1) && lane < T ? anc : 0;
-}
-
-// Weight of a part in a merge: its sum times zero where it saw nothing, so that
-// a NaN among its scores stays.
-__device__ __forceinline__ float tree_weight(float m, float l, float M, float scale) {
-  return m == -__builtin_huge_valf() ? l * 0.f : __builtin_amdgcn_exp2f((m - M) * scale);
-}
-
-// Values of a node that are not finite would reach every row through 0 * inf:
-// they are zero in LDS and added here, to the rows that see their node.  bad,
-// sees: bits of the 32 nodes of the block; pf: this lane's 8 probabilities; vr:
-// the first node's raw value row.
-template <int D>
-__device__ __forceinline__ void add_not_finite(f32x4_t (&acc)[D / 16], const uint4 &pf, uint32_t bad, uint64_t sees,
-                                               const uint16_t *vr, int width) {
-  const int col = threadIdx.x & 15, grp = (threadIdx.x >> 4) & 3;
-  const u32x4_t w = {pf.x, pf.y, pf.z, pf.w};
-  for (; bad; bad &= bad - 1) {
-    const int i = __builtin_ctz(bad);
-    const uint32_t pair = w[(i >> 1) & 3];
-    const float pr = __shfl((i & 1) ? hi16(pair) : lo16(pair), col + 16 * (i >> 3), 64);
-    if (!((sees >> i) & 1)) continue;
-    const uint16_t *v = vr + (size_t)i * width + grp * 4;
-#pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t x = v[dt * 16 + e];
-        if ((x & 0x7f80u) == 0x7f80u) acc[dt][e] += pr * bf2f(x);
-      }
-  }
-}
-
-template <int D, int MTQ>
-__global__ void __launch_bounds__(64 * kTW, 2) tree_attn_kernel(const TreeAttnParams p) {
-  using LY = TreeLds<D>;
-  constexpr int RS = LY::RS;
-  constexpr int DS = D / 32, DT = D / 16, DTW = DT / kTW;
-  constexpr int LPR = D / 8, RPW = 64 / LPR;  // lanes per prepared row, rows per wave and pass
-  __shared__ __align__(16) unsigned char smem[LY::bytes];
-  uint16_t *s_q = reinterpret_cast<uint16_t *>(smem + LY::q);
-  f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::q);
-  uint16_t *s_k = reinterpret_cast<uint16_t *>(smem + LY::k);
-  uint16_t *s_v = reinterpret_cast<uint16_t *>(smem + LY::v);
-  float *s_m = reinterpret_cast<float *>(smem + LY::m);
-  float *s_l = reinterpret_cast<float *>(smem + LY::l);
-  int *s_bad = reinterpret_cast<int *>(smem + LY::bad);
-  uint32_t *s_flag = reinterpret_cast<uint32_t *>(smem + LY::flag);
-  const float NEG_INF = -__builtin_huge_valf();
-
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = lane & 15, grp = lane >> 4;
-
-  const TreeUnit u_ = tree_unit(p);
-  const int c = u_.c, cell = u_.cell, kvh = u_.kvh, b = u_.b, C = p.splits;  // one row group
-  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv;
-  const int rows = T * G;  // query rows, at most 16 * MTQ
-  const int width = (nq + 2 * nkv) * D;
-  const uint16_t *qkv = p.qkv + (size_t)b * T * width;
-  auto out_at = [&](int m, int k) { return p.ofrag ? p.out + frag_off(m, k, p.ofrag) : p.out + (size_t)m * nq * D + k; };
-
-  // The raw query rows of this lane, before anything that waits.
-  const int sub = lane % LPR, ch = sub * 8;
-  constexpr int QP = (16 * MTQ + kTW * RPW - 1) / (kTW * RPW);
-  uint4 qraw[QP];
-  int qt[QP];
-#pragma unroll
-  for (int i = 0; i < QP; ++i) {
-    const int r = min((i * kTW + wave) * RPW + lane / LPR, rows - 1);
-    qt[i] = r / G;
-    qraw[i] = ld16(qkv + (size_t)qt[i] * width + (size_t)(kvh * G + r % G) * D + ch);
-  }
-  const int up = lane < T ? p.parents[(size_t)b * T + lane] : -1;
-  const int L = p.lens[b];
-  if (L < 0 || L > p.cap - T) {
-    if (c == 0)
-      for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * kTW) {
-        const int r = i / (D / 4), k4 = i % (D / 4) * 4;
-        *reinterpret_cast<uint2 *>(out_at(b * T + r / G, (kvh * G + r % G) * D + k4)) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
-      }
-    return;
-  }
-  const TreeRun run = tree_run(p, L, c);
-  if (run.n_active < 0) return;
-  const int nb = run.nb, n_active = run.n_active, j0 = run.j0, j1 = run.j1;
-
-  const size_t slab = (size_t)cell * p.cap * D;
-  const uint16_t *kc = p.k_cache + slab, *vc = p.v_cache + slab;
-  struct Frag {
-    uint4 ka[DS], kb[DS], vf[DT];
-  };
-  // Key rows of tile a: 8*(m >> 2) + (m & 3), of tile b 4 further, so that a
-  // lane's 8 scores are 8 consecutive rows, the B operand of the P.V product.
-  const int ra = 8 * (col >> 2) + (col & 3);
-  auto load_block = [&](int j, Frag &f) {
-    const uint16_t *kp = kc + (size_t)(32 * j + ra) * D + 8 * grp;
-    const uint16_t *vp = vc + ((size_t)(4 * j + grp) * D + col) * 8;
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      f.ka[s] = ld_nt(kp + s * 32);
-      f.kb[s] = ld_nt(kp + 4 * D + s * 32);
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) f.vf[dt] = ld_nt(vp + dt * 128);
-  };
-  Frag f0, f1;
-  if (j0 + wave < min(j1, nb)) load_block(j0 + wave, f0);
-
-  // ---- 1. ancestor sets.
-  const uint64_t anc = tree_ancestors(up, T, lane);
-  const int depth = (int)__popcll(anc) - 1;  // -1: no node (its rows are prepared at L and dropped)
-  const int pos = depth > 0 ? L + depth : L;
-  const uint64_t nodes = __ballot(anc != 0);
-
-  // ---- 2. queries, and the new keys and values of this run's node blocks.
-  {
-    const uint4 w = ld16(p.q_norm_w + ch);
-    uint4 cw[QP], sw[QP];
-#pragma unroll
-    for (int i = 0; i < QP; ++i) {
-      const size_t at = (size_t)__shfl(pos, qt[i], 64) * D + ch;
-      cw[i] = ld16(p.cos_tab + at);
-      sw[i] = ld16(p.sin_tab + at);
-    }
-#pragma unroll
-    for (int i = 0; i < QP; ++i) {
-      const int r = (i * kTW + wave) * RPW + lane / LPR;
-      const uint4 q = head_row<D>(qraw[i], w, cw[i], sw[i], p.eps);
-      if (r < 16 * MTQ) *reinterpret_cast<uint4 *>(s_q + r * RS + ch) = q;
-    }
-  }
-  const int n0 = max(j0 - nb, 0) * 32, n1 = min((j1 - nb) * 32, kTreeMaxT);  // nodes of this run, n1 <= n0: none
-  if (n1 > n0) {
-    const uint4 w = ld16(p.k_norm_w + ch);
-    for (int t = n0 + wave * RPW + lane / LPR; t < n1; t += kTW * RPW) {
-      const bool node = (nodes >> t) & 1;
-      const int tr = min(t, T - 1);
-      const int pt = __shfl(pos, tr, 64);
-      const uint16_t *row = qkv + (size_t)tr * width + (size_t)(nq + kvh) * D + ch;
-      const uint4 cw = ld16(p.cos_tab + (size_t)pt * D + ch), sw = ld16(p.sin_tab + (size_t)pt * D + ch);
-      const uint4 k = head_row<D>(ld16(row), w, cw, sw, p.eps);
-      const uint4 v = ld16(row + (size_t)nkv * D);
-      if (node) {
-        const size_t at = ((size_t)cell * T + t) * D + ch;
-        *reinterpret_cast<uint4 *>(p.k_nodes + at) = k;
-        *reinterpret_cast<uint4 *>(p.v_nodes + at) = v;
-      }
-      *reinterpret_cast<uint4 *>(s_k + t * RS + ch) = k;
-      const uint64_t part = __ballot(!finite8(v)) >> (lane & ~(LPR - 1));
-      if (sub == 0) s_bad[t] = node && (part & ((1ull << LPR) - 1));
-      uint32_t vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // no node, or not finite (add_not_finite): zero
-        if (!node || (vw[e] & 0x7f80u) == 0x7f80u) vw[e] &= 0xffff0000u;
-        if (!node || (vw[e] & 0x7f800000u) == 0x7f800000u) vw[e] &= 0xffffu;
-      }
-      uint16_t *dst = s_v + ((size_t)(t >> 3) * D + ch) * 8 + (t & 7);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dst[16 * e] = (uint16_t)(vw[e] & 0xffffu);
-        dst[16 * e + 8] = (uint16_t)(vw[e] >> 16);
-      }
-    }
-  }
-  lds_barrier();
-  uint64_t badset = 0;
-  if (n1 > n0) badset = __ballot(lane >= n0 && lane < n1 && s_bad[lane]);
-
-  uint4 qf[MTQ][DS];
-  uint64_t sees[MTQ];
-  f32x4_t acc[MTQ][DT];
-  float m_run[MTQ], l_run[MTQ];
-#pragma unroll
-  for (int mt = 0; mt < MTQ; ++mt) {
-#pragma unroll
-    for (int s = 0; s < DS; ++s) qf[mt][s] = *reinterpret_cast<const uint4 *>(s_q + (mt * 16 + col) * RS + s * 32 + grp * 8);
-    sees[mt] = shfl64(anc, min(mt * 16 + col, rows - 1) / G);
-    m_run[mt] = NEG_INF;
-    l_run[mt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
-
-  // ---- 3. the blocks.
-  const float scale = p.scale_log2;
-  auto process = [&](Frag &f, int j) {
-    f32x4_t sa[MTQ], sb[MTQ];
-    if (j >= nb) {  // node rows 32*(j - nb) ..
-      const int t0 = 32 * (j - nb);
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        f.ka[s] = *reinterpret_cast<const uint4 *>(s_k + (t0 + ra) * RS + s * 32 + grp * 8);
-        f.kb[s] = *reinterpret_cast<const uint4 *>(s_k + (t0 + ra + 4) * RS + s * 32 + grp * 8);
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        f.vf[dt] = *reinterpret_cast<const uint4 *>(s_v + ((size_t)((t0 >> 3) + grp) * D + dt * 16 + col) * 8);
-    } else if (32 * j + 32 > L) {  // the last cached block: slots from L on hold anything
-      const int v0 = 32 * j + 8 * grp;
-      uint32_t keep[4];
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-        keep[d] = (v0 + 2 * d < L ? 0x0000ffffu : 0u) | (v0 + 2 * d + 1 < L ? 0xffff0000u : 0u);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        f.vf[dt].x &= keep[0];
-        f.vf[dt].y &= keep[1];
-        f.vf[dt].z &= keep[2];
-        f.vf[dt].w &= keep[3];
-      }
-    }
-#pragma unroll
-    for (int mt = 0; mt < MTQ; ++mt) {
-      sa[mt] = sb[mt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        sa[mt] = mfma16x16x32(f.ka[s], qf[mt][s], sa[mt]);
-        sb[mt] = mfma16x16x32(f.kb[s], qf[mt][s], sb[mt]);
-      }
-    }
-    if (32 * j + 32 > L || j >= nb) {
-#pragma unroll
-      for (int mt = 0; mt < MTQ; ++mt) {
-        const uint32_t bits = j >= nb ? (uint32_t)(sees[mt] >> (32 * (j - nb))) >> (8 * grp)
-                                      : (uint32_t)((1ull << min(max(L - 32 * j - 8 * grp, 0), 8)) - 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (!((bits >> i) & 1)) sa[mt][i] = NEG_INF;
-          if (!((bits >> (4 + i)) & 1)) sb[mt][i] = NEG_INF;
-        }
-      }
-    }
-#pragma unroll
-    for (int mt = 0; mt < MTQ; ++mt) {
-      const float bmax = fmaxf(fmaxf(fmaxf(sa[mt][0], sa[mt][1]), fmaxf(sa[mt][2], sa[mt][3])),
-                               fmaxf(fmaxf(sb[mt][0], sb[mt][1]), fmaxf(sb[mt][2], sb[mt][3])));
-      if (__any(bmax > m_run[mt])) {
-        const float m_new = fmaxf(m_run[mt], max_xor16_32(bmax));
-        const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[mt] - m_new) * scale);
-        l_run[mt] *= alpha;
-        m_run[mt] = m_new;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) acc[mt][dt] *= alpha;
-      }
-      const float mc = m_run[mt] == NEG_INF ? 0.f : m_run[mt] * scale;
-      float pj[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        pj[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? sa[mt][e] : sb[mt][e - 4], scale, -mc));
-      l_run[mt] += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
-      const uint4 pf = pack8(pj);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[mt][dt] = mfma16x16x32(f.vf[dt], pf, acc[mt][dt]);
-      if (j >= nb) {
-        const uint32_t bad = (uint32_t)(badset >> (32 * (j - nb)));
-        if (bad)
-          add_not_finite<D>(acc[mt], pf, bad, sees[mt] >> (32 * (j - nb)),
-                            qkv + (size_t)(32 * (j - nb)) * width + (size_t)(nq + nkv + kvh) * D, width);
-      }
-    }
-  };
-  const int jc = min(j1, nb);  // blocks before jc come from the cache
-  for (int j = j0 + wave; j < j1; j += 2 * kTW) {
-    if (j + kTW < jc) load_block(j + kTW, f1);
-    process(f0, j);
-    if (j + 2 * kTW < jc) load_block(j + 2 * kTW, f0);
-    if (j + kTW < j1) process(f1, j + kTW);
-  }
-
-  // ---- 4. merge.
-  const bool direct = n_active == 1;
-  constexpr int RG = 16 * MTQ;
-  constexpr size_t kPart = (size_t)RG * (D + 2);  // floats of a partial: acc [RG][D], m [RG], l [RG]
-  float *part0 = p.partial + (direct ? (size_t)0 : (size_t)cell * C * kPart);
-  float *part = part0 + (size_t)c * kPart;
-#pragma unroll
-  for (int mt = 0; mt < MTQ; ++mt) {
-    const int r = mt * 16 + col;
-    float lw = l_run[mt] + shfl_xor(l_run[mt], 16);
-    lw += shfl_xor(lw, 32);
-    __syncthreads();  // the queries / the previous tile's partials are consumed
-    if (grp == 0) {
-      s_m[wave * 16 + col] = m_run[mt];
-      s_l[wave * 16 + col] = lw;
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[mt][dt];
-    __syncthreads();
-    float M = NEG_INF;
-#pragma unroll
-    for (int w = 0; w < kTW; ++w) M = fmaxf(M, s_m[w * 16 + col]);
-    float sc[kTW], lsum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kTW; ++w) {
-      const float l = s_l[w * 16 + col];
-      sc[w] = tree_weight(s_m[w * 16 + col], l, M, scale);
-      lsum += l * sc[w];
-    }
-#pragma unroll
-    for (int i = 0; i < DTW; ++i) {
-      const int dt = wave + kTW * i;
-      f32x4_t tot = s_acc[dt * 64 + lane] * sc[0];
-#pragma unroll
-      for (int w = 1; w < kTW; ++w) tot += s_acc[(w * DT + dt) * 64 + lane] * sc[w];
-      if (r >= rows) continue;
-      if (direct) {
-        const int t = r / G, hq = r % G;
-        uint2 o = make_uint2(pack2(tot[0] / lsum, tot[1] / lsum), pack2(tot[2] / lsum, tot[3] / lsum));
-        if (!((nodes >> t) & 1)) o = make_uint2(0u, 0u);
-        *reinterpret_cast<uint2 *>(out_at(b * T + t, (kvh * G + hq) * D + dt * 16 + grp * 4)) = o;
-      } else {
-        store_coherent4(part + (size_t)r * D + dt * 16 + grp * 4, tot);
-      }
-    }
-    if (!direct && wave == 0 && grp == 0 && r < rows) {
-      store_coherent(part + (size_t)RG * D + r, M);
-      store_coherent(part + (size_t)RG * D + RG + r, lsum);
-    }
-  }
-  if (direct) return;
-  if (!arrive_last(p.counters + cell, (uint32_t)n_active, s_flag)) return;
-#pragma unroll
-  for (int mt = 0; mt < MTQ; ++mt) {
-    const int r = mt * 16 + col;
-    if (r >= rows) continue;
-    float M = NEG_INF;
-    for (int i = 0; i < n_active; ++i) M = fmaxf(M, load_coherent(part0 + i * kPart + (size_t)RG * D + r));
-    float lsum = 0.f;
-    f32x4_t o[DTW];
-#pragma unroll
-    for (int i = 0; i < DTW; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < n_active; ++i) {
-      const float *pr = part0 + i * kPart;
-      const float l = load_coherent(pr + (size_t)RG * D + RG + r);
-      const float w = tree_weight(load_coherent(pr + (size_t)RG * D + r), l, M, scale);
-      lsum += l * w;
-#pragma unroll
-      for (int k = 0; k < DTW; ++k) o[k] += load_coherent4(pr + (size_t)r * D + (wave + kTW * k) * 16 + grp * 4) * w;
-    }
-    const int t = r / G, hq = r % G;
-#pragma unroll
-    for (int k = 0; k < DTW; ++k) {
-      uint2 v = make_uint2(pack2(o[k][0] / lsum, o[k][1] / lsum), pack2(o[k][2] / lsum, o[k][3] / lsum));
-      if (!((nodes >> t) & 1)) v = make_uint2(0u, 0u);
-      *reinterpret_cast<uint2 *>(out_at(b * T + t, (kvh * G + hq) * D + (wave + kTW * k) * 16 + grp * 4)) = v;
-    }
-  }
-}
-
-// ---------------------------------------------------------------- many rows
-// From 33 query rows per kv head every wave has 16 * MT rows of its own and
-// the NW waves share the blocks through a ring in LDS, filled by
-// global_load_lds_dwordx4 with per-lane gather addresses so that every
-// fragment lands in MFMA operand order (as the prefill attention stages its
-// blocks):
-//   K fragment 2s + h: lane (c, g) holds row 8*(c >> 2) + (c & 3) + 4h of the
-//     block, channels 32s + 8g .. +8;
-//   V fragment dt: lane (c, g) holds channel 16dt + c, rows 8g .. 8g + 7.
-// The node blocks are prepared into the same order behind the ring.  A lane's
-// 16 * MT query rows are prepared in registers, where they are used: lane
-// (c, g) holds channels 32s + 8g .. +8 of row c for every s, so the rotation's
-// partner channel is the lane's own and only the sum of squares crosses lanes.
-// While block j's softmax runs on the vector units, the matrix cores form
-// block j + 1's scores, one MFMA per exponential.
-template <int D, int NT>
-struct WideLds {
-  static constexpr int KF = D / 16, VF = D / 16;  // fragments of a block
-  static constexpr int BV = (KF + VF) * 64;       // uint4 per block
-  static constexpr int RING = 4;
-  static constexpr int vecs = (RING + NT) * BV;   // NT node blocks
-};
 
 // Head RMSNorm and RoPE of one row spread over the four lanes of a column, 8
 // channels 32s + 8g .. of every k step s, with the bits of head_norm_rope:
@@ -578,6 +104,455 @@ __device__ __forceinline__ void head_frags(uint4 (&f)[D / 32], const uint16_t *w
   }
 }
 
+__device__ __forceinline__ bool finite8(const uint4 &v) {
+  auto two = [](uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; };
+  return two(v.x) && two(v.y) && two(v.z) && two(v.w);
+}
+
+// A workgroup's place: split c of row group g of cell = b * nkv + kvh.  The row
+// groups of one (cell, split) read the same keys and values: they get numbers
+// that are equal modulo 8, the number of XCDs, and close together, so that
+// they share an L2.
+struct TreeUnit {
+  int c, cell, g, kvh, b;
+};
+__device__ __forceinline__ TreeUnit tree_unit(const TreeAttnParams &p) {
+  const int ng = p.groups, units = p.batch * p.nkv * p.splits, whole = units & ~7;
+  TreeUnit r;
+  int unit;
+  if ((int)blockIdx.x < whole * ng) {
+    const int q = blockIdx.x >> 3;
+    r.g = q % ng;
+    unit = (q / ng) * 8 + (blockIdx.x & 7);
+  } else {
+    const int y = blockIdx.x - whole * ng;
+    r.g = y % ng;
+    unit = whole + y / ng;
+  }
+  r.c = unit % p.splits;
+  r.cell = unit / p.splits;
+  r.kvh = r.cell % p.nkv;
+  r.b = r.cell / p.nkv;
+  return r;
+}
+
+// The blocks j0 .. j1 - 1 of split c of a sequence of L cached slots, the first
+// nb of all from the cache; every one of the n_active splits holds some
+// (c >= n_active: n_active = -1), the last one the node blocks.
+struct TreeRun {
+  int nb, n_active, j0, j1;
+};
+__host__ __device__ __forceinline__ int tree_active(int splits, int min_blocks, int nb, int ntb) {
+  // at least tail / 2 + 1 blocks per split, so that the one before the last
+  // has one left
+  const int tail = kTailWeight * ntb, least = min_blocks > tail / 2 ? min_blocks : tail / 2 + 1;
+  const int n = (nb + tail) / least;
+  return n < 1 ? 1 : n < splits ? n : splits;
+}
+__device__ __forceinline__ TreeRun tree_run(const TreeAttnParams &p, int L, int c) {
+  TreeRun r;
+  r.nb = (L + 31) >> 5;
+  const int ntb = (p.t_rows + 31) >> 5, total = r.nb + kTailWeight * ntb;
+  r.n_active = tree_active(p.splits, p.min_blocks, r.nb, ntb);
+  r.j0 = min((int)((int64_t)total * c / r.n_active), r.nb);
+  r.j1 = c + 1 == r.n_active ? r.nb + ntb : min((int)((int64_t)total * (c + 1) / r.n_active), r.nb);
+  if (c >= r.n_active) r.n_active = -1;
+  return r;
+}
+
+// Lane t: the nodes from the root to node t as bits, 0 where row t holds none.
+// up: parents[t] as loaded (anything on lanes from T on).
+__device__ __forceinline__ uint64_t tree_ancestors(int up, int T, int lane) {
+  if (lane == 0) up = 0;
+  if (lane >= T || up < 0 || up > lane || (up == lane && lane > 0)) up = lane;  // no node: a root of its own
+  uint64_t anc = 1ull << lane;
+  for (int i = 0; i < 6; ++i) {
+    const int up2 = __shfl(up, up, 64);
+    anc |= shfl64(anc, up);
+    if (!__any(up2 != up)) break;
+    up = up2;
+  }
+  return (anc & 1) && lane < T ? anc : 0;
+}
+
+// Weight of a part in a merge: its sum times zero where it saw nothing, so that
+// a NaN among its scores stays.
+__device__ __forceinline__ float tree_weight(float m, float l, float M, float scale) {
+  return m == -__builtin_huge_valf() ? l * 0.f : __builtin_amdgcn_exp2f((m - M) * scale);
+}
+
+// Values of a node that are not finite would reach every row through 0 * inf:
+// they are zero in LDS and added here, to the rows that see their node.  bad,
+// sees: bits of the 32 nodes of the block; pf: this lane's 8 probabilities; vr:
+// the first node's raw value row.
+template <int D>
+__device__ __forceinline__ void add_not_finite(f32x4_t (&acc)[D / 16], const uint4 &pf, uint32_t bad, uint64_t sees,
+                                               const uint16_t *vr, int width) {
+  const int col = threadIdx.x & 15, grp = (threadIdx.x >> 4) & 3;
+  const u32x4_t w = {pf.x, pf.y, pf.z, pf.w};
+  for (; bad; bad &= bad - 1) {
+    const int i = __builtin_ctz(bad);
+    const uint32_t pair = w[(i >> 1) & 3];
+    const float pr = __shfl((i & 1) ? hi16(pair) : lo16(pair), col + 16 * (i >> 3), 64);
+    if (!((sees >> i) & 1)) continue;
+    const uint16_t *v = vr + (size_t)i * width + grp * 4;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = v[dt * 16 + e];
+        if ((x & 0x7f80u) == 0x7f80u) acc[dt][e] += pr * bf2f(x);
+      }
+  }
+}
+
+// Merge of the n partials of row r (acc [RG][D], m [RG], l [RG] each, RG * (D +
+// 2) floats apart): this thread's f32x4 at channels ch[k].  8 partials' loads
+// are in flight at a time.  Returns the row's sum.
+template <int D, int NV, bool COH>
+__device__ __forceinline__ float tree_merge(const float *part0, int n, int RG, int r, const int (&ch)[NV], float scale,
+                                            f32x4_t (&o)[NV]) {
+  const size_t stride = (size_t)RG * (D + 2);
+  auto ld1 = [](const float *q) { return COH ? load_coherent(q) : *q; };
+  auto ld4 = [](const float *q) { return COH ? load_coherent4(q) : *reinterpret_cast<const f32x4_t *>(q); };
+  float M = -__builtin_huge_valf(), l = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) o[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float mi[8], li[8];
+    f32x4_t a[NV][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float *pr = part0 + (size_t)min(i0 + i, n - 1) * stride;
+      mi[i] = ld1(pr + (size_t)RG * D + r);
+      li[i] = ld1(pr + (size_t)RG * D + RG + r);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) a[k][i] = ld4(pr + (size_t)r * D + ch[k]);
+    }
+    float Mn = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) Mn = fmaxf(Mn, i0 + i < n ? mi[i] : M);
+    const float w0 = tree_weight(M, l, Mn, scale);
+    l *= w0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) o[k] *= w0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= n) continue;
+      const float w = tree_weight(mi[i], li[i], Mn, scale);
+      l += li[i] * w;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) o[k] += a[k][i] * w;
+    }
+    M = Mn;
+  }
+  return l;
+}
+
+__device__ __forceinline__ uint16_t *tree_out(const TreeAttnParams &p, int m, int k) {
+  return p.ofrag ? p.out + frag_off(m, k, p.ofrag) : p.out + (size_t)m * p.nq * p.head_dim + k;
+}
+
+// The rows r0 .. r0 + rows - 1 of a sequence whose length is out of range.
+__device__ __forceinline__ void tree_nan_rows(const TreeAttnParams &p, int b, int kvh, int r0, int rows) {
+  const int D = p.head_dim, G = p.nq / p.nkv;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
+    const int r = r0 + i / (D / 4), k4 = i % (D / 4) * 4;
+    *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + r / G, (kvh * G + r % G) * D + k4)) =
+        make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+  }
+}
+
+// ----------------------------------------------------------------- few rows
+// Four waves hold the same 16 rows and take the run's blocks in turn, two
+// blocks in flight each: a key or value fragment goes straight from memory
+// into the registers of the one wave that uses it, and there is no barrier
+// before the merge.  The wave that takes a node block prepares its keys in
+// place and turns its values in LDS of its own.
+template <int D>
+struct NarrowLds {
+  static constexpr int v = 0;                                 // new values [8][D][8]
+  static constexpr int acc = v + kTreeMaxT * D * 2;           // waves' partials [kTW][D / 16][64] f32x4
+  static constexpr int m = acc + kTW * (D / 16) * 64 * 16;    // wave row maxima [kTW][16]
+  static constexpr int l = m + kTW * 16 * 4;                  // wave row sums [kTW][16]
+  static constexpr int flag = l + kTW * 16 * 4;
+  static constexpr int bytes = flag + 16;
+};
+
+template <int D>
+__global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttnParams p) {
+  using LY = NarrowLds<D>;
+  constexpr int DS = D / 32, DT = D / 16, DTW = DT / kTW, RG = 16;
+  __shared__ __align__(16) unsigned char smem[LY::bytes];
+  uint16_t *s_v = reinterpret_cast<uint16_t *>(smem + LY::v);
+  f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::acc);
+  float *s_m = reinterpret_cast<float *>(smem + LY::m);
+  float *s_l = reinterpret_cast<float *>(smem + LY::l);
+  uint32_t *s_flag = reinterpret_cast<uint32_t *>(smem + LY::flag);
+  const float NEG_INF = -__builtin_huge_valf();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+
+  const TreeUnit u_ = tree_unit(p);
+  const int c = u_.c, cell = u_.cell, g = u_.g, kvh = u_.kvh, b = u_.b;
+  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv;
+  const int r0 = g * RG, rows = min(RG, T * G - r0);
+  const int width = (nq + 2 * nkv) * D;
+  const uint16_t *qkv = p.qkv + (size_t)b * T * width;
+
+  // What does not depend on the length is loaded first.
+  const int row = r0 + min(col, rows - 1), rt = row / G;  // lane's query row and node
+  uint4 qf[DS];
+  {
+    const uint16_t *q = qkv + (size_t)rt * width + (size_t)(kvh * G + row % G) * D + 8 * grp;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[s] = ld16(q + 32 * s);
+  }
+  const int up = lane < T ? p.parents[(size_t)b * T + lane] : -1;
+  const int L = p.lens[b];
+  if (L < 0 || L > p.cap - T) {
+    if (c == 0) tree_nan_rows(p, b, kvh, r0, rows);
+    return;
+  }
+  const TreeRun run = tree_run(p, L, c);
+  if (run.n_active < 0) return;
+  const int nb = run.nb, n_active = run.n_active, j0 = run.j0, j1 = run.j1;
+
+  const size_t slab = (size_t)cell * p.cap * D;
+  const uint16_t *kc = p.k_cache + slab, *vc = p.v_cache + slab;
+  struct Frag {
+    uint4 ka[DS], kb[DS], vf[DT];
+  };
+  // Key rows of tile a: 8*(m >> 2) + (m & 3), of tile b 4 further, so that a
+  // lane's 8 scores are 8 consecutive rows, the B operand of the P.V product.
+  const int ra = 8 * (col >> 2) + (col & 3);
+  auto load_block = [&](int j, Frag &f) {
+    const uint16_t *kp = kc + (size_t)(32 * j + ra) * D + 8 * grp;
+    const uint16_t *vp = vc + ((size_t)(4 * j + grp) * D + col) * 8;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      f.ka[s] = ld_nt(kp + s * 32);
+      f.kb[s] = ld_nt(kp + 4 * D + s * 32);
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) f.vf[dt] = ld_nt(vp + dt * 128);
+  };
+  // The last split's node blocks go to its last waves, which take them first.
+  const int jc = min(j1, nb), tb = j1 > nb ? wave - (kTW - (j1 - nb)) : -1;
+  Frag f0, f1;
+  if (tb >= 0) {  // raw node rows: keys in place, values by rows (vf[0 .. 2 DS - 1])
+    const int ta = min(32 * tb + ra, T - 1), tc = min(32 * tb + ra + 4, T - 1);
+    const uint16_t *ka = qkv + (size_t)ta * width + (size_t)(nq + kvh) * D + 8 * grp;
+    const uint16_t *kb = qkv + (size_t)tc * width + (size_t)(nq + kvh) * D + 8 * grp;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      f1.ka[s] = ld16(ka + s * 32);
+      f1.kb[s] = ld16(kb + s * 32);
+      f1.vf[s] = ld16(ka + (size_t)nkv * D + s * 32);
+      f1.vf[DS + s] = ld16(kb + (size_t)nkv * D + s * 32);
+    }
+  }
+  if (j0 + wave < jc) load_block(j0 + wave, f0);
+
+  const uint64_t anc = tree_ancestors(up, T, lane);
+  const int depth = (int)__popcll(anc) - 1;  // -1: no node (its rows are prepared at L and dropped)
+  const int pos = depth > 0 ? L + depth : L;
+  const uint64_t nodes = __ballot(anc != 0);
+  const uint64_t sees = shfl64(anc, rt);
+  {
+    const size_t at = (size_t)__shfl(pos, rt, 64) * D + 8 * grp;
+    head_frags<D>(qf, p.q_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
+  }
+
+  f32x4_t acc[DT];
+  float m_run = NEG_INF, l_run = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const float scale = p.scale_log2;
+
+  // A node block's raw rows into operands; returns the nodes with a value that
+  // is not finite.
+  auto prepare = [&](int t0, Frag &f) -> uint32_t {
+    uint16_t *sv = s_v + (size_t)t0 * D;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int t = t0 + ra + 4 * h;
+      const bool node = (nodes >> t) & 1;
+      const size_t at = (size_t)__shfl(pos, min(t, T - 1), 64) * D + 8 * grp;
+      head_frags<D>(h ? f.kb : f.ka, p.k_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
+      bool fin = true;
+#pragma unroll
+      for (int s = 0; s < DS; ++s) {
+        const uint4 v = f.vf[DS * h + s];
+        fin = fin && finite8(v);
+        if (node && g == 0) {
+          const size_t o = ((size_t)cell * T + t) * D + 32 * s + 8 * grp;
+          *reinterpret_cast<uint4 *>(p.k_nodes + o) = h ? f.kb[s] : f.ka[s];
+          *reinterpret_cast<uint4 *>(p.v_nodes + o) = v;
+        }
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint16_t *dst = sv + ((size_t)((t - t0) >> 3) * D + 32 * s + 8 * grp) * 8 + (t & 7);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // no node, or not finite (add_not_finite): zero
+          if (!node || (w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
+          if (!node || (w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
+          dst[16 * e] = (uint16_t)(w[e] & 0xffffu);
+          dst[16 * e + 8] = (uint16_t)(w[e] >> 16);
+        }
+      }
+      // lane t: is row t of the block one of this tile's, and not finite?
+      const uint64_t nf = __ballot(node && !fin);
+      const uint32_t m16 = (uint32_t)((nf | nf >> 16 | nf >> 32 | nf >> 48) & 0xffffu);
+      bad |= (uint32_t)__ballot(lane < 32 && ((lane >> 2) & 1) == h && ((m16 >> (4 * (lane >> 3) + (lane & 3))) & 1));
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      f.vf[dt] = *reinterpret_cast<const uint4 *>(sv + ((size_t)grp * D + dt * 16 + col) * 8);
+    return bad;
+  };
+
+  // Block j, from the cache or (NODES) of nodes.
+  auto process = [&](Frag &f, int j, auto nodesc) {
+    constexpr bool NODES = decltype(nodesc)::value != 0;
+    uint32_t bad = 0;
+    if constexpr (NODES) {
+      bad = prepare(32 * (j - nb), f);
+    } else if (32 * j + 32 > L) {  // the last cached block: slots from L on hold anything
+      const int v0 = 32 * j + 8 * grp;
+      uint32_t keep[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        keep[d] = (v0 + 2 * d < L ? 0x0000ffffu : 0u) | (v0 + 2 * d + 1 < L ? 0xffff0000u : 0u);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        f.vf[dt].x &= keep[0];
+        f.vf[dt].y &= keep[1];
+        f.vf[dt].z &= keep[2];
+        f.vf[dt].w &= keep[3];
+      }
+    }
+    f32x4_t sa = f32x4_t{0.f, 0.f, 0.f, 0.f}, sb = sa;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      sa = mfma16x16x32(f.ka[s], qf[s], sa);
+      sb = mfma16x16x32(f.kb[s], qf[s], sb);
+    }
+    if (NODES || 32 * j + 32 > L) {
+      const uint32_t bits = NODES ? (uint32_t)(sees >> (32 * (j - nb))) >> (8 * grp)
+                                  : (uint32_t)((1ull << min(max(L - 32 * j - 8 * grp, 0), 8)) - 1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!((bits >> i) & 1)) sa[i] = NEG_INF;
+        if (!((bits >> (4 + i)) & 1)) sb[i] = NEG_INF;
+      }
+    }
+    const float bmax = fmaxf(fmaxf(fmaxf(sa[0], sa[1]), fmaxf(sa[2], sa[3])), fmaxf(fmaxf(sb[0], sb[1]), fmaxf(sb[2], sb[3])));
+    if (__any(bmax > m_run)) {  // some row's maximum moves
+      const float m_new = fmaxf(m_run, max_xor16_32(bmax));
+      const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale);
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+    }
+    const float mc = m_run == NEG_INF ? 0.f : m_run * scale;
+    float pj[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pj[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? sa[e] : sb[e - 4], scale, -mc));
+    l_run += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+    const uint4 pf = pack8(pj);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma16x16x32(f.vf[dt], pf, acc[dt]);
+    if constexpr (NODES) {
+      if (bad)
+        add_not_finite<D>(acc, pf, bad, sees >> (32 * (j - nb)),
+                          qkv + (size_t)(32 * (j - nb)) * width + (size_t)(nq + nkv + kvh) * D, width);
+    }
+  };
+  if (tb >= 0) process(f1, nb + tb, Int<1>{});
+  for (int j = j0 + wave; j < jc; j += 2 * kTW) {
+    if (j + kTW < jc) load_block(j + kTW, f1);
+    process(f0, j, Int<0>{});
+    if (j + 2 * kTW < jc) load_block(j + 2 * kTW, f0);
+    if (j + kTW < jc) process(f1, j + kTW, Int<0>{});
+  }
+
+  // ---- merge of the waves, in wave order.
+  float lw = l_run + shfl_xor(l_run, 16);
+  lw += shfl_xor(lw, 32);
+  if (grp == 0) {
+    s_m[wave * 16 + col] = m_run;
+    s_l[wave * 16 + col] = lw;
+  }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[dt];
+  lds_barrier();
+  float M = NEG_INF;
+#pragma unroll
+  for (int w = 0; w < kTW; ++w) M = fmaxf(M, s_m[w * 16 + col]);
+  float sc[kTW], l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kTW; ++w) {
+    const float li = s_l[w * 16 + col];
+    sc[w] = tree_weight(s_m[w * 16 + col], li, M, scale);
+    l += li * sc[w];
+  }
+  f32x4_t o[DTW];
+  int ch[DTW];
+#pragma unroll
+  for (int i = 0; i < DTW; ++i) {
+    const int dt = wave + kTW * i;
+    ch[i] = dt * 16 + grp * 4;
+    o[i] = s_acc[dt * 64 + lane] * sc[0];
+#pragma unroll
+    for (int w = 1; w < kTW; ++w) o[i] += s_acc[(w * DT + dt) * 64 + lane] * sc[w];
+  }
+  if (n_active > 1) {
+    constexpr size_t kPart = (size_t)RG * (D + 2);
+    float *part0 = p.partial + ((size_t)cell * p.groups + g) * p.splits * kPart;
+    float *part = part0 + (size_t)c * kPart;
+    if (col < rows) {
+#pragma unroll
+      for (int i = 0; i < DTW; ++i) store_coherent4(part + (size_t)col * D + ch[i], o[i]);
+      if (wave == 0 && grp == 0) {
+        store_coherent(part + (size_t)RG * D + col, M);
+        store_coherent(part + (size_t)RG * D + RG + col, l);
+      }
+    }
+    if (!arrive_last(p.counters + (size_t)cell * p.groups + g, (uint32_t)n_active, s_flag)) return;
+    l = tree_merge<D, DTW, true>(part0, n_active, RG, min(col, rows - 1), ch, scale, o);
+  }
+  if (col >= rows) return;
+  const float inv = 1.f / l;
+  const bool node = (nodes >> rt) & 1;
+#pragma unroll
+  for (int i = 0; i < DTW; ++i) {
+    uint2 v = make_uint2(pack2(o[i][0] * inv, o[i][1] * inv), pack2(o[i][2] * inv, o[i][3] * inv));
+    if (!node) v = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2 *>(tree_out(p, b * T + rt, (kvh * G + row % G) * D + ch[i])) = v;
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+// Every wave has 16 * MT rows of its own and the NW waves share the blocks
+// through a ring in LDS, filled by global_load_lds_dwordx4 with per-lane gather
+// addresses so that every fragment lands in MFMA operand order (as the prefill
+// attention stages its blocks):
+//   K fragment 2s + h: lane (c, g) holds row 8*(c >> 2) + (c & 3) + 4h of the
+//     block, channels 32s + 8g .. +8;
+//   V fragment dt: lane (c, g) holds channel 16dt + c, rows 8g .. 8g + 7.
+// The node blocks are prepared into the same order behind the ring.  While
+// block j's softmax runs on the vector units, the matrix cores form block j +
+// 1's scores, one MFMA per exponential.
+template <int D, int NT>
+struct WideLds {
+  static constexpr int KF = D / 16, VF = D / 16;  // fragments of a block
+  static constexpr int BV = (KF + VF) * 64;       // uint4 per block
+  static constexpr int RING = 4;
+  static constexpr int vecs = (RING + NT) * BV;   // NT node blocks
+};
+
 template <int D, int NW, int MT, int NT>
 __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 2) tree_wide_kernel(const TreeAttnParams p) {
   using LY = WideLds<D, NT>;
@@ -587,8 +562,8 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   static_assert(KF % NW == 0 || (KF + LY::VF) % NW == 0, "whole fragments per wave");
   __shared__ uint4 ring[LY::vecs];         // [RING + NT][fragment][lane]
   uint4 *const tail = ring + RING * BV;
-  // Flags of the nodes with a value that is not finite: in the last ring
-  // slot, which takes its first block after they were read.
+  // Rows with a value that is not finite, a word per key tile: in the last
+  // ring slot, which takes its first block after they were read.
   uint32_t *s_bad = reinterpret_cast<uint32_t *>(ring + (RING - 1) * BV);
   const float NEG_INF = -__builtin_huge_valf();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -602,8 +577,6 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   const int rows = min(RG, R - r0);
   const int width = (nq + 2 * nkv) * D;
   const uint16_t *qkv = p.qkv + (size_t)b * T * width;
-  auto out_at = [&](int m, int k) { return p.ofrag ? p.out + frag_off(m, k, p.ofrag) : p.out + (size_t)m * nq * D + k; };
-
   uint4 qf[MT][DS];
   int row[MT];
 #pragma unroll
@@ -616,11 +589,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   const int up = lane < T ? p.parents[(size_t)b * T + lane] : -1;
   const int L = p.lens[b];
   if (L < 0 || L > p.cap - T) {
-    if (c == 0)
-      for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * NW) {
-        const int r = r0 + i / (D / 4), k4 = i % (D / 4) * 4;
-        *reinterpret_cast<uint2 *>(out_at(b * T + r / G, (kvh * G + r % G) * D + k4)) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
-      }
+    if (c == 0) tree_nan_rows(p, b, kvh, r0, rows);
     return;
   }
   const TreeRun run = tree_run(p, L, c);
@@ -668,8 +637,18 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   uint64_t badset = 0;
   const int tb0 = max(j0 - nb, 0), tb1 = run.j1 - nb;  // node blocks, none when tb1 <= tb0
   if (tb1 > tb0) {
-    if (threadIdx.x < 2) s_bad[threadIdx.x] = 0;
-    lds_barrier();
+    // Value fragment dt of node block i / DT: its loads go out before the keys
+    // are worked on.
+    constexpr int VW = DT * NT / NW > 0 ? DT * NT / NW : 1;  // per wave, at most
+    uint32_t vr[VW][8];
+    const uint16_t *v0 = qkv + (size_t)(nq + nkv + kvh) * D + col;
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+      const int i = DT * tb0 + wave + NW * k;
+      if (i >= DT * tb1) break;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vr[k][e] = v0[(size_t)min(32 * (i / DT) + 8 * grp + e, T - 1) * width + 16 * (i % DT)];
+    }
     for (int i = 2 * tb0 + wave; i < 2 * tb1; i += NW) {  // key tile h of block i / 2
       const int h = i & 1, t = 32 * (i >> 1) + 8 * (col >> 2) + (col & 3) + 4 * h, tr = min(t, T - 1);
       const bool node = (nodes >> t) & 1;
@@ -688,7 +667,8 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
         tail[(i >> 1) * BV + (2 * s + h) * 64 + lane] = k[s];
         fin = fin && finite8(v[s]);
       }
-      if (node && !fin) atomicOr(s_bad + (t >> 5), 1u << (t & 31));
+      const uint64_t nf = __ballot(node && !fin);
+      if (lane == 0) s_bad[i] = (uint32_t)((nf | nf >> 16 | nf >> 32 | nf >> 48) & 0xffffu);
       if (node && g == 0) {
         const size_t o = ((size_t)cell * T + t) * D + 8 * grp;
 #pragma unroll
@@ -698,20 +678,21 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
         }
       }
     }
-    for (int i = DT * tb0 + wave; i < DT * tb1; i += NW) {  // value fragment dt of block i / DT
-      const int dt = i % DT, t0 = 32 * (i / DT) + 8 * grp;
-      const uint16_t *vr = qkv + (size_t)(nq + nkv + kvh) * D + 16 * dt + col;
-      uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = vr[(size_t)min(t0 + e, T - 1) * width];
+    for (int k = 0; k < VW; ++k) {
+      const int i = DT * tb0 + wave + NW * k;
+      if (i >= DT * tb1) break;
+      const int t0 = 32 * (i / DT) + 8 * grp;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)  // no node, or not finite (added below to the rows that see it): zero
-        if (!((nodes >> (t0 + e)) & 1) || (w[e] & 0x7f80u) == 0x7f80u) w[e] = 0;
-      tail[(i / DT) * BV + (KF + dt) * 64 + lane] =
-          make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+      for (int e = 0; e < 8; ++e)  // no node, or not finite (add_not_finite): zero
+        if (!((nodes >> (t0 + e)) & 1) || (vr[k][e] & 0x7f80u) == 0x7f80u) vr[k][e] = 0;
+      tail[(i / DT) * BV + (KF + i % DT) * 64 + lane] =
+          make_uint4(vr[k][0] | vr[k][1] << 16, vr[k][2] | vr[k][3] << 16, vr[k][4] | vr[k][5] << 16, vr[k][6] | vr[k][7] << 16);
     }
     lds_barrier();
-    badset = (uint64_t)s_bad[0] | (uint64_t)s_bad[1] << 32;
+    // lane t: its row's place among the key tiles
+    const int tile = 2 * (lane >> 5) + ((lane >> 2) & 1);
+    badset = __ballot(tile >= 2 * tb0 && tile < 2 * tb1 && ((s_bad[tile] >> (4 * ((lane >> 3) & 3) + (lane & 3))) & 1));
   }
 
   f32x4_t acc[MT][DT];
@@ -869,64 +850,56 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   }
   block(jj, s0, s1, Int<1>{});
 
-  // ---- output, or a partial per row and the merge by the last workgroup.
-  const bool direct = n_active == 1;
-  constexpr size_t kPart = (size_t)RG * (D + 2);
-  float *part0 = p.partial + (direct ? (size_t)0 : ((size_t)cell * ng + g) * C * kPart);
-  float lsum[MT];
+  // ---- output, or a partial per row (m = -inf and l = 0 where a row holds no
+  // node, which is how the merge knows it).
+  float *part = p.partial + (n_active == 1 ? (size_t)0 : (((size_t)cell * ng + g) * C + c) * ((size_t)RG * (D + 2)));
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
-    lsum[u] = l_run[u] + shfl_xor(l_run[u], 16);
-    lsum[u] += shfl_xor(lsum[u], 32);
-  }
-  auto store_rows = [&](int u, const f32x4_t (&o)[DT], float l) {
-    const int t = row[u] / G, hq = row[u] % G;
+    const int r = (wave * MT + u) * 16 + col, t = row[u] / G;
     const bool node = (nodes >> t) & 1;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      uint2 v = make_uint2(pack2(o[dt][0] / l, o[dt][1] / l), pack2(o[dt][2] / l, o[dt][3] / l));
-      if (!node) v = make_uint2(0u, 0u);
-      *reinterpret_cast<uint2 *>(out_at(b * T + t, (kvh * G + hq) * D + dt * 16 + grp * 4)) = v;
-    }
-  };
-  if (direct) {
-#pragma unroll
-    for (int u = 0; u < MT; ++u)
-      if ((wave * MT + u) * 16 + col < rows) store_rows(u, acc[u], lsum[u]);
-    return;
-  }
-  float *part = part0 + (size_t)c * kPart;
-#pragma unroll
-  for (int u = 0; u < MT; ++u) {
-    const int r = (wave * MT + u) * 16 + col;
+    float l = l_run[u] + shfl_xor(l_run[u], 16);
+    l += shfl_xor(l, 32);
     if (r >= rows) continue;
+    if (n_active == 1) {
+      const float inv = 1.f / l;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) store_coherent4(part + (size_t)r * D + dt * 16 + grp * 4, acc[u][dt]);
-    if (grp == 0) {
-      store_coherent(part + (size_t)RG * D + r, m_run[u]);
-      store_coherent(part + (size_t)RG * D + RG + r, lsum[u]);
+      for (int dt = 0; dt < DT; ++dt) {
+        uint2 v = make_uint2(pack2(acc[u][dt][0] * inv, acc[u][dt][1] * inv), pack2(acc[u][dt][2] * inv, acc[u][dt][3] * inv));
+        if (!node) v = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2 *>(tree_out(p, b * T + t, (kvh * G + row[u] % G) * D + dt * 16 + grp * 4)) = v;
+      }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + dt * 16 + grp * 4) = acc[u][dt];
+      if (grp == 0) {
+        part[(size_t)RG * D + r] = node ? m_run[u] : NEG_INF;
+        part[(size_t)RG * D + RG + r] = node ? l : 0.f;
+      }
     }
   }
-  if (!arrive_last(p.counters + (size_t)cell * ng + g, (uint32_t)n_active, reinterpret_cast<uint32_t *>(ring))) return;
-#pragma unroll
-  for (int u = 0; u < MT; ++u) {
-    const int r = (wave * MT + u) * 16 + col;
-    if (r >= rows) continue;
-    float M = NEG_INF, l = 0.f;
-    for (int i = 0; i < n_active; ++i) M = fmaxf(M, load_coherent(part0 + i * kPart + (size_t)RG * D + r));
-    f32x4_t o[DT];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < n_active; ++i) {
-      const float *pr = part0 + i * kPart;
-      const float li = load_coherent(pr + (size_t)RG * D + RG + r);
-      const float w = tree_weight(load_coherent(pr + (size_t)RG * D + r), li, M, scale);
-      l += li * w;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] += load_coherent4(pr + (size_t)r * D + dt * 16 + grp * 4) * w;
-    }
-    store_rows(u, o, l);
-  }
+}
+
+// Merge of the wide kernel's partials: D / 4 threads per row.
+template <int D>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p) {
+  constexpr int TR = D / 4;
+  const int T = p.t_rows, G = p.nq / p.nkv, R = T * G, RG = p.group_rows;
+  const int per = (R + 256 / TR - 1) / (256 / TR);  // workgroups per cell
+  const int cell = blockIdx.x / per, kvh = cell % p.nkv, b = cell / p.nkv;
+  const int r = (blockIdx.x - cell * per) * (256 / TR) + threadIdx.x / TR;
+  const int L = p.lens[b];
+  if (L < 0 || L > p.cap - T || r >= R) return;
+  const int n = tree_active(p.splits, p.min_blocks, (L + 31) >> 5, (T + 31) >> 5);
+  if (n == 1) return;  // written by the one workgroup
+  const int g = r / RG;
+  const int ch[1] = {(int)(threadIdx.x % TR) * 4};
+  f32x4_t o[1];
+  const float l = tree_merge<D, 1, false>(p.partial + ((size_t)cell * p.groups + g) * p.splits * ((size_t)RG * (D + 2)), n, RG,
+                                          r - g * RG, ch, p.scale_log2, o);
+  const float inv = 1.f / l;
+  uint2 v = make_uint2(pack2(o[0][0] * inv, o[0][1] * inv), pack2(o[0][2] * inv, o[0][3] * inv));
+  if (l == 0.f) v = make_uint2(0u, 0u);  // no node
+  *reinterpret_cast<uint2 *>(tree_out(p, b * T + r / G, (kvh * G + r % G) * D + ch[0])) = v;
 }
 
 template <int D>
@@ -934,8 +907,7 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
   const dim3 grid((unsigned)(p.batch * p.nkv * p.groups * p.splits));
   const bool two = p.t_rows > 32;  // node blocks
   switch (p.group_rows) {
-    case 16: hipLaunchKernelGGL((tree_attn_kernel<D, 1>), grid, dim3(64 * kTW), 0, s, p); break;
-    case 32: hipLaunchKernelGGL((tree_attn_kernel<D, 2>), grid, dim3(64 * kTW), 0, s, p); break;
+    case 16: hipLaunchKernelGGL((tree_narrow_kernel<D>), grid, dim3(64 * kTW), 0, s, p); return hipSuccess;
     case 64:
       if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 4, 1, 2>), grid, dim3(256), 0, s, p);
       else hipLaunchKernelGGL((tree_wide_kernel<D, 4, 1, 1>), grid, dim3(256), 0, s, p);
@@ -950,18 +922,22 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
       break;
     default: return hipErrorInvalidValue;
   }
+  if (p.splits > 1) {
+    const int rows = p.t_rows * (p.nq / p.nkv), per = 256 / (D / 4);
+    hipLaunchKernelGGL((tree_merge_kernel<D>), dim3(p.batch * p.nkv * ((rows + per - 1) / per)), dim3(256), 0, s, p);
+  }
   return hipSuccess;
 }
 
 }  // namespace
 
-// The row group (16 or 32: the narrow kernel, all rows; 64, 128 or 256: the
-// wide one) and the splits.
+// The row group (16: the narrow kernel; 64, 128 or 256: the wide one) and the
+// splits.
 void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int rows = p->t_rows * (p->nq / p->nkv);
   const int64_t cells = (int64_t)p->batch * p->nkv;
   const int blocks = p->cap / 32;
-  p->group_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  p->group_rows = rows <= 32 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
   p->min_blocks = 4;
   p->groups = (rows + p->group_rows - 1) / p->group_rows;
   if (splits == 0) {
