@@ -837,8 +837,7 @@ static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool 
   if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->parents ||
       !a->k_cache || !a->v_cache || !a->k_nodes || !a->v_nodes || !a->out)
     return set_error(QDEC_EINVAL, "qdec_tree_attn: null pointer argument");
-  if (p->splits > 1 && (!a->partial || !a->counters))
-    return set_error(QDEC_EINVAL, "qdec_tree_attn: more than one split needs partial and counters");
+  if (p->splits > 1 && !a->partial) return set_error(QDEC_EINVAL, "qdec_tree_attn: more than one split needs partial");
   if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
       !aligned16(a->sin_tab) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->k_nodes) ||
       !aligned16(a->v_nodes) || !aligned16(a->out) || !aligned16(a->partial))
@@ -851,7 +850,7 @@ static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool 
   p->k_nodes = reinterpret_cast<uint16_t *>(a->k_nodes);
   p->v_nodes = reinterpret_cast<uint16_t *>(a->v_nodes);
   p->out = reinterpret_cast<uint16_t *>(a->out);
-  p->partial = a->partial; p->counters = a->counters;
+  p->partial = a->partial;
   return QDEC_OK;
 }
 
@@ -862,7 +861,7 @@ int qdec_tree_attn_workspace(const qdec_tree_attn_args *a, size_t *partial_bytes
   const size_t cells = (size_t)p.batch * p.nkv * p.groups;
   if (partial_bytes)
     *partial_bytes = p.splits > 1 ? sizeof(float) * cells * p.splits * p.group_rows * (p.head_dim + 2) : 0;
-  if (counter_bytes) *counter_bytes = p.splits > 1 ? sizeof(uint32_t) * cells : 0;
+  if (counter_bytes) *counter_bytes = 0;
   return QDEC_OK;
 }
 

@@ -274,13 +274,12 @@ struct TreeAttnParams {
   const uint16_t *k_cache, *v_cache;
   uint16_t *k_nodes, *v_nodes, *out;
   float *partial;
-  uint32_t *counters;
   float eps;
   float scale_log2;  // log2(e) / sqrt(head_dim)
   int batch, t_rows, nq, nkv, head_dim, cap;
   int splits;      // workgroups per (sequence, kv head, row group)
   int min_blocks;  // 32-row blocks a workgroup gets before another one is used
-  int group_rows;  // query rows a workgroup takes: 16, 64, 128 or 256
+  int group_rows;  // query rows a workgroup takes: 16, 32, 128 or 256
   int groups;      // row groups: ceil(t_rows * nq / nkv / group_rows)
   int ofrag;       // > 0: out is written in fragment order with this many M tiles
 };

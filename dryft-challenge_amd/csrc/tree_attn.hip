@@ -8,8 +8,9 @@
 // which there are ceil(L / 32) in the cache and ceil(T / 32) of nodes behind
 // them; runs are equal to within a block whatever L is, the node blocks
 // counting for kTailWeight each (their rows are prepared first).  Two kernels:
-// tree_narrow_kernel, 16 rows per workgroup, whose waves split the run's
-// blocks, and tree_wide_kernel, 64 to 256 rows, whose waves split the rows.
+// tree_narrow_kernel, 16 or 32 rows per workgroup, all in every wave, whose
+// waves split the run's blocks; and tree_wide_kernel, 128 or 256 rows, 32 per
+// wave, whose waves share every block.
 //
 // Common to both:
 //   * Ancestor sets: lane t of a wave holds node t's set as 64 bits and a
@@ -25,10 +26,11 @@
 //     row c for every k step s, so the rotation's partner channel is the
 //     lane's own and only the sum of squares crosses lanes.  The node blocks'
 //     keys are prepared the same way as A operands.
-//   * With more than one workgroup per row group the partials go to memory and
-//     are merged in order: by the last workgroup to arrive (narrow), or by
-//     tree_merge_kernel (wide, whose partials are too much for one CU).  A part
-//     whose rows saw nothing has maximum -inf and sum 0.
+//   * With more than one split every workgroup leaves a partial (sums, running
+//     maximum and sum of a row) and tree_merge_kernel merges them in order.  (A
+//     merge by the last workgroup to arrive took 5.4 us for 8 splits of 16
+//     rows: its stores, the counter and its loads follow one another at memory
+//     latency.  The second launch takes 3.5, and every CU shares its work.)
 #include "dma_dev.h"
 #include "qdec_common.h"
 #include "qdec_kernels.h"
@@ -47,21 +49,24 @@ __device__ __forceinline__ uint64_t shfl64(uint64_t v, int l) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-// Head RMSNorm and RoPE of one row spread over the four lanes of a column, 8
-// channels 32s + 8g .. of every k step s, with the bits of head_norm_rope:
-// the same balanced sum over the channels (8 in the lane, 16 and 32 across
-// lanes, 64 and 128 in the lane).
+// 8 channels 32s + 8g .. of a row for every k step s: a head row spread over the
+// four lanes of a column.
 template <int D>
-__device__ __forceinline__ void head_frags(uint4 (&f)[D / 32], const uint16_t *w, const uint16_t *cos_t,
-                                           const uint16_t *sin_t, float eps) {
-  constexpr int DS = D / 32;
-  uint4 wv[DS], cv[DS], sv[DS];
+struct Head {
+  uint4 v[D / 32];
+  __device__ __forceinline__ void load(const uint16_t *p) {
 #pragma unroll
-  for (int s = 0; s < DS; ++s) {
-    cv[s] = ld16(cos_t + 32 * s);
-    sv[s] = ld16(sin_t + 32 * s);
-    wv[s] = ld16(w + 32 * s);
+    for (int s = 0; s < D / 32; ++s) v[s] = ld16(p + 32 * s);
   }
+};
+
+// Head RMSNorm (gain w) and RoPE (cos c, sin n) of such a row, with the bits of
+// head_norm_rope: the same balanced sum over the channels (8 in the lane, 16
+// and 32 across lanes, 64 and 128 in the lane).
+template <int D>
+__device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], const Head<D> &w, const Head<D> &cw, const Head<D> &sw,
+                                          float eps) {
+  constexpr int DS = D / 32;
   float part[DS];
 #pragma unroll
   for (int s = 0; s < DS; ++s) {
@@ -78,26 +83,23 @@ __device__ __forceinline__ void head_frags(uint4 (&f)[D / 32], const uint16_t *w
   if constexpr (DS == 4) ss = ss + (part[2] + part[3]);
   const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
 #pragma unroll
-  for (int s = 0; s < DS; ++s) {
-    float x[8], g[8];
-    unpack8(f[s], x);
-    unpack8(wv[s], g);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = g[e] * rbf(x[e] * rstd);
-    f[s] = pack8(x);
-  }
-#pragma unroll
   for (int s = 0; s < DS / 2; ++s) {
-    float lo[8], hi[8], c[8], n[8], o[8];
+    float lo[8], hi[8], g[8], c[8], n[8], o[8];
     unpack8(f[s], lo);
+    unpack8(w.v[s], g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = rbf(g[e] * rbf(lo[e] * rstd));
     unpack8(f[s + DS / 2], hi);
-    unpack8(cv[s], c);
-    unpack8(sv[s], n);
+    unpack8(w.v[s + DS / 2], g);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = rbf(g[e] * rbf(hi[e] * rstd));
+    unpack8(cw.v[s], c);
+    unpack8(sw.v[s], n);
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = rbf(lo[e] * c[e]) + rbf(-hi[e] * n[e]);
     f[s] = pack8(o);
-    unpack8(cv[s + DS / 2], c);
-    unpack8(sv[s + DS / 2], n);
+    unpack8(cw.v[s + DS / 2], c);
+    unpack8(sw.v[s + DS / 2], n);
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = rbf(hi[e] * c[e]) + rbf(lo[e] * n[e]);
     f[s + DS / 2] = pack8(o);
@@ -175,6 +177,12 @@ __device__ __forceinline__ uint64_t tree_ancestors(int up, int T, int lane) {
   return (anc & 1) && lane < T ? anc : 0;
 }
 
+// The running maximum only moves when a score exceeds it by kMaxSlack / scale:
+// probabilities then stay below 2^kMaxSlack, which fp32 sums and bf16 operands
+// carry as well as those below 1, and the sums are rescaled in a few of the
+// first blocks only.
+constexpr float kMaxSlack = 8.f;
+
 // Weight of a part in a merge: its sum times zero where it saw nothing, so that
 // a NaN among its scores stays.
 __device__ __forceinline__ float tree_weight(float m, float l, float M, float scale) {
@@ -206,51 +214,125 @@ __device__ __forceinline__ void add_not_finite(f32x4_t (&acc)[D / 16], const uin
   }
 }
 
-// Merge of the n partials of row r (acc [RG][D], m [RG], l [RG] each, RG * (D +
-// 2) floats apart): this thread's f32x4 at channels ch[k].  8 partials' loads
-// are in flight at a time.  Returns the row's sum.
-template <int D, int NV, bool COH>
-__device__ __forceinline__ float tree_merge(const float *part0, int n, int RG, int r, const int (&ch)[NV], float scale,
-                                            f32x4_t (&o)[NV]) {
-  const size_t stride = (size_t)RG * (D + 2);
-  auto ld1 = [](const float *q) { return COH ? load_coherent(q) : *q; };
-  auto ld4 = [](const float *q) { return COH ? load_coherent4(q) : *reinterpret_cast<const f32x4_t *>(q); };
-  float M = -__builtin_huge_valf(), l = 0.f;
+// A node row spread over D / 8 consecutive lanes, 8 channels each: RMSNorm and
+// RoPE of head_rows, the same bits.
+template <int D>
+__device__ __forceinline__ uint4 head_row(const uint4 &raw, const uint4 &w, const uint4 &cw, const uint4 &sw, float eps) {
+  constexpr int LPR = D / 8;
+  float x[8], g[8], c[8], s[8], y[8];
+  unpack8(raw, x);
+  unpack8(w, g);
+  unpack8(cw, c);
+  unpack8(sw, s);
+  float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
+             ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
+  ss += dpp_f<0xB1>(ss);                            // lane ^ 1
+  ss += dpp_f<0x4E>(ss);                            // lane ^ 2
+  ss += dpp_f<0x141>(ss);                           // the other quad of 8
+  if constexpr (LPR == 16) ss += dpp_f<0x140>(ss);  // the other 8 of 16
+  const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
 #pragma unroll
-  for (int k = 0; k < NV; ++k) o[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float mi[8], li[8];
-    f32x4_t a[NV][8];
+  for (int e = 0; e < 8; ++e) y[e] = rbf(g[e] * rbf(x[e] * rstd));
+  const uint4 mine = pack8(y);
+  uint4 other;  // channels i +- D / 2: bf16 values, so four words
+  other.x = (uint32_t)__shfl_xor((int)mine.x, LPR / 2, 64);
+  other.y = (uint32_t)__shfl_xor((int)mine.y, LPR / 2, 64);
+  other.z = (uint32_t)__shfl_xor((int)mine.z, LPR / 2, 64);
+  other.w = (uint32_t)__shfl_xor((int)mine.w, LPR / 2, 64);
+  float r[8];
+  unpack8(other, r);
+  const bool first = (threadIdx.x & (LPR - 1)) < LPR / 2;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float *pr = part0 + (size_t)min(i0 + i, n - 1) * stride;
-      mi[i] = ld1(pr + (size_t)RG * D + r);
-      li[i] = ld1(pr + (size_t)RG * D + RG + r);
-#pragma unroll
-      for (int k = 0; k < NV; ++k) a[k][i] = ld4(pr + (size_t)r * D + ch[k]);
-    }
-    float Mn = M;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) Mn = fmaxf(Mn, i0 + i < n ? mi[i] : M);
-    const float w0 = tree_weight(M, l, Mn, scale);
-    l *= w0;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) o[k] *= w0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= n) continue;
-      const float w = tree_weight(mi[i], li[i], Mn, scale);
-      l += li[i] * w;
-#pragma unroll
-      for (int k = 0; k < NV; ++k) o[k] += a[k][i] * w;
-    }
-    M = Mn;
-  }
-  return l;
+  for (int e = 0; e < 8; ++e) y[e] = rbf(y[e] * c[e]) + rbf((first ? -r[e] : r[e]) * s[e]);
+  return pack8(y);
 }
+
+// The node blocks, prepared by all NW waves of the workgroup into LDS in operand
+// order (fragments as the wide kernel's ring holds them): wave and lane take
+// rows (k * NW + wave) * RPW + lane / LPR, 8 channels of each.  load() issues the
+// raw rows, before the lengths' and sets' dependent work; store() does the
+// rest.  One wave alone took 5 us for 32 rows.
+template <int D, int NW, int NT>
+struct TreeTail {
+  static constexpr int KF = D / 16, BV = D / 8 * 64;  // fragments of K, uint4 per block
+  static constexpr int LPR = D / 8, RPW = 64 / LPR, N = (32 * NT + NW * RPW - 1) / (NW * RPW);
+  uint4 k[N], v[N];
+
+  static __device__ __forceinline__ int row(int i) {
+    return (i * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW + (threadIdx.x & 63) / LPR;
+  }
+  __device__ __forceinline__ void load(const TreeAttnParams &p, const uint16_t *qkv, int kvh, int ntb) {
+    const int width = (p.nq + 2 * p.nkv) * D, ch = threadIdx.x % LPR * 8;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i * NW * RPW >= 32 * ntb) break;
+      const uint16_t *x = qkv + (size_t)min(row(i), p.t_rows - 1) * width + (size_t)(p.nq + kvh) * D + ch;
+      k[i] = ld16(x);
+      v[i] = ld16(x + (size_t)p.nkv * D);
+    }
+  }
+  // s_bad: 32 words per block.  pos, nodes: as the kernels hold them.  The
+  // workgroup has to meet before it reads.
+  __device__ __forceinline__ void store(const TreeAttnParams &p, uint4 *tail, int *s_bad, int cell, bool keep, int ntb,
+                                        int pos, uint64_t nodes) {
+    const int lane = threadIdx.x & 63, sub = lane % LPR, ch = sub * 8, T = p.t_rows;
+    const uint4 w = ld16(p.k_norm_w + ch);
+    uint4 cw[N], sw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i * NW * RPW >= 32 * ntb) break;
+      const size_t at = (size_t)__shfl(pos, min(row(i), T - 1), 64) * D + ch;
+      cw[i] = ld16(p.cos_tab + at);
+      sw[i] = ld16(p.sin_tab + at);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i * NW * RPW >= 32 * ntb) break;
+      const int t = row(i), r = t & 31;
+      const bool node = (nodes >> t) & 1;
+      const uint4 kr = head_row<D>(k[i], w, cw[i], sw[i], p.eps);
+      if (node && keep) {
+        const size_t o = ((size_t)cell * T + t) * D + ch;
+        *reinterpret_cast<uint4 *>(p.k_nodes + o) = kr;
+        *reinterpret_cast<uint4 *>(p.v_nodes + o) = v[i];
+      }
+      const uint64_t nf = __ballot(!finite8(v[i])) >> (lane & ~(LPR - 1));
+      if (t >= 32 * ntb) continue;  // (more rows per pass than a block has)
+      if (sub == 0) s_bad[t] = node && (nf & ((1ull << LPR) - 1));
+      uint4 *blk = tail + (t >> 5) * BV;
+      // K fragment 2s + h, lane (c, g): row 8*(c >> 2) + (c & 3) + 4h, channels 32s + 8g ..
+      blk[(2 * (sub >> 2) + ((r >> 2) & 1)) * 64 + 4 * (r >> 3) + (r & 3) + 16 * (sub & 3)] = kr;
+      // V fragment dt, lane (c, g): channel 16dt + c, rows 8g ..
+      uint16_t *dst = reinterpret_cast<uint16_t *>(blk + (KF + (ch >> 4)) * 64 + (ch & 15) + 16 * (r >> 3)) + (r & 7);
+      uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // no node, or not finite (add_not_finite): zero
+        if (!node || (x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
+        if (!node || (x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
+        dst[16 * e] = (uint16_t)(x[e] & 0xffffu);
+        dst[16 * e + 8] = (uint16_t)(x[e] >> 16);
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ uint16_t *tree_out(const TreeAttnParams &p, int m, int k) {
   return p.ofrag ? p.out + frag_off(m, k, p.ofrag) : p.out + (size_t)m * p.nq * p.head_dim + k;
+}
+// Four channels of query row r of a kv head: o / l, zeros where the row holds no
+// node.
+__device__ __forceinline__ void tree_store(const TreeAttnParams &p, int b, int kvh, int r, int ch, const f32x4_t &o,
+                                           float inv, bool node) {
+  const int G = p.nq / p.nkv;
+  uint2 v = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+  if (!node) v = make_uint2(0u, 0u);
+  *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + r / G, (kvh * G + r % G) * p.head_dim + ch)) = v;
+}
+// The partial of (cell, row group, split): acc [RG][D], m [RG], l [RG], with m =
+// -inf and l = 0 where a row saw nothing or holds no node.
+template <int D>
+__device__ __forceinline__ float *tree_part(const TreeAttnParams &p, int cell, int g, int c) {
+  return p.partial + (((size_t)cell * p.groups + g) * p.splits + c) * ((size_t)p.group_rows * (D + 2));
 }
 
 // The rows r0 .. r0 + rows - 1 of a sequence whose length is out of range.
@@ -264,31 +346,33 @@ __device__ __forceinline__ void tree_nan_rows(const TreeAttnParams &p, int b, in
 }
 
 // ----------------------------------------------------------------- few rows
-// Four waves hold the same 16 rows and take the run's blocks in turn, two
-// blocks in flight each: a key or value fragment goes straight from memory
-// into the registers of the one wave that uses it, and there is no barrier
-// before the merge.  The wave that takes a node block prepares its keys in
-// place and turns its values in LDS of its own.
-template <int D>
+// Four waves hold the same 16 * MT rows and take the run's blocks in turn, two
+// blocks in flight each: a key or value fragment goes straight from memory into
+// the registers of the one wave that uses it, and there is no barrier before
+// the merge of the waves, but for the one after the node blocks' preparation in
+// the last split.  With one M tile every wave
+// prepares the queries for itself, in registers; with more, wave u prepares
+// tile u and the operands stay in LDS (in registers they spilled: two blocks and
+// 64 rows' sums are 256).
+template <int D, int MT, int NT>
 struct NarrowLds {
-  static constexpr int v = 0;                                 // new values [8][D][8]
-  static constexpr int acc = v + kTreeMaxT * D * 2;           // waves' partials [kTW][D / 16][64] f32x4
-  static constexpr int m = acc + kTW * (D / 16) * 64 * 16;    // wave row maxima [kTW][16]
-  static constexpr int l = m + kTW * 16 * 4;                  // wave row sums [kTW][16]
-  static constexpr int flag = l + kTW * 16 * 4;
-  static constexpr int bytes = flag + 16;
+  static constexpr int tail = 0;                            // node blocks in operand order
+  static constexpr int bad = tail + NT * (D / 8) * 64 * 16;  // node rows with a value that is not finite
+  static constexpr int acc = bad + kTreeMaxT * 4;        // waves' sums of an M tile [kTW][D / 16][64] f32x4
+  static constexpr int m = acc + kTW * (D / 16) * 64 * 16;  // wave row maxima [MT][kTW][16]
+  static constexpr int l = m + MT * kTW * 16 * 4;        // wave row sums
+  static constexpr int q = l + MT * kTW * 16 * 4;        // query operands [MT][D / 32][64] (MT > 1)
+  static constexpr int bytes = q + (MT > 1 ? MT * (D / 32) * 1024 : 0);
 };
 
-template <int D>
-__global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttnParams p) {
-  using LY = NarrowLds<D>;
-  constexpr int DS = D / 32, DT = D / 16, DTW = DT / kTW, RG = 16;
+template <int D, int MT, int NT>
+__global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(const TreeAttnParams p) {
+  using LY = NarrowLds<D, MT, NT>;
+  constexpr int DS = D / 32, DT = D / 16, DTW = DT / kTW, RG = 16 * MT;
   __shared__ __align__(16) unsigned char smem[LY::bytes];
-  uint16_t *s_v = reinterpret_cast<uint16_t *>(smem + LY::v);
   f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::acc);
   float *s_m = reinterpret_cast<float *>(smem + LY::m);
   float *s_l = reinterpret_cast<float *>(smem + LY::l);
-  uint32_t *s_flag = reinterpret_cast<uint32_t *>(smem + LY::flag);
   const float NEG_INF = -__builtin_huge_valf();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -300,11 +384,17 @@ __global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttn
   const int width = (nq + 2 * nkv) * D;
   const uint16_t *qkv = p.qkv + (size_t)b * T * width;
 
-  // What does not depend on the length is loaded first.
-  const int row = r0 + min(col, rows - 1), rt = row / G;  // lane's query row and node
+  // What does not depend on the length is loaded first: the tile of query rows
+  // that this wave prepares.
+  uint4 *s_q = reinterpret_cast<uint4 *>(smem + LY::q);
   uint4 qf[DS];
+  const int mine = MT == 1 ? 0 : min(wave, MT - 1);
+  int rt[MT];  // the lane's query rows' nodes
+#pragma unroll
+  for (int u = 0; u < MT; ++u) rt[u] = (r0 + min(u * 16 + col, rows - 1)) / G;
+  const int qr = r0 + min(mine * 16 + col, rows - 1), qt = qr / G;
   {
-    const uint16_t *q = qkv + (size_t)rt * width + (size_t)(kvh * G + row % G) * D + 8 * grp;
+    const uint16_t *q = qkv + (size_t)qt * width + (size_t)(kvh * G + qr - qt * G) * D + 8 * grp;
 #pragma unroll
     for (int s = 0; s < DS; ++s) qf[s] = ld16(q + 32 * s);
   }
@@ -337,87 +427,68 @@ __global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttn
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) f.vf[dt] = ld_nt(vp + dt * 128);
   };
-  // The last split's node blocks go to its last waves, which take them first.
-  const int jc = min(j1, nb), tb = j1 > nb ? wave - (kTW - (j1 - nb)) : -1;
+  const int jc = min(j1, nb), ntb = max(j1 - nb, 0);  // the last split has the node blocks
+  uint4 *tail = reinterpret_cast<uint4 *>(smem + LY::tail);
+  int *s_bad = reinterpret_cast<int *>(smem + LY::bad);
+  TreeTail<D, kTW, NT> nt;
+  if (ntb > 0) nt.load(p, qkv, kvh, ntb);
   Frag f0, f1;
-  if (tb >= 0) {  // raw node rows: keys in place, values by rows (vf[0 .. 2 DS - 1])
-    const int ta = min(32 * tb + ra, T - 1), tc = min(32 * tb + ra + 4, T - 1);
-    const uint16_t *ka = qkv + (size_t)ta * width + (size_t)(nq + kvh) * D + 8 * grp;
-    const uint16_t *kb = qkv + (size_t)tc * width + (size_t)(nq + kvh) * D + 8 * grp;
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      f1.ka[s] = ld16(ka + s * 32);
-      f1.kb[s] = ld16(kb + s * 32);
-      f1.vf[s] = ld16(ka + (size_t)nkv * D + s * 32);
-      f1.vf[DS + s] = ld16(kb + (size_t)nkv * D + s * 32);
-    }
-  }
   if (j0 + wave < jc) load_block(j0 + wave, f0);
 
   const uint64_t anc = tree_ancestors(up, T, lane);
   const int depth = (int)__popcll(anc) - 1;  // -1: no node (its rows are prepared at L and dropped)
   const int pos = depth > 0 ? L + depth : L;
   const uint64_t nodes = __ballot(anc != 0);
-  const uint64_t sees = shfl64(anc, rt);
+  uint64_t sees[MT];
+#pragma unroll
+  for (int u = 0; u < MT; ++u) sees[u] = shfl64(anc, rt[u]);
   {
-    const size_t at = (size_t)__shfl(pos, rt, 64) * D + 8 * grp;
-    head_frags<D>(qf, p.q_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
+    const size_t at = (size_t)__shfl(pos, qt, 64) * D + 8 * grp;
+    Head<D> qw, cw, sw;
+    qw.load(p.q_norm_w + 8 * grp);
+    cw.load(p.cos_tab + at);
+    sw.load(p.sin_tab + at);
+    head_rows<D>(qf, qw, cw, sw, p.eps);
+  }
+  if constexpr (MT > 1) {
+    if (wave < MT) {
+#pragma unroll
+      for (int s = 0; s < DS; ++s) s_q[(wave * DS + s) * 64 + lane] = qf[s];
+    }
+  }
+  uint64_t badset = 0;
+  if (ntb > 0) {
+    nt.store(p, tail, s_bad, cell, g == 0, ntb, pos, nodes);
+    lds_barrier();
+    badset = __ballot(lane < 32 * ntb && s_bad[lane]);
+  } else if (MT > 1) {
+    lds_barrier();
   }
 
-  f32x4_t acc[DT];
-  float m_run = NEG_INF, l_run = 0.f;
+  f32x4_t acc[MT][DT];
+  float m_run[MT], l_run[MT];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int u = 0; u < MT; ++u) {
+    m_run[u] = NEG_INF;
+    l_run[u] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[u][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
   const float scale = p.scale_log2;
-
-  // A node block's raw rows into operands; returns the nodes with a value that
-  // is not finite.
-  auto prepare = [&](int t0, Frag &f) -> uint32_t {
-    uint16_t *sv = s_v + (size_t)t0 * D;
-    uint32_t bad = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = t0 + ra + 4 * h;
-      const bool node = (nodes >> t) & 1;
-      const size_t at = (size_t)__shfl(pos, min(t, T - 1), 64) * D + 8 * grp;
-      head_frags<D>(h ? f.kb : f.ka, p.k_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
-      bool fin = true;
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        const uint4 v = f.vf[DS * h + s];
-        fin = fin && finite8(v);
-        if (node && g == 0) {
-          const size_t o = ((size_t)cell * T + t) * D + 32 * s + 8 * grp;
-          *reinterpret_cast<uint4 *>(p.k_nodes + o) = h ? f.kb[s] : f.ka[s];
-          *reinterpret_cast<uint4 *>(p.v_nodes + o) = v;
-        }
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint16_t *dst = sv + ((size_t)((t - t0) >> 3) * D + 32 * s + 8 * grp) * 8 + (t & 7);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // no node, or not finite (add_not_finite): zero
-          if (!node || (w[e] & 0x7f80u) == 0x7f80u) w[e] &= 0xffff0000u;
-          if (!node || (w[e] & 0x7f800000u) == 0x7f800000u) w[e] &= 0xffffu;
-          dst[16 * e] = (uint16_t)(w[e] & 0xffffu);
-          dst[16 * e + 8] = (uint16_t)(w[e] >> 16);
-        }
-      }
-      // lane t: is row t of the block one of this tile's, and not finite?
-      const uint64_t nf = __ballot(node && !fin);
-      const uint32_t m16 = (uint32_t)((nf | nf >> 16 | nf >> 32 | nf >> 48) & 0xffffu);
-      bad |= (uint32_t)__ballot(lane < 32 && ((lane >> 2) & 1) == h && ((m16 >> (4 * (lane >> 3) + (lane & 3))) & 1));
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      f.vf[dt] = *reinterpret_cast<const uint4 *>(sv + ((size_t)grp * D + dt * 16 + col) * 8);
-    return bad;
-  };
+  const float slack = kMaxSlack / scale;
 
   // Block j, from the cache or (NODES) of nodes.
   auto process = [&](Frag &f, int j, auto nodesc) {
     constexpr bool NODES = decltype(nodesc)::value != 0;
-    uint32_t bad = 0;
     if constexpr (NODES) {
-      bad = prepare(32 * (j - nb), f);
+      const uint4 *B = tail + (j - nb) * ((D / 8) * 64) + lane;
+#pragma unroll
+      for (int s = 0; s < DS; ++s) {
+        f.ka[s] = B[(2 * s) * 64];
+        f.kb[s] = B[(2 * s + 1) * 64];
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) f.vf[dt] = B[(D / 16 + dt) * 64];
     } else if (32 * j + 32 > L) {  // the last cached block: slots from L on hold anything
       const int v0 = 32 * j + 8 * grp;
       uint32_t keep[4];
@@ -432,45 +503,59 @@ __global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttn
         f.vf[dt].w &= keep[3];
       }
     }
-    f32x4_t sa = f32x4_t{0.f, 0.f, 0.f, 0.f}, sb = sa;
+    f32x4_t sa[MT], sb[MT];
 #pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      sa = mfma16x16x32(f.ka[s], qf[s], sa);
-      sb = mfma16x16x32(f.kb[s], qf[s], sb);
-    }
-    if (NODES || 32 * j + 32 > L) {
-      const uint32_t bits = NODES ? (uint32_t)(sees >> (32 * (j - nb))) >> (8 * grp)
-                                  : (uint32_t)((1ull << min(max(L - 32 * j - 8 * grp, 0), 8)) - 1);
+    for (int u = 0; u < MT; ++u) {
+      sa[u] = sb[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!((bits >> i) & 1)) sa[i] = NEG_INF;
-        if (!((bits >> (4 + i)) & 1)) sb[i] = NEG_INF;
+      for (int s = 0; s < DS; ++s) {
+        const uint4 q = MT > 1 ? s_q[(u * DS + s) * 64 + lane] : qf[s];
+        sa[u] = mfma16x16x32(f.ka[s], q, sa[u]);
+        sb[u] = mfma16x16x32(f.kb[s], q, sb[u]);
       }
     }
-    const float bmax = fmaxf(fmaxf(fmaxf(sa[0], sa[1]), fmaxf(sa[2], sa[3])), fmaxf(fmaxf(sb[0], sb[1]), fmaxf(sb[2], sb[3])));
-    if (__any(bmax > m_run)) {  // some row's maximum moves
-      const float m_new = fmaxf(m_run, max_xor16_32(bmax));
-      const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * scale);
-      l_run *= alpha;
-      m_run = m_new;
+    if (NODES || 32 * j + 32 > L) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+      for (int u = 0; u < MT; ++u) {
+        const uint32_t bits = NODES ? (uint32_t)(sees[u] >> (32 * (j - nb))) >> (8 * grp)
+                                    : (uint32_t)((1ull << min(max(L - 32 * j - 8 * grp, 0), 8)) - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!((bits >> i) & 1)) sa[u][i] = NEG_INF;
+          if (!((bits >> (4 + i)) & 1)) sb[u][i] = NEG_INF;
+        }
+      }
     }
-    const float mc = m_run == NEG_INF ? 0.f : m_run * scale;
-    float pj[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) pj[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? sa[e] : sb[e - 4], scale, -mc));
-    l_run += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
-    const uint4 pf = pack8(pj);
+    for (int u = 0; u < MT; ++u) {
+      const float bmax = fmaxf(fmaxf(fmaxf(sa[u][0], sa[u][1]), fmaxf(sa[u][2], sa[u][3])),
+                               fmaxf(fmaxf(sb[u][0], sb[u][1]), fmaxf(sb[u][2], sb[u][3])));
+      if (__any(bmax > m_run[u] + slack)) {
+        const float m_new = fmaxf(m_run[u], max_xor16_32(bmax));
+        const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
+        l_run[u] *= alpha;
+        m_run[u] = m_new;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma16x16x32(f.vf[dt], pf, acc[dt]);
-    if constexpr (NODES) {
-      if (bad)
-        add_not_finite<D>(acc, pf, bad, sees >> (32 * (j - nb)),
-                          qkv + (size_t)(32 * (j - nb)) * width + (size_t)(nq + nkv + kvh) * D, width);
+        for (int dt = 0; dt < DT; ++dt) acc[u][dt] *= alpha;
+      }
+      const float mc = m_run[u] == NEG_INF ? 0.f : m_run[u] * scale;
+      float pj[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        pj[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? sa[u][e] : sb[u][e - 4], scale, -mc));
+      l_run[u] += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
+      const uint4 pf = pack8(pj);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[u][dt] = mfma16x16x32(f.vf[dt], pf, acc[u][dt]);
+      if constexpr (NODES) {
+        const uint32_t bad = (uint32_t)(badset >> (32 * (j - nb)));
+        if (bad)
+          add_not_finite<D>(acc[u], pf, bad, sees[u] >> (32 * (j - nb)),
+                            qkv + (size_t)(32 * (j - nb)) * width + (size_t)(nq + nkv + kvh) * D, width);
+      }
     }
   };
-  if (tb >= 0) process(f1, nb + tb, Int<1>{});
+  if (wave >= kTW - ntb) process(f1, nb + wave - (kTW - ntb), Int<1>{});  // the last waves
   for (int j = j0 + wave; j < jc; j += 2 * kTW) {
     if (j + kTW < jc) load_block(j + kTW, f1);
     process(f0, j, Int<0>{});
@@ -478,59 +563,52 @@ __global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttn
     if (j + kTW < jc) process(f1, j + kTW, Int<0>{});
   }
 
-  // ---- merge of the waves, in wave order.
-  float lw = l_run + shfl_xor(l_run, 16);
-  lw += shfl_xor(lw, 32);
-  if (grp == 0) {
-    s_m[wave * 16 + col] = m_run;
-    s_l[wave * 16 + col] = lw;
-  }
+  // ---- merge of the waves, in wave order; output or partial.
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[dt];
-  lds_barrier();
-  float M = NEG_INF;
-#pragma unroll
-  for (int w = 0; w < kTW; ++w) M = fmaxf(M, s_m[w * 16 + col]);
-  float sc[kTW], l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kTW; ++w) {
-    const float li = s_l[w * 16 + col];
-    sc[w] = tree_weight(s_m[w * 16 + col], li, M, scale);
-    l += li * sc[w];
-  }
-  f32x4_t o[DTW];
-  int ch[DTW];
-#pragma unroll
-  for (int i = 0; i < DTW; ++i) {
-    const int dt = wave + kTW * i;
-    ch[i] = dt * 16 + grp * 4;
-    o[i] = s_acc[dt * 64 + lane] * sc[0];
-#pragma unroll
-    for (int w = 1; w < kTW; ++w) o[i] += s_acc[(w * DT + dt) * 64 + lane] * sc[w];
-  }
-  if (n_active > 1) {
-    constexpr size_t kPart = (size_t)RG * (D + 2);
-    float *part0 = p.partial + ((size_t)cell * p.groups + g) * p.splits * kPart;
-    float *part = part0 + (size_t)c * kPart;
-    if (col < rows) {
-#pragma unroll
-      for (int i = 0; i < DTW; ++i) store_coherent4(part + (size_t)col * D + ch[i], o[i]);
-      if (wave == 0 && grp == 0) {
-        store_coherent(part + (size_t)RG * D + col, M);
-        store_coherent(part + (size_t)RG * D + RG + col, l);
-      }
+  for (int u = 0; u < MT; ++u) {
+    float lw = l_run[u] + shfl_xor(l_run[u], 16);
+    lw += shfl_xor(lw, 32);
+    if (grp == 0) {
+      s_m[(u * kTW + wave) * 16 + col] = m_run[u];
+      s_l[(u * kTW + wave) * 16 + col] = lw;
     }
-    if (!arrive_last(p.counters + (size_t)cell * p.groups + g, (uint32_t)n_active, s_flag)) return;
-    l = tree_merge<D, DTW, true>(part0, n_active, RG, min(col, rows - 1), ch, scale, o);
   }
-  if (col >= rows) return;
-  const float inv = 1.f / l;
-  const bool node = (nodes >> rt) & 1;
+  float *part = n_active > 1 ? tree_part<D>(p, cell, g, c) : nullptr;
 #pragma unroll
-  for (int i = 0; i < DTW; ++i) {
-    uint2 v = make_uint2(pack2(o[i][0] * inv, o[i][1] * inv), pack2(o[i][2] * inv, o[i][3] * inv));
-    if (!node) v = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2 *>(tree_out(p, b * T + rt, (kvh * G + row % G) * D + ch[i])) = v;
+  for (int u = 0; u < MT; ++u) {
+    if (u > 0) lds_barrier();  // the previous tile's sums are consumed
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[u][dt];
+    lds_barrier();
+    float M = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < kTW; ++w) M = fmaxf(M, s_m[(u * kTW + w) * 16 + col]);
+    float sc[kTW], l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTW; ++w) {
+      const float li = s_l[(u * kTW + w) * 16 + col];
+      sc[w] = tree_weight(s_m[(u * kTW + w) * 16 + col], li, M, scale);
+      l += li * sc[w];
+    }
+    const float inv = 1.f / l;
+    const int r = u * 16 + col;
+    const bool node = (nodes >> rt[u]) & 1;
+#pragma unroll
+    for (int i = 0; i < DTW; ++i) {
+      const int dt = wave + kTW * i, ch = dt * 16 + grp * 4;
+      f32x4_t o = s_acc[dt * 64 + lane] * sc[0];
+#pragma unroll
+      for (int w = 1; w < kTW; ++w) o += s_acc[(w * DT + dt) * 64 + lane] * sc[w];
+      if (r >= rows) continue;
+      if (n_active == 1)
+        tree_store(p, b, kvh, r0 + r, ch, o, inv, node);
+      else
+        *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + ch) = o;
+    }
+    if (n_active > 1 && wave == 0 && grp == 0 && r < rows) {
+      part[(size_t)RG * D + r] = node ? M : NEG_INF;
+      part[(size_t)RG * D + RG + r] = node ? l : 0.f;
+    }
   }
 }
 
@@ -545,33 +623,37 @@ __global__ void __launch_bounds__(64 * kTW, 2) tree_narrow_kernel(const TreeAttn
 // The node blocks are prepared into the same order behind the ring.  While
 // block j's softmax runs on the vector units, the matrix cores form block j +
 // 1's scores, one MFMA per exponential.
-template <int D, int NT>
+// What bounds it are the LDS reads (a block's 16 KiB, D = 128, serve a wave's 32
+// rows) and the matrix cores, which take as long.  (64 rows per wave would
+// halve the reads, but then the sums live in the accumulation registers, and
+// the scores with them: every score tile moved between the two files.)
+template <int D, int NW, int NT>
 struct WideLds {
   static constexpr int KF = D / 16, VF = D / 16;  // fragments of a block
   static constexpr int BV = (KF + VF) * 64;       // uint4 per block
-  static constexpr int RING = 4;
+  static constexpr int RING = NW == 8 ? 8 : 4;    // 8 waves: one workgroup per CU, 4: two
   static constexpr int vecs = (RING + NT) * BV;   // NT node blocks
 };
 
-template <int D, int NW, int MT, int NT>
+template <int D, int NW, int NT>
 __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 2) tree_wide_kernel(const TreeAttnParams p) {
-  using LY = WideLds<D, NT>;
+  using LY = WideLds<D, NW, NT>;
+  constexpr int MT = 2;
   constexpr int DS = D / 32, DT = D / 16, KF = LY::KF, BV = LY::BV, RING = LY::RING;
   constexpr int FPW = (KF + LY::VF) / NW;  // fragments each wave loads per block
   constexpr int RG = 16 * MT * NW;         // rows of a group
-  static_assert(KF % NW == 0 || (KF + LY::VF) % NW == 0, "whole fragments per wave");
+  static_assert((KF + LY::VF) % NW == 0 && (RING - 2) * FPW < 64, "whole fragments per wave, counted in vmcnt");
   __shared__ uint4 ring[LY::vecs];         // [RING + NT][fragment][lane]
   uint4 *const tail = ring + RING * BV;
-  // Rows with a value that is not finite, a word per key tile: in the last
-  // ring slot, which takes its first block after they were read.
-  uint32_t *s_bad = reinterpret_cast<uint32_t *>(ring + (RING - 1) * BV);
+  // Node rows with a value that is not finite: in the last ring slot, which
+  // takes its first block after they were read.
+  int *s_bad = reinterpret_cast<int *>(ring + (RING - 1) * BV);
   const float NEG_INF = -__builtin_huge_valf();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
 
   const TreeUnit u_ = tree_unit(p);
   const int c = u_.c, cell = u_.cell, g = u_.g, kvh = u_.kvh, b = u_.b;
-  const int ng = p.groups, C = p.splits;
   const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv;
   const int R = T * G, r0 = g * RG;
   const int rows = min(RG, R - r0);
@@ -620,6 +702,10 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   for (int jj = 0; jj < RING - 1; ++jj)
     if (jj < nd) dma_block(jj);
 
+  const int ntb = max(run.j1 - nb, 0);  // the last split has the node blocks
+  TreeTail<D, NW, NT> nt;
+  if (ntb > 0) nt.load(p, qkv, kvh, ntb);
+
   // ---- ancestor sets and queries.
   const uint64_t anc = tree_ancestors(up, T, lane);
   const int depth = (int)__popcll(anc) - 1;  // -1: no node (its rows are prepared at L and dropped)
@@ -630,69 +716,20 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   for (int u = 0; u < MT; ++u) {
     sees[u] = shfl64(anc, row[u] / G);
     const size_t at = (size_t)__shfl(pos, row[u] / G, 64) * D + 8 * grp;
-    head_frags<D>(qf[u], p.q_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
+    Head<D> qw, cw, sw;
+    qw.load(p.q_norm_w + 8 * grp);
+    cw.load(p.cos_tab + at);
+    sw.load(p.sin_tab + at);
+    head_rows<D>(qf[u], qw, cw, sw, p.eps);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);  // one tile's tables at a time (registers)
   }
 
-  // ---- the node blocks of this run.
+  // ---- the node blocks.
   uint64_t badset = 0;
-  const int tb0 = max(j0 - nb, 0), tb1 = run.j1 - nb;  // node blocks, none when tb1 <= tb0
-  if (tb1 > tb0) {
-    // Value fragment dt of node block i / DT: its loads go out before the keys
-    // are worked on.
-    constexpr int VW = DT * NT / NW > 0 ? DT * NT / NW : 1;  // per wave, at most
-    uint32_t vr[VW][8];
-    const uint16_t *v0 = qkv + (size_t)(nq + nkv + kvh) * D + col;
-#pragma unroll
-    for (int k = 0; k < VW; ++k) {
-      const int i = DT * tb0 + wave + NW * k;
-      if (i >= DT * tb1) break;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) vr[k][e] = v0[(size_t)min(32 * (i / DT) + 8 * grp + e, T - 1) * width + 16 * (i % DT)];
-    }
-    for (int i = 2 * tb0 + wave; i < 2 * tb1; i += NW) {  // key tile h of block i / 2
-      const int h = i & 1, t = 32 * (i >> 1) + 8 * (col >> 2) + (col & 3) + 4 * h, tr = min(t, T - 1);
-      const bool node = (nodes >> t) & 1;
-      const uint16_t *kr = qkv + (size_t)tr * width + (size_t)(nq + kvh) * D + 8 * grp;
-      uint4 k[DS], v[DS];
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        k[s] = ld16(kr + 32 * s);
-        v[s] = ld16(kr + (size_t)nkv * D + 32 * s);
-      }
-      const size_t at = (size_t)__shfl(pos, tr, 64) * D + 8 * grp;
-      head_frags<D>(k, p.k_norm_w + 8 * grp, p.cos_tab + at, p.sin_tab + at, p.eps);
-      bool fin = true;
-#pragma unroll
-      for (int s = 0; s < DS; ++s) {
-        tail[(i >> 1) * BV + (2 * s + h) * 64 + lane] = k[s];
-        fin = fin && finite8(v[s]);
-      }
-      const uint64_t nf = __ballot(node && !fin);
-      if (lane == 0) s_bad[i] = (uint32_t)((nf | nf >> 16 | nf >> 32 | nf >> 48) & 0xffffu);
-      if (node && g == 0) {
-        const size_t o = ((size_t)cell * T + t) * D + 8 * grp;
-#pragma unroll
-        for (int s = 0; s < DS; ++s) {
-          *reinterpret_cast<uint4 *>(p.k_nodes + o + 32 * s) = k[s];
-          *reinterpret_cast<uint4 *>(p.v_nodes + o + 32 * s) = v[s];
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < VW; ++k) {
-      const int i = DT * tb0 + wave + NW * k;
-      if (i >= DT * tb1) break;
-      const int t0 = 32 * (i / DT) + 8 * grp;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)  // no node, or not finite (add_not_finite): zero
-        if (!((nodes >> (t0 + e)) & 1) || (vr[k][e] & 0x7f80u) == 0x7f80u) vr[k][e] = 0;
-      tail[(i / DT) * BV + (KF + i % DT) * 64 + lane] =
-          make_uint4(vr[k][0] | vr[k][1] << 16, vr[k][2] | vr[k][3] << 16, vr[k][4] | vr[k][5] << 16, vr[k][6] | vr[k][7] << 16);
-    }
+  if (ntb > 0) {
+    nt.store(p, tail, s_bad, cell, g == 0, ntb, pos, nodes);
     lds_barrier();
-    // lane t: its row's place among the key tiles
-    const int tile = 2 * (lane >> 5) + ((lane >> 2) & 1);
-    badset = __ballot(tile >= 2 * tb0 && tile < 2 * tb1 && ((s_bad[tile] >> (4 * ((lane >> 3) & 3) + (lane & 3))) & 1));
+    badset = __ballot(lane < 32 * ntb && s_bad[lane]);
   }
 
   f32x4_t acc[MT][DT];
@@ -723,13 +760,15 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   // Block jj (if from the cache) is in LDS after every wave has waited for
   // its own loads of it, `newest` being the last block issued.
   auto await = [&](int jj, int newest) {
-    const int younger = min(newest, nd - 1) - jj;
-    if (younger >= 2)
-      __builtin_amdgcn_s_waitcnt(vmcnt_enc(2 * FPW) & ~(15 << 8));
-    else if (younger == 1)
-      __builtin_amdgcn_s_waitcnt(vmcnt_enc(FPW) & ~(15 << 8));
-    else
-      __builtin_amdgcn_s_waitcnt(kVmcnt0 & ~(15 << 8));
+    switch (min(newest, nd - 1) - jj) {  // younger blocks may stay in flight
+      case 6: if constexpr (RING >= 8) { __builtin_amdgcn_s_waitcnt(vmcnt_enc(6 * FPW) & ~(15 << 8)); break; } [[fallthrough]];
+      case 5: if constexpr (RING >= 8) { __builtin_amdgcn_s_waitcnt(vmcnt_enc(5 * FPW) & ~(15 << 8)); break; } [[fallthrough]];
+      case 4: if constexpr (RING >= 8) { __builtin_amdgcn_s_waitcnt(vmcnt_enc(4 * FPW) & ~(15 << 8)); break; } [[fallthrough]];
+      case 3: if constexpr (RING >= 8) { __builtin_amdgcn_s_waitcnt(vmcnt_enc(3 * FPW) & ~(15 << 8)); break; } [[fallthrough]];
+      case 2: __builtin_amdgcn_s_waitcnt(vmcnt_enc(2 * FPW) & ~(15 << 8)); break;
+      case 1: __builtin_amdgcn_s_waitcnt(vmcnt_enc(FPW) & ~(15 << 8)); break;
+      default: __builtin_amdgcn_s_waitcnt(kVmcnt0 & ~(15 << 8));
+    }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
@@ -743,7 +782,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   if (RING - 1 < nd) dma_block(RING - 1);
   read_k(min(1, n - 1));
 
-  const float scale = p.scale_log2;
+  const float scale = p.scale_log2, slack = kMaxSlack / scale;
   auto block = [&](int jj, Scores &S, Scores &N, auto lastc) {
     constexpr bool LAST = decltype(lastc)::value != 0;
     const int j = j0 + jj;
@@ -763,7 +802,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
     for (int u = 0; u < MT; ++u) {
       const float bmax = fmaxf(fmaxf(fmaxf(S.a[u][0], S.a[u][1]), fmaxf(S.a[u][2], S.a[u][3])),
                                fmaxf(fmaxf(S.b[u][0], S.b[u][1]), fmaxf(S.b[u][2], S.b[u][3])));
-      if (!__any(bmax > m_run[u])) continue;  // no row's maximum moves
+      if (!__any(bmax > m_run[u] + slack)) continue;
       const float m_new = fmaxf(m_run[u], max_xor16_32(bmax));
       const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
       l_run[u] *= alpha;
@@ -850,24 +889,19 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   }
   block(jj, s0, s1, Int<1>{});
 
-  // ---- output, or a partial per row (m = -inf and l = 0 where a row holds no
-  // node, which is how the merge knows it).
-  float *part = p.partial + (n_active == 1 ? (size_t)0 : (((size_t)cell * ng + g) * C + c) * ((size_t)RG * (D + 2)));
+  // ---- output or partial.
+  float *part = n_active > 1 ? tree_part<D>(p, cell, g, c) : nullptr;
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
-    const int r = (wave * MT + u) * 16 + col, t = row[u] / G;
-    const bool node = (nodes >> t) & 1;
+    const int r = (wave * MT + u) * 16 + col;
+    const bool node = (nodes >> (row[u] / G)) & 1;
     float l = l_run[u] + shfl_xor(l_run[u], 16);
     l += shfl_xor(l, 32);
     if (r >= rows) continue;
     if (n_active == 1) {
       const float inv = 1.f / l;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint2 v = make_uint2(pack2(acc[u][dt][0] * inv, acc[u][dt][1] * inv), pack2(acc[u][dt][2] * inv, acc[u][dt][3] * inv));
-        if (!node) v = make_uint2(0u, 0u);
-        *reinterpret_cast<uint2 *>(tree_out(p, b * T + t, (kvh * G + row[u] % G) * D + dt * 16 + grp * 4)) = v;
-      }
+      for (int dt = 0; dt < DT; ++dt) tree_store(p, b, kvh, row[u], dt * 16 + grp * 4, acc[u][dt], inv, node);
     } else {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + dt * 16 + grp * 4) = acc[u][dt];
@@ -879,27 +913,51 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   }
 }
 
-// Merge of the wide kernel's partials: D / 4 threads per row.
+// Merge of the splits' partials, in order: D / 4 threads per query row, the loads
+// of 8 partials in flight at a time.
 template <int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p) {
   constexpr int TR = D / 4;
-  const int T = p.t_rows, G = p.nq / p.nkv, R = T * G, RG = p.group_rows;
+  const int R = p.t_rows * (p.nq / p.nkv), RG = p.group_rows;
   const int per = (R + 256 / TR - 1) / (256 / TR);  // workgroups per cell
   const int cell = blockIdx.x / per, kvh = cell % p.nkv, b = cell / p.nkv;
   const int r = (blockIdx.x - cell * per) * (256 / TR) + threadIdx.x / TR;
   const int L = p.lens[b];
-  if (L < 0 || L > p.cap - T || r >= R) return;
-  const int n = tree_active(p.splits, p.min_blocks, (L + 31) >> 5, (T + 31) >> 5);
+  if (L < 0 || L > p.cap - p.t_rows || r >= R) return;
+  const int n = tree_active(p.splits, p.min_blocks, (L + 31) >> 5, (p.t_rows + 31) >> 5);
   if (n == 1) return;  // written by the one workgroup
-  const int g = r / RG;
-  const int ch[1] = {(int)(threadIdx.x % TR) * 4};
-  f32x4_t o[1];
-  const float l = tree_merge<D, 1, false>(p.partial + ((size_t)cell * p.groups + g) * p.splits * ((size_t)RG * (D + 2)), n, RG,
-                                          r - g * RG, ch, p.scale_log2, o);
-  const float inv = 1.f / l;
-  uint2 v = make_uint2(pack2(o[0][0] * inv, o[0][1] * inv), pack2(o[0][2] * inv, o[0][3] * inv));
-  if (l == 0.f) v = make_uint2(0u, 0u);  // no node
-  *reinterpret_cast<uint2 *>(tree_out(p, b * T + r / G, (kvh * G + r % G) * D + ch[0])) = v;
+  const int g = r / RG, rg = r - g * RG, ch = (int)(threadIdx.x % TR) * 4;
+  const float *part = tree_part<D>(p, cell, g, 0);
+  const size_t stride = (size_t)RG * (D + 2);
+  const float scale = p.scale_log2;
+  float M = -__builtin_huge_valf(), l = 0.f;
+  f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float mi[8], li[8];
+    f32x4_t a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float *pr = part + (size_t)min(i0 + i, n - 1) * stride;
+      mi[i] = pr[(size_t)RG * D + rg];
+      li[i] = pr[(size_t)RG * D + RG + rg];
+      a[i] = *reinterpret_cast<const f32x4_t *>(pr + (size_t)rg * D + ch);
+    }
+    float Mn = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) Mn = fmaxf(Mn, mi[i]);  // (the last partial repeats)
+    const float w0 = tree_weight(M, l, Mn, scale);
+    l *= w0;
+    o *= w0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= n) continue;
+      const float w = tree_weight(mi[i], li[i], Mn, scale);
+      l += li[i] * w;
+      o += a[i] * w;
+    }
+    M = Mn;
+  }
+  tree_store(p, b, kvh, r, ch, o, 1.f / l, l != 0.f);  // (a node's sum is not 0)
 }
 
 template <int D>
@@ -907,18 +965,21 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
   const dim3 grid((unsigned)(p.batch * p.nkv * p.groups * p.splits));
   const bool two = p.t_rows > 32;  // node blocks
   switch (p.group_rows) {
-    case 16: hipLaunchKernelGGL((tree_narrow_kernel<D>), grid, dim3(64 * kTW), 0, s, p); return hipSuccess;
-    case 64:
-      if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 4, 1, 2>), grid, dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((tree_wide_kernel<D, 4, 1, 1>), grid, dim3(256), 0, s, p);
+    case 16:
+      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 2>), grid, dim3(64 * kTW), 0, s, p);
+      else hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 1>), grid, dim3(64 * kTW), 0, s, p);
+      break;
+    case 32:
+      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 2>), grid, dim3(64 * kTW), 0, s, p);
+      else hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 1>), grid, dim3(64 * kTW), 0, s, p);
       break;
     case 128:
-      if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 4, 2, 2>), grid, dim3(256), 0, s, p);
-      else hipLaunchKernelGGL((tree_wide_kernel<D, 4, 2, 1>), grid, dim3(256), 0, s, p);
+      if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 4, 2>), grid, dim3(256), 0, s, p);
+      else hipLaunchKernelGGL((tree_wide_kernel<D, 4, 1>), grid, dim3(256), 0, s, p);
       break;
     case 256:
-      if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 8, 2, 2>), grid, dim3(512), 0, s, p);
-      else hipLaunchKernelGGL((tree_wide_kernel<D, 8, 2, 1>), grid, dim3(512), 0, s, p);
+      if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 8, 2>), grid, dim3(512), 0, s, p);
+      else hipLaunchKernelGGL((tree_wide_kernel<D, 8, 1>), grid, dim3(512), 0, s, p);
       break;
     default: return hipErrorInvalidValue;
   }
@@ -931,17 +992,17 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 
 }  // namespace
 
-// The row group (16: the narrow kernel; 64, 128 or 256: the wide one) and the
-// splits.
+// The row group (16 or 32: the narrow kernel; 128 or 256: the wide one) and
+// the splits.
 void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int rows = p->t_rows * (p->nq / p->nkv);
   const int64_t cells = (int64_t)p->batch * p->nkv;
   const int blocks = p->cap / 32;
-  p->group_rows = rows <= 32 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  p->group_rows = rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
   p->min_blocks = 4;
   p->groups = (rows + p->group_rows - 1) / p->group_rows;
   if (splits == 0) {
-    const int64_t fill = p->group_rows == 256 ? 256 : 512;  // workgroups the CUs hold at once
+    const int64_t fill = p->group_rows == 16 || p->group_rows == 128 ? 512 : 256;  // workgroups the CUs hold at once
     splits = (int)std::max<int64_t>(1, std::min<int64_t>(fill / (cells * p->groups), blocks / p->min_blocks));
   }
   p->splits = std::min(splits, 256);

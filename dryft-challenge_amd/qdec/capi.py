@@ -110,8 +110,8 @@ class TreeDraftArgs(ctypes.Structure):
 class TreeAttnArgs(ctypes.Structure):
     _fields_ = [("qkv", P), ("q_norm_w", P), ("k_norm_w", P), ("cos_tab", P), ("sin_tab", P), ("lens", P),
                 ("parents", P), ("k_cache", P), ("v_cache", P), ("k_nodes", P), ("v_nodes", P), ("out", P),
-                ("partial", P), ("counters", P), ("eps", F32), ("sm_scale", F32), ("batch", I32),
-                ("t_rows", I32), ("nq", I32), ("nkv", I32), ("head_dim", I32), ("cap", I32), ("splits", I32),
+                ("partial", P), ("eps", F32), ("sm_scale", F32), ("batch", I32), ("t_rows", I32), ("nq", I32),
+                ("nkv", I32), ("head_dim", I32), ("cap", I32), ("splits", I32),
                 ("out_frag", I32)]
 
 

@@ -510,9 +510,10 @@ int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
  * they were.  A length with lens[b] < 0 or lens[b] + t_rows > cap reads and
  * writes no cache or node memory; the rows of sequence b become NaN.
  * The cached slots and the nodes are dealt in 32-row blocks, evenly, to
- * `splits` workgroups per 64 query rows of a (sequence, kv head), fewer for a
- * short cache; the last one to finish merges their partials in order.  So a
- * result depends on splits, lens[b] and t_rows, never on timing. */
+ * `splits` workgroups per row group of a (sequence, kv head), fewer for a short
+ * cache; with splits > 1 they leave partials that a second launch merges in
+ * order.  So a result depends on splits, lens[b] and the call's shape, never on
+ * timing.  partial is scratch: calls that overlap in time must not share it. */
 typedef struct {
   const void *qkv;        /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
   const void *q_norm_w;   /* [head_dim] bf16 */
@@ -526,8 +527,7 @@ typedef struct {
   void *k_nodes;          /* [batch][nkv][t_rows][head_dim] bf16 out */
   void *v_nodes;          /* the same */
   void *out;              /* [batch*t_rows, nq*head_dim] bf16 */
-  float *partial;         /* split partials (qdec_tree_attn_workspace) */
-  uint32_t *counters;     /* zeroed arrival counters (qdec_tree_attn_workspace) */
+  float *partial;         /* split partials, 16-byte aligned (qdec_tree_attn_workspace) */
   float eps;
   float sm_scale;         /* 1/sqrt(head_dim) */
   int32_t batch;
@@ -540,6 +540,8 @@ typedef struct {
   int32_t out_frag;       /* 1: out in the fragment order of qdec_gemm_args */
 } qdec_tree_attn_args;
 int qdec_tree_attn(const qdec_tree_attn_args *a, qdec_stream_t stream);
+/* Bytes of `partial`; counter_bytes, as in the other queries, is 0: there are no
+ * counters. */
 int qdec_tree_attn_workspace(const qdec_tree_attn_args *a, size_t *partial_bytes, size_t *counter_bytes);
 
 /* Greedy acceptance on a tree: from the root, as long as some child of the

@@ -80,7 +80,7 @@ CASES = [
     ("tree_attn", attn, dict(k_nodes=None), -1, "null"),
     ("tree_attn", attn, dict(out=None), -1, "null"),
     ("tree_attn", attn, dict(splits=2, partial=None), -1, "partial"),
-    ("tree_attn", attn, dict(splits=2, counters=None), -1, "counters"),
+    ("tree_attn", attn, dict(splits=2, partial=8), -2, "aligned"),
     ("tree_attn", attn, dict(qkv=8), -2, "aligned"),
     ("tree_attn", attn, dict(cos_tab=24), -2, "aligned"),
     ("tree_attn", attn, dict(v_nodes=18), -2, "aligned"),
@@ -118,15 +118,12 @@ def test_null_args(qlib, name):
 
 def test_workspace(qlib):
     assert qlib.tree_attn_workspace(attn(splits=1)) == (0, 0)
-    # a partial is 16, 32, 64, 128 or 256 rows (a group of them from 257) of D + 2 floats
-    assert qlib.tree_attn_workspace(attn(splits=3)) == (4 * 16 * 3 * 32 * 130, 4 * 16)
-    assert qlib.tree_attn_workspace(attn(splits=2, head_dim=64, t_rows=1)) == (4 * 16 * 2 * 16 * 66, 4 * 16)
-    for nq, t in ((64, 9), (40, 64), (8, 64), (128, 64)):
-        pb, cb = qlib.tree_attn_workspace(attn(splits=2, nq=nq, t_rows=t))
-        groups = cb // (4 * 16)
-        assert pb % (4 * 16 * 2 * 130 * groups) == 0 and pb >= 4 * 16 * 2 * 130 * t * (nq // 8)
+    # a partial holds whole row groups, D + 2 floats a row; no counters
+    for nq, t, d in ((32, 8, 128), (32, 1, 64), (64, 9, 128), (40, 64, 128), (8, 64, 128), (128, 64, 64)):
+        pb, cb = qlib.tree_attn_workspace(attn(splits=3, nq=nq, t_rows=t, head_dim=d))
+        assert cb == 0 and pb % (4 * 16 * 3 * (d + 2)) == 0 and pb >= 4 * 16 * 3 * (d + 2) * t * (nq // 8)
     # splits = 0: the shape decides, and no more than one per four blocks of the cache
     pb, cb = qlib.tree_attn_workspace(attn(batch=1, cap=128))
     assert (pb, cb) == (0, 0)
     pb, cb = qlib.tree_attn_workspace(attn(batch=1, cap=1 << 20))
-    assert pb > 0 and cb == 4 * 8
+    assert pb > 0 and cb == 0
