@@ -268,6 +268,15 @@ hipError_t launch_accept(const int64_t *out_tok, const int64_t *draft, int64_t *
 // ---- tree speculation (tree.hip, tree_attn.hip)
 constexpr int kTreeMaxT = QDEC_TREE_MAX_T;
 constexpr int kTreeMaxMatches = QDEC_TREE_MAX_MATCHES;
+// n / d for 0 <= n < 2^31 as one multiplication and a shift.
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1u << s) < d) ++s;  // d <= 2^s, d <= 2^30
+  return FastDiv{d, (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
+}
 struct TreeAttnParams {
   const uint16_t *qkv, *q_norm_w, *k_norm_w, *cos_tab, *sin_tab;
   const int32_t *lens, *parents;
@@ -277,10 +286,11 @@ struct TreeAttnParams {
   float eps;
   float scale_log2;  // log2(e) / sqrt(head_dim)
   int batch, t_rows, nq, nkv, head_dim, cap;
-  int splits;      // workgroups per (sequence, kv head, row group)
+  int splits;      // workgroups per (sequence, kv head, row group), on average
   int min_blocks;  // 32-row blocks a workgroup gets before another one is used
   int group_rows;  // query rows a workgroup takes: 16, 32, 128 or 256
   int groups;      // row groups: ceil(t_rows * nq / nkv / group_rows)
+  FastDiv by_groups, by_nkv, by_g;  // g: query heads per kv head
   int ofrag;       // > 0: out is written in fragment order with this many M tiles
 };
 void tree_attn_plan(TreeAttnParams *p, int splits);

@@ -18,9 +18,9 @@
 //     rounds.  A set that does not reach the root is no node's.  The depth is
 //     the size of the set less one.
 //   * Per block S^T = K . Q^T (v_mfma_f32_16x16x32_bf16), online softmax in
-//     base 2 on fp32 scores, O^T += V^T . P^T (P rounded to bf16, the operand
-//     type).  The running maximum is only moved, and the sums rescaled, in
-//     blocks where some row's maximum grows.
+//     base 2 on fp32 scores, O^T += V^T . P^T with P in two bf16 parts.  What is
+//     rounded to bf16, because a matrix instruction or a buffer takes it, is
+//     rounded once: queries, node keys, the parts of P, the output.
 //   * A lane's query rows are prepared in registers, in the place where the
 //     MFMA's B operand wants them: lane (c, g) holds channels 32s + 8g .. +8 of
 //     row c for every k step s, so the rotation's partner channel is the
@@ -60,27 +60,24 @@ struct Head {
   }
 };
 
-// Head RMSNorm (gain w) and RoPE (cos c, sin n) of such a row, with the bits of
-// head_norm_rope: the same balanced sum over the channels (8 in the lane, 16
-// and 32 across lanes, 64 and 128 in the lane).
+// Head RMSNorm (gain w) and RoPE (cos c, sin n) of such a row, in fp32; one
+// rounding to bf16, the operand type, at the end.
 template <int D>
 __device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], const Head<D> &w, const Head<D> &cw, const Head<D> &sw,
                                           float eps) {
   constexpr int DS = D / 32;
-  float part[DS];
+  float ss = 0.f;
 #pragma unroll
   for (int s = 0; s < DS; ++s) {
     float x[8];
     unpack8(f[s], x);
-    float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
-               ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
-    ss = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
-    part[s] = __uint_as_float(b[0]) + __uint_as_float(b[1]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
   }
-  float ss = part[0] + part[1];
-  if constexpr (DS == 4) ss = ss + (part[2] + part[3]);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
+  ss = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
+  ss = __uint_as_float(b[0]) + __uint_as_float(b[1]);
   const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
 #pragma unroll
   for (int s = 0; s < DS / 2; ++s) {
@@ -88,22 +85,34 @@ __device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], const Head<D> &w, 
     unpack8(f[s], lo);
     unpack8(w.v[s], g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] = rbf(g[e] * rbf(lo[e] * rstd));
+    for (int e = 0; e < 8; ++e) lo[e] *= rstd * g[e];
     unpack8(f[s + DS / 2], hi);
     unpack8(w.v[s + DS / 2], g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hi[e] = rbf(g[e] * rbf(hi[e] * rstd));
+    for (int e = 0; e < 8; ++e) hi[e] *= rstd * g[e];
     unpack8(cw.v[s], c);
     unpack8(sw.v[s], n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = rbf(lo[e] * c[e]) + rbf(-hi[e] * n[e]);
+    for (int e = 0; e < 8; ++e) o[e] = lo[e] * c[e] - hi[e] * n[e];
     f[s] = pack8(o);
     unpack8(cw.v[s + DS / 2], c);
     unpack8(sw.v[s + DS / 2], n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = rbf(hi[e] * c[e]) + rbf(lo[e] * n[e]);
+    for (int e = 0; e < 8; ++e) o[e] = hi[e] * c[e] + lo[e] * n[e];
     f[s + DS / 2] = pack8(o);
   }
+}
+
+// Eight probabilities as two bf16 operands whose sum has 16 bits of them: with
+// one operand their rounding is, beside the output's own, the largest error of
+// the result (1.7 times the output's rounding alone; 1.4 with two).
+__device__ __forceinline__ void split8(const float (&p)[8], uint4 &hi, uint4 &lo) {
+  hi = pack8(p);
+  float h[8], d[8];
+  unpack8(hi, h);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] = p[e] - h[e];
+  lo = pack8(d);
 }
 
 __device__ __forceinline__ bool finite8(const uint4 &v) {
@@ -111,54 +120,108 @@ __device__ __forceinline__ bool finite8(const uint4 &v) {
   return two(v.x) && two(v.y) && two(v.z) && two(v.w);
 }
 
-// A workgroup's place: split c of row group g of cell = b * nkv + kvh.  The row
-// groups of one (cell, split) read the same keys and values: they get numbers
-// that are equal modulo 8, the number of XCDs, and close together, so that
-// they share an L2.
+__device__ __forceinline__ int div_by(const FastDiv &d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0, 2 to rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2, 3
+  return v;
+}
+
+// The splits are dealt to the sequences in proportion to their blocks, so that
+// the workgroups' runs are about equal in a batch of unequal lengths: of a kv
+// head's batch * splits workgroups, sequence b's are first .. first + n - 1.
+struct TreeDeal {
+  int b, L, n, first;  // n = 0: a workgroup that is left over
+};
+__device__ __forceinline__ bool tree_valid(const TreeAttnParams &p, int L) { return L >= 0 && L <= p.cap - p.t_rows; }
+// Blocks of a sequence of L slots (one where L is out of range).
+__device__ __forceinline__ int tree_weight_of(const TreeAttnParams &p, int L) {
+  return tree_valid(p, L) ? ((L + 31) >> 5) + kTailWeight * ((p.t_rows + 31) >> 5) : 1;
+}
+// Sequence b's workgroups end at E(b) = b + 1 + round(W(b) * batch * (splits - 1)
+// / W(batch - 1)), W the running sum of the weights: one each, the others in
+// proportion, batch * splits in all however the quotient rounds (it never
+// falls as W grows).  A split that would get fewer than `least` blocks is left
+// out; least >= kTailWeight per node block keeps the splits before the last
+// one from being empty.
+template <bool BY_SEQ>  // at = a sequence, else a workgroup
+__device__ __forceinline__ TreeDeal tree_deal(const TreeAttnParams &p, int at) {
+  const int B = p.batch, S = p.splits, lane = threadIdx.x & 63;
+  if (S == 1) return TreeDeal{at, p.lens[at], 1, at};
+  const int least = max(p.min_blocks, kTailWeight * ((p.t_rows + 31) >> 5));
+  auto active = [&](int w, int n) { return w < 2 * least ? 1 : min(n, w / least); };
+  if (B == 1) {
+    const int L = p.lens[0], n = active(tree_weight_of(p, L), S);
+    return TreeDeal{0, L, BY_SEQ || at < n ? n : 0, 0};
+  }
+  int total = 0;
+  for (int b0 = 0; b0 < B; b0 += 64)
+    total += __builtin_amdgcn_readlane(wave_scan(b0 + lane < B ? tree_weight_of(p, p.lens[min(b0 + lane, B - 1)]) : 0), 63);
+  const int spare = B * (S - 1);
+  const float ratio = (float)spare / (float)total;
+  int sum = 0, base = 0;  // weights and workgroups of the 64s before
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int b = b0 + lane, L = p.lens[min(b, B - 1)], w = b < B ? tree_weight_of(p, L) : 0;
+    const int W = sum + wave_scan(w);
+    const int end = min(b, B - 1) + 1 + min(spare, (int)((float)W * ratio + 0.5f));
+    int hit = at - b0;
+    if constexpr (!BY_SEQ) {
+      const uint64_t m = __ballot(end > at);
+      hit = m ? __builtin_ctzll(m) : 64;
+    }
+    if (hit < 64) {
+      hit = __builtin_amdgcn_readfirstlane(hit);
+      const int first = hit > 0 ? __builtin_amdgcn_readlane(end, max(hit - 1, 0)) : base;
+      const int n = active(__builtin_amdgcn_readlane(w, hit), __builtin_amdgcn_readlane(end, hit) - first);
+      return TreeDeal{b0 + hit, __builtin_amdgcn_readlane(L, hit), BY_SEQ || at - first < n ? n : 0, first};
+    }
+    sum = __builtin_amdgcn_readlane(W, 63);
+    base = __builtin_amdgcn_readlane(end, 63);
+  }
+  return TreeDeal{0, 0, 0, 0};
+}
+
+// A workgroup's place: row group g of unit = w * nkv + kvh, w its number among
+// the kv head's.  The row groups of one unit read the same keys and values:
+// they get numbers that are equal modulo 8, the number of XCDs, and close
+// together, so that they share an L2.
 struct TreeUnit {
-  int c, cell, g, kvh, b;
+  int unit, w, g, kvh;
 };
 __device__ __forceinline__ TreeUnit tree_unit(const TreeAttnParams &p) {
-  const int ng = p.groups, units = p.batch * p.nkv * p.splits, whole = units & ~7;
+  const int ng = p.groups, x = blockIdx.x, whole = (p.batch * p.nkv * p.splits) & ~7;
   TreeUnit r;
-  int unit;
-  if ((int)blockIdx.x < whole * ng) {
-    const int q = blockIdx.x >> 3;
-    r.g = q % ng;
-    unit = (q / ng) * 8 + (blockIdx.x & 7);
-  } else {
-    const int y = blockIdx.x - whole * ng;
-    r.g = y % ng;
-    unit = whole + y / ng;
+  r.unit = x;
+  r.g = 0;
+  if (ng > 1) {
+    const bool main = x < whole * ng;
+    const int y = main ? x >> 3 : x - whole * ng, q = div_by(p.by_groups, y);
+    r.g = y - q * ng;
+    r.unit = main ? q * 8 + (x & 7) : whole + q;
   }
-  r.c = unit % p.splits;
-  r.cell = unit / p.splits;
-  r.kvh = r.cell % p.nkv;
-  r.b = r.cell / p.nkv;
+  r.w = div_by(p.by_nkv, r.unit);
+  r.kvh = r.unit - r.w * p.nkv;
   return r;
 }
 
-// The blocks j0 .. j1 - 1 of split c of a sequence of L cached slots, the first
-// nb of all from the cache; every one of the n_active splits holds some
-// (c >= n_active: n_active = -1), the last one the node blocks.
+// The blocks j0 .. j1 - 1 of split c of n, the first nb of all from the cache,
+// the node blocks (the last split's) behind them.
 struct TreeRun {
-  int nb, n_active, j0, j1;
+  int nb, j0, j1;
 };
-__host__ __device__ __forceinline__ int tree_active(int splits, int min_blocks, int nb, int ntb) {
-  // at least tail / 2 + 1 blocks per split, so that the one before the last
-  // has one left
-  const int tail = kTailWeight * ntb, least = min_blocks > tail / 2 ? min_blocks : tail / 2 + 1;
-  const int n = (nb + tail) / least;
-  return n < 1 ? 1 : n < splits ? n : splits;
-}
-__device__ __forceinline__ TreeRun tree_run(const TreeAttnParams &p, int L, int c) {
+__device__ __forceinline__ TreeRun tree_run(const TreeAttnParams &p, int L, int c, int n) {
   TreeRun r;
   r.nb = (L + 31) >> 5;
   const int ntb = (p.t_rows + 31) >> 5, total = r.nb + kTailWeight * ntb;
-  r.n_active = tree_active(p.splits, p.min_blocks, r.nb, ntb);
-  r.j0 = min((int)((int64_t)total * c / r.n_active), r.nb);
-  r.j1 = c + 1 == r.n_active ? r.nb + ntb : min((int)((int64_t)total * (c + 1) / r.n_active), r.nb);
-  if (c >= r.n_active) r.n_active = -1;
+  const int each = total / n, more = total - each * n;
+  r.j0 = min(each * c + min(c, more), r.nb);
+  r.j1 = c + 1 == n ? r.nb + ntb : min(each * (c + 1) + min(c + 1, more), r.nb);
   return r;
 }
 
@@ -214,49 +277,43 @@ __device__ __forceinline__ void add_not_finite(f32x4_t (&acc)[D / 16], const uin
   }
 }
 
-// A node row spread over D / 8 consecutive lanes, 8 channels each: RMSNorm and
-// RoPE of head_rows, the same bits.
+// The same of a row spread over D / 8 consecutive lanes, 8 channels each.
 template <int D>
 __device__ __forceinline__ uint4 head_row(const uint4 &raw, const uint4 &w, const uint4 &cw, const uint4 &sw, float eps) {
   constexpr int LPR = D / 8;
-  float x[8], g[8], c[8], s[8], y[8];
+  float x[8], g[8], c[8], s[8], r[8];
   unpack8(raw, x);
   unpack8(w, g);
   unpack8(cw, c);
   unpack8(sw, s);
-  float ss = ((x[0] * x[0] + x[1] * x[1]) + (x[2] * x[2] + x[3] * x[3])) +
-             ((x[4] * x[4] + x[5] * x[5]) + (x[6] * x[6] + x[7] * x[7]));
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
   ss += dpp_f<0xB1>(ss);                            // lane ^ 1
   ss += dpp_f<0x4E>(ss);                            // lane ^ 2
   ss += dpp_f<0x141>(ss);                           // the other quad of 8
   if constexpr (LPR == 16) ss += dpp_f<0x140>(ss);  // the other 8 of 16
   const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = rbf(g[e] * rbf(x[e] * rstd));
-  const uint4 mine = pack8(y);
-  uint4 other;  // channels i +- D / 2: bf16 values, so four words
-  other.x = (uint32_t)__shfl_xor((int)mine.x, LPR / 2, 64);
-  other.y = (uint32_t)__shfl_xor((int)mine.y, LPR / 2, 64);
-  other.z = (uint32_t)__shfl_xor((int)mine.z, LPR / 2, 64);
-  other.w = (uint32_t)__shfl_xor((int)mine.w, LPR / 2, 64);
-  float r[8];
-  unpack8(other, r);
   const bool first = (threadIdx.x & (LPR - 1)) < LPR / 2;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = rbf(y[e] * c[e]) + rbf((first ? -r[e] : r[e]) * s[e]);
-  return pack8(y);
+  for (int e = 0; e < 8; ++e) x[e] *= rstd * g[e];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = shfl_xor(x[e], LPR / 2);  // channels i +- D / 2
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + (first ? -r[e] : r[e]) * s[e];
+  return pack8(x);
 }
 
 // The node blocks, prepared by all NW waves of the workgroup into LDS in operand
 // order (fragments as the wide kernel's ring holds them): wave and lane take
 // rows (k * NW + wave) * RPW + lane / LPR, 8 channels of each.  load() issues the
-// raw rows, before the lengths' and sets' dependent work; store() does the
-// rest.  One wave alone took 5 us for 32 rows.
+// raw rows, before the lengths' and sets' dependent work, load_tables() the
+// rotation tables' rows; store() does the rest.  One wave alone took 5 us for 32 rows.
 template <int D, int NW, int NT>
 struct TreeTail {
   static constexpr int KF = D / 16, BV = D / 8 * 64;  // fragments of K, uint4 per block
   static constexpr int LPR = D / 8, RPW = 64 / LPR, N = (32 * NT + NW * RPW - 1) / (NW * RPW);
-  uint4 k[N], v[N];
+  uint4 k[N], v[N], cw[N], sw[N], w;
 
   static __device__ __forceinline__ int row(int i) {
     return (i * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW + (threadIdx.x & 63) / LPR;
@@ -271,20 +328,21 @@ struct TreeTail {
       v[i] = ld16(x + (size_t)p.nkv * D);
     }
   }
-  // s_bad: 32 words per block.  pos, nodes: as the kernels hold them.  The
-  // workgroup has to meet before it reads.
-  __device__ __forceinline__ void store(const TreeAttnParams &p, uint4 *tail, int *s_bad, int cell, bool keep, int ntb,
-                                        int pos, uint64_t nodes) {
-    const int lane = threadIdx.x & 63, sub = lane % LPR, ch = sub * 8, T = p.t_rows;
-    const uint4 w = ld16(p.k_norm_w + ch);
-    uint4 cw[N], sw[N];
+  __device__ __forceinline__ void load_tables(const TreeAttnParams &p, int ntb, int pos) {
+    const int ch = threadIdx.x % LPR * 8;
+    w = ld16(p.k_norm_w + ch);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i * NW * RPW >= 32 * ntb) break;
-      const size_t at = (size_t)__shfl(pos, min(row(i), T - 1), 64) * D + ch;
+      const size_t at = (size_t)__shfl(pos, min(row(i), p.t_rows - 1), 64) * D + ch;
       cw[i] = ld16(p.cos_tab + at);
       sw[i] = ld16(p.sin_tab + at);
     }
+  }
+  // s_bad: 32 words per block.  The workgroup has to meet before it reads.
+  __device__ __forceinline__ void store(const TreeAttnParams &p, uint4 *tail, int *s_bad, int cell, bool keep, int ntb,
+                                        uint64_t nodes) {
+    const int lane = threadIdx.x & 63, sub = lane % LPR, ch = sub * 8, T = p.t_rows;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (i * NW * RPW >= 32 * ntb) break;
@@ -319,28 +377,27 @@ struct TreeTail {
 __device__ __forceinline__ uint16_t *tree_out(const TreeAttnParams &p, int m, int k) {
   return p.ofrag ? p.out + frag_off(m, k, p.ofrag) : p.out + (size_t)m * p.nq * p.head_dim + k;
 }
-// Four channels of query row r of a kv head: o / l, zeros where the row holds no
+// Four channels of node t's query head hq: o / l, zeros where the row holds no
 // node.
-__device__ __forceinline__ void tree_store(const TreeAttnParams &p, int b, int kvh, int r, int ch, const f32x4_t &o,
-                                           float inv, bool node) {
-  const int G = p.nq / p.nkv;
+__device__ __forceinline__ void tree_store(const TreeAttnParams &p, int b, int t, int hq, int ch, const f32x4_t &o, float inv,
+                                           bool node) {
   uint2 v = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
   if (!node) v = make_uint2(0u, 0u);
-  *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + r / G, (kvh * G + r % G) * p.head_dim + ch)) = v;
+  *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + t, hq * p.head_dim + ch)) = v;
 }
-// The partial of (cell, row group, split): acc [RG][D], m [RG], l [RG], with m =
-// -inf and l = 0 where a row saw nothing or holds no node.
+// The partial of a unit's row group: acc [RG][D], m [RG], l [RG], with m = -inf
+// and l = 0 where a row saw nothing or holds no node.
 template <int D>
-__device__ __forceinline__ float *tree_part(const TreeAttnParams &p, int cell, int g, int c) {
-  return p.partial + (((size_t)cell * p.groups + g) * p.splits + c) * ((size_t)p.group_rows * (D + 2));
+__device__ __forceinline__ float *tree_part(const TreeAttnParams &p, int unit, int g) {
+  return p.partial + ((size_t)unit * p.groups + g) * ((size_t)p.group_rows * (D + 2));
 }
 
 // The rows r0 .. r0 + rows - 1 of a sequence whose length is out of range.
 __device__ __forceinline__ void tree_nan_rows(const TreeAttnParams &p, int b, int kvh, int r0, int rows) {
-  const int D = p.head_dim, G = p.nq / p.nkv;
+  const int D = p.head_dim, G = p.by_g.d;
   for (int i = threadIdx.x; i < rows * (D / 4); i += blockDim.x) {
-    const int r = r0 + i / (D / 4), k4 = i % (D / 4) * 4;
-    *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + r / G, (kvh * G + r % G) * D + k4)) =
+    const int r = r0 + i / (D / 4), k4 = i % (D / 4) * 4, t = div_by(p.by_g, r);
+    *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + t, (kvh * G + r - t * G) * D + k4)) =
         make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
   }
 }
@@ -358,8 +415,8 @@ template <int D, int MT, int NT>
 struct NarrowLds {
   static constexpr int tail = 0;                            // node blocks in operand order
   static constexpr int bad = tail + NT * (D / 8) * 64 * 16;  // node rows with a value that is not finite
-  static constexpr int acc = bad + kTreeMaxT * 4;        // waves' sums of an M tile [kTW][D / 16][64] f32x4
-  static constexpr int m = acc + kTW * (D / 16) * 64 * 16;  // wave row maxima [MT][kTW][16]
+  static constexpr int acc = bad + kTreeMaxT * 4;        // waves' sums [MT][kTW][D / 16][64] f32x4
+  static constexpr int m = acc + MT * kTW * (D / 16) * 64 * 16;  // wave row maxima [MT][kTW][16]
   static constexpr int l = m + MT * kTW * 16 * 4;        // wave row sums
   static constexpr int q = l + MT * kTW * 16 * 4;        // query operands [MT][D / 32][64] (MT > 1)
   static constexpr int bytes = q + (MT > 1 ? MT * (D / 32) * 1024 : 0);
@@ -378,8 +435,11 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   const int col = lane & 15, grp = lane >> 4;
 
   const TreeUnit u_ = tree_unit(p);
-  const int c = u_.c, cell = u_.cell, g = u_.g, kvh = u_.kvh, b = u_.b;
-  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv;
+  const TreeDeal deal = tree_deal<false>(p, u_.w);
+  if (deal.n == 0) return;
+  const int kvh = u_.kvh, g = u_.g, b = deal.b, L = deal.L, n_active = deal.n, c = u_.w - deal.first;
+  const int cell = b * p.nkv + kvh;
+  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d;
   const int r0 = g * RG, rows = min(RG, T * G - r0);
   const int width = (nq + 2 * nkv) * D;
   const uint16_t *qkv = p.qkv + (size_t)b * T * width;
@@ -391,22 +451,20 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   const int mine = MT == 1 ? 0 : min(wave, MT - 1);
   int rt[MT];  // the lane's query rows' nodes
 #pragma unroll
-  for (int u = 0; u < MT; ++u) rt[u] = (r0 + min(u * 16 + col, rows - 1)) / G;
-  const int qr = r0 + min(mine * 16 + col, rows - 1), qt = qr / G;
+  for (int u = 0; u < MT; ++u) rt[u] = div_by(p.by_g, r0 + min(u * 16 + col, rows - 1));
+  const int qr = r0 + min(mine * 16 + col, rows - 1), qt = div_by(p.by_g, qr);
   {
     const uint16_t *q = qkv + (size_t)qt * width + (size_t)(kvh * G + qr - qt * G) * D + 8 * grp;
 #pragma unroll
     for (int s = 0; s < DS; ++s) qf[s] = ld16(q + 32 * s);
   }
   const int up = lane < T ? p.parents[(size_t)b * T + lane] : -1;
-  const int L = p.lens[b];
-  if (L < 0 || L > p.cap - T) {
+  if (!tree_valid(p, L)) {
     if (c == 0) tree_nan_rows(p, b, kvh, r0, rows);
     return;
   }
-  const TreeRun run = tree_run(p, L, c);
-  if (run.n_active < 0) return;
-  const int nb = run.nb, n_active = run.n_active, j0 = run.j0, j1 = run.j1;
+  const TreeRun run = tree_run(p, L, c, n_active);
+  const int nb = run.nb, j0 = run.j0, j1 = run.j1;
 
   const size_t slab = (size_t)cell * p.cap * D;
   const uint16_t *kc = p.k_cache + slab, *vc = p.v_cache + slab;
@@ -433,23 +491,28 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   TreeTail<D, kTW, NT> nt;
   if (ntb > 0) nt.load(p, qkv, kvh, ntb);
   Frag f0, f1;
-  if (j0 + wave < jc) load_block(j0 + wave, f0);
 
   const uint64_t anc = tree_ancestors(up, T, lane);
   const int depth = (int)__popcll(anc) - 1;  // -1: no node (its rows are prepared at L and dropped)
   const int pos = depth > 0 ? L + depth : L;
   const uint64_t nodes = __ballot(anc != 0);
   uint64_t sees[MT];
-#pragma unroll
-  for (int u = 0; u < MT; ++u) sees[u] = shfl64(anc, rt[u]);
+  // The tables of the rows' positions, then the first block: what follows works
+  // while the block is on its way.
+  Head<D> qw, cw, sw;
   {
     const size_t at = (size_t)__shfl(pos, qt, 64) * D + 8 * grp;
-    Head<D> qw, cw, sw;
     qw.load(p.q_norm_w + 8 * grp);
     cw.load(p.cos_tab + at);
     sw.load(p.sin_tab + at);
-    head_rows<D>(qf, qw, cw, sw, p.eps);
   }
+  if (ntb > 0) nt.load_tables(p, ntb, pos);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  if (j0 + wave < jc) load_block(j0 + wave, f0);
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+#pragma unroll
+  for (int u = 0; u < MT; ++u) sees[u] = shfl64(anc, rt[u]);
+  head_rows<D>(qf, qw, cw, sw, p.eps);
   if constexpr (MT > 1) {
     if (wave < MT) {
 #pragma unroll
@@ -458,7 +521,7 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   }
   uint64_t badset = 0;
   if (ntb > 0) {
-    nt.store(p, tail, s_bad, cell, g == 0, ntb, pos, nodes);
+    nt.store(p, tail, s_bad, cell, g == 0, ntb, nodes);
     lds_barrier();
     badset = __ballot(lane < 32 * ntb && s_bad[lane]);
   } else if (MT > 1) {
@@ -544,7 +607,10 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
       for (int e = 0; e < 8; ++e)
         pj[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(e < 4 ? sa[u][e] : sb[u][e - 4], scale, -mc));
       l_run[u] += ((pj[0] + pj[1]) + (pj[2] + pj[3])) + ((pj[4] + pj[5]) + (pj[6] + pj[7]));
-      const uint4 pf = pack8(pj);
+      uint4 pf, pl;
+      split8(pj, pf, pl);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[u][dt] = mfma16x16x32(f.vf[dt], pl, acc[u][dt]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[u][dt] = mfma16x16x32(f.vf[dt], pf, acc[u][dt]);
       if constexpr (NODES) {
@@ -572,14 +638,13 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
       s_m[(u * kTW + wave) * 16 + col] = m_run[u];
       s_l[(u * kTW + wave) * 16 + col] = lw;
     }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) s_acc[((u * kTW + wave) * DT + dt) * 64 + lane] = acc[u][dt];
   }
-  float *part = n_active > 1 ? tree_part<D>(p, cell, g, c) : nullptr;
+  lds_barrier();
+  float *part = n_active > 1 ? tree_part<D>(p, u_.unit, g) : nullptr;
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
-    if (u > 0) lds_barrier();  // the previous tile's sums are consumed
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[u][dt];
-    lds_barrier();
     float M = NEG_INF;
 #pragma unroll
     for (int w = 0; w < kTW; ++w) M = fmaxf(M, s_m[(u * kTW + w) * 16 + col]);
@@ -596,12 +661,12 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
 #pragma unroll
     for (int i = 0; i < DTW; ++i) {
       const int dt = wave + kTW * i, ch = dt * 16 + grp * 4;
-      f32x4_t o = s_acc[dt * 64 + lane] * sc[0];
+      f32x4_t o = s_acc[((u * kTW) * DT + dt) * 64 + lane] * sc[0];
 #pragma unroll
-      for (int w = 1; w < kTW; ++w) o += s_acc[(w * DT + dt) * 64 + lane] * sc[w];
+      for (int w = 1; w < kTW; ++w) o += s_acc[((u * kTW + w) * DT + dt) * 64 + lane] * sc[w];
       if (r >= rows) continue;
       if (n_active == 1)
-        tree_store(p, b, kvh, r0 + r, ch, o, inv, node);
+        tree_store(p, b, rt[u], kvh * G + r0 + r - rt[u] * G, ch, o, inv, node);
       else
         *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + ch) = o;
     }
@@ -653,30 +718,32 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   const int col = lane & 15, grp = lane >> 4;
 
   const TreeUnit u_ = tree_unit(p);
-  const int c = u_.c, cell = u_.cell, g = u_.g, kvh = u_.kvh, b = u_.b;
-  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv;
+  const TreeDeal deal = tree_deal<false>(p, u_.w);
+  if (deal.n == 0) return;
+  const int kvh = u_.kvh, g = u_.g, b = deal.b, L = deal.L, n_active = deal.n, c = u_.w - deal.first;
+  const int cell = b * p.nkv + kvh;
+  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d;
   const int R = T * G, r0 = g * RG;
   const int rows = min(RG, R - r0);
   const int width = (nq + 2 * nkv) * D;
   const uint16_t *qkv = p.qkv + (size_t)b * T * width;
   uint4 qf[MT][DS];
-  int row[MT];
+  int row[MT], rt[MT];
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
     row[u] = r0 + min((wave * MT + u) * 16 + col, rows - 1);
-    const uint16_t *q = qkv + (size_t)(row[u] / G) * width + (size_t)(kvh * G + row[u] % G) * D + 8 * grp;
+    rt[u] = div_by(p.by_g, row[u]);
+    const uint16_t *q = qkv + (size_t)rt[u] * width + (size_t)(kvh * G + row[u] - rt[u] * G) * D + 8 * grp;
 #pragma unroll
     for (int s = 0; s < DS; ++s) qf[u][s] = ld16(q + 32 * s);
   }
   const int up = lane < T ? p.parents[(size_t)b * T + lane] : -1;
-  const int L = p.lens[b];
-  if (L < 0 || L > p.cap - T) {
+  if (!tree_valid(p, L)) {
     if (c == 0) tree_nan_rows(p, b, kvh, r0, rows);
     return;
   }
-  const TreeRun run = tree_run(p, L, c);
-  if (run.n_active < 0) return;
-  const int nb = run.nb, n_active = run.n_active, j0 = run.j0, n = run.j1 - run.j0;
+  const TreeRun run = tree_run(p, L, c, n_active);
+  const int nb = run.nb, j0 = run.j0, n = run.j1 - run.j0;
   const int nd = max(0, min(run.j1, nb) - j0);  // of the n blocks, those from the cache
 
   // Block jj of this run into its ring slot: this wave gathers fragments wave,
@@ -714,8 +781,8 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   uint64_t sees[MT];
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
-    sees[u] = shfl64(anc, row[u] / G);
-    const size_t at = (size_t)__shfl(pos, row[u] / G, 64) * D + 8 * grp;
+    sees[u] = shfl64(anc, rt[u]);
+    const size_t at = (size_t)__shfl(pos, rt[u], 64) * D + 8 * grp;
     Head<D> qw, cw, sw;
     qw.load(p.q_norm_w + 8 * grp);
     cw.load(p.cos_tab + at);
@@ -727,7 +794,8 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   // ---- the node blocks.
   uint64_t badset = 0;
   if (ntb > 0) {
-    nt.store(p, tail, s_bad, cell, g == 0, ntb, pos, nodes);
+    nt.load_tables(p, ntb, pos);
+    nt.store(p, tail, s_bad, cell, g == 0, ntb, nodes);
     lds_barrier();
     badset = __ballot(lane < 32 * ntb && s_bad[lane]);
   }
@@ -814,7 +882,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
     const uint4 *B = src(jj);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) vf[dt] = B[(KF + dt) * 64];
-    uint4 pf[MT];
+    uint4 pf[MT], pl[MT];
     float pj[MT][8], mc[MT], psum[MT];
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
@@ -842,7 +910,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
       l_run[u] += psum[u];
-      pf[u] = pack8(pj[u]);
+      split8(pj[u], pf[u], pl[u]);
     }
     if constexpr (!LAST) {
       await(min(jj + 2, n - 1), jj + RING - 1);
@@ -863,6 +931,10 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
       }
     }
     if constexpr (!LAST) read_k(min(jj + 2, n - 1));
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int u = 0; u < MT; ++u) acc[u][dt] = mfma16x16x32(vf[dt], pl[u], acc[u][dt]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -890,18 +962,18 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   block(jj, s0, s1, Int<1>{});
 
   // ---- output or partial.
-  float *part = n_active > 1 ? tree_part<D>(p, cell, g, c) : nullptr;
+  float *part = n_active > 1 ? tree_part<D>(p, u_.unit, g) : nullptr;
 #pragma unroll
   for (int u = 0; u < MT; ++u) {
     const int r = (wave * MT + u) * 16 + col;
-    const bool node = (nodes >> (row[u] / G)) & 1;
+    const bool node = (nodes >> rt[u]) & 1;
     float l = l_run[u] + shfl_xor(l_run[u], 16);
     l += shfl_xor(l, 32);
     if (r >= rows) continue;
     if (n_active == 1) {
       const float inv = 1.f / l;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) tree_store(p, b, kvh, row[u], dt * 16 + grp * 4, acc[u][dt], inv, node);
+      for (int dt = 0; dt < DT; ++dt) tree_store(p, b, rt[u], kvh * G + row[u] - rt[u] * G, dt * 16 + grp * 4, acc[u][dt], inv, node);
     } else {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + dt * 16 + grp * 4) = acc[u][dt];
@@ -918,17 +990,17 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
 template <int D>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p) {
   constexpr int TR = D / 4;
-  const int R = p.t_rows * (p.nq / p.nkv), RG = p.group_rows;
-  const int per = (R + 256 / TR - 1) / (256 / TR);  // workgroups per cell
-  const int cell = blockIdx.x / per, kvh = cell % p.nkv, b = cell / p.nkv;
+  const int G = p.by_g.d, R = p.t_rows * G, RG = p.group_rows;
+  const int per = (R + 256 / TR - 1) / (256 / TR);  // workgroups per (sequence, kv head)
+  const int cell = blockIdx.x / per, b = div_by(p.by_nkv, cell), kvh = cell - b * p.nkv;
   const int r = (blockIdx.x - cell * per) * (256 / TR) + threadIdx.x / TR;
-  const int L = p.lens[b];
-  if (L < 0 || L > p.cap - p.t_rows || r >= R) return;
-  const int n = tree_active(p.splits, p.min_blocks, (L + 31) >> 5, (p.t_rows + 31) >> 5);
-  if (n == 1) return;  // written by the one workgroup
+  const TreeDeal deal = tree_deal<true>(p, b);
+  const int n = deal.n;
+  // one split: written by its workgroup, as the rows of a length out of range
+  if (n == 1 || !tree_valid(p, deal.L) || r >= R) return;
   const int g = r / RG, rg = r - g * RG, ch = (int)(threadIdx.x % TR) * 4;
-  const float *part = tree_part<D>(p, cell, g, 0);
-  const size_t stride = (size_t)RG * (D + 2);
+  const float *part = tree_part<D>(p, deal.first * p.nkv + kvh, g);
+  const size_t stride = (size_t)p.nkv * p.groups * RG * (D + 2);  // to the next workgroup's
   const float scale = p.scale_log2;
   float M = -__builtin_huge_valf(), l = 0.f;
   f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -957,7 +1029,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p)
     }
     M = Mn;
   }
-  tree_store(p, b, kvh, r, ch, o, 1.f / l, l != 0.f);  // (a node's sum is not 0)
+  const int t = div_by(p.by_g, r);
+  tree_store(p, b, t, kvh * G + r - t * G, ch, o, 1.f / l, l != 0.f);  // (a node's sum is not 0)
 }
 
 template <int D>
@@ -992,20 +1065,39 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 
 }  // namespace
 
-// The row group (16 or 32: the narrow kernel; 128 or 256: the wide one) and
-// the splits.
+// The row group and the splits.
+//
+// The narrow kernel reads the cache once per row group, from an L2 that its
+// groups share; the wide one once per 128 or 256 rows, but it waits at a barrier
+// per block.  The narrow one is ahead until its reads come to about 200 MB.
+// MI355X, us, 32 query heads on 8, narrow / wide: 64 nodes on 4100 slots (134 MB)
+// 25 / 32, 32 nodes on 2000 slots (33 MB) 16 / 21; 2 x 32 nodes on 8000 slots
+// (262 MB) 41 / 34, 64 nodes on 30000 (980 MB) 118 / 60.
+//
+// 16 rows per workgroup give more workgroups, 32 fewer reads: 16 while that
+// leaves fewer than 128 (16 nodes on 640 slots 11.4 / 12.5, on 4100 15.9 / 17.2;
+// 8 x 8 nodes on up to 1600 slots 19.2 / 17.3, 16 x 8 nodes on 3000 58 / 45).
+//
+// One workgroup per CU, none of fewer than four blocks of a full cache: more
+// splits read no faster and merge more (16 nodes on 4100 slots, 4 / 8 / 16 / 32
+// splits: 20 / 16 / 19 / 28).
 void tree_attn_plan(TreeAttnParams *p, int splits) {
-  const int rows = p->t_rows * (p->nq / p->nkv);
+  const int rows = p->t_rows * (p->nq / p->nkv), tiles = (rows + 15) / 16;
   const int64_t cells = (int64_t)p->batch * p->nkv;
   const int blocks = p->cap / 32;
-  p->group_rows = rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 ? 128 : 256;
+  const int64_t cache = cells * p->cap * p->head_dim * 4;  // bytes of both caches
+  if (rows > 64 && cache * ((rows + 31) / 32) > 200000000)
+    p->group_rows = rows <= 128 ? 128 : 256;
+  else
+    p->group_rows = rows <= 16 || cells * tiles < 128 ? 16 : 32;
   p->min_blocks = 4;
   p->groups = (rows + p->group_rows - 1) / p->group_rows;
-  if (splits == 0) {
-    const int64_t fill = p->group_rows == 16 || p->group_rows == 128 ? 512 : 256;  // workgroups the CUs hold at once
-    splits = (int)std::max<int64_t>(1, std::min<int64_t>(fill / (cells * p->groups), blocks / p->min_blocks));
-  }
+  if (splits == 0)
+    splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / (cells * p->groups), blocks / p->min_blocks));
   p->splits = std::min(splits, 256);
+  p->by_groups = fast_div(p->groups);
+  p->by_nkv = fast_div(p->nkv);
+  p->by_g = fast_div(p->nq / p->nkv);
 }
 
 hipError_t launch_tree_attn(const TreeAttnParams &p, hipStream_t s) {

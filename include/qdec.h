@@ -496,12 +496,12 @@ int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
 
 /* For every sequence b and node t (see above), from the raw projection row
  * qkv[b*t_rows + t]:
- *   q, k = per-head RMSNorm and RoPE at position lens[b] + depth(t), with the
- *          arithmetic and rounding points of qdec_attn;
+ *   q, k = per-head RMSNorm and RoPE at position lens[b] + depth(t), in fp32,
+ *          rounded to bf16 once (qdec_attn rounds where the reference does,
+ *          five times, so its keys differ by such roundings);
  *   out  = softmax(q . K^T / sqrt(D)) . V over cache slots 0 .. lens[b] - 1,
  *          node t's ancestors and node t itself: fp32 scores, statistics and
- *          accumulation, probabilities rounded to bf16 before the P.V product
- *          (the operand type of the matrix instruction), one rounding to bf16;
+ *          accumulation, probabilities in two bf16 parts, one rounding to bf16;
  *   k and the raw v go to k_nodes / v_nodes ([batch][nkv][t_rows][head_dim]).
  * The cache is only read: qdec_tree_commit appends what was accepted.  What a
  * row does not see (other branches, slots from lens[b] on) does not reach it,

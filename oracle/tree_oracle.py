@@ -74,21 +74,20 @@ def bf(x):
 
 
 def head_norm_rope(x, w, cos, sin, eps):
-    """Per-head RMSNorm and RoPE of ``[..., D]`` rows with the rounding points
-    of the decode attention: bf16 after the normalisation, the gain, each
-    product of the rotation and their sum."""
+    """Per-head RMSNorm and RoPE of ``[..., D]`` rows, unrounded."""
     D = x.shape[-1]
-    y = bf(w * bf(x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)))
+    y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w
     rot = torch.cat((-y[..., D // 2:], y[..., :D // 2]), -1)
-    return bf(bf(y * cos) + bf(rot * sin))
+    return y * cos + rot * sin
 
 
 def attention(qkv, parents, L, k_cache, v_cache, q_norm, k_norm, cos, sin, nq, nkv, eps):
     """One sequence.  ``qkv`` [T, (nq + 2 nkv) D], ``k_cache`` / ``v_cache``
-    [nkv, slots, D] (at least L slots), float64 throughout.  Returns ``out``
-    [T, nq, D], ``mag`` (the same sum over absolute values, the scale of its
-    rounding errors), and the nodes' keys and values [nkv, T, D] (NaN in rows
-    that hold no node)."""
+    [nkv, slots, D] (at least L slots), float64 throughout but for the queries
+    and node keys, which are rounded to bf16 once.  Returns ``out`` [T, nq, D],
+    ``mag`` (the same sum over absolute values, the scale of its rounding
+    errors), and the nodes' keys and values [nkv, T, D] (NaN in rows that hold
+    no node)."""
     T, D = len(parents), cos.shape[-1]
     up = ancestors(parents)
     x = qkv.double().view(T, nq + 2 * nkv, D)
@@ -103,8 +102,8 @@ def attention(qkv, parents, L, k_cache, v_cache, q_norm, k_norm, cos, sin, nq, n
             continue
         pos = L + len(up[t]) - 1
         c, s = cos[pos].double(), sin[pos].double()
-        q[t] = head_norm_rope(x[t, :nq], q_norm.double(), c, s, eps)
-        kn[:, t] = head_norm_rope(x[t, nq:nq + nkv], k_norm.double(), c, s, eps)
+        q[t] = bf(head_norm_rope(x[t, :nq], q_norm.double(), c, s, eps))
+        kn[:, t] = bf(head_norm_rope(x[t, nq:nq + nkv], k_norm.double(), c, s, eps))
         vn[:, t] = x[t, nq + nkv:]
     kc, vc = k_cache[:, :L].double(), v_cache[:, :L].double()
     for t in q:

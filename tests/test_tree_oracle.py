@@ -96,8 +96,8 @@ def test_attention_of_a_chain_is_causal_attention():
     cos, sin = torch.cat((ang.cos(),) * 2, 1), torch.cat((ang.sin(),) * 2, 1)
     out, mag, kn, vn = tree_oracle.attention(qkv, [-1, 0, 1, 2, 3], L, kc, vc, one, one, cos, sin, nq, nkv, 1e-6)
     x = qkv.view(T, nq + 2 * nkv, D)
-    q = torch.stack([tree_oracle.head_norm_rope(x[t, :nq], one.double(), cos[L + t].double(), sin[L + t].double(), 1e-6)
-                     for t in range(T)], 1)
+    q = torch.stack([tree_oracle.bf(tree_oracle.head_norm_rope(x[t, :nq], one.double(), cos[L + t].double(),
+                                                               sin[L + t].double(), 1e-6)) for t in range(T)], 1)
     keys, vals = torch.cat((kc, kn), 1).repeat_interleave(2, 0), torch.cat((vc, vn), 1).repeat_interleave(2, 0)
     s = q @ keys.transpose(1, 2).contiguous() / D ** 0.5
     s = s.masked_fill(torch.arange(L + T)[None] > L + torch.arange(T)[:, None], -torch.inf)
