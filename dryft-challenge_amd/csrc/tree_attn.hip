@@ -18,9 +18,14 @@
 //     rounds.  A set that does not reach the root is no node's.  The depth is
 //     the size of the set less one.
 //   * Per block S^T = K . Q^T (v_mfma_f32_16x16x32_bf16), online softmax in
-//     base 2 on fp32 scores, O^T += V^T . P^T with P in two bf16 parts.  What is
-//     rounded to bf16, because a matrix instruction or a buffer takes it, is
-//     rounded once: queries, node keys, the parts of P, the output.
+//     base 2 on fp32 scores, O^T += V^T . P^T.  The matrix instructions take
+//     bf16: P goes in as two parts whose sum has 16 bits of it, and so do the
+//     narrow kernel's queries (the wide one's, which is bound by its
+//     arithmetic, are rounded once).  Each of these roundings would otherwise
+//     add as much error to the result as its own rounding to bf16 (relative
+//     to 64 bits 0.0040 with q, k as qdec_attn rounds them and P rounded, 0.0024
+//     with P in two parts, 0.0017 with both: the output's rounding alone).
+//     Node keys are rounded once, to what k_nodes holds.
 //   * A lane's query rows are prepared in registers, in the place where the
 //     MFMA's B operand wants them: lane (c, g) holds channels 32s + 8g .. +8 of
 //     row c for every k step s, so the rotation's partner channel is the
@@ -60,11 +65,21 @@ struct Head {
   }
 };
 
-// Head RMSNorm (gain w) and RoPE (cos c, sin n) of such a row, in fp32; one
-// rounding to bf16, the operand type, at the end.
-template <int D>
-__device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], const Head<D> &w, const Head<D> &cw, const Head<D> &sw,
-                                          float eps) {
+// Eight numbers as two bf16 vectors whose sum has 16 bits of them.
+__device__ __forceinline__ void split8(const float (&p)[8], uint4 &hi, uint4 &lo) {
+  hi = pack8(p);
+  float h[8], d[8];
+  unpack8(hi, h);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) d[e] = p[e] - h[e];
+  lo = pack8(d);
+}
+
+// Head RMSNorm (gain w) and RoPE (cos c, sin n) of such a row, in fp32; rounded
+// to bf16, the operand type, at the end, lo taking what f leaves (LO).
+template <int D, bool LO>
+__device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], uint4 (&lo)[D / 32], const Head<D> &w, const Head<D> &cw,
+                                          const Head<D> &sw, float eps) {
   constexpr int DS = D / 32;
   float ss = 0.f;
 #pragma unroll
@@ -79,40 +94,34 @@ __device__ __forceinline__ void head_rows(uint4 (&f)[D / 32], const Head<D> &w, 
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(ss), __float_as_uint(ss), false, false);
   ss = __uint_as_float(b[0]) + __uint_as_float(b[1]);
   const float rstd = 1.0f / sqrtf(ss / (float)D + eps);
+  auto put = [&](int s, const float (&o)[8]) {
+    if constexpr (LO)
+      split8(o, f[s], lo[s]);
+    else
+      f[s] = pack8(o);
+  };
 #pragma unroll
   for (int s = 0; s < DS / 2; ++s) {
-    float lo[8], hi[8], g[8], c[8], n[8], o[8];
-    unpack8(f[s], lo);
+    float x[8], y[8], g[8], c[8], n[8], o[8];
+    unpack8(f[s], x);
     unpack8(w.v[s], g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) lo[e] *= rstd * g[e];
-    unpack8(f[s + DS / 2], hi);
+    for (int e = 0; e < 8; ++e) x[e] *= rstd * g[e];
+    unpack8(f[s + DS / 2], y);
     unpack8(w.v[s + DS / 2], g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) hi[e] *= rstd * g[e];
+    for (int e = 0; e < 8; ++e) y[e] *= rstd * g[e];
     unpack8(cw.v[s], c);
     unpack8(sw.v[s], n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = lo[e] * c[e] - hi[e] * n[e];
-    f[s] = pack8(o);
+    for (int e = 0; e < 8; ++e) o[e] = x[e] * c[e] - y[e] * n[e];
+    put(s, o);
     unpack8(cw.v[s + DS / 2], c);
     unpack8(sw.v[s + DS / 2], n);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = hi[e] * c[e] + lo[e] * n[e];
-    f[s + DS / 2] = pack8(o);
+    for (int e = 0; e < 8; ++e) o[e] = y[e] * c[e] + x[e] * n[e];
+    put(s + DS / 2, o);
   }
-}
-
-// Eight probabilities as two bf16 operands whose sum has 16 bits of them: with
-// one operand their rounding is, beside the output's own, the largest error of
-// the result (1.7 times the output's rounding alone; 1.4 with two).
-__device__ __forceinline__ void split8(const float (&p)[8], uint4 &hi, uint4 &lo) {
-  hi = pack8(p);
-  float h[8], d[8];
-  unpack8(hi, h);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) d[e] = p[e] - h[e];
-  lo = pack8(d);
 }
 
 __device__ __forceinline__ bool finite8(const uint4 &v) {
@@ -418,8 +427,8 @@ struct NarrowLds {
   static constexpr int acc = bad + kTreeMaxT * 4;        // waves' sums [MT][kTW][D / 16][64] f32x4
   static constexpr int m = acc + MT * kTW * (D / 16) * 64 * 16;  // wave row maxima [MT][kTW][16]
   static constexpr int l = m + MT * kTW * 16 * 4;        // wave row sums
-  static constexpr int q = l + MT * kTW * 16 * 4;        // query operands [MT][D / 32][64] (MT > 1)
-  static constexpr int bytes = q + (MT > 1 ? MT * (D / 32) * 1024 : 0);
+  static constexpr int q = l + MT * kTW * 16 * 4;        // query operands [MT][2][D / 32][64] (MT > 1)
+  static constexpr int bytes = q + (MT > 1 ? MT * (D / 32) * 2048 : 0);
 };
 
 template <int D, int MT, int NT>
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   // What does not depend on the length is loaded first: the tile of query rows
   // that this wave prepares.
   uint4 *s_q = reinterpret_cast<uint4 *>(smem + LY::q);
-  uint4 qf[DS];
+  uint4 qf[DS], ql[DS];  // the queries in two parts
   const int mine = MT == 1 ? 0 : min(wave, MT - 1);
   int rt[MT];  // the lane's query rows' nodes
 #pragma unroll
@@ -512,11 +521,14 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
 #pragma unroll
   for (int u = 0; u < MT; ++u) sees[u] = shfl64(anc, rt[u]);
-  head_rows<D>(qf, qw, cw, sw, p.eps);
+  head_rows<D, true>(qf, ql, qw, cw, sw, p.eps);
   if constexpr (MT > 1) {
     if (wave < MT) {
 #pragma unroll
-      for (int s = 0; s < DS; ++s) s_q[(wave * DS + s) * 64 + lane] = qf[s];
+      for (int s = 0; s < DS; ++s) {
+        s_q[(2 * wave * DS + s) * 64 + lane] = qf[s];
+        s_q[((2 * wave + 1) * DS + s) * 64 + lane] = ql[s];
+      }
     }
   }
   uint64_t badset = 0;
@@ -572,7 +584,10 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
       sa[u] = sb[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < DS; ++s) {
-        const uint4 q = MT > 1 ? s_q[(u * DS + s) * 64 + lane] : qf[s];
+        const uint4 q = MT > 1 ? s_q[(2 * u * DS + s) * 64 + lane] : qf[s];
+        const uint4 r = MT > 1 ? s_q[((2 * u + 1) * DS + s) * 64 + lane] : ql[s];
+        sa[u] = mfma16x16x32(f.ka[s], r, sa[u]);
+        sb[u] = mfma16x16x32(f.kb[s], r, sb[u]);
         sa[u] = mfma16x16x32(f.ka[s], q, sa[u]);
         sb[u] = mfma16x16x32(f.kb[s], q, sb[u]);
       }
@@ -787,7 +802,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
     qw.load(p.q_norm_w + 8 * grp);
     cw.load(p.cos_tab + at);
     sw.load(p.sin_tab + at);
-    head_rows<D>(qf[u], qw, cw, sw, p.eps);
+    head_rows<D, false>(qf[u], qf[u], qw, cw, sw, p.eps);
     __atomic_signal_fence(__ATOMIC_SEQ_CST);  // one tile's tables at a time (registers)
   }
 
