@@ -17,20 +17,28 @@ __device__ __forceinline__ int64_t lane_i64(int64_t v, int l) {
 
 // One workgroup per sequence.
 //   1. The history is scanned from its end in windows of kDraftU * 1024
-//      positions.  Position e ends an earlier occurrence of the pattern of n
-//      tokens when hist[e - i] = hist[L - i], i < n; ballots and a prefix over
-//      the waves append the hits of each pattern to its list in order, most
-//      recent first, until both lists are full.
+//      positions, the next window's loads in flight while one is searched in
+//      LDS.  Position e ends an earlier occurrence of the pattern of n tokens
+//      when hist[e - i] = hist[L - i], i < n.  A wave's hits are a ballot; one
+//      wave per pattern then appends them to its list in order, most recent
+//      first, while the others store the next window.  Both lists full ends
+//      the scan.
 //   2. The candidates' tokens go to LDS.
 //   3. The first wave builds the tree with one lane per node: a token's child
 //      is found by one ballot.
+// What bounds it: a history of 20K tokens is 160 KB through one CU.
 constexpr int kDraftThreads = 1024;
-constexpr int kDraftU = 4;
+constexpr int kDraftU = 8;
+constexpr int kDraftWindow = kDraftU * kDraftThreads;
+constexpr int kDraftGram = 64;  // tokens of a pattern, at most
 __global__ void __launch_bounds__(kDraftThreads) tree_draft_kernel(const qdec_tree_draft_args p) {
-  constexpr int NW = kDraftThreads / 64;
+  constexpr int NW = kDraftThreads / 64, WORDS = kDraftU * NW;
+  static_assert(WORDS == 128 && 2 * kTreeMaxMatches * (kTreeMaxT - 1) <= kDraftWindow, "two words per lane; the drafts fit");
+  __shared__ int64_t s_tok[kDraftWindow + kDraftGram];  // the window, newest first; then the drafts
+  __shared__ int64_t s_pat[kDraftGram];                 // the last tokens, newest first
+  __shared__ uint64_t s_hit[2][WORDS];
   __shared__ int s_end[2][kTreeMaxMatches];
-  __shared__ int s_cnt[2][kDraftU][NW];
-  __shared__ int64_t s_tok[2 * kTreeMaxMatches * (kTreeMaxT - 1)];
+  __shared__ int s_found[2];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int T = p.t_rows, K = p.depth, M = p.matches;
   const int64_t *h = p.hist + (size_t)b * p.cap;
@@ -38,59 +46,68 @@ __global__ void __launch_bounds__(kDraftThreads) tree_draft_kernel(const qdec_tr
   if (L < 0) L = 0;
   if (L >= p.cap) L = p.cap - 1;
   const int ngram[2] = {p.primary, p.backoff};
-  int found[2] = {0, 0};
-  const int64_t newest = h[L];
-  for (int top = T > 1 ? L - 1 : -1; top >= 0 && (found[0] < M || found[1] < M); top -= kDraftU * kDraftThreads) {
-    int64_t tok[kDraftU];
+  int64_t r[kDraftU], over = 0;
+  auto load = [&](int top) {
 #pragma unroll
     for (int u = 0; u < kDraftU; ++u) {
       const int e = top - u * kDraftThreads - tid;
-      tok[u] = e >= 0 ? h[e] : 0;
+      r[u] = e >= 0 ? h[e] : 0;
     }
-    uint64_t hit[2][kDraftU];
+    const int e = top - kDraftWindow - tid;
+    if (tid < kDraftGram) over = e >= 0 ? h[e] : 0;
+  };
+  if (tid < 2) s_found[tid] = 0;
+  if (tid < kDraftGram) s_pat[tid] = L >= tid ? h[L - tid] : 0;
+  if (T > 1) load(L - 1);
+  for (int top = T > 1 ? L - 1 : -1; top >= 0; top -= kDraftWindow) {
+#pragma unroll
+    for (int u = 0; u < kDraftU; ++u) s_tok[u * kDraftThreads + tid] = r[u];
+    if (tid < kDraftGram) s_tok[kDraftWindow + tid] = over;
+    __syncthreads();  // the window; the hits of the one before are listed
+    if (s_found[0] == M && s_found[1] == M) break;
+    if (top >= kDraftWindow) load(top - kDraftWindow);
+    const int64_t newest = s_pat[0];
 #pragma unroll
     for (int u = 0; u < kDraftU; ++u) {
-      const int e = top - u * kDraftThreads - tid;
-      const bool last = e >= 0 && tok[u] == newest;
+      const int q = u * kDraftThreads + tid, e = top - q;
+      const bool last = e >= 0 && s_tok[q] == newest;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         bool ok = last && e >= ngram[w] - 1;
-        for (int i = 1; i < ngram[w] && ok; ++i) ok = h[e - i] == h[L - i];
-        hit[w][u] = __ballot(ok);
-        if (lane == 0) s_cnt[w][u][wave] = __popcll(hit[w][u]);
+        for (int i = 1; i < ngram[w] && ok; ++i) ok = s_tok[q + i] == s_pat[i];
+        const uint64_t hit = __ballot(ok);
+        if (lane == 0) s_hit[w][u * NW + wave] = hit;
       }
     }
     __syncthreads();
+    if (wave < 2) {  // word k: window positions (k / NW) * 1024 + (k % NW) * 64 + bit
+      uint64_t bits[2] = {s_hit[wave][2 * lane], s_hit[wave][2 * lane + 1]};
+      const int count = __popcll(bits[0]) + __popcll(bits[1]), upto = wave_scan(count);
+      const int had = s_found[wave];
+      int at = had + upto - count;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-#pragma unroll
-      for (int u = 0; u < kDraftU; ++u) {
-        int before = found[w], total = 0;
-        for (int i = 0; i < NW; ++i) {
-          const int c = s_cnt[w][u][i];
-          if (i < wave) before += c;
-          total += c;
-        }
-        const int at = before + __popcll(hit[w][u] & ((1ull << lane) - 1));
-        if (((hit[w][u] >> lane) & 1) && at < M) s_end[w][at] = top - u * kDraftThreads - tid;
-        found[w] = min(found[w] + total, M);
+      for (int k = 0; k < 2; ++k) {
+        const int word = 2 * lane + k, q = word / NW * kDraftThreads + word % NW * 64;
+        for (; bits[k] && at < M; bits[k] &= bits[k] - 1) s_end[wave][at++] = top - q - __builtin_ctzll(bits[k]);
       }
+      if (lane == 63) s_found[wave] = min(M, had + upto);
     }
-    __syncthreads();
   }
-  const int total = found[0] + found[1];
+  __syncthreads();
+  const int found = s_found[0], total = found + s_found[1];
   for (int i = tid; i < total * K; i += kDraftThreads) {
     const int m = i / K, at = i - m * K;
-    const int e = m < found[0] ? s_end[0][m] : s_end[1][m - found[0]];
+    const int e = m < found ? s_end[0][m] : s_end[1][m - found];
     s_tok[i] = e + 1 + at <= L ? h[e + 1 + at] : 0;
   }
   __syncthreads();
   if (wave) return;
+  const int64_t newest = s_pat[0];
   int64_t id = newest;  // lane t: node t's token and parent
   int par = -1;
   int count = 1;
   for (int m = 0; m < total && count < T; ++m) {
-    const int e = m < found[0] ? s_end[0][m] : s_end[1][m - found[0]];
+    const int e = m < found ? s_end[0][m] : s_end[1][m - found];
     const int n = min(K, L - e);
     const int64_t mine = s_tok[m * K + min(lane, K - 1)];
     int cur = 0;
