@@ -25,6 +25,9 @@ Public surface (the reference's engine/engine.py:215-241, 1024-1063):
   per sequence, longest-prefix acceptance and rollback by length.  The
   kernels give every row the same arithmetic whatever the row count, so the
   emitted tokens are exactly those of the plain greedy path.
+* Optional tree speculation (``speculate="tree"``): several earlier
+  continuations merged into a tree of drafts and verified in one pass, the
+  accepted path's keys and values appended to the cache (``qdec.tree``).
 * The engine never falls back to another implementation: a missing or
   failing kernel library raises.
 """
@@ -42,6 +45,7 @@ if _HERE not in sys.path:
 from qdec import capi, selfcheck  # noqa: E402
 from qdec.checkpoint import load_config, load_tensors  # noqa: E402
 from qdec.runtime import DecodeState, DeviceModel, max_rows_per_seq  # noqa: E402
+from qdec.tree import TreeDecoder, tree_nodes  # noqa: E402
 
 # Decode steps queued ahead of the one being handed to the caller (as the
 # reference, engine/engine.py:66); one before the first token.
@@ -85,9 +89,11 @@ class _Shape:
         # shape must chunk alike to produce the same bits.
         self.spec_k = spec_k(batch, engine.model.cfg.group)
         slack = 2 * (self.spec_k + 1)
+        self.tree_t = tree_nodes(batch) if speculate == "tree" else 0
+        slack = max(slack, 2 * self.tree_t)  # a walk past the last token, and the next pass's nodes
         self.capacity = prompt_len + new_tokens + slack
-        max_t = (self.spec_k + 1) if (speculate and self.spec_k) else 16
-        self.state = DecodeState(engine.model, batch, self.capacity, max_t=max_t)
+        max_t = (self.spec_k + 1) if (speculate and speculate != "tree" and self.spec_k) else 16
+        self.state = DecodeState(engine.model, batch, self.capacity, max_t=max_t, tree_t=self.tree_t)
         self.graph = None
         self.spec_graph = None
         self.host = torch.empty((new_tokens, batch), dtype=torch.int64, pin_memory=True)
@@ -97,8 +103,9 @@ class _Shape:
 
 
 class Engine:
-    def __init__(self, model_path: str, speculate: bool = False, mega=None) -> None:
+    def __init__(self, model_path: str, speculate: "bool | str" = False, mega=None) -> None:
         """Load the checkpoint at ``model_path`` (HF layout, local files only).
+        ``speculate``: True drafts one chain per sequence, "tree" a tree.
         ``mega``: try one launch per layer for plain decode (None: MEGA_ENABLED)."""
         start = time.perf_counter()
         if not torch.cuda.is_available():
@@ -142,7 +149,7 @@ class Engine:
         # Known-answer checks of every kernel family on this device, with the
         # model's own weights and plans; raises on a mismatch (no fallback).
         selfcheck.run(DecodeState(self.model, 1, 64, max_t=1))
-        self.speculate = bool(speculate)
+        self.speculate = speculate if speculate == "tree" else bool(speculate)
         self.spec_gate = True  # speculation falls back to plain steps when drafts do not pay
         self.use_graphs = use_graphs
         self.mega = MEGA_ENABLED if mega is None else bool(mega)
@@ -160,8 +167,10 @@ class Engine:
         sh = _Shape(self, batch, prompt_len, new_tokens, self.speculate)
         # Known-answer checks of this shape's own plans (every row count it
         # replays) before it serves; raises, and the shape is not kept.
-        t_rows = (1, sh.spec_k + 1) if (self.speculate and sh.spec_k) else (1,)
+        t_rows = (1, sh.spec_k + 1) if (self.speculate and self.speculate != "tree" and sh.spec_k) else (1,)
         selfcheck.run_shape(sh.state, t_rows)
+        if sh.tree_t:
+            selfcheck.run_tree(sh.state)
         if self.use_graphs:
             sh.graph = self._capture(lambda: sh.state.step(t_rows=1))
             if self.mega and not self.speculate and sh.state.layer_supported():
@@ -346,12 +355,17 @@ class Engine:
 
         batch, prompt_len = ids.shape
         sh = self._shape_for(batch, prompt_len, steps)
-        if sh.spec_k == 0:  # no room for drafts at this batch size
+        tree = self.speculate == "tree"
+        if (sh.tree_t if tree else sh.spec_k) == 0:  # no room for drafts at this batch size
             yield from self._generate_plain(sh, ids, steps)
             self.stats["spec"] = {"iterations": steps - 1, "verify_iterations": 0, "plain_iterations": steps - 1}
             return
         dec = getattr(sh, "spec", None)
         if dec is None:
-            dec = sh.spec = SpecDecoder(self, sh.state, SPEC_PRIMARY, SPEC_BACKOFF, sh.spec_k)
+            if tree:
+                dec = TreeDecoder(self, sh.state, SPEC_PRIMARY, SPEC_BACKOFF)
+            else:
+                dec = SpecDecoder(self, sh.state, SPEC_PRIMARY, SPEC_BACKOFF, sh.spec_k)
+            sh.spec = dec
         yield from dec.generate(ids, steps, gate=self.spec_gate)
         self.stats["spec"] = dec.last_stats

@@ -19,7 +19,9 @@ stream, so it can be captured into a hipGraph as is.
 
 Per-role launch plans are functions of the matrix shape only, never of the
 row count: that keeps every output element's summation order the same for a
-1-row and a 36-row call (the basis of lossless speculation).
+1-row and a 36-row call (the basis of lossless speculation).  A tree pass
+(``tree_t`` nodes per sequence) runs the same projections around
+``qdec_tree_attn``, whose sums are its own.
 
 ``Prefill`` fills the cache from a prompt with the prefill kernels: every
 prompt position of every sequence goes through a layer at once (in position
@@ -372,6 +374,11 @@ def max_rows_per_seq(batch, requested=ATTN_MAX_T, group=4):
     return max(1, min(requested, cap, GEMM_MAX_ROWS // batch))
 
 
+def max_tree_nodes(batch):
+    """Nodes per sequence of a tree pass: GEMM_MAX_ROWS rows in all."""
+    return min(capi.TREE_MAX_T, GEMM_MAX_ROWS // batch)
+
+
 def attn_chunk(batch, nkv, cap):
     """Slots per attention workgroup (a multiple of 32; absolute-slot
     chunking).  Measured on MI355X with 4-wave workgroups (graph-replayed,
@@ -510,7 +517,7 @@ class DeviceModel:
 class DecodeState:
     """Buffers for one (batch, capacity) shape and the step over them."""
 
-    def __init__(self, model, batch, capacity, max_t=1, keep_logits=False):
+    def __init__(self, model, batch, capacity, max_t=1, keep_logits=False, tree_t=0):
         c = model.cfg
         self.model, self.lib = model, model.lib
         self.batch = batch
@@ -518,7 +525,12 @@ class DecodeState:
         self.max_t = max_rows_per_seq(batch, max_t, c.group)
         if batch > GEMM_MAX_ROWS:
             raise ValueError(f"batch {batch} > {GEMM_MAX_ROWS} rows per step")
-        self.max_rows = batch * self.max_t
+        # Nodes per sequence of a tree pass (0: none): their attention takes
+        # any number up to TREE_MAX_T, so only the GEMMs' rows bound them.
+        if not 0 <= tree_t <= max_tree_nodes(batch):
+            raise ValueError(f"tree_t {tree_t} not in [0, {max_tree_nodes(batch)}] at batch {batch}")
+        self.tree_t = tree_t
+        self.max_rows = batch * max(self.max_t, tree_t)
         dev, bf = model.device, torch.bfloat16
         L, H, D = c.n_layers, c.hidden, c.head_dim
         self.chunk = attn_chunk(batch, c.nkv, self.cap)
@@ -574,7 +586,8 @@ class DecodeState:
         gw = 0
         gc = 1
         for role in ("qkv", "o", "gate_up", "down", "lm"):
-            for t in range(1, self.max_t + 1):  # the plan (and its workspace) depends on the row count
+            # the plan (and its workspace) depends on the row count
+            for t in sorted({*range(1, self.max_t + 1), *((tree_t,) if tree_t else ())}):
                 a = self._gemm_args(role, 0, batch * t, hand=self.hand_over)
                 pb, cb = self.lib.gemm_workspace(a)
                 gw, gc = max(gw, pb), max(gc, cb)
@@ -584,6 +597,17 @@ class DecodeState:
         aw = max(aw, self.lib.attn_workspace(self._attn_args(0, 1, partials=True))[0])
         self.attn_partial = torch.zeros((max(aw, 16) // 4 + 4,), dtype=torch.float32, device=dev)
         self.attn_counters = torch.zeros((max(ac, 4) // 4 + 4,), dtype=torch.int32, device=dev)
+        if tree_t:
+            # A tree's nodes keep their keys and values beside the cache until
+            # qdec_tree_commit appends the accepted path's.
+            node_shape = (L, batch, c.nkv, tree_t, D)
+            self.k_nodes = torch.zeros(node_shape, dtype=bf, device=dev)
+            self.v_nodes = torch.zeros(node_shape, dtype=bf, device=dev)
+            self.parents = torch.full((batch * tree_t,), -1, dtype=torch.int32, device=dev)
+            self.path = torch.full((batch * tree_t,), -1, dtype=torch.int32, device=dev)
+            self.naccept = torch.zeros((batch,), dtype=torch.int32, device=dev)
+            tw, _ = self.lib.tree_attn_workspace(self._tree_args(0))
+            self.tree_partial = torch.zeros((max(tw, 16) // 4 + 4,), dtype=torch.float32, device=dev)
         self._gemm_cache = {}
         self._attn_cache = {}
         self.layer_launch = False  # plain steps as one qdec_layer launch per layer
@@ -775,16 +799,54 @@ class DecodeState:
         a.strided = 1 if (ATTN_STRIDED and self.attn_waves == 8 and self.chunk < self.cap) else 0
         return a
 
+    def _tree_args(self, layer):
+        m, c = self.model, self.model.cfg
+        a = capi.TreeAttnArgs()
+        a.qkv, a.q_norm_w, a.k_norm_w = self.qkv.data_ptr(), m.q_norm[layer].data_ptr(), m.k_norm[layer].data_ptr()
+        a.cos_tab, a.sin_tab, a.lens = self.cos.data_ptr(), self.sin.data_ptr(), self.lens.data_ptr()
+        a.parents = self.parents.data_ptr()
+        a.k_cache, a.v_cache = self.k_cache[layer].data_ptr(), self.v_cache[layer].data_ptr()
+        a.k_nodes, a.v_nodes = self.k_nodes[layer].data_ptr(), self.v_nodes[layer].data_ptr()
+        a.out = self.attn_out.data_ptr()
+        if hasattr(self, "tree_partial"):
+            a.partial = self.tree_partial.data_ptr()
+        a.eps, a.sm_scale = c.eps, c.head_dim ** -0.5
+        a.batch, a.t_rows, a.nq, a.nkv, a.head_dim = self.batch, self.tree_t, c.nq, c.nkv, c.head_dim
+        a.cap, a.splits = self.cap, 0
+        a.out_frag = 1 if self.batch * self.tree_t >= FRAG_ROWS else 0
+        return a
+
+    def tree_commit(self, stream=None):
+        """The keys and values of the nodes on ``path`` (``naccept[b] + 1`` of
+        them per sequence) into the cache slots that end at ``lens[b]``, in
+        every layer."""
+        c = self.model.cfg
+        a = capi.TreeCommitArgs(k_nodes=self.k_nodes.data_ptr(), v_nodes=self.v_nodes.data_ptr(),
+                                k_cache=self.k_cache.data_ptr(), v_cache=self.v_cache.data_ptr(),
+                                path=self.path.data_ptr(), naccept=self.naccept.data_ptr(),
+                                lens=self.lens.data_ptr(), n_layers=c.n_layers, batch=self.batch,
+                                t_rows=self.tree_t, nkv=c.nkv, head_dim=c.head_dim, cap=self.cap)
+        self.lib.tree_commit(a, (stream or torch.cuda.current_stream(self.model.device)).cuda_stream)
+
     # ---------------------------------------------------------------- step
-    def run_step(self, t_rows=1, lm_head=True, ids_out=None, advance=True, stream=None):
+    def run_step(self, t_rows=1, lm_head=True, ids_out=None, advance=True, stream=None, tree=False):
         """One forward of ``t_rows`` rows per sequence at positions
         ``lens[b] .. lens[b] + t_rows - 1`` (device ``lens``), fed from
         ``ids[b * t_rows + t]``.
 
         With ``lm_head`` the greedy pick of every row goes to ``ids_out``
         (default ``ids``: the next step's input) and, with ``advance``,
-        ``lens[b] += 1`` (plain decode; requires ``t_rows == 1``)."""
-        if t_rows < 1 or t_rows > self.max_t:
+        ``lens[b] += 1`` (plain decode; requires ``t_rows == 1``).
+
+        With ``tree`` the rows are the ``t_rows`` = ``tree_t`` nodes of
+        ``parents`` at positions ``lens[b]`` + depth; their keys and values go
+        to ``k_nodes`` / ``v_nodes`` and the cache is only read."""
+        if tree:
+            if not self.tree_t or t_rows != self.tree_t:
+                raise ValueError(f"t_rows {t_rows} of a tree pass is not the state's tree_t {self.tree_t}")
+            if advance:
+                raise ValueError("a tree pass does not advance the lengths")
+        elif t_rows < 1 or t_rows > self.max_t:
             raise ValueError(f"t_rows {t_rows} not in [1, {self.max_t}]")
         if advance and lm_head and t_rows != 1:
             raise ValueError("advance needs t_rows == 1")
@@ -795,14 +857,17 @@ class DecodeState:
         e.ids, e.emb, e.h = self.ids.data_ptr(), m.emb.data_ptr(), self.h.data_ptr()
         e.rows, e.hidden, e.vocab = rows, c.hidden, c.vocab
         lib.embed(e, s)
-        pm = self._merge_in_o(t_rows)
-        by_layer = self.layer_launch and t_rows == 1
+        pm = not tree and self._merge_in_o(t_rows)
+        by_layer = self.layer_launch and t_rows == 1 and not tree
         for i in range(c.n_layers):
             if by_layer:
                 lib.layer(self._layer_args[i], s)
                 continue
             lib.gemm(self._cached_gemm("qkv", i, rows), s)
-            lib.attn(self._cached_attn(i, t_rows, pm), s)
+            if tree:
+                lib.tree_attn(self._cached_tree(i), s)
+            else:
+                lib.attn(self._cached_attn(i, t_rows, pm), s)
             lib.gemm(self._cached_gemm("o", i, rows, self._cached_attn(i, t_rows, pm) if pm else None), s)
             lib.gemm(self._cached_gemm("gate_up", i, rows), s)
             lib.gemm(self._cached_gemm("down", i, rows), s)
@@ -827,9 +892,15 @@ class DecodeState:
             self._attn_cache[key] = a
         return a
 
-    def step(self, t_rows=1, lm_head=True, ids_out=None, advance=True, stream=None):
+    def _cached_tree(self, layer):
+        a = self._attn_cache.get(("tree", layer))
+        if a is None:
+            a = self._attn_cache[("tree", layer)] = self._tree_args(layer)
+        return a
+
+    def step(self, t_rows=1, lm_head=True, ids_out=None, advance=True, stream=None, tree=False):
         """One forward (``run_step``); the name every caller captures."""
-        self.run_step(t_rows=t_rows, lm_head=lm_head, ids_out=ids_out, advance=advance, stream=stream)
+        self.run_step(t_rows=t_rows, lm_head=lm_head, ids_out=ids_out, advance=advance, stream=stream, tree=tree)
 
     # ------------------------------------------------ one layer per launch
     def layer_supported(self):

@@ -16,7 +16,9 @@ step replays are exercised:
 * the attention at cache length 0: every head's output is the new value row,
   and the value row lands in cache slot 0;
 * the n-gram drafter and the acceptance rule on a short history with a
-  known match.
+  known match;
+* for a shape with tree passes, the tree's drafter, attention, acceptance and
+  commit through the shape's own buffers (``run_tree``).
 
 A mismatch raises ``QdecError``: the engine never falls back to another
 implementation.
@@ -483,4 +485,132 @@ def run_shape(state, t_rows=(1,)):
             _fail("embed", f"{R} rows: gathered rows differ from the embedding")
         _shape_gemms(state, t)
         _shape_attention(state, t)
+    torch.cuda.synchronize(dev)
+
+
+def run_tree(state):
+    """Known-answer checks of a tree pass of ``state`` (``tree_t`` nodes), on
+    its own buffers: embedding, projections and lm_head at its row count as
+    ``run_shape`` checks them, and the four kernels of a tree iteration:
+
+    * the drafter on a history with two known continuations;
+    * the attention over a cache whose values are all one row, with a star of
+      nodes that carry that row too: a softmax average of equal rows is that
+      row (its weights sum to 1 to far less than half a bf16 step, so the sum
+      rounds back to it).  One node's key and value and
+      every slot past the length are NaN: only that node may see it;
+    * the acceptance of one draft, and its node's key and value in the cache
+      slots it takes, with every other slot as it was."""
+    m, lib, c = state.model, state.lib, state.model.cfg
+    dev = m.device
+    s = torch.cuda.current_stream(dev).cuda_stream
+    B, T, D, nq, nkv, cap = state.batch, state.tree_t, c.head_dim, c.nq, c.nkv, state.cap
+    R, G = B * T, c.nq // c.nkv
+    ids = (torch.arange(R, device=dev, dtype=torch.int64) * 7919 + 13) % c.vocab
+    state.ids[:R].copy_(ids)
+    lib.embed(capi.EmbedArgs(ids=state.ids.data_ptr(), emb=m.emb.data_ptr(), h=state.h.data_ptr(), rows=R,
+                             hidden=c.hidden, vocab=c.vocab), s)
+    if not torch.equal(state.h[:R].float(), _tiled_rows(m.emb, c.vocab, c.hidden, ids)):
+        _fail("embed", f"{R} rows: gathered rows differ from the embedding")
+    _shape_gemms(state, T)
+
+    # ---- drafter: after [5, 6, 7], most recently 4, before that 8 9
+    line = torch.tensor([5, 6, 7, 8, 9, 5, 6, 7, 4, 5, 6, 7], dtype=torch.int64)
+    hist = torch.zeros((B, len(line) + 8), dtype=torch.int64, device=dev)
+    hist[:, :len(line)] = line.to(dev)
+    hl = torch.full((B,), len(line) - 1, dtype=torch.int32, device=dev)
+    lib.tree_draft(capi.TreeDraftArgs(hist=hist.data_ptr(), lens=hl.data_ptr(), ids=state.ids.data_ptr(),
+                                      parents=state.parents.data_ptr(), batch=B, cap=hist.shape[1], t_rows=T,
+                                      primary=3, backoff=3, depth=2, matches=2), s)
+    nodes = ([(7, -1), (4, 0), (5, 1), (8, 0), (9, 3)] + [(0, -1)] * T)[:T]
+    want = torch.tensor(nodes * B, dtype=torch.int64)
+    got = torch.stack((state.ids[:R].cpu(), state.parents[:R].cpu().long()), -1)
+    if not torch.equal(got, want):
+        _fail("tree_draft", f"(token, parent) {got.tolist()}, expected {want.tolist()}")
+
+    # ---- attention: a star, one leaf NaN, the cache's rows all equal
+    g = torch.Generator(device="cpu").manual_seed(977 + R)
+    lens = [max(0, cap - 2 * T - 37 * b) for b in range(B)]
+    row = torch.randn((B, nkv, D), generator=g).to(torch.bfloat16)
+    kc, vc = state.k_cache[0], state.v_cache[0]
+    past = (torch.arange(cap)[None] >= torch.tensor(lens)[:, None]).to(dev)[:, None, :, None]  # [B, 1, cap, 1]
+    k0 = torch.randn(kc.shape, generator=torch.Generator(device=dev).manual_seed(5), device=dev)
+    k0 = k0.masked_fill(past, float("nan")).to(torch.bfloat16)
+    v0 = row.to(dev).float()[:, :, None].expand(kc.shape).masked_fill(past, float("nan")).to(torch.bfloat16)
+    v8 = vc.view(B, nkv, cap // 8, D, 8)  # channel-major: slot s, channel d at [s // 8, d, s % 8]
+
+    def cached_v():
+        return v8.permute(0, 1, 2, 4, 3).reshape(B, nkv, cap, D)
+
+    kc.copy_(k0)
+    v8.copy_(v0.view(B, nkv, cap // 8, 8, D).permute(0, 1, 2, 4, 3))
+    qkv = torch.randn((B, T, nq + 2 * nkv, D), generator=g).to(torch.bfloat16)
+    qkv[:, :, nq + nkv:] = row[:, None]
+    bad = [1 + b % (T - 1) for b in range(B)]
+    for b in range(B):
+        qkv[b, bad[b], nq:] = float("nan")
+    state.qkv[:R].copy_(qkv.reshape(R, -1).to(dev))
+    state.lens.copy_(torch.tensor(lens, dtype=torch.int32, device=dev))
+    state.parents[:R].view(B, T).fill_(0)
+    a = state._tree_args(0)
+    lib.tree_attn(a, s)
+    out = _get_rows(state.attn_out, R, nq * D, a.out_frag).cpu().view(B, T, nq * D)
+    want = row.repeat_interleave(G, 1).view(B, 1, nq * D).expand(B, T, nq * D).clone()
+    for b in range(B):
+        want[b, bad[b]] = out[b, bad[b]]
+        if not bool(out[b, bad[b]].isnan().all()):
+            _fail("tree attention", f"sequence {b}: a NaN node is not in its own row")
+    if not torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)):
+        _fail("tree attention", f"{R} rows: rows differ from the one value row of cache and nodes")
+    if not torch.equal(state.v_nodes[0].cpu().nan_to_num(7.0),
+                       qkv[:, :, nq + nkv:].transpose(1, 2).nan_to_num(7.0)):
+        _fail("tree attention", f"{R} rows: node value rows differ")
+
+    # ---- acceptance of each sequence's last good leaf, and its commit
+    leaf = [T - 1 if T > 2 and bad[b] != T - 1 else (T - 2 if T > 2 else 0) for b in range(B)]
+    ids = torch.arange(R, dtype=torch.int64) + 1
+    pick = torch.zeros(R, dtype=torch.int64)
+    for b in range(B):
+        pick[b * T] = ids[b * T + leaf[b]] if leaf[b] else 0
+        pick[b * T + leaf[b]] = 0 if not leaf[b] else R + 1
+    state.ids[:R].copy_(ids)
+    state.out_tok[:R].copy_(pick)
+    hist = torch.zeros((B, cap), dtype=torch.int64, device=dev)
+    emit = torch.zeros(R, dtype=torch.int64, device=dev)
+    lib.tree_accept(capi.TreeAcceptArgs(
+        out_tok=state.out_tok.data_ptr(), ids=state.ids.data_ptr(), parents=state.parents.data_ptr(),
+        hist=hist.data_ptr(), lens=state.lens.data_ptr(), lens_out=state.lens.data_ptr(),
+        naccept=state.naccept.data_ptr(), path=state.path.data_ptr(), emit=emit.data_ptr(), batch=B, cap=cap,
+        t_rows=T, stop_len=cap), s)
+    walks = [[0, leaf[b]] if leaf[b] else [0] for b in range(B)]
+    for b in range(B):
+        toks = [int(pick[b * T + t]) for t in walks[b]]
+        n, pad = len(toks), [-1] * (T - len(toks))
+        got = (state.path[b * T:(b + 1) * T].tolist(), emit[b * T:(b + 1) * T].tolist(), int(state.naccept[b]),
+               int(state.lens[b]), hist[b, lens[b] + 1:lens[b] + 1 + n].tolist())
+        if got != (walks[b] + pad, toks + pad, n - 1, lens[b] + n, toks):
+            _fail("tree_accept", f"sequence {b}: path, tokens, accepted, length, history {got}")
+    if c.n_layers > 1:
+        state.k_nodes[-1].fill_(2.0)
+        state.v_nodes[-1].fill_(3.0)
+        state.k_cache[-1].zero_()
+        state.v_cache[-1].zero_()
+    state.tree_commit()
+    for b in range(B):
+        for i, t in enumerate(walks[b]):
+            k0[b, :, lens[b] + i] = state.k_nodes[0, b, :, t]
+            v0[b, :, lens[b] + i] = row[b].to(dev)
+    if not (torch.equal(kc.nan_to_num(7.0), k0.nan_to_num(7.0))
+            and torch.equal(cached_v().nan_to_num(7.0), v0.nan_to_num(7.0))):
+        _fail("tree_commit", f"{R} rows: the cache differs from the accepted nodes appended to it")
+    if c.n_layers > 1:
+        slots = sum(len(w) for w in walks) * nkv * D
+        if (float(state.k_cache[-1].float().sum()), float(state.v_cache[-1].float().sum())) != (2.0 * slots, 3.0 * slots):
+            _fail("tree_commit", f"{R} rows: the last layer's cache differs from its accepted nodes")
+    state.k_cache.zero_()
+    state.v_cache.zero_()
+    state.k_nodes.zero_()
+    state.v_nodes.zero_()
+    state.parents.fill_(-1)
+    state.lens.zero_()
     torch.cuda.synchronize(dev)

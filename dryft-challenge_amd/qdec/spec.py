@@ -124,15 +124,18 @@ class AcceptancePredictor:
             L = len(ix.hist) - 1
             while pend and pend[0][0] + self.k <= L:
                 L0, d = pend.popleft()
-                follow = ix.hist[L0 + 1:L0 + 1 + self.k]
-                a = 0
-                while a < self.k and d[a] == follow[a]:
-                    a += 1
+                a = self._accepted(d, ix.hist[L0 + 1:L0 + 1 + self.k])
                 self.recent.append(a + 1)
                 self.positions += 1
                 self.hits += a > 0
                 self.total += a + 1
             pend.append((L, ix.draft(L)))
+
+    def _accepted(self, d, follow):
+        a = 0
+        while a < self.k and d[a] == follow[a]:
+            a += 1
+        return a
 
     def predicted(self):
         """Tokens per sequence a verify iteration is expected to emit (1.0
@@ -147,18 +150,32 @@ class SpecDecoder:
         self.engine, self.state, self.lib = engine, state, state.lib
         self.primary, self.backoff, self.k = primary, backoff, k
         self.T = k + 1
-        B, dev = state.batch, state.model.device
         if k < 1:
             raise ValueError("speculation needs k >= 1 drafts")
-        if self.T > state.max_t:
-            raise ValueError(f"verify rows {self.T} > state max_t {state.max_t}")
-        self.hist = torch.zeros((B, state.cap), dtype=torch.int64, device=dev)
-        self.draft = torch.zeros((B * k,), dtype=torch.int64, device=dev)
-        self.naccept = torch.zeros((B,), dtype=torch.int32, device=dev)
+        self._buffers()
+        self.hist = torch.zeros((state.batch, state.cap), dtype=torch.int64, device=state.model.device)
         self.graphs = {}       # k -> graph, for the current stop length
         self.graph_stop = None
         self.cost_ratio = None  # time of a verify iteration / a k = 0 iteration
         self.last_stats = {}
+
+    def _buffers(self):
+        st, dev = self.state, self.state.model.device
+        if self.T > st.max_t:
+            raise ValueError(f"verify rows {self.T} > state max_t {st.max_t}")
+        self.draft = torch.zeros((st.batch * self.k,), dtype=torch.int64, device=dev)
+        self.naccept = torch.zeros((st.batch,), dtype=torch.int32, device=dev)
+        self.tokens = st.out_tok  # row b * (k + 1) + i: the i-th token sequence b emits
+
+    def _predictor(self):
+        return AcceptancePredictor(self.state.batch, self.primary, self.backoff, self.k)
+
+    def _rows(self, k):
+        """Rows per sequence of an iteration with k drafts in a chain."""
+        return k + 1
+
+    def _checked(self, toks):
+        return self.engine._checked(toks)
 
     def _draft(self, k):
         """Write the verify rows ``ids[b*(k+1) ..]`` = [current token, k
@@ -232,7 +249,7 @@ class SpecDecoder:
         first = self.engine._checked(st.ids[:B].to("cpu", non_blocking=False).tolist())
         out = [[t] for t in first]
         counts = [1] * B
-        pred = AcceptancePredictor(B, self.primary, self.backoff, self.k)
+        pred = self._predictor()
         for b, row in enumerate(prompt.tolist()):
             pred.start(b, row, first[b])
         yield [out[b][0] for b in range(B)]
@@ -254,7 +271,8 @@ class SpecDecoder:
             kinds[slot] = k
             self._run(k, stop_len)
             h_acc[slot].copy_(self.naccept, non_blocking=True)
-            h_tok[slot, :B * (k + 1)].copy_(st.out_tok[:B * (k + 1)], non_blocking=True)
+            n = B * self._rows(k)
+            h_tok[slot, :n].copy_(self.tokens[:n], non_blocking=True)
             events[slot].record()
 
         # Every iteration emits >= 1 token per live sequence, so at most
@@ -268,9 +286,9 @@ class SpecDecoder:
             events[slot].synchronize()
             done += 1
             k = kinds[slot]
-            Tk = k + 1
+            Tk = self._rows(k)
             acc = h_acc[slot].tolist()
-            tok = self.engine._checked(h_tok[slot, :B * (k + 1)].tolist())
+            tok = self._checked(h_tok[slot, :B * Tk].tolist())
             gained, live = 0, 0
             for b in range(B):
                 if counts[b] >= steps:
