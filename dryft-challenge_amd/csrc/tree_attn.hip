@@ -1069,22 +1069,24 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 
 }  // namespace
 
-// The row group and the splits.
+// The row group and the splits.  Below, us on MI355X with 32 query heads on 8.
 //
 // The narrow kernel reads the cache once per row group, from an L2 that its
 // groups share; the wide one once per 128 or 256 rows, but it waits at a barrier
-// per block.  The narrow one is ahead until its reads come to about 200 MB.
-// MI355X, us, 32 query heads on 8, narrow / wide: 64 nodes on 4100 slots (134 MB)
-// 25 / 32, 32 nodes on 2000 slots (33 MB) 16 / 21; 2 x 32 nodes on 8000 slots
-// (262 MB) 41 / 34, 64 nodes on 30000 (980 MB) 118 / 60.
+// per block.  The narrow one is ahead until its reads come to about 200 MB:
+// narrow / wide, 32 nodes on 1100 slots (18 MB) 14 / 19, 64 nodes on 4200 (138 MB)
+// 26.5 / 32, 2 x 32 nodes on 8300 (272 MB) 43 / 37, 64 on 30000 (980 MB) 106 / 72.
 //
-// 16 rows per workgroup give more workgroups, 32 fewer reads: 16 while that
-// leaves fewer than 128 (16 nodes on 640 slots 11.4 / 12.5, on 4100 15.9 / 17.2;
-// 8 x 8 nodes on up to 1600 slots 19.2 / 17.3, 16 x 8 nodes on 3000 58 / 45).
+// 16 rows per workgroup give more workgroups, 32 half the reads.  16 where 32
+// would leave CUs idle and the reads are under 130 MB: 16 / 32 rows, 16 nodes on
+// 1100 slots (18 MB) 11.7 / 13.2, on 4200 (69 MB) 15.9 / 17.6, 2 x 16 nodes on 4200
+// (138 MB) 23.5 / 22.5, 32 nodes on 8300 (272 MB) 33 / 27, 16 on 30000 58 / 45.
 //
 // One workgroup per CU, none of fewer than four blocks of a full cache: more
 // splits read no faster and merge more (16 nodes on 4100 slots, 4 / 8 / 16 / 32
-// splits: 20 / 16 / 19 / 28).
+// splits: 20 / 16 / 19 / 28).  Of the wide kernel's 128 rows a CU holds two
+// workgroups, which pays from 24 blocks each: 2 x 32 nodes on 30000 slots, one / two
+// 84 / 75, on 8300 (8 blocks each) 37 / 39.5.
 void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int rows = p->t_rows * (p->nq / p->nkv), tiles = (rows + 15) / 16;
   const int64_t cells = (int64_t)p->batch * p->nkv;
@@ -1093,11 +1095,15 @@ void tree_attn_plan(TreeAttnParams *p, int splits) {
   if (rows > 64 && cache * ((rows + 31) / 32) > 200000000)
     p->group_rows = rows <= 128 ? 128 : 256;
   else
-    p->group_rows = rows <= 16 || cells * tiles < 128 ? 16 : 32;
+    p->group_rows = rows <= 16 || (cells * tiles < 128 && cache * tiles < 130000000) ? 16 : 32;
   p->min_blocks = 4;
   p->groups = (rows + p->group_rows - 1) / p->group_rows;
-  if (splits == 0)
-    splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / (cells * p->groups), blocks / p->min_blocks));
+  if (splits == 0) {
+    const int64_t units = cells * p->groups;
+    int64_t n = std::min<int64_t>(256 / units, blocks / p->min_blocks);
+    if (p->group_rows == 128 && blocks >= 24 * (512 / units)) n = std::max(n, 512 / units);
+    splits = (int)std::max<int64_t>(1, n);
+  }
   p->splits = std::min(splits, 256);
   p->by_groups = fast_div(p->groups);
   p->by_nkv = fast_div(p->nkv);
