@@ -65,6 +65,8 @@ struct Head {
   }
 };
 
+__device__ __forceinline__ uint4 vec(const u32x4_t &v) { return make_uint4(v[0], v[1], v[2], v[3]); }
+
 // Eight numbers as two bf16 vectors whose sum has 16 bits of them.
 __device__ __forceinline__ void split8(const float (&p)[8], uint4 &hi, uint4 &lo) {
   hi = pack8(p);
@@ -690,27 +692,40 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
 //     block, channels 32s + 8g .. +8;
 //   V fragment dt: lane (c, g) holds channel 16dt + c, rows 8g .. 8g + 7.
 // The node blocks are prepared into the same order behind the ring.  While
-// block j's softmax runs on the vector units, the matrix cores form block j +
-// 1's scores, one MFMA per exponential.
-// What bounds it are the LDS reads (a block's 16 KiB, D = 128, serve a wave's 32
-// rows) and the matrix cores, which take as long.  (64 rows per wave would
-// halve the reads, but then the sums live in the accumulation registers, and
-// the scores with them: every score tile moved between the two files.)
+// block j's exponentials run on the vector units, the matrix cores form block j +
+// 1's scores, one MFMA per exponential; the probabilities' low parts are formed
+// between the products of the high ones, the next scores' maxima between those of
+// the low ones.  The values are read as the keys' registers come free and the
+// other way round.  Cached blocks before the last run without its checks, and the
+// workgroup meets every second block when the ring has 8 slots.
+//
+// MI355X, 2 x 64 nodes, 64 query heads on 8, 30000 slots: 174 us, 0.75 PFLOP/s (1.1
+// with both parts of the probabilities).  A block of 256 rows takes about 2700
+// cycles of a CU, of which the matrix cores have 1560 and the LDS reads 530; the
+// rest is the two waves of a SIMD waiting for each other's vector instructions.
+// (209 us with the checks in every block and the softmax's steps one after the
+// other.  64 rows per wave would halve the LDS reads, but then the sums live in
+// the accumulation registers, and the scores with them: every score tile moved
+// between the two files.)
 template <int D, int NW, int NT>
 struct WideLds {
   static constexpr int KF = D / 16, VF = D / 16;  // fragments of a block
   static constexpr int BV = (KF + VF) * 64;       // uint4 per block
-  static constexpr int RING = NW == 8 ? 8 : 4;    // 8 waves: one workgroup per CU, 4: two
+  static constexpr int RING = NW == 8 ? 8 : 4;    // 4 waves: 8 slots take 2 us longer to fill
   static constexpr int vecs = (RING + NT) * BV;   // NT node blocks
 };
 
 template <int D, int NW, int NT>
-__global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 2) tree_wide_kernel(const TreeAttnParams p) {
+// 512 threads also where it runs with 256: the registers of two waves per SIMD.
+// More would be accumulation registers (64 nodes on 30000 slots, 16 query heads on
+// 8: 47.5 us, 54 with them).
+__global__ void __launch_bounds__(512, 2) tree_wide_kernel(const TreeAttnParams p) {
   using LY = WideLds<D, NW, NT>;
   constexpr int MT = 2;
   constexpr int DS = D / 32, DT = D / 16, KF = LY::KF, BV = LY::BV, RING = LY::RING;
   constexpr int FPW = (KF + LY::VF) / NW;  // fragments each wave loads per block
   constexpr int RG = 16 * MT * NW;         // rows of a group
+  constexpr bool PAIRS = RING >= 8;        // one barrier per two blocks: the ring holds blocks jj .. jj + 3 meanwhile
   static_assert((KF + LY::VF) % NW == 0 && (RING - 2) * FPW < 64, "whole fragments per wave, counted in vmcnt");
   __shared__ uint4 ring[LY::vecs];         // [RING + NT][fragment][lane]
   uint4 *const tail = ring + RING * BV;
@@ -763,7 +778,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
 #pragma unroll
     for (int i = 0; i < FPW; ++i) {
       const int f = wave + NW * i;
-      if (f < KF)
+      if (NW * (i + 1) <= KF || (NW * i < KF && f < KF))
         dma16u(kc + at + 4 * D * (f & 1) + 32 * (f >> 1), koff, base + f * 1024);
       else
         dma16u(vc + at + (f - KF) * 128, voff, base + f * 1024);
@@ -824,6 +839,11 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   };
   struct Scores {
     f32x4_t a[MT], b[MT];
+    float mx[MT];  // a lane's largest
+    __device__ __forceinline__ float at(int u, int e) const { return e < 4 ? a[u][e] : b[u][e - 4]; }
+    __device__ __forceinline__ void max_to(int u, int e) {  // entries up to odd e
+      mx[u] = fmaxf(e == 1 ? at(u, 0) : fmaxf(mx[u], at(u, e - 1)), at(u, e));
+    }
   };
   auto score1 = [&](Scores &S, int s, int u, int h) {
     f32x4_t &d = h ? S.b[u] : S.a[u];
@@ -850,15 +870,24 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
   Scores s0, s1;
 #pragma unroll
   for (int i = 0; i < 2 * DS * MT; ++i) score1(s0, i / (2 * MT), (i >> 1) % MT, i & 1);
+#pragma unroll
+  for (int i = 1; i < 8 * MT; i += 2) s0.max_to(i >> 3, i & 7);
   await(min(1, n - 1), RING - 2);
   if (RING - 1 < nd) dma_block(RING - 1);
+  int issued = RING - 1;  // the newest block asked for, if there is one
   read_k(min(1, n - 1));
 
   const float scale = p.scale_log2, slack = kMaxSlack / scale;
-  auto block = [&](int jj, Scores &S, Scores &N, auto lastc) {
-    constexpr bool LAST = decltype(lastc)::value != 0;
+  // AHEAD: 2 or 3, the workgroup meets and blocks up to jj + AHEAD are in LDS
+  // after that; 0, the last meeting covers this block; -1, the last block.
+  // INNER: blocks up to jj + RING are whole ones from the cache and the last
+  // meeting brought its loads up to date.
+  auto block = [&](int jj, Scores &S, Scores &N, auto ahead, auto inner) {
+    constexpr int AHEAD = decltype(ahead)::value;
+    constexpr bool LAST = AHEAD < 0, INNER = decltype(inner)::value != 0;
+    auto at = [&](int k) { return INNER ? ring + (k & (RING - 1)) * BV + lane : src(k); };
     const int j = j0 + jj;
-    if (32 * j + 32 > L) {  // the last cached block, or nodes
+    if (!INNER && 32 * j + 32 > L) {  // the last cached block, or nodes
 #pragma unroll
       for (int u = 0; u < MT; ++u) {
         const uint32_t bits = j >= nb ? (uint32_t)(sees[u] >> (32 * (j - nb))) >> (8 * grp)
@@ -868,26 +897,33 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
           if (!((bits >> i) & 1)) S.a[u][i] = NEG_INF;
           if (!((bits >> (4 + i)) & 1)) S.b[u][i] = NEG_INF;
         }
+#pragma unroll
+        for (int e = 1; e < 8; e += 2) S.max_to(u, e);
       }
     }
+    if (__builtin_expect(__any(S.mx[0] > m_run[0] + slack || S.mx[1] > m_run[1] + slack), 0)) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      const float bmax = fmaxf(fmaxf(fmaxf(S.a[u][0], S.a[u][1]), fmaxf(S.a[u][2], S.a[u][3])),
-                               fmaxf(fmaxf(S.b[u][0], S.b[u][1]), fmaxf(S.b[u][2], S.b[u][3])));
-      if (!__any(bmax > m_run[u] + slack)) continue;
-      const float m_new = fmaxf(m_run[u], max_xor16_32(bmax));
-      const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
-      l_run[u] *= alpha;
-      m_run[u] = m_new;
+      for (int u = 0; u < MT; ++u) {
+        const float m_new = fmaxf(m_run[u], max_xor16_32(S.mx[u]));
+        const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
+        l_run[u] *= alpha;
+        m_run[u] = m_new;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[u][dt] *= alpha;
+        for (int dt = 0; dt < DT; ++dt) acc[u][dt] *= alpha;
+      }
     }
     uint4 vf[DT];
-    const uint4 *B = src(jj);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) vf[dt] = B[(KF + dt) * 64];
-    uint4 pf[MT], pl[MT];
+    const uint4 *B = at(jj) + KF * 64;
+    auto read_v = [&](int dt) {
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      vf[dt] = B[dt * 64];
+      vf[dt + 1] = B[(dt + 1) * 64];
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    };
+    read_v(0);
+    u32x4_t ph[MT], pl[MT];  // the probabilities' two parts
     float pj[MT][8], mc[MT], psum[MT];
+    auto high = [&](int u, int e) { ph[u][e >> 1] = pack2(pj[u][e - 1], pj[u][e]); };  // e odd
 #pragma unroll
     for (int u = 0; u < MT; ++u) {
       mc[u] = m_run[u] == NEG_INF ? 0.f : m_run[u] * scale;
@@ -898,7 +934,7 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int i = u * 8 + e;  // MFMA i of the scores: k step, tile, row half
-        float x = e < 4 ? S.a[u][e] : S.b[u][e - 4];
+        float x = S.at(u, e);
         pin(x);
         pj[u][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -mc[u]));
         if constexpr (!LAST) {
@@ -907,20 +943,29 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
             pin((i & 1) ? N.b[(i >> 1) % MT] : N.a[(i >> 1) % MT]);
           }
         }
+        if (i % 4 == 3 && i / 2 + 1 < DT) read_v(i / 2 + 1);  // as the keys' registers come free
         if (i > 0) psum[(i - 1) >> 3] += pj[(i - 1) >> 3][(i - 1) & 7];
+        if (i > 0 && !(i & 1)) high((i - 1) >> 3, (i - 1) & 7);
         pin(pj[u][e]);
       }
     psum[MT - 1] += pj[MT - 1][7];
+    high(MT - 1, 7);
 #pragma unroll
-    for (int u = 0; u < MT; ++u) {
-      l_run[u] += psum[u];
-      split8(pj[u], pf[u], pl[u]);
+    for (int u = 0; u < MT; ++u) l_run[u] += psum[u];
+    if constexpr (INNER && AHEAD > 0) {
+      constexpr int STEP = AHEAD - 1;  // blocks between meetings
+      __builtin_amdgcn_s_waitcnt(vmcnt_enc((RING - AHEAD - STEP) * FPW) & ~(15 << 8));
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int i = STEP - 1; i >= 0; --i) dma_block(jj + RING - i);
+      issued = jj + RING;
+    } else if constexpr (AHEAD > 0) {
+      await(min(jj + AHEAD, n - 1), issued);
+      for (; issued < jj + RING; ++issued)  // slots up to jj's were read by all
+        if (issued + 1 < nd) dma_block(issued + 1);
     }
-    if constexpr (!LAST) {
-      await(min(jj + 2, n - 1), jj + RING - 1);
-      if (jj + RING < nd) dma_block(jj + RING);
-    }
-    if (j < nb && 32 * j + 32 > L) {  // slots from L on hold anything
+    if (!INNER && j < nb && 32 * j + 32 > L) {  // slots from L on hold anything
       uint32_t keep[4];
       const int sb = 32 * j + 8 * grp;
 #pragma unroll
@@ -934,36 +979,64 @@ __global__ void __launch_bounds__(64 * NW, D == 128 && NW == 4 && NT == 2 ? 1 : 
         vf[dt].w &= keep[3];
       }
     }
-    if constexpr (!LAST) read_k(min(jj + 2, n - 1));
+    const uint4 *K2 = at(INNER ? jj + 2 : min(jj + 2, n - 1));
+    constexpr int VPM = 8 / DT;  // probabilities per MFMA
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int i = 0; i < DT * MT; ++i) {
+      const int dt = i / MT, u = i % MT;
+      acc[u][dt] = mfma16x16x32(vf[dt], vec(ph[u]), acc[u][dt]);
 #pragma unroll
-      for (int u = 0; u < MT; ++u) acc[u][dt] = mfma16x16x32(vf[dt], pl[u], acc[u][dt]);
+      for (int x = i * VPM; x < (i + 1) * VPM; ++x) {
+        const int w = x >> 3, e = x & 7;
+        pj[w][e] -= (e & 1) ? hi16(ph[w][e >> 1]) : lo16(ph[w][e >> 1]);
+        if (e & 1) pl[w][e >> 1] = pack2(pj[w][e - 1], pj[w][e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int i = 0; i < DT * MT; ++i) {
+      const int dt = i / MT, u = i % MT;
+      acc[u][dt] = mfma16x16x32(vf[dt], vec(pl[u]), acc[u][dt]);
+      if constexpr (!LAST) {
 #pragma unroll
-      for (int u = 0; u < MT; ++u) acc[u][dt] = mfma16x16x32(vf[dt], pf[u], acc[u][dt]);
-    if (j >= nb) {
+        for (int x = i * VPM; x < (i + 1) * VPM; ++x)
+          if (x & 1) N.max_to(x >> 3, x & 7);
+        if (u == MT - 1) {  // as the values' registers come free
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+          kf[dt] = K2[dt * 64];
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!INNER && j >= nb) {
       const uint32_t bad = (uint32_t)(badset >> (32 * (j - nb)));
       if (bad) {
 #pragma unroll
         for (int u = 0; u < MT; ++u)
-          add_not_finite<D>(acc[u], pf[u], bad, sees[u] >> (32 * (j - nb)),
+          add_not_finite<D>(acc[u], vec(ph[u]), bad, sees[u] >> (32 * (j - nb)),
                             qkv + (size_t)(32 * (j - nb)) * width + (size_t)(nq + nkv + kvh) * D, width);
       }
     }
   };
   int jj = 0;
   if (!(n & 1)) {  // pairs, then the last block by itself
-    block(0, s0, s1, Int<0>{});
+    block(0, s0, s1, Int<2>{}, Int<0>{});
     s0 = s1;
     jj = 1;
   }
-  for (; jj + 1 < n; jj += 2) {
-    block(jj, s0, s1, Int<0>{});
-    block(jj + 1, s1, s0, Int<0>{});
+  constexpr Int<PAIRS ? 3 : 2> first;
+  constexpr Int<PAIRS ? 0 : 2> second;
+  while (jj + 1 < n) {
+    block(jj, s0, s1, first, Int<0>{});
+    block(jj + 1, s1, s0, second, Int<0>{});
+    jj += 2;
+    for (; jj + 1 + RING < nd; jj += 2) {
+      block(jj, s0, s1, first, Int<1>{});
+      block(jj + 1, s1, s0, second, Int<1>{});
+    }
   }
-  block(jj, s0, s1, Int<1>{});
+  block(jj, s0, s1, Int<-1>{}, Int<0>{});
 
   // ---- output or partial.
   float *part = n_active > 1 ? tree_part<D>(p, u_.unit, g) : nullptr;
@@ -1072,10 +1145,12 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 // The row group and the splits.  Below, us on MI355X with 32 query heads on 8.
 //
 // The narrow kernel reads the cache once per row group, from an L2 that its
-// groups share; the wide one once per 128 or 256 rows, but it waits at a barrier
-// per block.  The narrow one is ahead until its reads come to about 200 MB:
-// narrow / wide, 32 nodes on 1100 slots (18 MB) 14 / 19, 64 nodes on 4200 (138 MB)
-// 26.5 / 32, 2 x 32 nodes on 8300 (272 MB) 43 / 37, 64 on 30000 (980 MB) 106 / 72.
+// groups share; the wide one once per 128 or 256 rows, but its pipeline takes
+// longer to fill.  The narrow one is ahead until its reads come to about 130 MB
+// (200 MB against 256 rows): narrow / wide, 32 nodes on 1100 slots (18 MB) 14 / 19,
+// 2 x 32 on 4200 (138 MB) 28 / 27, 4 x 16 on 8300 (272 MB) 47 / 42, 32 on 30000
+// (492 MB) 67 / 43; 64 nodes on 4200 (138 MB) 26.5 / 31, on 8300 (272 MB) 39 / 37, on
+// 30000 (980 MB) 106 / 61.
 //
 // 16 rows per workgroup give more workgroups, 32 half the reads.  16 where 32
 // would leave CUs idle and the reads are under 130 MB: 16 / 32 rows, 16 nodes on
@@ -1084,15 +1159,13 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 //
 // One workgroup per CU, none of fewer than four blocks of a full cache: more
 // splits read no faster and merge more (16 nodes on 4100 slots, 4 / 8 / 16 / 32
-// splits: 20 / 16 / 19 / 28).  Of the wide kernel's 128 rows a CU holds two
-// workgroups, which pays from 24 blocks each: 2 x 32 nodes on 30000 slots, one / two
-// 84 / 75, on 8300 (8 blocks each) 37 / 39.5.
+// splits: 20 / 16 / 19 / 28; 2 x 32 nodes on 30000 slots, 16 / 32: 65 / 71).
 void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int rows = p->t_rows * (p->nq / p->nkv), tiles = (rows + 15) / 16;
   const int64_t cells = (int64_t)p->batch * p->nkv;
   const int blocks = p->cap / 32;
   const int64_t cache = cells * p->cap * p->head_dim * 4;  // bytes of both caches
-  if (rows > 64 && cache * ((rows + 31) / 32) > 200000000)
+  if (rows > 32 && cache * ((rows + 31) / 32) > (rows <= 128 ? 130000000 : 200000000))
     p->group_rows = rows <= 128 ? 128 : 256;
   else
     p->group_rows = rows <= 16 || (cells * tiles < 128 && cache * tiles < 130000000) ? 16 : 32;
@@ -1101,7 +1174,6 @@ void tree_attn_plan(TreeAttnParams *p, int splits) {
   if (splits == 0) {
     const int64_t units = cells * p->groups;
     int64_t n = std::min<int64_t>(256 / units, blocks / p->min_blocks);
-    if (p->group_rows == 128 && blocks >= 24 * (512 / units)) n = std::max(n, 512 / units);
     splits = (int)std::max<int64_t>(1, n);
   }
   p->splits = std::min(splits, 256);
