@@ -26,7 +26,9 @@ __device__ __forceinline__ int64_t lane_i64(int64_t v, int l) {
 //   2. The candidates' tokens go to LDS.
 //   3. The first wave builds the tree with one lane per node: a token's child
 //      is found by one ballot.
-// What bounds it: a history of 20K tokens is 160 KB through one CU.
+// What bounds it: a history of 20K tokens is 160 KB through one CU.  MI355X: 16
+// histories of 8000 to 32000 tokens 16.6 us (36 with every position's pattern read
+// from memory), one of 600 tokens 3.6.
 constexpr int kDraftThreads = 1024;
 constexpr int kDraftU = 8;
 constexpr int kDraftWindow = kDraftU * kDraftThreads;
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(kDraftThreads) tree_draft_kernel(const qdec_tr
 }
 
 // One wave per sequence, one lane per node: a step down the tree is one
-// ballot over the lanes.
+// ballot over the lanes.  The launch bounds it (MI355X: one sequence 1.6 us, 32 2.6).
 __global__ void __launch_bounds__(64) tree_accept_kernel(const qdec_tree_accept_args p) {
   const int b = blockIdx.x, lane = threadIdx.x;
   const int T = p.t_rows;
@@ -170,7 +172,9 @@ __global__ void __launch_bounds__(64) tree_accept_kernel(const qdec_tree_accept_
 
 // One workgroup per (kv head, sequence, layer): the node rows of the path are
 // 16-byte vectors; keys go to their slot's row as they are, the 8 channels of
-// a value vector to their places of the channel-major cache.
+// a value vector to their places of the channel-major cache.  A path has few rows,
+// so the launch and one load after another bound it: MI355X, 36 layers of 8 kv
+// heads, one sequence 2.9 us, eight 5.7.
 template <int D>
 __global__ void __launch_bounds__(256) tree_commit_kernel(const qdec_tree_commit_args p) {
   const int kvh = blockIdx.x, b = blockIdx.y;

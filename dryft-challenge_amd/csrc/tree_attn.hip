@@ -410,7 +410,12 @@ __device__ __forceinline__ void tree_nan_rows(const TreeAttnParams &p, int b, in
 // the last split.  With one M tile every wave
 // prepares the queries for itself, in registers; with more, wave u prepares
 // tile u and the operands stay in LDS (in registers they spilled: two blocks and
-// 64 rows' sums are 256).
+// 32 rows' sums are 192).
+//
+// What bounds it: the cache read when it is long (MI355X, 32 x 4 nodes on 2000 to
+// 4224 slots, 16 query heads on 8: 75 us, 5.4 TB/s), else the chain of dependent
+// loads before the first block (16 nodes on 640 slots: 8 us, 4 of them that; 64 nodes
+// on 4100: 23, at 10 TB/s from L2).
 template <int D, int MT, int NT>
 struct NarrowLds {
   static constexpr int tail = 0;                            // node blocks in operand order
