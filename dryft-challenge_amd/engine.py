@@ -74,6 +74,13 @@ def spec_k(batch, group=4):
     return max(0, min(SPEC_K_MAX, 16 // batch - 1, max_rows_per_seq(batch, group=group) - 1))
 
 
+def speculation(mode):
+    """``Engine.speculate`` of a constructor's argument: "tree" or a bool."""
+    if isinstance(mode, str) and mode != "tree":
+        raise ValueError(f'speculate is a bool or "tree" (got {mode!r})')
+    return mode if isinstance(mode, str) else bool(mode)
+
+
 def _log(message):
     print(f"[engine] {message}", file=sys.stderr, flush=True)
 
@@ -149,7 +156,7 @@ class Engine:
         # Known-answer checks of every kernel family on this device, with the
         # model's own weights and plans; raises on a mismatch (no fallback).
         selfcheck.run(DecodeState(self.model, 1, 64, max_t=1))
-        self.speculate = speculate if speculate == "tree" else bool(speculate)
+        self.speculate = speculation(speculate)
         self.spec_gate = True  # speculation falls back to plain steps when drafts do not pay
         self.use_graphs = use_graphs
         self.mega = MEGA_ENABLED if mega is None else bool(mega)

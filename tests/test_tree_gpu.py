@@ -287,6 +287,72 @@ def test_attention_values_that_are_not_finite_stay_in_their_branch(lib):
     assert torch.equal(ref.rows()[:, sees2][..., rest], got[:, sees2][..., rest])
 
 
+# Shapes of the many-row kernel: 128 or 256 query rows per workgroup, up to 32 or
+# up to 64 nodes, both head sizes; it takes over by what a full cache would cost
+# to read, so the capacities are large and the lengths need not be.
+WIDE = [(16, 32, 8, 128, 16416, 128), (24, 32, 8, 128, 11040, 128), (64, 16, 8, 128, 8320, 128),
+        (20, 64, 8, 128, 10304, 256), (64, 64, 8, 128, 3200, 256), (64, 4, 2, 64, 66560, 128),
+        (10, 16, 2, 64, 87296, 128), (33, 16, 2, 64, 45184, 256), (9, 32, 2, 64, 82016, 256)]
+
+
+def wide(c, group_rows):
+    """The call's row groups are the many-row kernel's, as the partials' size shows."""
+    rows = c.T * (c.nq // c.nkv)
+    a = capi.TreeAttnArgs.from_buffer_copy(c.a)
+    a.splits = 2
+    groups = -(-rows // group_rows)
+    return c.lib.tree_attn_workspace(a)[0] == 4 * c.B * c.nkv * 2 * groups * group_rows * (c.D + 2)
+
+
+@pytest.mark.parametrize("T,nq,nkv,D,cap,group_rows", WIDE)
+def test_attention_many_rows(lib, T, nq, nkv, D, cap, group_rows):
+    """Runs of no, one, two, an odd and an even number of blocks, shorter and
+    longer than the ring, ragged ends, one workgroup or several."""
+    for i, (L, splits) in enumerate([(0, 1), (1, 0), (32, 1), (33, 2), (255, 1), (256, 1), (290, 1), (320, 3), (700, 1),
+                                     (737, 1), (1500, 2), (2049, 5), (min(cap - T, 6000), 1), (cap - T, 0)]):
+        c = Attn(lib, [L], T, nq, nkv, D, ["holes", "random", "short", "star"][i % 4], splits=splits, seed=i, cap=cap)
+        assert wide(c, group_rows)
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("T,nq,nkv,cap,group_rows", [(40, 64, 8, 2560, 256), (40, 16, 8, 5600, 128), (9, 32, 8, 11008, 128)])
+def test_attention_many_rows_values_that_are_not_finite(lib, T, nq, nkv, cap, group_rows):
+    """As above: such a node reaches the rows that see it, and no other."""
+    par = ([-1, 0, 0, 1, 2, 0, 5, 3] + [7] * 64)[:T]
+
+    def call():
+        c = Attn(lib, [50, 0, 1000], T, nq, nkv, 128, "chain", splits=2, seed=4, cap=cap)
+        assert wide(c, group_rows)
+        c.trees = [par] * 3
+        c.parents.copy_(i32(c.trees))
+        return c, c.qkv.view(3, T, nq + 2 * nkv, 128)
+
+    c, x = call()
+    x[:, 2, nq + nkv:, 3] = float("inf")
+    x[:, 2, nq + nkv:, 4] = NAN
+    x[:, 5, nq:nq + nkv] = NAN
+    c.run()
+    torch.cuda.synchronize()
+    up = tree_oracle.ancestors(par)
+    sees2 = torch.tensor([2 in u for u in up], device=DEV)
+    sees5 = torch.tensor([5 in u for u in up], device=DEV)
+    rest = torch.ones(128, dtype=torch.bool, device=DEV)
+    rest[3:5] = False
+    got = c.rows()
+    assert got[:, sees5].isnan().all()
+    assert torch.isposinf(got[:, sees2][..., 3]).all() and got[:, sees2][..., 4].isnan().all()
+    ref, y = call()
+    y.copy_(x)
+    y[:, 2, nq + nkv:, 3:5] = 0
+    y[:, 5, nq:nq + nkv] = 1
+    ref.run()
+    torch.cuda.synchronize()
+    assert got[:, sees2][..., rest].isfinite().all() and got[:, ~sees2 & ~sees5].isfinite().all()
+    assert torch.equal(ref.rows()[:, ~sees2 & ~sees5], got[:, ~sees2 & ~sees5])
+    assert torch.equal(ref.rows()[:, sees2][..., rest], got[:, sees2][..., rest])
+
+
 @pytest.mark.parametrize("L", [-1, -(1 << 31), 57, 64, (1 << 31) - 1])
 @pytest.mark.parametrize("splits", [1, 4])
 def test_attention_invalid_length(lib, L, splits):

@@ -63,3 +63,10 @@ def test_nodes_per_sequence(batch):
     n = tree_nodes(batch)
     assert n == 0 or 2 <= n <= min(max_tree_nodes(batch), capi.TREE_MAX_T) and batch * n <= GEMM_MAX_ROWS
     assert 1 <= TREE_DEPTH < capi.TREE_MAX_T and 1 <= TREE_MATCHES <= capi.TREE_MAX_MATCHES
+
+
+def test_engine_speculation_modes():
+    from engine import speculation
+    assert [speculation(m) for m in (False, True, None, 1, "tree")] == [False, True, False, True, "tree"]
+    with pytest.raises(ValueError, match="speculate"):
+        speculation("chain")
