@@ -147,6 +147,30 @@ def test_long_walks(model, B, S, n, width):
         assert dec.last_stats["iterations"] <= -(-(n - 1) // per) + 1
 
 
+@pytest.mark.parametrize("B", [1, 3, 16, 32])
+def test_widest_trees(model, B):
+    """States of as many nodes as the GEMMs take: the known-answer checks, and
+    planted walks."""
+    from qdec import selfcheck
+    from qdec.runtime import DecodeState, max_tree_nodes
+    from qdec.tree import TreeDecoder
+    name, cfg, eng, ora = model
+    S, n, T = 24, 10, max_tree_nodes(B)
+    prompt = motif_prompts(cfg["vocab_size"], B, S, 55 + B)
+    eng.speculate = False
+    plain = list(eng.generate(prompt.tolist(), n))
+    st = DecodeState(eng.model, B, S + n + 2 * T, max_t=16, tree_t=T)
+    selfcheck.run_tree(st)
+    graphs, eng.use_graphs = eng.use_graphs, False
+    try:
+        dec = TreeDecoder(eng, st, 3, 2)
+        dec._draft = planted(dec, plain, S, 1 if T > 2 else 0)
+        steps = list(dec.generate(prompt, n, gate=False))
+    finally:
+        eng.use_graphs = graphs
+    check_prefix(judge(ora, prompt, steps), steps, plain)
+
+
 def test_iteration_captured_and_replayed(model):
     """One whole iteration as a graph, replayed with other work between,
     against eager iterations from the same start: every buffer bit for bit."""
