@@ -413,9 +413,9 @@ __device__ __forceinline__ void tree_nan_rows(const TreeAttnParams &p, int b, in
 // 32 rows' sums are 192).
 //
 // What bounds it: the cache read when it is long (MI355X, 32 x 4 nodes on 2000 to
-// 4224 slots, 16 query heads on 8: 75 us, 5.4 TB/s), else the chain of dependent
+// 4224 slots, 16 query heads on 8: 74 us, 5.5 TB/s), else the chain of dependent
 // loads before the first block (16 nodes on 640 slots: 8 us, 4 of them that; 64 nodes
-// on 4100: 23, at 10 TB/s from L2).
+// on 4100: 22, at 10 TB/s from L2).
 template <int D, int MT, int NT>
 struct NarrowLds {
   static constexpr int tail = 0;                            // node blocks in operand order
@@ -427,8 +427,10 @@ struct NarrowLds {
   static constexpr int bytes = q + (MT > 1 ? MT * (D / 32) * 2048 : 0);
 };
 
-template <int D, int MT, int NT>
-__global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(const TreeAttnParams p) {
+// 512 threads for the registers, as the wide kernel's (with accumulation registers
+// the two M tiles were 2% slower).
+template <int D, int MT, int NT, bool SHARED>
+__global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParams p) {
   using LY = NarrowLds<D, MT, NT>;
   constexpr int DS = D / 32, DT = D / 16, DTW = DT / kTW, RG = 16 * MT;
   __shared__ __align__(16) unsigned char smem[LY::bytes];
@@ -479,16 +481,21 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
   // Key rows of tile a: 8*(m >> 2) + (m & 3), of tile b 4 further, so that a
   // lane's 8 scores are 8 consecutive rows, the B operand of the P.V product.
   const int ra = 8 * (col >> 2) + (col & 3);
+  // A key load takes half a cache line per row and the next one the other half: it
+  // stays in the caches meanwhile.  A value load takes whole lines, which only other
+  // row groups (SHARED) read again.  us with non-temporal loads of neither / values only /
+  // both, on one cache again and again: 32 x 4 nodes on 2000 to 4224 slots, one row
+  // group, 79 / 66 / 75; 2 x 16 on 8300, two, 26 / 28 / 29.
   auto load_block = [&](int j, Frag &f) {
     const uint16_t *kp = kc + (size_t)(32 * j + ra) * D + 8 * grp;
     const uint16_t *vp = vc + ((size_t)(4 * j + grp) * D + col) * 8;
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
-      f.ka[s] = ld_nt(kp + s * 32);
-      f.kb[s] = ld_nt(kp + 4 * D + s * 32);
+      f.ka[s] = ld16(kp + s * 32);
+      f.kb[s] = ld16(kp + 4 * D + s * 32);
     }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) f.vf[dt] = ld_nt(vp + dt * 128);
+    for (int dt = 0; dt < DT; ++dt) f.vf[dt] = SHARED ? ld16(vp + dt * 128) : ld_nt(vp + dt * 128);
   };
   const int jc = min(j1, nb), ntb = max(j1 - nb, 0);  // the last split has the node blocks
   uint4 *tail = reinterpret_cast<uint4 *>(smem + LY::tail);
@@ -580,6 +587,7 @@ __global__ void __launch_bounds__(64 * kTW, MT == 1 ? 2 : 1) tree_narrow_kernel(
       sa[u] = sb[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < DS; ++s) {
+        if (MT > 1 && s % 2 == 0) __atomic_signal_fence(__ATOMIC_SEQ_CST);  // a few operands at a time (registers)
         const uint4 q = MT > 1 ? s_q[(2 * u * DS + s) * 64 + lane] : qf[s];
         const uint4 r = MT > 1 ? s_q[((2 * u + 1) * DS + s) * 64 + lane] : ql[s];
         sa[u] = mfma16x16x32(f.ka[s], r, sa[u]);
@@ -1120,13 +1128,15 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
   const dim3 grid((unsigned)(p.batch * p.nkv * p.groups * p.splits));
   const bool two = p.t_rows > 32;  // node blocks
   switch (p.group_rows) {
-    case 16:
-      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 2>), grid, dim3(64 * kTW), 0, s, p);
-      else hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 1>), grid, dim3(64 * kTW), 0, s, p);
+    case 16:  // more than 32 nodes are more than one group
+      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 2, true>), grid, dim3(64 * kTW), 0, s, p);
+      else if (p.groups > 1) hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 1, true>), grid, dim3(64 * kTW), 0, s, p);
+      else hipLaunchKernelGGL((tree_narrow_kernel<D, 1, 1, false>), grid, dim3(64 * kTW), 0, s, p);
       break;
-    case 32:
-      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 2>), grid, dim3(64 * kTW), 0, s, p);
-      else hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 1>), grid, dim3(64 * kTW), 0, s, p);
+    case 32:  // more than 32 nodes are more than one group
+      if (two) hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 2, true>), grid, dim3(64 * kTW), 0, s, p);
+      else if (p.groups > 1) hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 1, true>), grid, dim3(64 * kTW), 0, s, p);
+      else hipLaunchKernelGGL((tree_narrow_kernel<D, 2, 1, false>), grid, dim3(64 * kTW), 0, s, p);
       break;
     case 128:
       if (two) hipLaunchKernelGGL((tree_wide_kernel<D, 4, 2>), grid, dim3(256), 0, s, p);
@@ -1151,16 +1161,15 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 //
 // The narrow kernel reads the cache once per row group, from an L2 that its
 // groups share; the wide one once per 128 or 256 rows, but its pipeline takes
-// longer to fill.  The narrow one is ahead until its reads come to about 130 MB
-// (200 MB against 256 rows): narrow / wide, 32 nodes on 1100 slots (18 MB) 14 / 19,
-// 2 x 32 on 4200 (138 MB) 28 / 27, 4 x 16 on 8300 (272 MB) 47 / 42, 32 on 30000
-// (492 MB) 67 / 43; 64 nodes on 4200 (138 MB) 26.5 / 31, on 8300 (272 MB) 39 / 37, on
-// 30000 (980 MB) 106 / 61.
+// longer to fill.  The narrow one is ahead until its reads come to about 200 MB,
+// and with up to 64 rows always: narrow / wide, 2 x 32 nodes on 4200 slots (138 MB)
+// 26 / 26.5, on 8300 (272 MB) 37 / 33, 32 on 30000 (492 MB) 53 / 43; 64 nodes on 8300
+// (272 MB) 37 / 37.5, on 30000 (980 MB) 89 / 65; 4 x 16 nodes on 30000 118 / 119.
 //
 // 16 rows per workgroup give more workgroups, 32 half the reads.  16 where 32
 // would leave CUs idle and the reads are under 130 MB: 16 / 32 rows, 16 nodes on
-// 1100 slots (18 MB) 11.7 / 13.2, on 4200 (69 MB) 15.9 / 17.6, 2 x 16 nodes on 4200
-// (138 MB) 23.5 / 22.5, 32 nodes on 8300 (272 MB) 33 / 27, 16 on 30000 58 / 45.
+// 4100 slots (67 MB) 15.3 / 17.1, 32 on 2000 (65 MB) 15.4 / 15.9, on 4200 (138 MB)
+// 20.5 / 19.2, 2 x 16 on 4200 (138 MB) 21.9 / 20.4.
 //
 // One workgroup per CU, none of fewer than four blocks of a full cache: more
 // splits read no faster and merge more (16 nodes on 4100 slots, 4 / 8 / 16 / 32
@@ -1170,7 +1179,7 @@ void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int64_t cells = (int64_t)p->batch * p->nkv;
   const int blocks = p->cap / 32;
   const int64_t cache = cells * p->cap * p->head_dim * 4;  // bytes of both caches
-  if (rows > 32 && cache * ((rows + 31) / 32) > (rows <= 128 ? 130000000 : 200000000))
+  if (rows > 64 && cache * ((rows + 31) / 32) > 200000000)
     p->group_rows = rows <= 128 ? 128 : 256;
   else
     p->group_rows = rows <= 16 || (cells * tiles < 128 && cache * tiles < 130000000) ? 16 : 32;

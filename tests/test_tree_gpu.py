@@ -290,9 +290,9 @@ def test_attention_values_that_are_not_finite_stay_in_their_branch(lib):
 # Shapes of the many-row kernel: 128 or 256 query rows per workgroup, up to 32 or
 # up to 64 nodes, both head sizes; it takes over by what a full cache would cost
 # to read, so the capacities are large and the lengths need not be.
-WIDE = [(16, 32, 8, 128, 16416, 128), (24, 32, 8, 128, 11040, 128), (64, 16, 8, 128, 8320, 128),
-        (20, 64, 8, 128, 10304, 256), (64, 64, 8, 128, 3200, 256), (64, 4, 2, 64, 66560, 128),
-        (10, 16, 2, 64, 87296, 128), (33, 16, 2, 64, 45184, 256), (9, 32, 2, 64, 82016, 256)]
+WIDE = [(17, 32, 8, 128, 16416, 128), (27, 32, 8, 128, 12256, 128), (64, 16, 8, 128, 12256, 128),
+        (20, 64, 8, 128, 10304, 256), (64, 64, 8, 128, 3200, 256), (64, 4, 2, 64, 97728, 128),
+        (10, 16, 2, 64, 130400, 128), (33, 16, 2, 64, 45184, 256), (9, 32, 2, 64, 82016, 256)]
 
 
 def wide(c, group_rows):
@@ -316,7 +316,7 @@ def test_attention_many_rows(lib, T, nq, nkv, D, cap, group_rows):
         c.check()
 
 
-@pytest.mark.parametrize("T,nq,nkv,cap,group_rows", [(40, 64, 8, 2560, 256), (40, 16, 8, 5600, 128), (9, 32, 8, 11008, 128)])
+@pytest.mark.parametrize("T,nq,nkv,cap,group_rows", [(40, 64, 8, 2560, 256), (40, 16, 8, 5600, 128), (17, 32, 8, 5600, 128)])
 def test_attention_many_rows_values_that_are_not_finite(lib, T, nq, nkv, cap, group_rows):
     """As above: such a node reaches the rows that see it, and no other."""
     par = ([-1, 0, 0, 1, 2, 0, 5, 3] + [7] * 64)[:T]
