@@ -386,10 +386,17 @@ __device__ __forceinline__ void tree_store(const TreeAttnParams &p, int b, int t
   *reinterpret_cast<uint2 *>(tree_out(p, b * p.t_rows + t, hq * p.head_dim + ch)) = v;
 }
 // The partial of a unit's row group: acc [RG][D], m [RG], l [RG], with m = -inf
-// and l = 0 where a row saw nothing or holds no node.
+// and l = 0 where a row holds no node.
 template <int D>
 __device__ __forceinline__ float *tree_part(const TreeAttnParams &p, int unit, int g) {
   return p.partial + ((size_t)unit * p.groups + g) * ((size_t)p.group_rows * (D + 2));
+}
+
+// The sum of a partial: not 0 for a node, whatever it saw (scores of -inf only have
+// the sum 0, weight 0 beside others and a NaN result by themselves).
+__device__ __forceinline__ float part_sum(bool node, float m, float l) {
+  if (!node) return 0.f;
+  return m == -__builtin_huge_valf() && l == 0.f ? 1.f : l;
 }
 
 // The rows r0 .. r0 + rows - 1 of a sequence whose length is out of range.
@@ -691,7 +698,7 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
     }
     if (n_active > 1 && wave == 0 && grp == 0 && r < rows) {
       part[(size_t)RG * D + r] = node ? M : NEG_INF;
-      part[(size_t)RG * D + RG + r] = node ? l : 0.f;
+      part[(size_t)RG * D + RG + r] = part_sum(node, M, l);
     }
   }
 }
@@ -1069,7 +1076,7 @@ __global__ void __launch_bounds__(512, 2) tree_wide_kernel(const TreeAttnParams 
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + dt * 16 + grp * 4) = acc[u][dt];
       if (grp == 0) {
         part[(size_t)RG * D + r] = node ? m_run[u] : NEG_INF;
-        part[(size_t)RG * D + RG + r] = node ? l : 0.f;
+        part[(size_t)RG * D + RG + r] = part_sum(node, m_run[u], l);
       }
     }
   }
@@ -1093,6 +1100,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p)
   const size_t stride = (size_t)p.nkv * p.groups * RG * (D + 2);  // to the next workgroup's
   const float scale = p.scale_log2;
   float M = -__builtin_huge_valf(), l = 0.f;
+  bool node = false;
   f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < n; i0 += 8) {
     float mi[8], li[8];
@@ -1116,11 +1124,12 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p)
       const float w = tree_weight(mi[i], li[i], Mn, scale);
       l += li[i] * w;
       o += a[i] * w;
+      node |= li[i] != 0.f;
     }
     M = Mn;
   }
   const int t = div_by(p.by_g, r);
-  tree_store(p, b, t, kvh * G + r - t * G, ch, o, 1.f / l, l != 0.f);  // (a node's sum is not 0)
+  tree_store(p, b, t, kvh * G + r - t * G, ch, o, 1.f / l, node);
 }
 
 template <int D>

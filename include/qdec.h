@@ -505,7 +505,8 @@ int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
  *   k and the raw v go to k_nodes / v_nodes ([batch][nkv][t_rows][head_dim]).
  * The cache is only read: qdec_tree_commit appends what was accepted.  What a
  * row does not see (other branches, slots from lens[b] on) does not reach it,
- * whatever it holds, NaN and infinities included.
+ * whatever it holds, NaN and infinities included.  Cached keys and values that a
+ * row does see are taken to be finite: infinite ones come out as NaN.
  * A row that holds no node: out is zero, its k_nodes / v_nodes are left as
  * they were.  A length with lens[b] < 0 or lens[b] + t_rows > cap reads and
  * writes no cache or node memory; the rows of sequence b become NaN.

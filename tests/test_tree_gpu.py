@@ -353,6 +353,33 @@ def test_attention_many_rows_values_that_are_not_finite(lib, T, nq, nkv, cap, gr
     assert torch.equal(ref.rows()[:, sees2][..., rest], got[:, sees2][..., rest])
 
 
+@pytest.mark.parametrize("T,nq,nkv,cap", [(4, 8, 2, 512), (40, 8, 2, 512), (64, 64, 8, 6304)])
+@pytest.mark.parametrize("splits", [1, 2, 3])
+def test_attention_scores_that_overflow(lib, T, nq, nkv, cap, splits):
+    """Every score between nodes is -inf.  Beside cached keys of score 0 a node has
+    weight 0 and a row is the mean of the cached values; with scores of -inf
+    everywhere it is NaN, as the softmax is, in one split as in several."""
+    c = Attn(lib, [300], T, nq, nkv, 128, "holes", splits=splits, seed=T, cap=cap)
+    c.qkv.view(T, nq + 2 * nkv, 128)[c.live, :nq + nkv] = 1
+    c.qn.fill_(1e20)
+    c.kn.fill_(-1e20)
+    c.cos.fill_(1)
+    c.sin.fill_(0)
+    c.k[:, :, :300] = 0
+    c.run()
+    torch.cuda.synchronize()
+    got = c.rows()[0].double()
+    v = c.v_rows[0, :, :300].double()
+    ref = v.mean(1).repeat_interleave(nq // nkv, 0)
+    mag = v.abs().mean(1).repeat_interleave(nq // nkv, 0)
+    assert (got[~c.live] == 0).all()
+    assert ((got[c.live] - ref).abs() <= bound(ref, mag, 300, T)).all()
+    c.k[:, :, :300] = -1e20
+    c.run()
+    torch.cuda.synchronize()
+    assert c.rows()[0][c.live].isnan().all() and (c.rows()[0][~c.live] == 0).all()
+
+
 @pytest.mark.parametrize("L", [-1, -(1 << 31), 57, 64, (1 << 31) - 1])
 @pytest.mark.parametrize("splits", [1, 4])
 def test_attention_invalid_length(lib, L, splits):
