@@ -27,7 +27,7 @@ __device__ __forceinline__ int64_t lane_i64(int64_t v, int l) {
 //   3. The first wave builds the tree with one lane per node: a token's child
 //      is found by one ballot.
 // What bounds it: a history of 20K tokens is 160 KB through one CU.  MI355X: 16
-// histories of 8000 to 32000 tokens 16.6 us (36 with every position's pattern read
+// histories of 8000 to 32000 tokens 15.6 us (36 with every position's pattern read
 // from memory), one of 600 tokens 3.6.
 constexpr int kDraftThreads = 1024;
 constexpr int kDraftU = 8;
@@ -69,17 +69,25 @@ __global__ void __launch_bounds__(kDraftThreads) tree_draft_kernel(const qdec_tr
     if (s_found[0] == M && s_found[1] == M) break;
     if (top >= kDraftWindow) load(top - kDraftWindow);
     const int64_t newest = s_pat[0];
+    uint64_t last[kDraftU];  // the newest token itself: most waves go no further
+#pragma unroll
+    for (int u = 0; u < kDraftU; ++u) {
+      const int q = u * kDraftThreads + tid;
+      last[u] = __ballot(q <= top && s_tok[q] == newest);
+    }
 #pragma unroll
     for (int u = 0; u < kDraftU; ++u) {
       const int q = u * kDraftThreads + tid, e = top - q;
-      const bool last = e >= 0 && s_tok[q] == newest;
+      uint64_t hit[2] = {0, 0};
+      if (last[u]) {
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        bool ok = last && e >= ngram[w] - 1;
-        for (int i = 1; i < ngram[w] && ok; ++i) ok = s_tok[q + i] == s_pat[i];
-        const uint64_t hit = __ballot(ok);
-        if (lane == 0) s_hit[w][u * NW + wave] = hit;
+        for (int w = 0; w < 2; ++w) {
+          bool ok = ((last[u] >> lane) & 1) && e >= ngram[w] - 1;
+          for (int i = 1; i < ngram[w] && ok; ++i) ok = s_tok[q + i] == s_pat[i];
+          hit[w] = __ballot(ok);
+        }
       }
+      if (lane < 2) s_hit[lane][u * NW + wave] = lane ? hit[1] : hit[0];
     }
     __syncthreads();
     if (wave < 2) {  // word k: window positions (k / NW) * 1024 + (k % NW) * 64 + bit
