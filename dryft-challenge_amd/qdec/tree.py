@@ -42,9 +42,9 @@ from .runtime import max_tree_nodes
 from .spec import AcceptancePredictor, NgramIndex, SpecDecoder
 
 # Rows of a tree pass, all sequences together.  Qwen3-4B's size, 1024 cached
-# slots, batch 1 / 4 / 8, ms per iteration: plain 2.15 / 2.31 / 2.51, 16 rows 2.76 /
-# 2.82 / 2.87, 32 rows 3.10 / 3.15 / 3.17, 48 rows 3.60 / 3.66 / 3.72, 64 rows 3.95 /
-# 4.00 / 4.09: the second 16 rows cost 11%, the next ones 16% and 10%.
+# slots, batch 1 / 4 / 8, ms per iteration: plain 2.15 / 2.31 / 2.51, 16 rows 2.75 /
+# 2.83 / 2.95, 32 rows 3.07 / 3.21 / 3.23, 48 rows 3.50 / 3.63 / 3.76, 64 rows 3.91 /
+# 4.03 / 4.14: the second 16 rows cost 12%, the next ones 14% and 11%.
 TREE_ROWS = 32
 TREE_DEPTH = 8      # tokens taken from one earlier occurrence
 TREE_MATCHES = 8    # earlier occurrences per pattern
