@@ -187,9 +187,10 @@ template <int D>
 __global__ void __launch_bounds__(256) tree_commit_kernel(const qdec_tree_commit_args p) {
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int T = p.t_rows;
-  const int a = p.naccept[b], n = a + 1, L = p.lens[b];
+  const int a = p.naccept[b], L = p.lens[b];
   const int *path = p.path + (size_t)b * T;
-  if (a < 0 || a >= T || L < n || L > p.cap || path[0] != 0) return;
+  if (a < 0 || a >= T || L <= a || L > p.cap || path[0] != 0) return;
+  const int n = a + 1;
   const int lane = threadIdx.x & 63;
   const int node = lane < n ? path[lane] : 0;  // every wave holds the path
   if (__any(node < 0 || node >= T)) return;

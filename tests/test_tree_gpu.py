@@ -618,7 +618,7 @@ def test_commit(lib, T, nkv, D, layers):
         seqs.append((rnd.randint(n, cap) if i > 1 else (n if i else cap), [0] + sorted(rnd.sample(range(1, T), n - 1)), n - 1))
     seqs += [(40, [-1] * T, 0),  # frozen
              (40, [0, T][:T], min(1, T - 1)) if T > 1 else (40, [-1], 0), (40, [0, -2][:T] if T > 1 else [-1], min(1, T - 1)),
-             (cap + 1, [0], 0), (0, [0], 0), (-(1 << 31), [0], 0), ((1 << 31) - 1, [0], 0), (40, list(range(T)), T), (40, [0], -1), (40, [1] if T > 1 else [-1], 0)]
+             (cap + 1, [0], 0), (0, [0], 0), (-(1 << 31), [0], 0), ((1 << 31) - 1, [0], 0), (40, list(range(T)), T), (40, [0], (1 << 31) - 1), (40, [0], -1), (40, [1] if T > 1 else [-1], 0)]
     B = len(seqs)
     kn, vn = (torch.randn((layers, B, nkv, T, D), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
     k = torch.randn((layers, B, nkv, cap, D), generator=g, device=DEV).to(torch.bfloat16)
