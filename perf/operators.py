@@ -292,10 +292,9 @@ def _prepare_own(st):
         if k in fields:
             setattr(a, k, v)
     if c["kind"] == "attn":
-        pb, cb = lib.tree_attn_workspace(a)
+        pb, _ = lib.tree_attn_workspace(a)  # no counters
         st["partial"] = torch.zeros((max(pb, 16) // 4,), dtype=torch.float32, device=DEV)
-        st["counters"] = torch.zeros((max(cb, 4) // 4,), dtype=torch.int32, device=DEV)
-        a.partial, a.counters = st["partial"].data_ptr(), st["counters"].data_ptr()
+        a.partial = st["partial"].data_ptr()
     st["args"] = a
 
 
