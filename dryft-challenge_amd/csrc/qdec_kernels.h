@@ -286,11 +286,11 @@ struct TreeAttnParams {
   float eps;
   float scale_log2;  // log2(e) / sqrt(head_dim)
   int batch, t_rows, nq, nkv, head_dim, cap;
-  int splits;      // workgroups per (sequence, kv head, row group), on average
+  int splits;      // workgroups per (sequence, kv head, row group), at most
   int min_blocks;  // 32-row blocks a workgroup gets before another one is used
   int group_rows;  // query rows a workgroup takes: 16, 32, 128 or 256
   int groups;      // row groups: ceil(t_rows * nq / nkv / group_rows)
-  FastDiv by_groups, by_nkv, by_g;  // g: query heads per kv head
+  FastDiv by_groups, by_nkv, by_splits, by_g;  // g: query heads per kv head
   int ofrag;       // > 0: out is written in fragment order with this many M tiles
 };
 void tree_attn_plan(TreeAttnParams *p, int splits);

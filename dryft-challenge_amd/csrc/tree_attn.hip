@@ -133,66 +133,26 @@ __device__ __forceinline__ bool finite8(const uint4 &v) {
 
 __device__ __forceinline__ int div_by(const FastDiv &d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
 
-// The splits are dealt to the sequences in proportion to their blocks, so that
-// the workgroups' runs are about equal in a batch of unequal lengths: of a kv
-// head's batch * splits workgroups, sequence b's are first .. first + n - 1.
-struct TreeDeal {
-  int b, L, n, first;  // n = 0: a workgroup that is left over
-};
 __device__ __forceinline__ bool tree_valid(const TreeAttnParams &p, int L) { return L >= 0 && L <= p.cap - p.t_rows; }
-// Blocks of a sequence of L slots (one where L is out of range).
-__device__ __forceinline__ int tree_weight_of(const TreeAttnParams &p, int L) {
-  return tree_valid(p, L) ? ((L + 31) >> 5) + kTailWeight * ((p.t_rows + 31) >> 5) : 1;
-}
-// Sequence b's workgroups end at E(b) = b + 1 + round(W(b) * batch * (splits - 1)
-// / W(batch - 1)), W the running sum of the weights: one each, the others in
-// proportion, batch * splits in all however the quotient rounds (it never
-// falls as W grows).  A split that would get fewer than `least` blocks is left
-// out; least >= kTailWeight per node block keeps the splits before the last
-// one from being empty.
-template <bool BY_SEQ>  // at = a sequence, else a workgroup
-__device__ __forceinline__ TreeDeal tree_deal(const TreeAttnParams &p, int at) {
-  const int B = p.batch, S = p.splits, lane = threadIdx.x & 63;
-  if (S == 1) return TreeDeal{at, p.lens[at], 1, at};
-  const int least = max(p.min_blocks, kTailWeight * ((p.t_rows + 31) >> 5));
-  auto active = [&](int w, int n) { return w < 2 * least ? 1 : min(n, w / least); };
-  if (B == 1) {
-    const int L = p.lens[0], n = active(tree_weight_of(p, L), S);
-    return TreeDeal{0, L, BY_SEQ || at < n ? n : 0, 0};
-  }
-  int total = 0;
-  for (int b0 = 0; b0 < B; b0 += 64)
-    total += __builtin_amdgcn_readlane(wave_scan(b0 + lane < B ? tree_weight_of(p, p.lens[min(b0 + lane, B - 1)]) : 0), 63);
-  const int spare = B * (S - 1);
-  const float ratio = (float)spare / (float)total;
-  int sum = 0, base = 0;  // weights and workgroups of the 64s before
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane, L = p.lens[min(b, B - 1)], w = b < B ? tree_weight_of(p, L) : 0;
-    const int W = sum + wave_scan(w);
-    const int end = min(b, B - 1) + 1 + min(spare, (int)((float)W * ratio + 0.5f));
-    int hit = at - b0;
-    if constexpr (!BY_SEQ) {
-      const uint64_t m = __ballot(end > at);
-      hit = m ? __builtin_ctzll(m) : 64;
-    }
-    if (hit < 64) {
-      hit = __builtin_amdgcn_readfirstlane(hit);
-      const int first = hit > 0 ? __builtin_amdgcn_readlane(end, max(hit - 1, 0)) : base;
-      const int n = active(__builtin_amdgcn_readlane(w, hit), __builtin_amdgcn_readlane(end, hit) - first);
-      return TreeDeal{b0 + hit, __builtin_amdgcn_readlane(L, hit), BY_SEQ || at - first < n ? n : 0, first};
-    }
-    sum = __builtin_amdgcn_readlane(W, 63);
-    base = __builtin_amdgcn_readlane(end, 63);
-  }
-  return TreeDeal{0, 0, 0, 0};
+// Workgroups that share a sequence of L slots: `splits`, or fewer where they
+// would get less than `least` blocks each (>= kTailWeight per node block, so that
+// none before the last is empty); one where L is out of range.  The other
+// sequences' lengths do not count, so that they do not move this one's sums.  us,
+// this / the batch's splits dealt by the sequences' lengths: 8 x 8 nodes on 0 to
+// 1600 slots, 32 query heads on 8, 17.4 / 17.4; 4 x 8 on 0 to 4000 18.5 / 19.0;
+// 2 x 16 on 0 and 8000 22.6 / 21.3; 4 x 32 on 0 to 15000, 64 heads, 83 / 68.
+__device__ __forceinline__ int tree_active(const TreeAttnParams &p, int L) {
+  const int tail = kTailWeight * ((p.t_rows + 31) >> 5), least = max(p.min_blocks, tail);
+  const int blocks = tree_valid(p, L) ? ((L + 31) >> 5) + tail : 1;
+  return blocks < 2 * least ? 1 : min(p.splits, blocks / least);
 }
 
-// A workgroup's place: row group g of unit = w * nkv + kvh, w its number among
-// the kv head's.  The row groups of one unit read the same keys and values:
+// A workgroup's place: row group g of unit = (b * splits + c) * nkv + kvh, split c
+// of sequence b.  The row groups of one unit read the same keys and values:
 // they get numbers that are equal modulo 8, the number of XCDs, and close
 // together, so that they share an L2.
 struct TreeUnit {
-  int unit, w, g, kvh;
+  int unit, b, c, g, kvh;
 };
 __device__ __forceinline__ TreeUnit tree_unit(const TreeAttnParams &p) {
   const int ng = p.groups, x = blockIdx.x, whole = (p.batch * p.nkv * p.splits) & ~7;
@@ -205,8 +165,10 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeAttnParams &p) {
     r.g = y - q * ng;
     r.unit = main ? q * 8 + (x & 7) : whole + q;
   }
-  r.w = div_by(p.by_nkv, r.unit);
-  r.kvh = r.unit - r.w * p.nkv;
+  const int w = div_by(p.by_nkv, r.unit);
+  r.kvh = r.unit - w * p.nkv;
+  r.b = div_by(p.by_splits, w);
+  r.c = w - r.b * p.splits;
   return r;
 }
 
@@ -449,9 +411,8 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
   const int col = lane & 15, grp = lane >> 4;
 
   const TreeUnit u_ = tree_unit(p);
-  const TreeDeal deal = tree_deal<false>(p, u_.w);
-  if (deal.n == 0) return;
-  const int kvh = u_.kvh, g = u_.g, b = deal.b, L = deal.L, n_active = deal.n, c = u_.w - deal.first;
+  const int kvh = u_.kvh, g = u_.g, b = u_.b, c = u_.c, L = p.lens[b], n_active = tree_active(p, L);
+  if (c >= n_active) return;
   const int cell = b * p.nkv + kvh;
   const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d;
   const int r0 = g * RG, rows = min(RG, T * G - r0);
@@ -757,9 +718,8 @@ __global__ void __launch_bounds__(512, 2) tree_wide_kernel(const TreeAttnParams 
   const int col = lane & 15, grp = lane >> 4;
 
   const TreeUnit u_ = tree_unit(p);
-  const TreeDeal deal = tree_deal<false>(p, u_.w);
-  if (deal.n == 0) return;
-  const int kvh = u_.kvh, g = u_.g, b = deal.b, L = deal.L, n_active = deal.n, c = u_.w - deal.first;
+  const int kvh = u_.kvh, g = u_.g, b = u_.b, c = u_.c, L = p.lens[b], n_active = tree_active(p, L);
+  if (c >= n_active) return;
   const int cell = b * p.nkv + kvh;
   const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d;
   const int R = T * G, r0 = g * RG;
@@ -1091,12 +1051,11 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p)
   const int per = (R + 256 / TR - 1) / (256 / TR);  // workgroups per (sequence, kv head)
   const int cell = blockIdx.x / per, b = div_by(p.by_nkv, cell), kvh = cell - b * p.nkv;
   const int r = (blockIdx.x - cell * per) * (256 / TR) + threadIdx.x / TR;
-  const TreeDeal deal = tree_deal<true>(p, b);
-  const int n = deal.n;
+  const int n = tree_active(p, p.lens[b]);
   // one split: written by its workgroup, as the rows of a length out of range
-  if (n == 1 || !tree_valid(p, deal.L) || r >= R) return;
+  if (n == 1 || r >= R) return;
   const int g = r / RG, rg = r - g * RG, ch = (int)(threadIdx.x % TR) * 4;
-  const float *part = tree_part<D>(p, deal.first * p.nkv + kvh, g);
+  const float *part = tree_part<D>(p, b * p.splits * p.nkv + kvh, g);
   const size_t stride = (size_t)p.nkv * p.groups * RG * (D + 2);  // to the next workgroup's
   const float scale = p.scale_log2;
   float M = -__builtin_huge_valf(), l = 0.f;
@@ -1202,6 +1161,7 @@ void tree_attn_plan(TreeAttnParams *p, int splits) {
   p->splits = std::min(splits, 256);
   p->by_groups = fast_div(p->groups);
   p->by_nkv = fast_div(p->nkv);
+  p->by_splits = fast_div(p->splits);
   p->by_g = fast_div(p->nq / p->nkv);
 }
 
