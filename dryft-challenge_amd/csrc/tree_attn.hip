@@ -207,6 +207,15 @@ __device__ __forceinline__ uint64_t tree_ancestors(int up, int T, int lane) {
 // carry as well as those below 1, and the sums are rescaled in a few of the
 // first blocks only.
 constexpr float kMaxSlack = 8.f;
+// Moves a row's running maximum m to a block's maximum `top` if that exceeds it by
+// the slack (only then, so that no other row of the wave decides where this one
+// rescales) and returns the factor of its sums.
+__device__ __forceinline__ float raise_max(float &m, float top, float slack, float scale) {
+  if (!(top > m + slack)) return 1.f;
+  const float alpha = __builtin_amdgcn_exp2f((m - top) * scale);
+  m = top;
+  return alpha;
+}
 
 // Weight of a part in a merge: its sum times zero where it saw nothing, so that
 // a NaN among its scores stays.
@@ -581,10 +590,8 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
       const float bmax = fmaxf(fmaxf(fmaxf(sa[u][0], sa[u][1]), fmaxf(sa[u][2], sa[u][3])),
                                fmaxf(fmaxf(sb[u][0], sb[u][1]), fmaxf(sb[u][2], sb[u][3])));
       if (__any(bmax > m_run[u] + slack)) {
-        const float m_new = fmaxf(m_run[u], max_xor16_32(bmax));
-        const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
+        const float alpha = raise_max(m_run[u], max_xor16_32(bmax), slack, scale);
         l_run[u] *= alpha;
-        m_run[u] = m_new;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[u][dt] *= alpha;
       }
@@ -884,10 +891,8 @@ __global__ void __launch_bounds__(512, 2) tree_wide_kernel(const TreeAttnParams 
     if (__builtin_expect(__any(S.mx[0] > m_run[0] + slack || S.mx[1] > m_run[1] + slack), 0)) {
 #pragma unroll
       for (int u = 0; u < MT; ++u) {
-        const float m_new = fmaxf(m_run[u], max_xor16_32(S.mx[u]));
-        const float alpha = m_new == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m_run[u] - m_new) * scale);
+        const float alpha = raise_max(m_run[u], max_xor16_32(S.mx[u]), slack, scale);
         l_run[u] *= alpha;
-        m_run[u] = m_new;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[u][dt] *= alpha;
       }

@@ -1,5 +1,7 @@
-"""What a result of the tree attention depends on: the splits, its sequence's
-length and the call's shape.  The other sequences' lengths do not move its bits."""
+"""What a result of the tree attention depends on: a row's bits follow from its
+own query, what it sees, the splits, its sequence's length and the call's shape.
+Neither the other sequences' lengths nor the other rows of its own sequence
+move them."""
 
 import pytest
 import torch
@@ -45,3 +47,26 @@ def test_other_lengths_move_nothing(lib, T, nq, nkv, D, cap, splits, rows, at): 
     for s in seen[1:]:
         for x, y in zip(seen[0], s):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("T,nq,nkv,D,cap,splits,rows", [(3, 8, 2, 128, 4096, 1, 16), (4, 8, 8, 64, 4096, 2, 16),
+                                                        (16, 32, 8, 128, 2080, 1, 32), (27, 32, 8, 128, 12256, 2, 128),
+                                                        (64, 64, 8, 128, 3200, 1, 256)])
+def test_other_rows_move_nothing(lib, T, nq, nkv, D, cap, splits, rows):  # noqa: F811
+    """The last node's query changes: only its own rows do.  Scores of the cache
+    grow with the slot, by more than the running maximum's slack again and again,
+    at different slots for different rows."""
+    L = 1500
+    c = Attn(lib, [L] * 4, T, nq, nkv, D, "star", splits=splits, cap=cap, seed=D + T)
+    assert group_rows(c, rows)
+    c.k[:, :, :L] *= torch.linspace(0.1, 6, L, device=DEV)[None, None, :, None].to(torch.bfloat16)
+    x = c.qkv.view(4, T, nq + 2 * nkv, D)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    seen = []
+    for _ in range(6):
+        c.run()
+        c.check()
+        seen.append(bits(c.rows()[:, :T - 1]))
+        x[:, T - 1, :nq] = torch.randn((4, nq, D), generator=g, device=DEV).sign().to(torch.bfloat16)
+    for s in seen[1:]:
+        assert torch.equal(seen[0][0], s[0])
