@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "qdec_common.h"
@@ -837,6 +838,10 @@ static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool 
   if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->parents ||
       !a->k_cache || !a->v_cache || !a->k_nodes || !a->v_nodes || !a->out)
     return set_error(QDEC_EINVAL, "qdec_tree_attn: null pointer argument");
+  // The running maximum moves in steps of kTreeMaxSlack / scale.
+  if (!(p->scale_log2 > 0.f) || !std::isfinite(p->scale_log2) || !std::isfinite(kTreeMaxSlack / p->scale_log2))
+    return set_error(QDEC_EINVAL, "qdec_tree_attn: sm_scale %g is not positive, or it or its reciprocal leaves fp32's range",
+                     (double)a->sm_scale);
   if (p->splits > 1 && !a->partial) return set_error(QDEC_EINVAL, "qdec_tree_attn: more than one split needs partial");
   if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
       !aligned16(a->sin_tab) || !aligned16(a->k_cache) || !aligned16(a->v_cache) || !aligned16(a->k_nodes) ||

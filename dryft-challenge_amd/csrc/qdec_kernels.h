@@ -268,6 +268,7 @@ hipError_t launch_accept(const int64_t *out_tok, const int64_t *draft, int64_t *
 // ---- tree speculation (tree.hip, tree_attn.hip)
 constexpr int kTreeMaxT = QDEC_TREE_MAX_T;
 constexpr int kTreeMaxMatches = QDEC_TREE_MAX_MATCHES;
+constexpr float kTreeMaxSlack = 8.f;  // by which scores exceed their running maximum before it moves, in powers of 2
 // n / d for 0 <= n < 2^31 as one multiplication and a shift.
 struct FastDiv {
   uint32_t d, mul, shift;

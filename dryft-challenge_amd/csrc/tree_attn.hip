@@ -202,11 +202,10 @@ __device__ __forceinline__ uint64_t tree_ancestors(int up, int T, int lane) {
   return (anc & 1) && lane < T ? anc : 0;
 }
 
-// The running maximum only moves when a score exceeds it by kMaxSlack / scale:
-// probabilities then stay below 2^kMaxSlack, which fp32 sums and bf16 operands
+// The running maximum only moves when a score exceeds it by kTreeMaxSlack / scale:
+// probabilities then stay below 2^kTreeMaxSlack, which fp32 sums and bf16 operands
 // carry as well as those below 1, and the sums are rescaled in a few of the
 // first blocks only.
-constexpr float kMaxSlack = 8.f;
 // Moves a row's running maximum m to a block's maximum `top` if that exceeds it by
 // the slack (only then, so that no other row of the wave decides where this one
 // rescales) and returns the factor of its sums.
@@ -530,7 +529,7 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
     for (int dt = 0; dt < DT; ++dt) acc[u][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   const float scale = p.scale_log2;
-  const float slack = kMaxSlack / scale;
+  const float slack = kTreeMaxSlack / scale;
 
   // Block j, from the cache or (NODES) of nodes.
   auto process = [&](Frag &f, int j, auto nodesc) {
@@ -864,7 +863,7 @@ __global__ void __launch_bounds__(512, 2) tree_wide_kernel(const TreeAttnParams 
   int issued = RING - 1;  // the newest block asked for, if there is one
   read_k(min(1, n - 1));
 
-  const float scale = p.scale_log2, slack = kMaxSlack / scale;
+  const float scale = p.scale_log2, slack = kTreeMaxSlack / scale;
   // AHEAD: 2 or 3, the workgroup meets and blocks up to jj + AHEAD are in LDS
   // after that; 0, the last meeting covers this block; -1, the last block.
   // INNER: blocks up to jj + RING are whole ones from the cache and the last

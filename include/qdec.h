@@ -530,7 +530,7 @@ typedef struct {
   void *out;              /* [batch*t_rows, nq*head_dim] bf16 */
   float *partial;         /* split partials, 16-byte aligned (qdec_tree_attn_workspace) */
   float eps;
-  float sm_scale;         /* 1/sqrt(head_dim) */
+  float sm_scale;         /* 1/sqrt(head_dim); positive */
   int32_t batch;
   int32_t t_rows;         /* 1..64 */
   int32_t nq;             /* a multiple of nkv, at most 16 per kv head */
