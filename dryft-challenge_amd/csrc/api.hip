@@ -830,8 +830,11 @@ static int plan_tree_attn(const qdec_tree_attn_args *a, TreeAttnParams *p, bool 
   p->head_dim = a->head_dim; p->cap = a->cap;
   p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
   tree_attn_plan(p, a->splits);
-  // workgroups of the launches (at most 128 per cell in the merge), numbered in 31 bits
-  if ((int64_t)p->batch * p->nkv * std::max(p->groups * p->splits, 128) > 0x7fffffff)
+  // A launch's work items are numbered in 32 bits.
+  const int rows = p->t_rows * (p->nq / p->nkv), per = 1024 / p->head_dim;  // rows of a merge workgroup
+  const int64_t items = std::max(p->groups * p->splits * (p->group_rows == 256 ? 512 : 256),
+                                 p->splits > 1 ? (rows + per - 1) / per * 256 : 0);
+  if ((int64_t)p->batch * p->nkv * items > 0xffffffffll)
     return set_error(QDEC_EUNSUPPORTED, "qdec_tree_attn: batch %d x nkv %d x %d row groups x %d splits", p->batch,
                      p->nkv, p->groups, p->splits);
   if (!need_scratch) return QDEC_OK;
