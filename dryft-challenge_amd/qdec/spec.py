@@ -156,7 +156,7 @@ class SpecDecoder:
         self.hist = torch.zeros((state.batch, state.cap), dtype=torch.int64, device=state.model.device)
         self.graphs = {}       # k -> graph, for the current stop length
         self.graph_stop = None
-        self.cost_ratio = None  # time of a verify iteration / a k = 0 iteration
+        self.cost_ratio = None  # cost of a verify iteration / a k = 0 iteration; None: to be timed
         self.last_stats = {}
 
     def _buffers(self):

@@ -24,13 +24,13 @@ rounds a node's key once where the plain step rounds it where the reference
 does, and its attention sums in its own order, so at a near-tie the pick may
 differ from the plain step's, as between two batch sizes of most engines; the
 chain of ``qdec.spec`` is the mode that reproduces the plain stream bit for
-bit.  With the gate the choice between the two kinds of iteration depends on a
-measured time; without it a run repeats its tokens.
+bit.  Which kind of iteration runs follows from the tokens and the shape
+(``tree_cost``), never from a clock: the same call gives the same tokens every time.
 
 The acceptance gate is ``qdec.spec``'s: the drafter's rule restated on the host
 (``TreeIndex``) scores every position with what a tree pass there would have
-emitted, and tree passes run while that beats their measured cost; otherwise a
-plain step keeps the history.
+emitted, and tree passes run while that beats their cost; otherwise a plain step
+keeps the history.
 """
 
 import bisect
@@ -38,7 +38,7 @@ import bisect
 import torch
 
 from . import capi
-from .runtime import max_tree_nodes
+from .runtime import GEMM_MAX_ROWS, max_tree_nodes
 from .spec import AcceptancePredictor, NgramIndex, SpecDecoder
 
 # Rows of a tree pass, all sequences together.  Qwen3-4B's size, 1024 cached
@@ -48,6 +48,22 @@ from .spec import AcceptancePredictor, NgramIndex, SpecDecoder
 TREE_ROWS = 32
 TREE_DEPTH = 8      # tokens taken from one earlier occurrence
 TREE_MATCHES = 8    # earlier occurrences per pattern
+# What a row past the plain step's adds to an iteration, in plain steps.
+TREE_ROW_COST = 0.0135
+
+
+def tree_cost(batch, nodes):
+    """Plain steps that a tree pass of ``nodes`` rows per sequence costs: a part
+    per row more, smaller where the plain step is itself of many rows.  A rule, not
+    a time measured beside the run: the gate compares with it, and with a measured
+    time the tokens at a near-tie would follow the clock.
+
+    MI355X, rule / measured at 100, 1024 and 8192 cached slots.  Qwen3-4B's size,
+    32 rows: batch 1 1.41 / 1.40 1.41 1.44, 2 1.39 / 1.34 1.36 1.25, 4 1.35 / 1.31
+    1.38 1.28, 8 1.28 / 1.24 1.28 1.16, 16 1.16 / 1.04 1.07 1.04; 64 rows at 1024
+    slots: batch 1 1.84 / 1.82, 4 1.76 / 1.74, 8 1.66 / 1.65.  28 layers of hidden
+    2048, 32 rows: batch 1 1.41 / 1.42 1.32 1.32, 4 1.35 / 1.23 1.24 1.22."""
+    return 1.0 + TREE_ROW_COST * batch * (nodes - 1) * (1.0 - batch / GEMM_MAX_ROWS)
 
 
 def tree_nodes(batch):
@@ -108,6 +124,7 @@ class TreeDecoder(SpecDecoder):
             raise ValueError(f"tree speculation needs a state with tree_t >= 2 (got {state.tree_t})")
         self.matches = matches
         super().__init__(engine, state, primary, backoff, depth)
+        self.cost_ratio = tree_cost(state.batch, state.tree_t)
 
     def _buffers(self):
         st, dev = self.state, self.state.model.device
@@ -124,12 +141,6 @@ class TreeDecoder(SpecDecoder):
     def _checked(self, toks):
         self.engine._checked([t for t in toks if t != -1])  # -1: past a sequence's walk
         return toks
-
-    def _ensure_graphs(self, stop_len):
-        if not (self.graphs and self.graph_stop == stop_len):
-            # The cost ratio is measured near the lengths it will judge.
-            self.state.lens.fill_(max(0, stop_len - 8 * (self.k + 1)))
-        super()._ensure_graphs(stop_len)
 
     def _stream(self):
         return torch.cuda.current_stream(self.state.model.device).cuda_stream
