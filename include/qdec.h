@@ -496,9 +496,11 @@ int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
 
 /* For every sequence b and node t (see above), from the raw projection row
  * qkv[b*t_rows + t]:
- *   q, k = per-head RMSNorm and RoPE at position lens[b] + depth(t), in fp32,
- *          rounded to bf16 once (qdec_attn rounds where the reference does,
- *          five times, so its keys differ by such roundings);
+ *   q, k = per-head RMSNorm and RoPE at position lens[b] + depth(t), in fp32; k
+ *          rounded to bf16 once (qdec_attn rounds where the reference does, five
+ *          times, so its keys differ by such roundings), q entering the products
+ *          in two bf16 parts (16 bits of it) or, in a call of many query rows per
+ *          kv head over a large cache, rounded once;
  *   out  = softmax(q . K^T / sqrt(D)) . V over cache slots 0 .. lens[b] - 1,
  *          node t's ancestors and node t itself: fp32 scores, statistics and
  *          accumulation, probabilities in two bf16 parts, one rounding to bf16;
@@ -513,8 +515,10 @@ int qdec_tree_draft(const qdec_tree_draft_args *a, qdec_stream_t stream);
  * The cached slots and the nodes are dealt in 32-row blocks, evenly, to
  * `splits` workgroups per row group of a (sequence, kv head), fewer for a short
  * cache; with splits > 1 they leave partials that a second launch merges in
- * order.  So a result depends on splits, lens[b] and the call's shape, never on
- * timing.  partial is scratch: calls that overlap in time must not share it. */
+ * order.  So a row's bits follow from what it sees, splits, lens[b] and the call's
+ * shape -- batch, t_rows, nq, nkv, head_dim and cap, which also choose the
+ * precision of q -- and neither from timing nor from the other sequences or the
+ * other branches.  partial is scratch: calls that overlap in time must not share it. */
 typedef struct {
   const void *qkv;        /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
   const void *q_norm_w;   /* [head_dim] bf16 */

@@ -81,10 +81,10 @@ def head_norm_rope(x, w, cos, sin, eps):
     return y * cos + rot * sin
 
 
-def attention(qkv, parents, L, k_cache, v_cache, q_norm, k_norm, cos, sin, nq, nkv, eps):
+def attention(qkv, parents, L, k_cache, v_cache, q_norm, k_norm, cos, sin, nq, nkv, eps, round_q=bf):
     """One sequence.  ``qkv`` [T, (nq + 2 nkv) D], ``k_cache`` / ``v_cache``
     [nkv, slots, D] (at least L slots), float64 throughout but for the queries
-    and node keys, which are rounded to bf16 once.  Returns ``out`` [T, nq, D],
+    (``round_q``) and node keys, which are rounded to bf16 once.  Returns ``out`` [T, nq, D],
     ``mag`` (the same sum over absolute values, the scale of its rounding
     errors), and the nodes' keys and values [nkv, T, D] (NaN in rows that hold
     no node)."""
@@ -102,7 +102,7 @@ def attention(qkv, parents, L, k_cache, v_cache, q_norm, k_norm, cos, sin, nq, n
             continue
         pos = L + len(up[t]) - 1
         c, s = cos[pos].double(), sin[pos].double()
-        q[t] = bf(head_norm_rope(x[t, :nq], q_norm.double(), c, s, eps))
+        q[t] = round_q(head_norm_rope(x[t, :nq], q_norm.double(), c, s, eps))
         kn[:, t] = bf(head_norm_rope(x[t, nq:nq + nkv], k_norm.double(), c, s, eps))
         vn[:, t] = x[t, nq + nkv:]
     kc, vc = k_cache[:, :L].double(), v_cache[:, :L].double()
