@@ -23,9 +23,10 @@
 //     narrow kernel's queries (the wide one's, which is bound by its
 //     arithmetic, are rounded once).  Each of these roundings would otherwise
 //     add as much error to the result as its own rounding to bf16 (relative
-//     to 64 bits 0.0040 with q, k as qdec_attn rounds them and P rounded, 0.0024
+//     to 64 bits 0.0040 with q, k as qdec_attn rounds them and P rounded, 0.0023
 //     with P in two parts, 0.0017 with both: the output's rounding alone).
-//     Node keys are rounded once, to what k_nodes holds.
+//     Node keys are rounded once, to what k_nodes holds: up to 0.0020 where the
+//     nodes outweigh the cache.
 //   * A lane's query rows are prepared in registers, in the place where the
 //     MFMA's B operand wants them: lane (c, g) holds channels 32s + 8g .. +8 of
 //     row c for every k step s, so the rotation's partner channel is the
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
   // stays in the caches meanwhile.  A value load takes whole lines, which only other
   // row groups (SHARED) read again.  us with non-temporal loads of neither / values only /
   // both, on one cache again and again: 32 x 4 nodes on 2000 to 4224 slots, one row
-  // group, 79 / 66 / 75; 2 x 16 on 8300, two, 26 / 28 / 29.
+  // group, 81 / 68 / 76; 2 x 16 on 8300, two, 25 / 28 / 30.
   auto load_block = [&](int j, Frag &f) {
     const uint16_t *kp = kc + (size_t)(32 * j + ra) * D + 8 * grp;
     const uint16_t *vp = vc + ((size_t)(4 * j + grp) * D + col) * 8;
@@ -686,12 +687,12 @@ __global__ void __launch_bounds__(512, 2) tree_narrow_kernel(const TreeAttnParam
 // other way round.  Cached blocks before the last run without its checks, and the
 // workgroup meets every second block when the ring has 8 slots.
 //
-// MI355X, 2 x 64 nodes, 64 query heads on 8, 30000 slots: 174 us, 0.75 PFLOP/s (1.1
-// with both parts of the probabilities).  A block of 256 rows takes about 2700
+// MI355X, 2 x 64 nodes, 64 query heads on 8, 30000 slots: 178 us at full clock, 0.74
+// PFLOP/s (1.1 with both parts of the probabilities), and 8 for the merge.  A block of 256 rows takes about 2700
 // cycles of a CU, of which the matrix cores have 1560 and the LDS reads 530; the
 // rest is the two waves of a SIMD waiting for each other's vector instructions.
-// (209 us with the checks in every block and the softmax's steps one after the
-// other.  64 rows per wave would halve the LDS reads, but then the sums live in
+// (The call took 209 us with the checks in every block and the softmax's steps one
+// after the other, 184 now.  64 rows per wave would halve the LDS reads, but then the sums live in
 // the accumulation registers, and the scores with them: every score tile moved
 // between the two files.)
 template <int D, int NW, int NT>
@@ -1135,17 +1136,17 @@ hipError_t launch_d(const TreeAttnParams &p, hipStream_t s) {
 // groups share; the wide one once per 128 or 256 rows, but its pipeline takes
 // longer to fill.  The narrow one is ahead until its reads come to about 200 MB,
 // and with up to 64 rows always: narrow / wide, 2 x 32 nodes on 4200 slots (138 MB)
-// 26 / 26.5, on 8300 (272 MB) 37 / 33, 32 on 30000 (492 MB) 53 / 43; 64 nodes on 8300
-// (272 MB) 37 / 37.5, on 30000 (980 MB) 89 / 65; 4 x 16 nodes on 30000 118 / 119.
+// 24.8 / 25.6, on 8300 (272 MB) 34.9 / 31.7, 32 on 30000 (492 MB) 52 / 44; 64 nodes on
+// 8300 (272 MB) 36.3 / 37.5, on 30000 (980 MB) 88 / 63; 4 x 16 nodes on 30000 114 / 119.
 //
 // 16 rows per workgroup give more workgroups, 32 half the reads.  16 where 32
 // would leave CUs idle and the reads are under 130 MB: 16 / 32 rows, 16 nodes on
-// 4100 slots (67 MB) 15.3 / 17.1, 32 on 2000 (65 MB) 15.4 / 15.9, on 4200 (138 MB)
-// 20.5 / 19.2, 2 x 16 on 4200 (138 MB) 21.9 / 20.4.
+// 4100 slots (67 MB) 15.1 / 17.0, 32 on 2000 (65 MB) 15.2 / 16.1, on 4200 (138 MB)
+// 20.1 / 19.2, 2 x 16 on 4200 (138 MB) 20.5 / 19.4.
 //
 // One workgroup per CU, none of fewer than four blocks of a full cache: more
 // splits read no faster and merge more (16 nodes on 4100 slots, 4 / 8 / 16 / 32
-// splits: 20 / 16 / 19 / 28; 2 x 32 nodes on 30000 slots, 16 / 32: 65 / 71).
+// splits: 19 / 15.5 / 18.5 / 27; 2 x 32 nodes on 30000 slots, 8 / 16 / 32: 92 / 63 / 67).
 void tree_attn_plan(TreeAttnParams *p, int splits) {
   const int rows = p->t_rows * (p->nq / p->nkv), tiles = (rows + 15) / 16;
   const int64_t cells = (int64_t)p->batch * p->nkv;
