@@ -904,6 +904,135 @@ int qdec_tree_commit(const qdec_tree_commit_args *a, qdec_stream_t stream) {
   return launch_status(launch_tree_commit(*a, (hipStream_t)stream), "qdec_tree_commit");
 }
 
+// ------------------------------------------------------------ 8-bit KV cache
+// What kv8_store, kv8_load and kv8_attn all require of a cache.
+static int kv8_shape(const char *fn, int batch, int nkv, int head_dim, int cap) {
+  if (head_dim != 128 && head_dim != 64) return set_error(QDEC_EUNSUPPORTED, "%s: head_dim %d (128 or 64)", fn, head_dim);
+  if (batch < 1 || batch > 16383 || nkv < 1 || nkv > 65535)
+    return set_error(QDEC_EINVAL, "%s: batch %d not in [1, 16383], or nkv %d not in [1, 65535]", fn, batch, nkv);
+  if (cap < kKv8Block || cap % kKv8Block)
+    return set_error(QDEC_EINVAL, "%s: cap %d not a positive multiple of %d", fn, cap, kKv8Block);
+  return QDEC_OK;
+}
+
+extern "C++" template <class A>
+static int plan_kv8_copy(const char *fn, const A *a, Kv8CopyParams *p) {
+  if (!a) return set_error(QDEC_EINVAL, "%s: null args", fn);
+  const int rc = kv8_shape(fn, a->batch, a->nkv, a->head_dim, a->cap);
+  if (rc != QDEC_OK) return rc;
+  if (a->slab_cap < 32 || a->slab_cap % 32)
+    return set_error(QDEC_EINVAL, "%s: slab_cap %d not a positive multiple of 32", fn, a->slab_cap);
+  if (!a->k_slab || !a->v_slab || !a->k8 || !a->v8 || !a->k_scale || !a->v_scale)
+    return set_error(QDEC_EINVAL, "%s: null pointer argument", fn);
+  if (!aligned16(a->k_slab) || !aligned16(a->v_slab) || !aligned16(a->k8) || !aligned16(a->v8) || !aligned16(a->k_scale) ||
+      !aligned16(a->v_scale))
+    return set_error(QDEC_EALIGN, "%s: slabs, caches and scales must be 16-byte aligned", fn);
+  *p = Kv8CopyParams{};
+  p->k_slab = reinterpret_cast<uint16_t *>(const_cast<void *>(static_cast<const void *>(a->k_slab)));
+  p->v_slab = reinterpret_cast<uint16_t *>(const_cast<void *>(static_cast<const void *>(a->v_slab)));
+  p->k8 = reinterpret_cast<int8_t *>(const_cast<void *>(static_cast<const void *>(a->k8)));
+  p->v8 = reinterpret_cast<int8_t *>(const_cast<void *>(static_cast<const void *>(a->v8)));
+  p->k_scale = const_cast<float *>(a->k_scale);
+  p->v_scale = const_cast<float *>(a->v_scale);
+  p->cells = (int64_t)a->batch * a->nkv;
+  p->nkv = a->nkv; p->head_dim = a->head_dim; p->cap = a->cap; p->slab_cap = a->slab_cap; p->n = a->n;
+  return QDEC_OK;
+}
+
+// A launch's work items are numbered in 32 bits.
+static int kv8_copy_grid(const char *fn, const Kv8CopyParams &p) {
+  if (p.cells * p.groups > (1ll << 26) - 8) return set_error(QDEC_EUNSUPPORTED, "%s: %lld (sequence, kv head) pairs x %d slots", fn, (long long)p.cells, p.n);
+  return QDEC_OK;
+}
+
+int qdec_kv8_store(const qdec_kv8_store_args *a, qdec_stream_t stream) {
+  Kv8CopyParams p;
+  int rc = plan_kv8_copy("qdec_kv8_store", a, &p);
+  if (rc != QDEC_OK) return rc;
+  if (a->pos0 < 0 || a->n < 1 || (int64_t)a->pos0 + a->n > std::min(a->cap, a->slab_cap))
+    return set_error(QDEC_EINVAL, "qdec_kv8_store: slots %d + %d of cap %d, slab_cap %d", a->pos0, a->n, a->cap, a->slab_cap);
+  p.pos0 = a->pos0;
+  p.groups = (a->pos0 + a->n - 1) / 16 - a->pos0 / 16 + 1;
+  rc = kv8_copy_grid("qdec_kv8_store", p);
+  if (rc != QDEC_OK) return rc;
+  return launch_status(launch_kv8_store(p, (hipStream_t)stream), "qdec_kv8_store");
+}
+
+int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream) {
+  Kv8CopyParams p;
+  int rc = plan_kv8_copy("qdec_kv8_load", a, &p);
+  if (rc != QDEC_OK) return rc;
+  if (a->n < 1 || a->n > a->slab_cap) return set_error(QDEC_EINVAL, "qdec_kv8_load: n %d not in [1, slab_cap %d]", a->n, a->slab_cap);
+  p.starts = a->starts;
+  p.groups = (a->n + 15) / 16;
+  rc = kv8_copy_grid("qdec_kv8_load", p);
+  if (rc != QDEC_OK) return rc;
+  return launch_status(launch_kv8_load(p, (hipStream_t)stream), "qdec_kv8_load");
+}
+
+static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool need_scratch) {
+  if (!a) return set_error(QDEC_EINVAL, "qdec_kv8_attn: null args");
+  const int rc = kv8_shape("qdec_kv8_attn", a->batch, a->nkv, a->head_dim, a->cap);
+  if (rc != QDEC_OK) return rc;
+  if (a->nq < a->nkv || a->nq % a->nkv)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: nq %d / nkv %d (whole query heads per kv head)", a->nq, a->nkv);
+  if (a->t_rows < 1 || a->t_rows > kKv8MaxT || a->t_rows > a->cap)
+    return set_error(QDEC_EINVAL, "qdec_kv8_attn: t_rows %d not in [1, %d]", a->t_rows, kKv8MaxT);
+  if ((int64_t)a->t_rows * (a->nq / a->nkv) > 64)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: t_rows %d x %d query heads per kv head (at most 64 rows)", a->t_rows,
+                     a->nq / a->nkv);
+  if (a->splits < 0 || a->splits > 256) return set_error(QDEC_EINVAL, "qdec_kv8_attn: splits %d not in [0, 256]", a->splits);
+  if (a->out_frag != 0 && a->out_frag != 1) return set_error(QDEC_EINVAL, "qdec_kv8_attn: out_frag %d not 0 or 1", a->out_frag);
+  *p = Kv8AttnParams{};
+  p->eps = a->eps;
+  p->scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p->batch = a->batch; p->t_rows = a->t_rows; p->nq = a->nq; p->nkv = a->nkv;
+  p->head_dim = a->head_dim; p->cap = a->cap;
+  p->splits = a->splits ? a->splits : kv8_attn_splits(a->batch, a->nkv, a->cap);
+  p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
+  // A launch's work items are numbered in 32 bits.
+  const int64_t tiles = (a->t_rows * (a->nq / a->nkv) + 15) / 16;
+  if ((int64_t)p->batch * p->nkv * p->splits * tiles * 512 > 0xffffffffll)
+    return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: batch %d x nkv %d x %d splits", p->batch, p->nkv, p->splits);
+  if (!need_scratch) return QDEC_OK;
+  if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->k8 || !a->v8 || !a->k_scale ||
+      !a->v_scale || !a->out)
+    return set_error(QDEC_EINVAL, "qdec_kv8_attn: null pointer argument");
+  if (p->splits > 1 && !a->partial) return set_error(QDEC_EINVAL, "qdec_kv8_attn: more than one split needs partial");
+  if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
+      !aligned16(a->sin_tab) || !aligned16(a->k8) || !aligned16(a->v8) || !aligned16(a->k_scale) || !aligned16(a->v_scale) ||
+      !aligned16(a->out) || !aligned16(a->partial))
+    return set_error(QDEC_EALIGN, "qdec_kv8_attn: tensor pointers must be 16-byte aligned");
+  auto u16 = [](const void *x) { return reinterpret_cast<const uint16_t *>(x); };
+  p->qkv = u16(a->qkv); p->q_norm_w = u16(a->q_norm_w); p->k_norm_w = u16(a->k_norm_w);
+  p->cos_tab = u16(a->cos_tab); p->sin_tab = u16(a->sin_tab);
+  p->lens = a->lens;
+  p->k8 = reinterpret_cast<int8_t *>(a->k8);
+  p->v8 = reinterpret_cast<int8_t *>(a->v8);
+  p->k_scale = a->k_scale;
+  p->v_scale = a->v_scale;
+  p->out = reinterpret_cast<uint16_t *>(a->out);
+  p->partial = a->partial;
+  return QDEC_OK;
+}
+
+int qdec_kv8_attn_workspace(const qdec_kv8_attn_args *a, size_t *partial_bytes, size_t *counter_bytes) {
+  Kv8AttnParams p;
+  const int rc = plan_kv8_attn(a, &p, false);
+  if (rc != QDEC_OK) return rc;
+  const size_t rows = (size_t)p.batch * p.t_rows * p.nq;
+  if (partial_bytes) *partial_bytes = p.splits > 1 ? sizeof(float) * rows * p.splits * (p.head_dim + 2) : 0;
+  if (counter_bytes) *counter_bytes = 0;
+  return QDEC_OK;
+}
+
+int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream) {
+  Kv8AttnParams p;
+  const int rc = plan_kv8_attn(a, &p, true);
+  if (rc != QDEC_OK) return rc;
+  return launch_status(launch_kv8_attn(p, (hipStream_t)stream), "qdec_kv8_attn");
+}
+
 // ------------------------------------------------------------- prefill
 static int rownorm(const qdec_rownorm_args *a, const float *parts, int nparts, void *merged, qdec_stream_t stream) {
   if (!a || !a->x || !a->out) return set_error(QDEC_EINVAL, "qdec_rownorm: null pointer");

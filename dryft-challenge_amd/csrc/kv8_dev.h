@@ -1,0 +1,52 @@
+// Arithmetic of the 8-bit KV cache, shared by its kernels.
+//
+// A row x of D channels is held as q = round(127 x / top), top = max|x|, ties to
+// even, and scale = top / 127; it stands for q * scale, off by half a step or
+// less.  (One scale for each token and head: a scale over several tokens would
+// have to grow as louder ones arrive, rounding what is there a second time, and
+// a row's bits would depend on how many rows its pass had.)  127 x of a bf16 x has 15
+// bits, so in fp32 it is exact and only the division rounds: quotients that
+// are halves, as of x = top / 2, come out as such, and no other quotient of two
+// bf16 numbers is within 2^-9 of one.  A row with an infinity or a NaN gets the
+// scale NaN, one with top below 2^-100, whose reciprocals would leave fp32's
+// range, the scale 0.
+#pragma once
+
+#include "qdec_common.h"
+
+namespace qdec {
+
+constexpr float kKv8Tiny = 7.8886090522101180541e-31f;  // 2^-100
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float kv8_scale(float top, bool finite) {
+  return finite ? (top < kKv8Tiny ? 0.f : top / 127.f) : __builtin_nanf("");
+}
+// What (127 / 256) x is divided by (the 256 keeps 127 x in range): top / 256, or
+// infinity where all are held as 0.
+__device__ __forceinline__ float kv8_div(float top, bool finite) {
+  return finite && top >= kKv8Tiny ? top * 0.00390625f : __builtin_huge_valf();
+}
+// An int8 in the low byte.  (0 for x = NaN and x = inf, whose div is infinite.)
+__device__ __forceinline__ uint32_t kv8_round(float x, float div) {
+  const float q = rintf((0.49609375f * x) / div);
+  return (uint32_t)(int)(q == q ? q : 0.f) & 0xffu;
+}
+
+// Maximum over the 64 lanes of a wave, over 16-lane rows, of numbers >= 0.
+__device__ __forceinline__ float row16_maxf(float v) {
+  v = fmaxf(v, dpp_f<0xB1>(v));
+  v = fmaxf(v, dpp_f<0x4E>(v));
+  v = fmaxf(v, dpp_f<0x141>(v));
+  return fmaxf(v, dpp_f<0x140>(v));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = row16_maxf(v);
+  return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
+}
+
+__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+}  // namespace qdec

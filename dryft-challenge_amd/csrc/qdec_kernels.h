@@ -300,4 +300,34 @@ hipError_t launch_tree_draft(const qdec_tree_draft_args &a, hipStream_t s);
 hipError_t launch_tree_accept(const qdec_tree_accept_args &a, hipStream_t s);
 hipError_t launch_tree_commit(const qdec_tree_commit_args &a, hipStream_t s);
 
+// ---- 8-bit KV cache (kv8.hip, kv8_attn.hip)
+constexpr int kKv8Block = 64;  // slots of a block: one wave's work between two looks at the running maximum
+constexpr int kKv8MaxT = 16;   // query rows per sequence
+struct Kv8CopyParams {         // kv8_store, kv8_load
+  uint16_t *k_slab, *v_slab;
+  int8_t *k8, *v8;
+  float *k_scale, *v_scale;
+  const int32_t *starts;  // kv8_load: first slot per sequence, or NULL: 0
+  int64_t cells;          // batch * nkv
+  int nkv, head_dim, cap, slab_cap, pos0, n;
+  int groups;             // 16-slot groups per cell
+};
+hipError_t launch_kv8_store(const Kv8CopyParams &p, hipStream_t s);
+hipError_t launch_kv8_load(const Kv8CopyParams &p, hipStream_t s);
+struct Kv8AttnParams {
+  const uint16_t *qkv, *q_norm_w, *k_norm_w, *cos_tab, *sin_tab;
+  const int32_t *lens;
+  int8_t *k8, *v8;
+  float *k_scale, *v_scale;
+  uint16_t *out;
+  float *partial;
+  float eps;
+  float scale_log2;  // log2(e) / sqrt(head_dim)
+  int batch, t_rows, nq, nkv, head_dim, cap;
+  int splits;  // workgroups per (sequence, kv head): block j goes to workgroup j % splits
+  int ofrag;   // > 0: out is written in fragment order with this many M tiles
+};
+int kv8_attn_splits(int batch, int nkv, int cap);
+hipError_t launch_kv8_attn(const Kv8AttnParams &p, hipStream_t s);
+
 }  // namespace qdec

@@ -127,6 +127,23 @@ class TreeCommitArgs(ctypes.Structure):
                 ("head_dim", I32), ("cap", I32)]
 
 
+class Kv8StoreArgs(ctypes.Structure):
+    _fields_ = [("k_slab", P), ("v_slab", P), ("k8", P), ("v8", P), ("k_scale", P), ("v_scale", P), ("batch", I32),
+                ("nkv", I32), ("head_dim", I32), ("cap", I32), ("slab_cap", I32), ("pos0", I32), ("n", I32)]
+
+
+class Kv8LoadArgs(ctypes.Structure):
+    _fields_ = [("k8", P), ("v8", P), ("k_scale", P), ("v_scale", P), ("starts", P), ("k_slab", P), ("v_slab", P),
+                ("batch", I32), ("nkv", I32), ("head_dim", I32), ("cap", I32), ("slab_cap", I32), ("n", I32)]
+
+
+class Kv8AttnArgs(ctypes.Structure):
+    _fields_ = [("qkv", P), ("q_norm_w", P), ("k_norm_w", P), ("cos_tab", P), ("sin_tab", P), ("lens", P),
+                ("k8", P), ("v8", P), ("k_scale", P), ("v_scale", P), ("out", P), ("partial", P), ("eps", F32),
+                ("sm_scale", F32), ("batch", I32), ("t_rows", I32), ("nq", I32), ("nkv", I32), ("head_dim", I32),
+                ("cap", I32), ("splits", I32), ("out_frag", I32)]
+
+
 def declared_functions(header=HEADER):
     """Names of every function declared in include/qdec.h."""
     with open(header) as f:
@@ -159,6 +176,8 @@ class Lib:
                          ("qdec_ngram_draft", DraftArgs), ("qdec_spec_accept", AcceptArgs),
                          ("qdec_tree_draft", TreeDraftArgs), ("qdec_tree_attn", TreeAttnArgs),
                          ("qdec_tree_accept", TreeAcceptArgs), ("qdec_tree_commit", TreeCommitArgs),
+                         ("qdec_kv8_store", Kv8StoreArgs), ("qdec_kv8_load", Kv8LoadArgs),
+                         ("qdec_kv8_attn", Kv8AttnArgs),
                          ("qdec_rownorm", RownormArgs), ("qdec_prefill_gemm", PgemmArgs),
                          ("qdec_prefill_qk", PrefillQkArgs), ("qdec_prefill_attn", PrefillAttnArgs)):
             fn = getattr(so, name)
@@ -169,7 +188,7 @@ class Lib:
         so.qdec_layer.argtypes = [ctypes.POINTER(LayerArgs), P]
         so.qdec_layer.restype = ctypes.c_int
         for name, st in (("qdec_gemm_workspace", GemmArgs), ("qdec_attn_workspace", AttnArgs),
-                         ("qdec_tree_attn_workspace", TreeAttnArgs)):
+                         ("qdec_tree_attn_workspace", TreeAttnArgs), ("qdec_kv8_attn_workspace", Kv8AttnArgs)):
             fn = getattr(so, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.POINTER(ctypes.c_size_t),
                            ctypes.POINTER(ctypes.c_size_t)]
@@ -249,6 +268,15 @@ class Lib:
     def tree_commit(self, args, stream):
         self._check("qdec_tree_commit", self.so.qdec_tree_commit(ctypes.byref(args), stream))
 
+    def kv8_store(self, args, stream):
+        self._check("qdec_kv8_store", self.so.qdec_kv8_store(ctypes.byref(args), stream))
+
+    def kv8_load(self, args, stream):
+        self._check("qdec_kv8_load", self.so.qdec_kv8_load(ctypes.byref(args), stream))
+
+    def kv8_attn(self, args, stream):
+        self._check("qdec_kv8_attn", self.so.qdec_kv8_attn(ctypes.byref(args), stream))
+
     def rownorm(self, args, stream):
         self._check("qdec_rownorm", self.so.qdec_rownorm(ctypes.byref(args), stream))
 
@@ -293,6 +321,12 @@ class Lib:
         pb, cb = ctypes.c_size_t(), ctypes.c_size_t()
         self._check("qdec_tree_attn_workspace",
                     self.so.qdec_tree_attn_workspace(ctypes.byref(args), ctypes.byref(pb), ctypes.byref(cb)))
+        return pb.value, cb.value
+
+    def kv8_attn_workspace(self, args):
+        pb, cb = ctypes.c_size_t(), ctypes.c_size_t()
+        self._check("qdec_kv8_attn_workspace",
+                    self.so.qdec_kv8_attn_workspace(ctypes.byref(args), ctypes.byref(pb), ctypes.byref(cb)))
         return pb.value, cb.value
 
 

@@ -599,6 +599,112 @@ typedef struct {
 } qdec_tree_commit_args;
 int qdec_tree_commit(const qdec_tree_commit_args *a, qdec_stream_t stream);
 
+/* ------------------------------------------------------ 8-bit KV cache */
+
+/* Keys and values held as int8 with one fp32 scale for each slot and kv head:
+ * half the cache's bytes, so half the read that bounds decoding long contexts,
+ * and twice the slots.  A row x of head_dim channels is held as q =
+ * round(127 x / max|x|), ties to even, and scale = max|x| / 127; it stands for
+ * q * scale.  A row with max|x| < 2^-100 is held as zeros with scale 0; one with
+ * an infinity or a NaN gets the scale NaN and reads back as NaN.  No slot's
+ * bits depend on another's: a slot that is written again, or rolled back by its
+ * sequence's length, leaves no trace in its neighbours.  No counterpart in the
+ * reference, whose cache is bf16 (engine/engine.py:289-301).
+ *   k8              : [batch][nkv][cap][head_dim] int8, per layer
+ *   v8              : [batch][nkv][cap/16][head_dim][16] int8, per layer: 16
+ *                     consecutive slots of one channel are 16 contiguous bytes
+ *   k_scale, v_scale: [batch][nkv][cap] float, per layer
+ * cap is a multiple of 64.  bf16 slabs beside it (k_slab, v_slab) have the
+ * layouts of the K and V cache slabs with slab_cap slots, a multiple of 32. */
+
+/* Slots pos0 .. pos0 + n - 1 of every sequence and kv head from the bf16 slabs
+ * into the 8-bit cache, the same slot numbers; the other slots are left as they
+ * were.  The prompt path's write: qdec_prefill_qk leaves a layer's keys and
+ * values in the slabs. */
+typedef struct {
+  const void *k_slab;  /* [batch][nkv][slab_cap][head_dim] bf16 */
+  const void *v_slab;  /* [batch][nkv][slab_cap/8][head_dim][8] bf16 */
+  void *k8;
+  void *v8;
+  float *k_scale;
+  float *v_scale;
+  int32_t batch;
+  int32_t nkv;
+  int32_t head_dim;    /* 128 or 64 */
+  int32_t cap;         /* slots per sequence of the 8-bit cache */
+  int32_t slab_cap;    /* slots per sequence of the slabs */
+  int32_t pos0;
+  int32_t n;           /* >= 1; pos0 + n <= cap and <= slab_cap */
+} qdec_kv8_store_args;
+int qdec_kv8_store(const qdec_kv8_store_args *a, qdec_stream_t stream);
+
+/* Slots starts[b] .. starts[b] + n - 1 of every sequence b of the 8-bit cache
+ * into slots 0 .. n - 1 of the bf16 slabs, as bf16(q * scale); the slabs' other
+ * slots are left as they were.  A slot outside [0, cap) reads nothing and becomes
+ * NaN. */
+typedef struct {
+  const void *k8;
+  const void *v8;
+  const float *k_scale;
+  const float *v_scale;
+  const int32_t *starts; /* [batch], or NULL: 0 */
+  void *k_slab;          /* out */
+  void *v_slab;          /* out */
+  int32_t batch;
+  int32_t nkv;
+  int32_t head_dim;      /* 128 or 64 */
+  int32_t cap;
+  int32_t slab_cap;
+  int32_t n;             /* 1 .. slab_cap */
+} qdec_kv8_load_args;
+int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
+
+/* qdec_attn over the 8-bit cache.  For every sequence b and query row t <
+ * t_rows, from the raw projection row qkv[b*t_rows + t]:
+ *   q, k = per-head RMSNorm and RoPE at position lens[b] + t, in fp32 (qdec_attn
+ *          rounds where the reference does, five times);
+ *   k and the raw v go into cache slot lens[b] + t as above;
+ *   out  = softmax(q . K^T * sm_scale) . V over slots 0 .. lens[b] + t as the
+ *          cache holds them, the new ones included: fp32 statistics and
+ *          accumulation, q in two fp16 parts (22 bits), p * v_scale in fp16,
+ *          one rounding to bf16.
+ * What a row does not see does not reach it, whatever its slot or scale holds.  A length
+ * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
+ * of sequence b become NaN.
+ * Slots are dealt in blocks of 64, block j to workgroup j % splits of its
+ * (sequence, kv head); with splits > 1 a second launch merges the workgroups'
+ * partials, in order.  So a row's bits follow from what it sees and from splits,
+ * never from t_rows, the other sequences or timing; 0 splits takes a number that
+ * follows from batch, nkv and cap.  partial is scratch: calls that overlap in
+ * time must not share it. */
+typedef struct {
+  const void *qkv;      /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
+  const void *q_norm_w; /* [head_dim] bf16 */
+  const void *k_norm_w; /* [head_dim] bf16 */
+  const void *cos_tab;  /* [cap, head_dim] bf16 */
+  const void *sin_tab;  /* [cap, head_dim] bf16 */
+  const int32_t *lens;  /* [batch] slots already in the cache per sequence */
+  void *k8;             /* this layer's cache */
+  void *v8;
+  float *k_scale;
+  float *v_scale;
+  void *out;            /* [batch*t_rows, nq*head_dim] bf16 */
+  float *partial;       /* split partials, 16-byte aligned (qdec_kv8_attn_workspace) */
+  float eps;
+  float sm_scale;       /* 1/sqrt(head_dim) */
+  int32_t batch;
+  int32_t t_rows;       /* 1..16 */
+  int32_t nq;           /* a multiple of nkv; t_rows * nq / nkv at most 64 */
+  int32_t nkv;
+  int32_t head_dim;     /* 128 or 64 */
+  int32_t cap;          /* slots per sequence, multiple of 64 */
+  int32_t splits;       /* 1..256, or 0: chosen from the shape */
+  int32_t out_frag;     /* 1: out in the fragment order of qdec_gemm_args */
+} qdec_kv8_attn_args;
+int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream);
+/* Bytes of `partial`; counter_bytes, as in the other queries, is 0. */
+int qdec_kv8_attn_workspace(const qdec_kv8_attn_args *a, size_t *partial_bytes, size_t *counter_bytes);
+
 /* ------------------------------------------------------------ prefill */
 
 /* Prompt processing: every prompt position of every sequence in one forward
