@@ -28,6 +28,9 @@ Public surface (the reference's engine/engine.py:215-241, 1024-1063):
 * Optional tree speculation (``speculate="tree"``): several earlier
   continuations merged into a tree of drafts and verified in one pass, the
   accepted path's keys and values appended to the cache (``qdec.tree``).
+* Optional 8-bit KV cache (``kv_cache="int8"``): keys and values as int8 with a
+  scale for each token and kv head, written and attended over by the decode
+  kernels themselves (qdec_kv8_attn): half the cache's bytes.
 * The engine never falls back to another implementation: a missing or
   failing kernel library raises.
 """
@@ -81,6 +84,21 @@ def speculation(mode):
     return mode if isinstance(mode, str) else bool(mode)
 
 
+def cache_kind(kind):
+    """``Engine.kv_cache`` of a constructor's argument: "bf16" or "int8"."""
+    if kind not in ("bf16", "int8"):
+        raise ValueError(f'kv_cache is "bf16" or "int8" (got {kind!r})')
+    return kind
+
+
+def check_modes(kv_cache, speculate, mega):
+    """Refuse what an 8-bit cache does not come with."""
+    if cache_kind(kv_cache) == "int8" and speculate == "tree":
+        raise ValueError('speculate="tree" reads a bf16 cache (kv_cache="int8"; speculate=True takes either)')
+    if kv_cache == "int8" and mega:
+        raise ValueError('mega=True reads a bf16 cache (kv_cache="int8")')
+
+
 def _log(message):
     print(f"[engine] {message}", file=sys.stderr, flush=True)
 
@@ -89,7 +107,7 @@ class _Shape:
     """Per (batch, prompt, new tokens) state: decode state, graphs, host ring."""
 
     def __init__(self, engine, batch, prompt_len, new_tokens, speculate):
-        self.key = (batch, prompt_len, new_tokens, speculate)
+        self.key = (batch, prompt_len, new_tokens, speculate, engine.kv_cache)
         self.batch = batch
         # The verify slack is reserved in both modes: attention chunking is a
         # function of (batch, capacity), and plain and speculative runs of one
@@ -100,7 +118,8 @@ class _Shape:
         slack = max(slack, 2 * self.tree_t)  # a walk past the last token, and the next pass's nodes
         self.capacity = prompt_len + new_tokens + slack
         max_t = (self.spec_k + 1) if (speculate and speculate != "tree" and self.spec_k) else 16
-        self.state = DecodeState(engine.model, batch, self.capacity, max_t=max_t, tree_t=self.tree_t)
+        self.state = DecodeState(engine.model, batch, self.capacity, max_t=max_t, tree_t=self.tree_t,
+                                 kv8=engine.kv_cache == "int8")
         self.graph = None
         self.spec_graph = None
         self.host = torch.empty((new_tokens, batch), dtype=torch.int64, pin_memory=True)
@@ -110,29 +129,32 @@ class _Shape:
 
 
 class Engine:
-    def __init__(self, model_path: str, speculate: "bool | str" = False, mega=None) -> None:
+    def __init__(self, model_path: str, speculate: "bool | str" = False, mega=None, kv_cache: str = "bf16") -> None:
         """Load the checkpoint at ``model_path`` (HF layout, local files only).
         ``speculate``: True drafts one chain per sequence, "tree" a tree.
-        ``mega``: try one launch per layer for plain decode (None: MEGA_ENABLED)."""
+        ``mega``: try one launch per layer for plain decode (None: MEGA_ENABLED).
+        ``kv_cache``: "int8" holds keys and values in 8 bits (not with "tree" or
+        ``mega``)."""
+        check_modes(kv_cache, speculation(speculate), mega)
         start = time.perf_counter()
         if not torch.cuda.is_available():
             raise RuntimeError("Engine needs a HIP device (torch.cuda.is_available() is False)")
         cfg = load_config(model_path)
         tensors = load_tensors(model_path)
-        self._setup(cfg, tensors, speculate, mega=mega)
+        self._setup(cfg, tensors, speculate, mega=mega, kv_cache=kv_cache)
         del tensors
         _log(f"engine ready in {time.perf_counter() - start:.1f}s "
              f"({self.model.weight_bytes() / 1e9:.2f} GB of packed weights)")
 
     @classmethod
-    def from_tensors(cls, cfg, tensors, speculate=False, use_graphs=True, mega=None):
+    def from_tensors(cls, cfg, tensors, speculate=False, use_graphs=True, mega=None, kv_cache="bf16"):
         """Build around in-memory HF-named tensors (tests)."""
         self = cls.__new__(cls)
-        self._setup(cfg, tensors, speculate, use_graphs, mega=mega)
+        self._setup(cfg, tensors, speculate, use_graphs, mega=mega, kv_cache=kv_cache)
         return self
 
     @classmethod
-    def from_model(cls, model, device="cuda:0", use_triton=True, use_graphs=True):
+    def from_model(cls, model, device="cuda:0", use_triton=True, use_graphs=True, kv_cache="bf16"):
         """The reference's test hook (engine/engine.py:243-248): build around
         an already-loaded Transformers Qwen3 model (its config and weights).
         The engine runs its HIP kernels on ``device`` (a HIP device) or
@@ -146,9 +168,10 @@ class Engine:
                              "kernels (use_triton=True runs them)")
         cfg = model.config.to_dict()
         tensors = {k: v.detach() for k, v in model.state_dict().items()}
-        return cls.from_tensors(cfg, tensors, use_graphs=use_graphs)
+        return cls.from_tensors(cfg, tensors, use_graphs=use_graphs, kv_cache=kv_cache)
 
-    def _setup(self, cfg, tensors, speculate, use_graphs=True, mega=None):
+    def _setup(self, cfg, tensors, speculate, use_graphs=True, mega=None, kv_cache="bf16"):
+        check_modes(kv_cache, speculation(speculate), mega)
         self.device = torch.device("cuda:0")
         torch.cuda.set_device(self.device)
         self.lib = capi.lib()
@@ -156,6 +179,7 @@ class Engine:
         # Known-answer checks of every kernel family on this device, with the
         # model's own weights and plans; raises on a mismatch (no fallback).
         selfcheck.run(DecodeState(self.model, 1, 64, max_t=1))
+        self.kv_cache = kv_cache
         self.speculate = speculation(speculate)
         self.spec_gate = True  # speculation falls back to plain steps when drafts do not pay
         self.use_graphs = use_graphs
@@ -165,7 +189,8 @@ class Engine:
 
     # ----------------------------------------------------------- per shape
     def _shape_for(self, batch, prompt_len, new_tokens):
-        key = (batch, prompt_len, new_tokens, self.speculate)
+        check_modes(self.kv_cache, self.speculate, False)  # (attributes a caller may set)
+        key = (batch, prompt_len, new_tokens, self.speculate, self.kv_cache)
         if self.shape is not None and self.shape.key == key:
             return self.shape
         self.shape = None
@@ -183,8 +208,9 @@ class Engine:
             if self.mega and not self.speculate and sh.state.layer_supported():
                 self._try_mega(sh, prompt_len, new_tokens)
         self.shape = sh
+        cache = "8-bit cache" if sh.state.kv8 else f"attention chunk {sh.state.chunk}"
         _log(f"shape B={batch} S={prompt_len} N={new_tokens}: capacity {sh.state.cap}, "
-             f"attention chunk {sh.state.chunk}, graph={'yes' if sh.graph else 'no'}, "
+             f"{cache}, graph={'yes' if sh.graph else 'no'}, "
              f"setup {time.perf_counter() - start:.2f}s")
         return sh
 

@@ -23,6 +23,10 @@ row count: that keeps every output element's summation order the same for a
 (``tree_t`` nodes per sequence) runs the same projections around
 ``qdec_tree_attn``, whose sums are its own.
 
+With ``kv8`` the cache holds keys and values as int8 with a scale for each slot
+and kv head (include/qdec.h, "8-bit KV cache"): half the bytes, so that long
+contexts decode faster and twice the slots fit.  Steps run ``qdec_kv8_attn``.
+
 ``Prefill`` fills the cache from a prompt with the prefill kernels: every
 prompt position of every sequence goes through a layer at once (in position
 chunks of about ``PREFILL_ROWS`` rows), so each weight matrix is read once
@@ -37,6 +41,7 @@ import torch
 from . import capi
 
 GEMM_MAX_ROWS = 64
+KV8_BLOCK = 64  # the 8-bit cache's slots come in whole blocks (kKv8Block of qdec_kernels.h)
 GEMM_WIDE_MIN_ROWS = 9  # of qdec_gemm_wide
 ATTN_MAX_T = 16
 # Rows (sequences x positions) of one prefill chunk: activations of 32K rows
@@ -517,11 +522,14 @@ class DeviceModel:
 class DecodeState:
     """Buffers for one (batch, capacity) shape and the step over them."""
 
-    def __init__(self, model, batch, capacity, max_t=1, keep_logits=False, tree_t=0):
+    def __init__(self, model, batch, capacity, max_t=1, keep_logits=False, tree_t=0, kv8=False):
         c = model.cfg
         self.model, self.lib = model, model.lib
         self.batch = batch
-        self.cap = round_up(capacity, 32)
+        self.kv8 = kv8
+        self.cap = round_up(capacity, KV8_BLOCK if kv8 else 32)
+        if kv8 and tree_t:
+            raise ValueError("tree passes read a bf16 cache (kv8 state)")
         self.max_t = max_rows_per_seq(batch, max_t, c.group)
         if batch > GEMM_MAX_ROWS:
             raise ValueError(f"batch {batch} > {GEMM_MAX_ROWS} rows per step")
@@ -537,8 +545,14 @@ class DecodeState:
         self.attn_waves = state_attn_waves(batch, c.nkv, D, self.cap)
         assert self.attn_waves == 4 or self.max_t <= 8
         cache_shape = (L, batch, c.nkv, self.cap, D)
-        self.k_cache = torch.zeros(cache_shape, dtype=bf, device=dev)
-        self.v_cache = torch.zeros(cache_shape, dtype=bf, device=dev)
+        if kv8:
+            self.k8 = torch.zeros(cache_shape, dtype=torch.int8, device=dev)
+            self.v8 = torch.zeros((L, batch, c.nkv, self.cap // 16, D, 16), dtype=torch.int8, device=dev)
+            self.k_scale = torch.zeros(cache_shape[:-1], dtype=torch.float32, device=dev)
+            self.v_scale = torch.zeros(cache_shape[:-1], dtype=torch.float32, device=dev)
+        else:
+            self.k_cache = torch.zeros(cache_shape, dtype=bf, device=dev)
+            self.v_cache = torch.zeros(cache_shape, dtype=bf, device=dev)
         self.layer_elems = batch * c.nkv * self.cap * D
         R = self.max_rows
         # The residual stream alternates between two buffers: the down
@@ -593,8 +607,11 @@ class DecodeState:
                 gw, gc = max(gw, pb), max(gc, cb)
         self.gemm_partial = torch.zeros((max(gw, 16) // 4 + 4,), dtype=torch.float32, device=dev)
         self.gemm_counters = torch.zeros((max(gc, 4) // 4 + 4,), dtype=torch.int32, device=dev)
-        aw, ac = self.lib.attn_workspace(self._attn_args(0, self.max_t))
-        aw = max(aw, self.lib.attn_workspace(self._attn_args(0, 1, partials=True))[0])
+        if kv8:
+            aw, ac = self.lib.kv8_attn_workspace(self._kv8_args(0, self.max_t))
+        else:
+            aw, ac = self.lib.attn_workspace(self._attn_args(0, self.max_t))
+            aw = max(aw, self.lib.attn_workspace(self._attn_args(0, 1, partials=True))[0])
         self.attn_partial = torch.zeros((max(aw, 16) // 4 + 4,), dtype=torch.float32, device=dev)
         self.attn_counters = torch.zeros((max(ac, 4) // 4 + 4,), dtype=torch.int32, device=dev)
         if tree_t:
@@ -620,7 +637,8 @@ class DecodeState:
         the merged output.  The O-side merge takes 4 query heads per kv
         head; other shapes merge in the attention."""
         c = self.model.cfg
-        return t_rows == 1 and self.batch <= MERGE_IN_O_MAX_BATCH and c.group == 4 and c.head_dim == 128
+        return (t_rows == 1 and self.batch <= MERGE_IN_O_MAX_BATCH and c.group == 4 and c.head_dim == 128
+                and not self.kv8)
 
     def _resident(self, a, role):
         """Whether the call ``a`` of ``role`` (resident still 0) runs
@@ -799,6 +817,25 @@ class DecodeState:
         a.strided = 1 if (ATTN_STRIDED and self.attn_waves == 8 and self.chunk < self.cap) else 0
         return a
 
+    def kv8_held(self, layer):
+        """The fields of one layer's 8-bit cache in the kv8 calls' arguments."""
+        c = self.model.cfg
+        return dict(k8=self.k8[layer].data_ptr(), v8=self.v8[layer].data_ptr(), k_scale=self.k_scale[layer].data_ptr(),
+                    v_scale=self.v_scale[layer].data_ptr(), batch=self.batch, nkv=c.nkv, head_dim=c.head_dim,
+                    cap=self.cap)
+
+    def _kv8_args(self, layer, t_rows):
+        m, c = self.model, self.model.cfg
+        a = capi.Kv8AttnArgs(**self.kv8_held(layer))
+        a.qkv, a.q_norm_w, a.k_norm_w = self.qkv.data_ptr(), m.q_norm[layer].data_ptr(), m.k_norm[layer].data_ptr()
+        a.cos_tab, a.sin_tab, a.lens = self.cos.data_ptr(), self.sin.data_ptr(), self.lens.data_ptr()
+        a.out = self.attn_out.data_ptr()
+        if hasattr(self, "attn_partial"):
+            a.partial = self.attn_partial.data_ptr()
+        a.eps, a.sm_scale, a.t_rows, a.nq, a.splits = c.eps, c.head_dim ** -0.5, t_rows, c.nq, 0
+        a.out_frag = 1 if self.batch * t_rows >= FRAG_ROWS else 0
+        return a
+
     def _tree_args(self, layer):
         m, c = self.model, self.model.cfg
         a = capi.TreeAttnArgs()
@@ -866,6 +903,8 @@ class DecodeState:
             lib.gemm(self._cached_gemm("qkv", i, rows), s)
             if tree:
                 lib.tree_attn(self._cached_tree(i), s)
+            elif self.kv8:
+                lib.kv8_attn(self._cached_kv8(i, t_rows), s)
             else:
                 lib.attn(self._cached_attn(i, t_rows, pm), s)
             lib.gemm(self._cached_gemm("o", i, rows, self._cached_attn(i, t_rows, pm) if pm else None), s)
@@ -892,6 +931,12 @@ class DecodeState:
             self._attn_cache[key] = a
         return a
 
+    def _cached_kv8(self, layer, t_rows):
+        a = self._attn_cache.get(("kv8", layer, t_rows))
+        if a is None:
+            a = self._attn_cache[("kv8", layer, t_rows)] = self._kv8_args(layer, t_rows)
+        return a
+
     def _cached_tree(self, layer):
         a = self._attn_cache.get(("tree", layer))
         if a is None:
@@ -907,7 +952,8 @@ class DecodeState:
         """Whether qdec_layer takes this state's plain decode steps: up to
         LAYER_MAX_BATCH sequences (its O stage always merges the attention
         partials, whatever MERGE_IN_O_MAX_BATCH says for five launches)."""
-        return self.batch <= LAYER_MAX_BATCH and self.model.cfg.group == 4 and self.model.cfg.head_dim == 128
+        return (self.batch <= LAYER_MAX_BATCH and self.model.cfg.group == 4 and self.model.cfg.head_dim == 128
+                and not self.kv8)
 
     def layer_attn_args(self, layer):
         """The attention stage of qdec_layer: this state's arguments with
@@ -935,7 +981,7 @@ class DecodeState:
         another order than this state's plans, so its rows are not
         bit-identical to theirs (within the logit tolerance instead)."""
         if not self.layer_supported():
-            raise ValueError(f"qdec_layer takes at most {LAYER_MAX_BATCH} sequences (batch {self.batch})")
+            raise ValueError(f"qdec_layer takes at most {LAYER_MAX_BATCH} sequences (batch {self.batch}) and a bf16 cache")
         c, dev = self.model.cfg, self.model.device
         if getattr(self, "layer_plan", None) is None:
             self.layer_plan = torch.zeros((c.n_layers, capi.LAYER_PLAN_BYTES), dtype=torch.uint8, device=dev)
@@ -1037,6 +1083,12 @@ class Prefill:
     rows) where a width is no multiple of 128.  After the last chunk the final row
     of each sequence goes through the decode lm_head + argmax.
 
+    With an 8-bit cache the layer's keys and values go to a pair of bf16 slabs
+    of one layer, from there into the cache (qdec_kv8_store), and the slots so
+    far come back from it (qdec_kv8_load) before the attention: every row
+    attends over what the cache holds, as the steps after it do, in whatever
+    chunks the prompt ran.
+
     Replaces engine/engine.py:448-490 (``_layers_forward`` over the whole
     prompt, ``_attend_prefill``, ``_prefill``)."""
 
@@ -1059,6 +1111,33 @@ class Prefill:
         self._skinny_bufs, self._skinny_calls = None, {}
         self._split_bufs = None
         self._gemm_scratch = None
+        self._slabs = None
+
+    def _kv_slabs(self, S):
+        """(K, V, slots) that the prompt kernels of a layer write and read: with
+        an 8-bit cache a pair of slabs all layers share, for S slots."""
+        c, st = self.state.model.cfg, self.state
+        if self._slabs is None or self._slabs[2] < S:
+            self._slabs = None
+            cap = round_up(S, KV8_BLOCK)
+            shape = (st.batch, c.nkv, cap, c.head_dim)
+            k, v = (torch.zeros(shape, dtype=torch.bfloat16, device=st.model.device) for _ in range(2))
+            self._slabs = (k, v, cap)
+        return self._slabs
+
+    def _attend(self, qk, at, layer, s):
+        """Head norm, RoPE, cache fill and attention of a chunk in ``layer``."""
+        st, lib, m = self.state, self.state.lib, self.state.model
+        qk.q_norm_w, qk.k_norm_w = m.q_norm[layer].data_ptr(), m.k_norm[layer].data_ptr()
+        if not st.kv8:
+            qk.k_cache, qk.v_cache = st.k_cache[layer].data_ptr(), st.v_cache[layer].data_ptr()
+        lib.prefill_qk(qk, s)
+        if st.kv8:
+            held = dict(k_slab=qk.k_cache, v_slab=qk.v_cache, slab_cap=qk.cap, **st.kv8_held(layer))
+            lib.kv8_store(capi.Kv8StoreArgs(pos0=qk.pos0, n=qk.t_rows, **held), s)
+            lib.kv8_load(capi.Kv8LoadArgs(n=qk.pos0 + qk.t_rows, **held), s)
+        at.k_cache, at.v_cache = qk.k_cache, qk.v_cache
+        lib.prefill_attn(at, s)
 
     def _skinny_layers(self, R):
         """Every layer's four products over all R prompt rows (row b*S + t)
@@ -1209,10 +1288,13 @@ class Prefill:
             qk.qkv, qk.cos_tab, qk.sin_tab = self.qkv.data_ptr(), st.cos.data_ptr(), st.sin.data_ptr()
             qk.eps, qk.batch, qk.t_rows, qk.pos0 = c.eps, B, T, c0
             qk.nq, qk.nkv, qk.head_dim, qk.cap = c.nq, c.nkv, D, st.cap
+            if st.kv8:
+                k, v, qk.cap = self._kv_slabs(S)
+                qk.k_cache, qk.v_cache = k.data_ptr(), v.data_ptr()
             at = capi.PrefillAttnArgs()
             at.qkv, at.out, at.sm_scale = self.qkv.data_ptr(), self.att.data_ptr(), D ** -0.5
             at.batch, at.t_rows, at.pos0, at.nq, at.nkv = B, T, c0, c.nq, c.nkv
-            at.head_dim, at.cap, at.tiles = D, st.cap, tiles
+            at.head_dim, at.cap, at.tiles = D, qk.cap, tiles
             if wide or narrow:
                 at.tiles = -(-R // 16)  # the fragment order of qdec_gemm
                 product = lib.gemm_wide if wide else lib.gemm
@@ -1222,11 +1304,7 @@ class Prefill:
                                                 else (self._gemm_layers(R), None, 0, self.h))
                 for i, (g_qkv, g_o, g_gu, g_dn) in enumerate(layers):
                     product(g_qkv, s)
-                    qk.q_norm_w, qk.k_norm_w = m.q_norm[i].data_ptr(), m.k_norm[i].data_ptr()
-                    qk.k_cache, qk.v_cache = st.k_cache[i].data_ptr(), st.v_cache[i].data_ptr()
-                    lib.prefill_qk(qk, s)
-                    at.k_cache, at.v_cache = qk.k_cache, qk.v_cache
-                    lib.prefill_attn(at, s)
+                    self._attend(qk, at, i, s)
                     product(g_o, s)
                     product(g_gu, s)
                     product(g_dn, s)
@@ -1274,11 +1352,7 @@ class Prefill:
                 norm_rows(m.in_w[i])
                 g_qkv.w = m.w_qkv[i].data_ptr()
                 lib.prefill_gemm(g_qkv, s)
-                qk.q_norm_w, qk.k_norm_w = m.q_norm[i].data_ptr(), m.k_norm[i].data_ptr()
-                qk.k_cache, qk.v_cache = st.k_cache[i].data_ptr(), st.v_cache[i].data_ptr()
-                lib.prefill_qk(qk, s)
-                at.k_cache, at.v_cache = qk.k_cache, qk.v_cache
-                lib.prefill_attn(at, s)
+                self._attend(qk, at, i, s)
                 res_product(g_o, m.w_o[i], sp_o)
                 norm_rows(m.post_w[i])
                 g_gu.w = m.w_gu[i].data_ptr()

@@ -17,6 +17,8 @@ step replays are exercised:
   and the value row lands in cache slot 0;
 * the n-gram drafter and the acceptance rule on a short history with a
   known match;
+* for a shape with an 8-bit cache, its attention and its prompts' store and
+  read back (``run_shape``);
 * for a shape with tree passes, the tree's drafter, attention, acceptance and
   commit through the shape's own buffers (``run_tree``).
 
@@ -458,6 +460,99 @@ def _shape_attention(state, t):
     state.lens.zero_()
 
 
+def _shape_kv8(state, t):
+    """The 8-bit cache's attention of a step over t rows per sequence, as
+    ``_shape_attention``: one cached key of 127 s on two channels (held exactly)
+    draws the whole softmax weight, and the value rows are whole numbers whose
+    largest is 127, so that they are held exactly with scale 1.  Then the new rows
+    in the cache, and the slots before them through qdec_kv8_load and back
+    through qdec_kv8_store: the same bytes."""
+    m, lib, c = state.model, state.lib, state.model.cfg
+    dev = m.device
+    s = torch.cuda.current_stream(dev).cuda_stream
+    B, D, nkv, nq, cap = state.batch, c.head_dim, c.nkv, c.nq, state.cap
+    G, R = nq // nkv, B * t
+    g = torch.Generator(device="cpu").manual_seed(4242 + R)
+    qw = m.q_norm[0].float().cpu()
+    half = D // 2
+    j = max(range(8), key=lambda i: float(qw[half - 1 - i].abs() + qw[D - 1 - i].abs()))
+    i1, i2 = half - 1 - j, D - 1 - j
+    rstd = 1.0 / (2.0 / D + c.eps) ** 0.5
+    q1, q2 = float(qw[i1]) * rstd, float(qw[i2]) * rstd
+    if abs(q1) + abs(q2) < 1e-3:
+        _fail("8-bit attention", "q-norm weights of the lowest-frequency RoPE pairs are all ~0; no known-answer query")
+    alpha = 400.0 / ((D ** -0.5) * 1.4426950408889634 * (abs(q1) + abs(q2)))
+    lens = [max(1, cap - t - 1 - (37 * b) % max(1, cap // 4)) for b in range(B)]
+    hot = torch.tensor([[((b * 131 + h * 71 + 11) * 977) % lens[b] for h in range(nkv)] for b in range(B)])
+
+    def whole(*shape):  # value rows that 8 bits hold as they are
+        v = torch.randint(-127, 128, shape, generator=g)
+        v[..., 5] = 127
+        return v
+
+    k8, v8, ks, vs = state.k8[0], state.v8[0], state.k_scale[0], state.v_scale[0]
+    k8.zero_()
+    bi = torch.arange(B)[:, None].expand(B, nkv).reshape(-1).to(dev)
+    hi = torch.arange(nkv)[None, :].expand(B, nkv).reshape(-1).to(dev)
+    hs = hot.reshape(-1).to(dev)
+    hot_key = torch.zeros(D, dtype=torch.int8)
+    hot_key[i1] = 127 if q1 >= 0 else -127
+    hot_key[i2] = 127 if q2 >= 0 else -127
+    k8[bi, hi, hs] = hot_key.to(dev)
+    ks.fill_(alpha / 127.0)
+    few = whole(1, nkv, 97, D).to(dev, torch.int8)  # rows 0 .. 96 over and over
+    rows = few[:, :, torch.arange(cap, device=dev) % 97].expand(B, nkv, cap, D)
+    v8.copy_(rows.reshape(B, nkv, cap // 16, 16, D).transpose(3, 4))
+    vs.fill_(1.0)
+    past = torch.arange(cap, device=dev)[None] >= torch.tensor(lens, device=dev)[:, None]  # [B, cap]
+    ks.masked_fill_(past[:, None], float("nan"))
+    vs.masked_fill_(past[:, None], float("nan"))
+    qkv = torch.zeros((R, c.n_qkv), dtype=torch.bfloat16)
+    qkv[:, [h * D + i1 for h in range(nq)]] = 1.0
+    qkv[:, [h * D + i2 for h in range(nq)]] = 1.0
+    vnew = whole(R, nkv, D)
+    qkv[:, (nq + nkv) * D:] = vnew.view(R, nkv * D).to(torch.bfloat16)
+    state.qkv[:R].copy_(qkv.to(dev))
+    state.lens.copy_(torch.tensor(lens, dtype=torch.int32, device=dev))
+    hv = rows[bi, hi, hs].view(B, nkv, D)
+    want = hv.repeat_interleave(G, 1).reshape(B, 1, nq * D).expand(B, t, nq * D).reshape(R, nq * D).to(torch.bfloat16)
+    a = state._kv8_args(0, t)
+    lib.kv8_attn(a, s)
+    got = _get_rows(state.attn_out, R, nq * D, a.out_frag)
+    if not torch.equal(got, want):
+        bad = int((got != want).any(-1).sum())
+        _fail("8-bit attention", f"{R} rows: {bad} rows differ from the hot slot's value row")
+    pos = torch.tensor(lens)[:, None] + torch.arange(t)[None, :]  # [B, t]
+    b3 = torch.arange(B)[:, None, None].expand(B, t, nkv).reshape(-1).to(dev)
+    h3 = torch.arange(nkv)[None, None, :].expand(B, t, nkv).reshape(-1).to(dev)
+    p3 = pos[:, :, None].expand(B, t, nkv).reshape(-1).to(dev)
+    if not (torch.equal(v8[b3, h3, p3 // 16, :, p3 % 16].long().cpu(), vnew.reshape(-1, D))
+            and bool((vs[b3, h3, p3] == 1.0).all())):
+        _fail("8-bit attention", f"{R} rows: new value rows not written to their cache slots")
+    if bool((k8[b3, h3, p3] != 0).any()) or bool((ks[b3, h3, p3] != 0).any()):
+        _fail("8-bit attention", f"{R} rows: new (zero) key rows not written to their cache slots")
+    # ---- the shortest sequence's slots read back and stored again
+    n = min(lens)
+    slots = -(-n // 32) * 32
+    k, v = (torch.zeros((B, nkv, slots, D), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    held = dict(k_slab=k.data_ptr(), v_slab=v.data_ptr(), slab_cap=slots, n=n, **state.kv8_held(0))
+    before = [x.clone() for x in (k8, v8, ks, vs)]
+    lib.kv8_load(capi.Kv8LoadArgs(**held), s)
+    back = v.view(B, nkv, slots // 8, D, 8).transpose(3, 4).reshape(B, nkv, slots, D)[:, :, :n]
+    if not torch.equal(back, rows[:, :, :n].to(torch.bfloat16)):
+        _fail("kv8_load", f"{int((back != rows[:, :, :n]).sum())} of {back.numel()} values differ")
+    k8[:, :, :n].zero_()
+    v8.zero_()
+    lib.kv8_store(capi.Kv8StoreArgs(pos0=0, **held), s)
+    again = v8.transpose(3, 4).reshape(B, nkv, cap, D)[:, :, :n]
+    if not (torch.equal(k8, before[0]) and torch.equal(again, rows[:, :, :n]) and bool((vs[:, :, :n] == 1.0).all())
+            and torch.equal(vs[:, :, n:].nan_to_num(7.0), before[3][:, :, n:].nan_to_num(7.0))):
+        _fail("kv8_store", "slots read back and stored again differ")
+    for x in (k8, v8, ks, vs):
+        x.zero_()
+    state.lens.zero_()
+
+
 def run_shape(state, t_rows=(1,)):
     """Known-answer checks of one decode shape's own launch plans, on its own
     buffers, before it serves (the reference checks each new shape's fused
@@ -484,7 +579,7 @@ def run_shape(state, t_rows=(1,)):
         if not torch.equal(state.h[:R].float(), _tiled_rows(m.emb, c.vocab, c.hidden, ids)):
             _fail("embed", f"{R} rows: gathered rows differ from the embedding")
         _shape_gemms(state, t)
-        _shape_attention(state, t)
+        (_shape_kv8 if state.kv8 else _shape_attention)(state, t)
     torch.cuda.synchronize(dev)
 
 

@@ -157,8 +157,9 @@ class Qwen3Oracle:
     bf16 checkpoints stay exactly representable in fp32).  ``cfg`` is the HF
     config dict."""
 
-    def __init__(self, cfg, tensors, mode="bf16", attn="decode"):
+    def __init__(self, cfg, tensors, mode="bf16", attn="decode", hold=lambda rows: rows):
         self.mode, self.attn = mode, attn
+        self.hold = hold  # what a cache makes of the key and value rows [..., D] written to it
         self.hidden = cfg["hidden_size"]
         self.inter = cfg["intermediate_size"]
         self.n_layers = cfg["num_hidden_layers"]
@@ -228,8 +229,8 @@ class Qwen3Oracle:
             q = head_norm_rope(q, ly["qn"], cos, sin, self.eps, mode)
             k = head_norm_rope(k, ly["kn"], cos, sin, self.eps, mode)
             for b in range(B):
-                kc[i, b, :, pos[b]] = k[b].transpose(0, 1)
-                vc[i, b, :, pos[b]] = v[b].transpose(0, 1)
+                kc[i, b, :, pos[b]] = self.hold(k[b].transpose(0, 1))
+                vc[i, b, :, pos[b]] = self.hold(v[b].transpose(0, 1))
             # [B, nkv, G*T, D] query rows grouped by kv head
             qg = q.permute(0, 2, 1, 3).reshape(B, self.nkv, G, T, self.d).reshape(B, self.nkv, G * T, self.d)
             vis = visible[:, None, None, :, :].expand(B, 1, G, T, cap).reshape(B, 1, G * T, cap)
