@@ -998,6 +998,8 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
   if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->k8 || !a->v8 || !a->k_scale ||
       !a->v_scale || !a->out)
     return set_error(QDEC_EINVAL, "qdec_kv8_attn: null pointer argument");
+  if (!(p->scale_log2 > 0.f) || !std::isfinite(p->scale_log2))
+    return set_error(QDEC_EINVAL, "qdec_kv8_attn: sm_scale %g is not positive and finite", (double)a->sm_scale);
   if (p->splits > 1 && !a->partial) return set_error(QDEC_EINVAL, "qdec_kv8_attn: more than one split needs partial");
   if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
       !aligned16(a->sin_tab) || !aligned16(a->k8) || !aligned16(a->v8) || !aligned16(a->k_scale) || !aligned16(a->v_scale) ||

@@ -52,13 +52,8 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_store_kernel(const Kv8CopyPar
     if constexpr (LPR == 16) top = fmaxf(top, dpp_f<0x140>(top));
     const uint64_t bad = __ballot(!fin) >> (lane & ~(LPR - 1));
     fin = (bad & ((1ull << LPR) - 1)) == 0;
-    const float div = kv8_div(top, fin);
-    uint2 q = make_uint2(0u, 0u);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      q.x |= kv8_round(x[e], div) << (8 * e);
-      q.y |= kv8_round(x[4 + e], div) << (8 * e);
-    }
+    const Kv8Div div(top, fin);
+    const uint2 q = make_uint2(div.four(x[0], x[1], x[2], x[3]), div.four(x[4], x[5], x[6], x[7]));
     if (in) {
       *reinterpret_cast<uint2 *>(k8 + (size_t)slot * D + ch) = q;
       if (lane % LPR == 0) kscale[slot] = kv8_scale(top, fin);
@@ -91,9 +86,9 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_store_kernel(const Kv8CopyPar
     }
     top = wave_max(top);
     fin = __all(fin);
-    const float div = kv8_div(top, fin);
+    const Kv8Div div(top, fin);
 #pragma unroll
-    for (int j = 0; j < CPL; ++j) q[j][i >> 2] |= kv8_round(x[j], div) << (8 * (i & 3));
+    for (int j = 0; j < CPL; ++j) q[j][i >> 2] |= (div.one(x[j]) & 0xffu) << (8 * (i & 3));
     const int slot = s0 + i;
     if (lane == 0 && slot >= p.pos0 && slot < s1) vscale[slot] = kv8_scale(top, fin);
   }

@@ -2,8 +2,9 @@
 // quantised write of the new rows folded in: t_rows query rows per sequence,
 // row t at position lens[b] + t over slots 0 .. lens[b] + t.
 //
-// A workgroup of 8 waves takes up to 16 query rows and the 64-slot blocks j = c,
-// c + splits, ... of one (sequence, kv head), its wave w every eighth of those.  Blocks are dealt by
+// A workgroup of 8 waves takes up to 16 query rows of one (sequence, kv head) and
+// the runs c, c + splits, ... of 8 consecutive 64-slot blocks, its wave w one block
+// of each.  Blocks are dealt by
 // absolute slot numbers and a row is rescaled by its own scores alone, so a
 // row's bits do not depend on t_rows.  Per block
 // (v_mfma_f32_16x16x32_f16):
@@ -31,7 +32,6 @@ namespace qdec {
 namespace {
 
 constexpr int kW = 8;       // waves of a workgroup
-constexpr int kPad = 8;     // fp16 behind an LDS query row (bank spread)
 
 __device__ __forceinline__ f32x4_t mfma_f16(const f16x8_t &a, const f16x8_t &b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -61,60 +61,80 @@ __device__ __forceinline__ void to_f16(const uint4 &v, f16x8_t &a, f16x8_t &b) {
 template <int I>
 __device__ __forceinline__ float row_lane(float v) { return dpp_f<0x150 + I>(v); }
 
+// The value of lane ^ X (16 or 32).
+template <int X>
+__device__ __forceinline__ float lane_xor(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const bool low = !(threadIdx.x & X);
+  if constexpr (X == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(low ? r[1] : r[0]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(low ? r[1] : r[0]);
+  }
+}
+__device__ __forceinline__ float sum_xor16_32(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // Head RMSNorm and RoPE of channels 2 lane, 2 lane + 1 of a row, in fp32 (lanes
 // from D / 2 on pass raw = 0).
 template <int D>
 __device__ __forceinline__ void norm_rope(uint32_t raw, uint32_t w, uint32_t cw, uint32_t sw, float eps, float &o0, float &o1) {
-  const int lane = threadIdx.x & 63;
   const float x0 = lo16(raw), x1 = hi16(raw);
   const float rstd = 1.0f / sqrtf(wave_sum(x0 * x0 + x1 * x1) / (float)D + eps);
   const float y0 = x0 * rstd * lo16(w), y1 = x1 * rstd * hi16(w);
-  const float p0 = shfl_xor(y0, D / 4), p1 = shfl_xor(y1, D / 4);
-  const bool first = (lane & (D / 2 - 1)) < D / 4;
-  o0 = y0 * lo16(cw) + (first ? -p0 : p0) * lo16(sw);
-  o1 = y1 * hi16(cw) + (first ? -p1 : p1) * hi16(sw);
+  // the first half's partner counts negative
+  const float sign = (threadIdx.x & (D / 4)) ? 1.f : -1.f;
+  o0 = y0 * lo16(cw) + lane_xor<D / 4>(y0) * (sign * lo16(sw));
+  o1 = y1 * hi16(cw) + lane_xor<D / 4>(y1) * (sign * hi16(sw));
 }
 
 // A row's power-of-two factor: 2^-e with 2^e <= max|x| < 2^(e+1), and 2^e.
 __device__ __forceinline__ void pow2_of(float top, float &down, float &up) {
-  const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 120);
-  down = __uint_as_float((uint32_t)(127 - e) << 23);
-  up = __uint_as_float((uint32_t)(127 + e) << 23);
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 27), 247);
+  down = __uint_as_float((uint32_t)(254 - e) << 23);
+  up = __uint_as_float((uint32_t)e << 23);
 }
 
-template <int D>
-struct Frag {  // one block
-  uint4 k[4][D / 64];  // MFMA rows tile: row r = slot 16 (r >> 2) + 4 tile + (r & 3); 16 channels 64 h + 16 grp
-  uint4 v[D / 16];     // channel 16 dt + col, slots 16 grp .. + 15
-  float ks, vs;        // scales of slot `lane`
-};
+// A row held in 8 bits: this lane's two values in the low bytes of q; its scale.
+__device__ __forceinline__ float hold2(float x0, float x1, uint32_t &q) {
+  const float top = wave_max(fmaxf(fabsf(x0), fabsf(x1)));
+  const bool fin = __all(finite_f(x0) && finite_f(x1));
+  const Kv8Div div(top, fin);
+  q = __builtin_amdgcn_perm(div.one(x1), div.one(x0), 0x0c0c0400u);
+  return kv8_scale(top, fin);
+}
 
 // LDS (bytes).
-template <int D>
+template <int D, bool PK>
 struct Lds {
-  static constexpr int RS = D + kPad;
-  static constexpr int q = 0;                            // [2][16][RS] fp16 query parts; then wave sums [kW][D / 16][64] f32x4
-  static constexpr int qn = 2 * 16 * RS * 2;
-  static constexpr int an = kW * (D / 16) * 64 * 16;
-  static constexpr int qs = q + (qn > an ? qn : an);     // [16] query rows' factors
-  static constexpr int k8 = qs + 16 * 4;                 // [kKv8MaxT][D]
-  static constexpr int v8 = k8 + kKv8MaxT * D;           // [2][D][16]
-  static constexpr int sk = v8 + 2 * D * 16;             // [kKv8MaxT]
+  static constexpr int RS = D + 8;                               // fp16 per query row (bank spread)
+  static constexpr int AC = PK ? 8 : 16;                         // columns of the sums
+  static constexpr int q = 0;                                    // [2][AC][RS] fp16 parts of the queries
+  static constexpr int acc = q + 2 * AC * RS * 2;                // [kW][D / 16][4][AC] f32x4
+  static constexpr int qs = acc + kW * (D / 16) * 4 * AC * 16;   // [16] query rows' factors
+  static constexpr int k8 = qs + 16 * 4;                         // [kKv8MaxT][D]
+  static constexpr int v8 = k8 + kKv8MaxT * D;                   // [2][D][16]
+  static constexpr int sk = v8 + 2 * D * 16;                     // [kKv8MaxT]
   static constexpr int sv = sk + kKv8MaxT * 4;
-  static constexpr int m = sv + kKv8MaxT * 4;            // [3][kW][16] wave statistics: maximum, sum, unit
+  static constexpr int m = sv + kKv8MaxT * 4;                    // [3][16][kW] wave statistics: maximum, sum, unit
   static constexpr int bytes = m + 3 * kW * 16 * 4;
 };
 
 // PK: at most 8 query rows in all, both parts in one tile.
 template <int D, bool PK>
 __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p) {
-  constexpr int NH = D / 64, DT = D / 16, LH = D / 2;
-  constexpr int QPW = 16 / kW, KPW = kKv8MaxT / kW;
-  using LY = Lds<D>;
-  constexpr int RS = LY::RS;
+  constexpr int NH = D / 64, DT = D / 16;
+  using LY = Lds<D, PK>;
+  constexpr int RS = LY::RS, AC = LY::AC;
   __shared__ __attribute__((aligned(16))) unsigned char smem[LY::bytes];
   _Float16 *s_q = reinterpret_cast<_Float16 *>(smem + LY::q);
-  f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::q);
+  f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::acc);
   float *s_qs = reinterpret_cast<float *>(smem + LY::qs);
   unsigned char *s_k8 = smem + LY::k8, *s_v8 = smem + LY::v8;
   float *s_sk = reinterpret_cast<float *>(smem + LY::sk), *s_sv = reinterpret_cast<float *>(smem + LY::sv);
@@ -131,28 +151,46 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   int8_t *k8 = p.k8 + cell * p.cap * D, *v8 = p.v8 + cell * p.cap * D;
   float *kscale = p.k_scale + cell * p.cap, *vscale = p.v_scale + cell * p.cap;
   const float NEG_INF = -__builtin_huge_valf();
-  const int blocks = p.cap / kKv8Block;
 
-  auto load_block = [&](int j, Frag<D> &f) {
+  // One block's keys, values and scales.  MFMA row r of K's tile t is slot 16 (r
+  // >> 2) + 4 t + (r & 3), its channels 64 h + 16 grp .. + 15; V's are channel 16 dt +
+  // col, slots 16 grp .. + 15; the scales those of slot `lane`.
+  uint4 kf[4][NH], vf[DT];
+  float ks, vs;
+  auto load_k = [&](int j) {
     const int s0 = j * kKv8Block;
     const int8_t *kb = k8 + (size_t)(s0 + 16 * (col >> 2) + (col & 3)) * D + 16 * grp;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int h = 0; h < NH; ++h) f.k[t][h] = ld_nt(kb + (4 * t) * D + 64 * h);
+      for (int h = 0; h < NH; ++h) kf[t][h] = ld_nt(kb + (4 * t) * D + 64 * h);
+    ks = __builtin_nontemporal_load(kscale + s0 + lane);
+  };
+  auto load_v = [&](int j) {
+    const int s0 = j * kKv8Block;
     const int8_t *vb = v8 + ((size_t)((s0 >> 4) + grp) * D + col) * 16;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) f.v[dt] = ld_nt(vb + dt * 256);
-    f.ks = kscale[s0 + lane];
-    f.vs = vscale[s0 + lane];
+    for (int dt = 0; dt < DT; ++dt) vf[dt] = ld_nt(vb + dt * 256);
+    vs = __builtin_nontemporal_load(vscale + s0 + lane);
   };
-  // This wave's i-th block; the first one's addresses do not depend on the length.
-  auto nth = [&](int i) { return c + C * (wave + kW * i); };
-  Frag<D> f0, f1;
-  if (nth(0) < blocks) load_block(nth(0), f0);
-
+  // This wave's first block, and one round's step.
+  const int j0 = kW * c + wave, step = kW * C;
+  // Rows to prepare: this tile's queries, then the new keys and values (for a
+  // workgroup that takes some of their blocks); row i on wave 7 - i % 8.  Waves with rows
+  // ask for their blocks behind them, the others at once: the first block's
+  // addresses do not depend on the length.
+  const int first = kW - 1 - wave;
+  const bool late = first < nr + T;
+  if (!late && j0 < p.cap / kKv8Block) {
+    load_k(j0);
+    load_v(j0);
+  }
+  const int ch = 2 * min(lane, D / 2 - 1);
+  const bool lv = lane < D / 2;
+  const uint16_t *rows = p.qkv + (size_t)b * T * width;
+  auto pair = [&](const uint16_t *x) { return *reinterpret_cast<const uint32_t *>(x + ch); };
   const int L = p.lens[b];
-  if (L < 0 || L > p.cap - T) {  // no cache access; the rows become NaN
+  if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
     if (c == 0)
       for (int i = threadIdx.x; i < nr * (D / 4); i += blockDim.x) {
         const int y = i / (D / 4), ch = (i - y * (D / 4)) * 4, r = r0 + y, row = b * T + r / G, k = (kvh * G + r % G) * D + ch;
@@ -162,66 +200,47 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     return;
   }
   const int last = L + T - 1, nb = last / kKv8Block + 1;
-  if (c >= nb) return;
-  if (nth(1) < nb) load_block(nth(1), f1);
-
-  // ---- the query rows in two fp16 parts, the new keys and values in 8 bits, to LDS
-  const int ch = 2 * min(lane, LH - 1);
-  const bool lv = lane < LH;
-  const uint16_t *rows = p.qkv + (size_t)b * T * width;
-  auto pair = [&](const uint16_t *x) { return *reinterpret_cast<const uint32_t *>(x + ch); };
-  const uint32_t qw = pair(p.q_norm_w), kw = pair(p.k_norm_w);
-  for (int i = 0; i < QPW; ++i) {
-    const int y = wave + kW * i, r = r0 + y;
-    if (y >= nr) break;
-    const int t = r / G, h = kvh * G + r - t * G;
+  if (kW * c >= nb) return;
+  const bool mine = (L / (kW * kKv8Block)) % C == c || ((nb - 1) / kW) % C == c;  // takes some of the new rows' blocks
+  const int jobs = mine ? nr + T : nr;
+  for (int i = first; i < jobs; i += kW) {
+    const bool query = i < nr;
+    const int r = r0 + i, t = query ? r / G : i - nr, head = query ? kvh * G + r - t * G : nq + kvh;
+    const uint16_t *x = rows + (size_t)t * width + (size_t)head * D;
+    const uint32_t raw = pair(x), vraw = query ? 0u : pair(x + (size_t)nkv * D), w = pair(query ? p.q_norm_w : p.k_norm_w);
+    const uint32_t cw = pair(p.cos_tab + (size_t)(L + t) * D), sw = pair(p.sin_tab + (size_t)(L + t) * D);
     float x0, x1;
-    norm_rope<D>(lv ? pair(rows + (size_t)t * width + (size_t)h * D) : 0u, qw, pair(p.cos_tab + (size_t)(L + t) * D),
-                 pair(p.sin_tab + (size_t)(L + t) * D), p.eps, x0, x1);
-    float down, up;
-    pow2_of(wave_max(lv ? fmaxf(fabsf(x0), fabsf(x1)) : 0.f), down, up);
-    x0 *= down;
-    x1 *= down;
-    const f16x2_t hi = {(_Float16)x0, (_Float16)x1};
-    const f16x2_t lo = {(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])};
-    if (lv) {
-      *reinterpret_cast<f16x2_t *>(s_q + y * RS + ch) = hi;
-      *reinterpret_cast<f16x2_t *>(s_q + (16 + y) * RS + ch) = lo;
-    }
-    if (lane == 0) s_qs[y] = up * p.scale_log2;
-  }
-  const int b_lo = L / kKv8Block, b_hi = last / kKv8Block;  // (new rows lie in two blocks at most)
-  const bool mine = b_lo % C == c || b_hi % C == c;
-  if (mine) {
-    for (int i = 0; i < KPW; ++i) {
-      const int t = wave + kW * i;
-      if (t >= T) break;
-      const uint16_t *x = rows + (size_t)t * width + (size_t)(nq + kvh) * D;
-      const uint32_t vr = lv ? pair(x + (size_t)nkv * D) : 0u;
-      float k0, k1;
-      norm_rope<D>(lv ? pair(x) : 0u, kw, pair(p.cos_tab + (size_t)(L + t) * D), pair(p.sin_tab + (size_t)(L + t) * D), p.eps,
-                   k0, k1);
-      if (!lv) k0 = k1 = 0.f;
-      const float v0 = lo16(vr), v1 = hi16(vr);
-      const float kt = wave_max(fmaxf(fabsf(k0), fabsf(k1))), vt = wave_max(fmaxf(fabsf(v0), fabsf(v1)));
-      const bool kf = __all(finite_f(k0) && finite_f(k1)), vf = __all(finite_f(v0) && finite_f(v1));
-      const float kd = kv8_div(kt, kf), vd = kv8_div(vt, vf);
-      const uint32_t q0 = kv8_round(k0, kd), q1 = kv8_round(k1, kd), w0 = kv8_round(v0, vd), w1 = kv8_round(v1, vd);
-      const int slot = L + t, gi = (slot >> 4) - (L >> 4), e = slot & 15;
-      const bool put = tile == 0 && (slot / kKv8Block) % C == c;
+    norm_rope<D>(lv ? raw : 0u, w, cw, sw, p.eps, x0, x1);
+    if (query) {
+      float down, up;
+      pow2_of(wave_max(lv ? fmaxf(fabsf(x0), fabsf(x1)) : 0.f), down, up);
+      x0 *= down;
+      x1 *= down;
+      const f16x2_t hi = {(_Float16)x0, (_Float16)x1};
+      const f16x2_t lo = {(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])};
       if (lv) {
-        *reinterpret_cast<uint16_t *>(s_k8 + t * D + ch) = (uint16_t)(q0 | (q1 << 8));
-        s_v8[(gi * D + ch) * 16 + e] = (unsigned char)w0;
-        s_v8[(gi * D + ch + 1) * 16 + e] = (unsigned char)w1;
+        *reinterpret_cast<f16x2_t *>(s_q + i * RS + ch) = hi;
+        *reinterpret_cast<f16x2_t *>(s_q + (AC + i) * RS + ch) = lo;
+      }
+      if (lane == 0) s_qs[i] = up * p.scale_log2;
+    } else {
+      const int slot = L + t, e = slot & 15;
+      const bool put = tile == 0 && (slot / (kW * kKv8Block)) % C == c;
+      uint32_t kq, vq;
+      const float sk = hold2(lv ? x0 : 0.f, lv ? x1 : 0.f, kq), sv = hold2(lv ? lo16(vraw) : 0.f, lv ? hi16(vraw) : 0.f, vq);
+      if (lv) {
+        unsigned char *vl = s_v8 + (((slot >> 4) - (L >> 4)) * D + ch) * 16 + e;
+        *reinterpret_cast<uint16_t *>(s_k8 + t * D + ch) = (uint16_t)kq;
+        vl[0] = (unsigned char)vq;
+        vl[16] = (unsigned char)(vq >> 8);
         if (put) {
-          *reinterpret_cast<uint16_t *>(k8 + (size_t)slot * D + ch) = (uint16_t)(q0 | (q1 << 8));
-          int8_t *vo = v8 + ((size_t)(slot >> 4) * D + ch) * 16 + e;
-          vo[0] = (int8_t)w0;
-          vo[16] = (int8_t)w1;
+          int8_t *vg = v8 + ((size_t)(slot >> 4) * D + ch) * 16 + e;
+          *reinterpret_cast<uint16_t *>(k8 + (size_t)slot * D + ch) = (uint16_t)kq;
+          vg[0] = (int8_t)vq;
+          vg[16] = (int8_t)(vq >> 8);
         }
       }
       if (lane == 0) {
-        const float sk = kv8_scale(kt, kf), sv = kv8_scale(vt, vf);
         s_sk[t] = sk;
         s_sv[t] = sv;
         if (put) {
@@ -231,6 +250,10 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       }
     }
   }
+  if (late && j0 < nb) {
+    load_k(j0);
+    load_v(j0);
+  }
   lds_barrier();
 
   // ---- this wave's blocks
@@ -238,8 +261,9 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const bool row_in = y < nr;
   const float qs = row_in ? s_qs[y] : 0.f;
   const int lim = row_in ? L + (r0 + y) / G : -1;  // the last slot the row sees
-  float m_run = NEG_INF, l_run = 0.f;
-  int unit = -200;  // 2^unit > |w| so far
+  // Of the blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
+  // units of 2^(unit - 15).
+  float m_run = NEG_INF, l_run = 0.f, unit = NEG_INF;
   f32x4_t acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -251,55 +275,54 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     for (int e = 0; e < 2; ++e) {
       auto part = [&](int i) {
         const f16x8_t z = {};
-        return row_in ? *reinterpret_cast<const f16x8_t *>(s_q + (16 * i + y) * RS + 64 * h + 16 * grp + 8 * e) : z;
+        return row_in ? *reinterpret_cast<const f16x8_t *>(s_q + (AC * i + y) * RS + 64 * h + 16 * grp + 8 * e) : z;
       };
       qh[h][e] = part(PK ? col >> 3 : 0);
       if constexpr (!PK) ql[h][e] = part(1);
     }
-
-  // The new rows of a block that holds some, from LDS.
-  auto patch = [&](Frag<D> &f, int s0) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int i = s0 + 16 * (col >> 2) + 4 * t + (col & 3) - L;
-      const bool is = (unsigned)i < (unsigned)T;
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(s_k8 + min(max(i, 0), kKv8MaxT - 1) * D + 64 * h + 16 * grp);
-        if (is) f.k[t][h] = x;
-      }
-    }
-    const int v0 = s0 + 16 * grp, gi = min(max((v0 >> 4) - (L >> 4), 0), 1);
-    uint32_t take[4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      take[d] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int s = v0 + 4 * d + e;
-        if (s >= L && s <= last) take[d] |= 0xffu << (8 * e);
-      }
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const uint4 x = *reinterpret_cast<const uint4 *>(s_v8 + (gi * D + dt * 16 + col) * 16);
-      uint4 &v = f.v[dt];
-      v.x = (v.x & ~take[0]) | (x.x & take[0]);
-      v.y = (v.y & ~take[1]) | (x.y & take[1]);
-      v.z = (v.z & ~take[2]) | (x.z & take[2]);
-      v.w = (v.w & ~take[3]) | (x.w & take[3]);
-    }
-    const int i = s0 + lane - L;
-    if ((unsigned)i < (unsigned)T) {
-      f.ks = s_sk[i];
-      f.vs = s_sv[i];
-    }
+  auto each = [&](auto fn) {
+    fn(Int<0>{}); fn(Int<1>{}); fn(Int<2>{}); fn(Int<3>{}); fn(Int<4>{}); fn(Int<5>{}); fn(Int<6>{}); fn(Int<7>{});
+    fn(Int<8>{}); fn(Int<9>{}); fn(Int<10>{}); fn(Int<11>{}); fn(Int<12>{}); fn(Int<13>{}); fn(Int<14>{}); fn(Int<15>{});
   };
 
-  auto process = [&](Frag<D> &f, int j) {
+  for (int j = j0; j < nb; j += step) {
     const int s0 = j * kKv8Block;
-    const bool edge = s0 + kKv8Block > L;  // slots that not every row sees
-    if (edge) patch(f, s0);
+    const bool edge = s0 + kKv8Block > L;  // slots that not every row sees, the new rows among them
+    if (edge) {                            // which come from LDS
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = s0 + 16 * (col >> 2) + 4 * t + (col & 3) - L;
+        const bool is = (unsigned)i < (unsigned)T;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(s_k8 + min(max(i, 0), kKv8MaxT - 1) * D + 64 * h + 16 * grp);
+          if (is) kf[t][h] = x;
+        }
+      }
+      const int v0 = s0 + 16 * grp, gi = min(max((v0 >> 4) - (L >> 4), 0), 1);
+      // byte i of this lane's 16: slot v0 + i, a new row's from L to `last`
+      auto from = [&](int s, int d) {  // dword d's bytes from slot s on
+        const int n = min(max(s - v0 - 4 * d, 0), 4);
+        return (uint32_t)(0xffffffffull << (8 * n));
+      };
+      uint32_t take[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d) take[d] = from(L, d) & ~from(last + 1, d);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(s_v8 + (gi * D + dt * 16 + col) * 16);
+        uint4 &v = vf[dt];
+        v.x = (v.x & ~take[0]) | (x.x & take[0]);
+        v.y = (v.y & ~take[1]) | (x.y & take[1]);
+        v.z = (v.z & ~take[2]) | (x.z & take[2]);
+        v.w = (v.w & ~take[3]) | (x.w & take[3]);
+      }
+      const int i = s0 + lane - L;
+      if ((unsigned)i < (unsigned)T) {
+        ks = s_sk[i];
+        vs = s_sv[i];
+      }
+    }
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -307,7 +330,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         f16x8_t a[2];
-        to_f16(f.k[t][h], a[0], a[1]);
+        to_f16(kf[t][h], a[0], a[1]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           hi = mfma_f16(a[e], qh[h][e], hi);
@@ -321,106 +344,108 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       }
     }
     // lane (col, grp) holds slots s0 + 16 grp + i of its row
-    auto each = [&](auto fn) {
-      fn(Int<0>{}); fn(Int<1>{}); fn(Int<2>{}); fn(Int<3>{}); fn(Int<4>{}); fn(Int<5>{}); fn(Int<6>{}); fn(Int<7>{});
-      fn(Int<8>{}); fn(Int<9>{}); fn(Int<10>{}); fn(Int<11>{}); fn(Int<12>{}); fn(Int<13>{}); fn(Int<14>{}); fn(Int<15>{});
-    };
-    const int seen = lim - s0 - 16 * grp;  // of them, those up to here
-    float top = NEG_INF;
     each([&](auto n) {
       constexpr int i = decltype(n)::value;
-      s[i] = s[i] * row_lane<i>(f.ks) * qs;
-      if (edge && i > seen) s[i] = NEG_INF;
-      top = fmaxf(top, s[i]);
+      s[i] *= row_lane<i>(ks);
+      pin(s[i]);
     });
-    const float m_new = fmaxf(m_run, max_xor16_32(top));
-    const float m_sub = m_new == NEG_INF ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_sub);
+    if (j + step < nb) load_k(j + step);
+    // of them, those up to `seen` (pins: a branch around the selects, not sixteen in every block)
+    int seen = lim - s0 - 16 * grp;
+    if (edge) {
+      pin(seen);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = i > seen ? NEG_INF : s[i];
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    const float m_old = m_run;
+    m_run = fmaxf(m_run, max_xor16_32(top));
+    const float mq = m_run == NEG_INF ? 0.f : m_run * qs;
     float psum = 0.f, big = 0.f;
     each([&](auto n) {
       constexpr int i = decltype(n)::value;
-      const float e = __builtin_amdgcn_exp2f(s[i] - m_sub);
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, -mq));
       psum += e;
-      const float w = e * row_lane<i>(f.vs);
-      s[i] = edge && i > seen ? 0.f : w;
-      big = fmaxf(big, s[i]);
+      s[i] = e * row_lane<i>(vs);
     });
+    if (edge) {
+      pin(seen);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = i > seen ? 0.f : s[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) big = fmaxf(big, s[i]);
+    const float alpha = m_old == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m_old - m_run) * qs);
     l_run = l_run * alpha + psum;
-    // The unit: above this block's w and, moved to the new maximum, above the old.
-    big = max_xor16_32(big);
-    const int ub = (int)(__float_as_uint(big) >> 23) - 126;
-    const int uo = unit - (int)fminf(m_new - m_run, 1000.f);
-    const int un = min(max(max(ub, uo), -100), 125);
-    const float ra = __builtin_ldexpf(alpha, max(unit - un, -300));
-    m_run = m_new;
-    unit = un;
-    const float to = __uint_as_float((uint32_t)(127 + 15 - un) << 23);
+    const float u_old = unit;
+    unit = fmaxf(unit, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
+    const float up = unit == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mq - unit + 15.f);
     f16x8_t w[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      w[0][e] = (_Float16)(s[e] * to);
-      w[1][e] = (_Float16)(s[8 + e] * to);
+      w[0][e] = (_Float16)(s[e] * up);
+      w[1][e] = (_Float16)(s[8 + e] * up);
+    }
+    if (__any(u_old < unit)) {
+      const float ra = u_old < unit ? __builtin_amdgcn_exp2f(u_old - unit) : 1.f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] *= ra;
     }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       f16x8_t a[2];
-      to_f16(f.v[dt], a[0], a[1]);
-      acc[dt] *= ra;
+      to_f16(vf[dt], a[0], a[1]);
       acc[dt] = mfma_f16(a[0], w[0], acc[dt]);
       acc[dt] = mfma_f16(a[1], w[1], acc[dt]);
     }
-  };
-  for (int i = 0; nth(i) < nb; i += 2) {
-    process(f0, nth(i));
-    if (nth(i + 2) < nb) load_block(nth(i + 2), f0);
-    if (nth(i + 1) < nb) {
-      process(f1, nth(i + 1));
-      if (nth(i + 3) < nb) load_block(nth(i + 3), f1);
-    }
+    if (j + step < nb) load_v(j + step);
   }
 
   // ---- the waves' sums, in wave order; then the output or a partial: the
   // normalised row, its maximum and its sum.
-  const int n_active = min(C, nb);
-  float *part = p.partial + (cell * C + c) * (size_t)(R * (D + 2));
-  const int r = r0 + y;
-  const bool out_in = row_in && !(PK && col >= 8);
-  float lw = l_run + shfl_xor(l_run, 16);
-  lw += shfl_xor(lw, 32);
-  lds_barrier();  // the queries have been read
-  if (grp == 0) {
-    s_m[wave * 16 + col] = m_run;
-    s_m[(kW + wave) * 16 + col] = lw;
-    s_m[(2 * kW + wave) * 16 + col] = __int_as_float(unit);
-  }
+  const int n_active = min(C, (nb + kW - 1) / kW), nw = min(nb - kW * c, kW);  // waves that had blocks
+  if (col < AC) {
+    const float lw = sum_xor16_32(l_run);
+    if (grp == 0) {
+      s_m[col * kW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
+      s_m[(16 + col) * kW + wave] = lw;
+      s_m[(32 + col) * kW + wave] = unit;
+    }
+    if (wave < nw) {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) s_acc[(wave * DT + dt) * 64 + lane] = acc[dt];
+      for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
+    }
+  }
   lds_barrier();
-  float M = NEG_INF, sum = 0.f, fac[kW];
-  int U = -1000;
+  if (!row_in || (PK && col >= 8)) return;
+  float mw[kW], lw[kW], uw[kW], M = NEG_INF, U = NEG_INF, sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < kW; ++w) M = fmaxf(M, s_m[w * 16 + col]);
+  for (int w = 0; w < kW; w += 4) {
+    *reinterpret_cast<f32x4_t *>(mw + w) = *reinterpret_cast<const f32x4_t *>(s_m + col * kW + w);
+    *reinterpret_cast<f32x4_t *>(lw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (16 + col) * kW + w);
+    *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * kW + w);
+  }
 #pragma unroll
   for (int w = 0; w < kW; ++w) {
-    const float mw = s_m[w * 16 + col];
-    if (mw != NEG_INF) U = max(U, __float_as_int(s_m[(2 * kW + w) * 16 + col]) - (int)fminf(M - mw, 1000.f));
+    M = fmaxf(M, mw[w]);
+    U = fmaxf(U, uw[w]);
   }
-  U = min(max(U, -100), 125);
 #pragma unroll
   for (int w = 0; w < kW; ++w) {
-    const float mw = s_m[w * 16 + col], l = s_m[(kW + w) * 16 + col];
-    const float e = mw == NEG_INF ? l * 0.f : __builtin_amdgcn_exp2f(mw - M);  // (a NaN among its scores stays)
-    sum += l * e;
-    fac[w] = __builtin_ldexpf(e, max(__float_as_int(s_m[(2 * kW + w) * 16 + col]) - U, -300));
+    // (a NaN among a wave's scores stays, also where it saw nothing else)
+    sum += lw[w] * (mw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M));
+    uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
   }
-  const float back = __builtin_ldexpf(1.f, U - 15);
+  const int r = r0 + y;
+  float *part = p.partial + (cell * C + c) * (size_t)(R * (D + 2));
+  const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = 1.f / sum;
   for (int dt = wave; dt < DT; dt += kW) {
-    f32x4_t o = s_acc[dt * 64 + lane] * fac[0];
+    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < nw; ++w) o += s_acc[((w * DT + dt) * 4 + grp) * AC + col] * uw[w];
 #pragma unroll
-    for (int w = 1; w < kW; ++w) o += s_acc[(w * DT + dt) * 64 + lane] * fac[w];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] / sum * back;
-    if (!out_in) continue;
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
     const int k = dt * 16 + grp * 4;
     if (n_active == 1) {
       const int t = r / G, row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
@@ -430,7 +455,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + k) = sum == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : o;
     }
   }
-  if (n_active > 1 && wave == 0 && grp == 0 && out_in) {
+  if (n_active > 1 && wave == 0 && grp == 0) {
     part[(size_t)R * D + r] = M;
     part[(size_t)R * D + R + r] = sum;
   }
@@ -444,7 +469,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   const int r = blockIdx.x * (256 / TR) + threadIdx.x / TR;
   const int L = p.lens[b];
   if (r >= R || L < 0 || L > p.cap - p.t_rows) return;
-  const int n = min(p.splits, (L + p.t_rows - 1) / kKv8Block + 1);
+  const int n = min(p.splits, (L + p.t_rows - 1) / (kKv8Block * kW) + 1);
   if (n == 1) return;  // written by its workgroup
   const int ch = (int)(threadIdx.x % TR) * 4;
   const size_t stride = (size_t)R * (D + 2);

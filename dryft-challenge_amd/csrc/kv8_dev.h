@@ -24,16 +24,28 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float kv8_scale(float top, bool finite) {
   return finite ? (top < kKv8Tiny ? 0.f : top / 127.f) : __builtin_nanf("");
 }
-// What (127 / 256) x is divided by (the 256 keeps 127 x in range): top / 256, or
-// infinity where all are held as 0.
-__device__ __forceinline__ float kv8_div(float top, bool finite) {
-  return finite && top >= kKv8Tiny ? top * 0.00390625f : __builtin_huge_valf();
-}
-// An int8 in the low byte.  (0 for x = NaN and x = inf, whose div is infinite.)
-__device__ __forceinline__ uint32_t kv8_round(float x, float div) {
-  const float q = rintf((0.49609375f * x) / div);
-  return (uint32_t)(int)(q == q ? q : 0.f) & 0xffu;
-}
+// Rounding of a row's values.  127 x / top as (127 / 256) x / (top / 256), which keeps
+// 127 x in range; the quotient by one step of refinement, which leaves a quotient
+// that fp32 can hold as it is; rounded by adding 1.5 * 2^23, whose sum's low bits are
+// the whole number.  A row held as zeros (and inf * 0 = NaN) has the reciprocal 0.
+struct Kv8Div {
+  float div, rcp;
+  __device__ __forceinline__ Kv8Div(float top, bool finite) {
+    const bool held = finite && top >= kKv8Tiny;
+    div = held ? top * 0.00390625f : 0.f;
+    rcp = held ? __builtin_amdgcn_rcpf(div) : 0.f;
+    rcp = __builtin_fmaf(__builtin_fmaf(-div, rcp, 1.f), rcp, rcp);
+  }
+  // An int8 in the low byte.
+  __device__ __forceinline__ uint32_t one(float x) const {
+    const float a = 0.49609375f * x, q = a * rcp;
+    return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, div, a), rcp, q) + 12582912.f);
+  }
+  __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
+    const uint32_t a = __builtin_amdgcn_perm(one(x1), one(x0), 0x0c0c0400u), b = __builtin_amdgcn_perm(one(x3), one(x2), 0x04000c0cu);
+    return a | b;
+  }
+};
 
 // Maximum over the 64 lanes of a wave, over 16-lane rows, of numbers >= 0.
 __device__ __forceinline__ float row16_maxf(float v) {

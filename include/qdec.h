@@ -671,7 +671,7 @@ int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
  * What a row does not see does not reach it, whatever its slot or scale holds.  A length
  * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
  * of sequence b become NaN.
- * Slots are dealt in blocks of 64, block j to workgroup j % splits of its
+ * Slots are dealt in runs of 512, run j to workgroup j % splits of its
  * (sequence, kv head); with splits > 1 a second launch merges the workgroups'
  * partials, in order.  So a row's bits follow from what it sees and from splits,
  * never from t_rows, the other sequences or timing; 0 splits takes a number that
@@ -691,7 +691,7 @@ typedef struct {
   void *out;            /* [batch*t_rows, nq*head_dim] bf16 */
   float *partial;       /* split partials, 16-byte aligned (qdec_kv8_attn_workspace) */
   float eps;
-  float sm_scale;       /* 1/sqrt(head_dim) */
+  float sm_scale;       /* 1/sqrt(head_dim); positive */
   int32_t batch;
   int32_t t_rows;       /* 1..16 */
   int32_t nq;           /* a multiple of nkv; t_rows * nq / nkv at most 64 */

@@ -23,7 +23,7 @@ def test_structs_match_header_fields():
 def fill(st, **kw):
     a = st()
     for f, t in a._fields_:
-        setattr(a, f, 16 if t is capi.P else 1)
+        setattr(a, f, 16 if t is capi.P else 1)  # (eps and sm_scale: 1)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -82,6 +82,10 @@ CASES = shared("kv8_store", store) + shared("kv8_load", load) + shared("kv8_attn
     ("kv8_attn", attn, dict(t_rows=0), -1, "t_rows"),
     ("kv8_attn", attn, dict(t_rows=17), -1, "t_rows"),
     ("kv8_attn", attn, dict(t_rows=9, nq=64), -3, "64 rows"),
+    ("kv8_attn", attn, dict(sm_scale=0.0), -1, "sm_scale"),
+    ("kv8_attn", attn, dict(sm_scale=-0.1), -1, "sm_scale"),
+    ("kv8_attn", attn, dict(sm_scale=math.inf), -1, "sm_scale"),
+    ("kv8_attn", attn, dict(sm_scale=math.nan), -1, "sm_scale"),
     ("kv8_attn", attn, dict(splits=-1), -1, "splits"),
     ("kv8_attn", attn, dict(splits=257), -1, "splits"),
     ("kv8_attn", attn, dict(out_frag=2), -1, "out_frag"),
