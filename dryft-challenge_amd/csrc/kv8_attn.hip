@@ -7,15 +7,16 @@
 // of each.  Blocks are dealt by
 // absolute slot numbers and a row is rescaled by its own scores alone, so a
 // row's bits do not depend on t_rows.  Per block
-// (v_mfma_f32_16x16x32_f16):
-//   S^T = K . Q^T.  K's 8 bits are fp16 integers: a byte under the exponent byte
-//     0x64 is 1024 + byte, so one byte permute makes two of them and one packed
-//     subtraction takes 1152 off.  Q is held in two fp16 parts (22 bits) of the
-//     row divided by a power of two; up to 8 query rows they are the two halves
-//     of one MFMA's 16 columns.
+//   S^T = K . Q^T (v_mfma_i32_16x16x64_i8), exact: K as it is held, q in 21 bits,
+//     relative to its row's largest, as three digits of 7 bits.  The columns that few
+//     query rows leave hold their other digits: up to 4 rows take one matrix instruction
+//     where fp16 parts of q took two, and K no conversion (5 of every 20 vector
+//     instructions of a block).
 //   p = 2^(S scale_k scale_q - m), fp32 statistics.
-//   O^T += V^T . W^T with w = p scale_v in fp16: 2^-11 relative, an eighth of the
-//     output's rounding.  fp16 reaches down to 2^-24 only, so a row's w are
+//   O^T += V^T . W^T (v_mfma_f32_16x16x32_f16) with w = p scale_v in fp16: 2^-11
+//     relative, an eighth of the output's rounding.  V's 8 bits are fp16 integers: a byte under
+//     the exponent byte 0x64 is 1024 + byte, so one byte permute makes two of them
+//     and one packed subtraction takes 1152 off.  fp16 reaches down to 2^-24 only, so a row's w are
 //     held in units of 2^(u - 15), 2^u above the largest |w| so far.
 // K's rows are dealt to MFMA rows so that a lane's 16 scores are the 16 slots of
 // one V group, the operand of the second product; slot l's scales sit in lane
@@ -33,6 +34,10 @@ namespace {
 
 constexpr int kW = 8;       // waves of a workgroup
 
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x4_t mfma_i8(const uint4 &a, const uint4 &b, i32x4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4_t mfma_f16(const f16x8_t &a, const f16x8_t &b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -94,11 +99,18 @@ __device__ __forceinline__ void norm_rope(uint32_t raw, uint32_t w, uint32_t cw,
   o1 = y1 * hi16(cw) + lane_xor<D / 4>(y1) * (sign * hi16(sw));
 }
 
-// A row's power-of-two factor: 2^-e with 2^e <= max|x| < 2^(e+1), and 2^e.
-__device__ __forceinline__ void pow2_of(float top, float &down, float &up) {
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 27), 247);
-  down = __uint_as_float((uint32_t)(254 - e) << 23);
-  up = __uint_as_float((uint32_t)e << 23);
+// The factors 2^(20 - e) and 2^(e - 20) of a row with 2^(e-1) <= max|x| < 2^e.
+__device__ __forceinline__ void grid_of(float top, float &down, float &up) {
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 47), 247) - 126;
+  down = __uint_as_float((uint32_t)(127 + 20 - e) << 23);
+  up = __uint_as_float((uint32_t)(127 - 20 + e) << 23);
+}
+// A whole number of at most 2^20 as a 2^14 + b 2^7 + c, each an int8 in its low byte.
+__device__ __forceinline__ void digits(int q, int &a, int &b, int &c) {
+  a = (q + (1 << 13)) >> 14;
+  q -= a << 14;
+  b = (q + 64) >> 7;
+  c = q - (b << 7);
 }
 
 // A row held in 8 bits: this lane's two values in the low bytes of q; its scale.
@@ -111,12 +123,11 @@ __device__ __forceinline__ float hold2(float x0, float x1, uint32_t &q) {
 }
 
 // LDS (bytes).
-template <int D, bool PK>
+template <int D, int AC>
 struct Lds {
-  static constexpr int RS = D + 8;                               // fp16 per query row (bank spread)
-  static constexpr int AC = PK ? 8 : 16;                         // columns of the sums
-  static constexpr int q = 0;                                    // [2][AC][RS] fp16 parts of the queries
-  static constexpr int acc = q + 2 * AC * RS * 2;                // [kW][D / 16][4][AC] f32x4
+  static constexpr int RS = D + 16;                              // bytes per query row (bank spread)
+  static constexpr int q = 0;                                    // [3][AC][RS] digits of the queries
+  static constexpr int acc = q + 3 * AC * RS;                    // [kW][D / 16][4][AC] f32x4
   static constexpr int qs = acc + kW * (D / 16) * 4 * AC * 16;   // [16] query rows' factors
   static constexpr int k8 = qs + 16 * 4;                         // [kKv8MaxT][D]
   static constexpr int v8 = k8 + kKv8MaxT * D;                   // [2][D][16]
@@ -126,14 +137,15 @@ struct Lds {
   static constexpr int bytes = m + 3 * kW * 16 * 4;
 };
 
-// PK: at most 8 query rows in all, both parts in one tile.
-template <int D, bool PK>
+// AC: 4, 8 or 16, the columns of 16 that query rows take, at most so many rows; the
+// others hold other digits of them.
+template <int D, int AC>
 __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p) {
   constexpr int NH = D / 64, DT = D / 16;
-  using LY = Lds<D, PK>;
-  constexpr int RS = LY::RS, AC = LY::AC;
+  using LY = Lds<D, AC>;
+  constexpr int RS = LY::RS;
   __shared__ __attribute__((aligned(16))) unsigned char smem[LY::bytes];
-  _Float16 *s_q = reinterpret_cast<_Float16 *>(smem + LY::q);
+  unsigned char *s_q = smem + LY::q;
   f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(smem + LY::acc);
   float *s_qs = reinterpret_cast<float *>(smem + LY::qs);
   unsigned char *s_k8 = smem + LY::k8, *s_v8 = smem + LY::v8;
@@ -212,17 +224,20 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     float x0, x1;
     norm_rope<D>(lv ? raw : 0u, w, cw, sw, p.eps, x0, x1);
     if (query) {
+      // 21 bits, relative to the row's largest, as three digits
+      if (!lv) x0 = x1 = 0.f;
+      const bool fin = __all(finite_f(x0) && finite_f(x1));
       float down, up;
-      pow2_of(wave_max(lv ? fmaxf(fabsf(x0), fabsf(x1)) : 0.f), down, up);
-      x0 *= down;
-      x1 *= down;
-      const f16x2_t hi = {(_Float16)x0, (_Float16)x1};
-      const f16x2_t lo = {(_Float16)(x0 - (float)hi[0]), (_Float16)(x1 - (float)hi[1])};
+      grid_of(wave_max(fmaxf(fabsf(x0), fabsf(x1))), down, up);
+      int d0[3], d1[3];
+      digits(fin ? (int)rintf(x0 * down) : 0, d0[0], d0[1], d0[2]);
+      digits(fin ? (int)rintf(x1 * down) : 0, d1[0], d1[1], d1[2]);
       if (lv) {
-        *reinterpret_cast<f16x2_t *>(s_q + i * RS + ch) = hi;
-        *reinterpret_cast<f16x2_t *>(s_q + (AC + i) * RS + ch) = lo;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<uint16_t *>(s_q + (k * AC + i) * RS + ch) = (uint16_t)((d0[k] & 0xff) | (d1[k] << 8));
       }
-      if (lane == 0) s_qs[i] = up * p.scale_log2;
+      if (lane == 0) s_qs[i] = fin ? up * p.scale_log2 : __builtin_nanf("");
     } else {
       const int slot = L + t, e = slot & 15;
       const bool put = tile == 0 && (slot / (kW * kKv8Block)) % C == c;
@@ -257,7 +272,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   lds_barrier();
 
   // ---- this wave's blocks
-  const int y = PK ? col & 7 : col;
+  const int y = col & (AC - 1);
   const bool row_in = y < nr;
   const float qs = row_in ? s_qs[y] : 0.f;
   const int lim = row_in ? L + (r0 + y) / G : -1;  // the last slot the row sees
@@ -267,18 +282,18 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   f32x4_t acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // Query operands: 8 channels 64 h + 16 grp + 8 e of the column's row.
-  f16x8_t qh[NH][2], ql[PK ? 1 : NH][2];
+  // Query operands: 16 channels 64 h + 16 grp of the column's row, the digits so that
+  // scores are (a 2^14 + c) + b 2^7 in every form: four columns each of a, b, c and
+  // nothing; eight of a and c, and b in a second operand; or three operands.
+  constexpr int NO = AC == 4 ? 1 : AC == 8 ? 2 : 3;
+  uint4 qf[NO][NH];
+  const float weight = AC == 16 ? 16384.f : AC == 8 ? (col < 8 ? 16384.f : 1.f) : col < 4 ? 16384.f : col < 8 ? 128.f : 1.f;
 #pragma unroll
-  for (int h = 0; h < NH; ++h)
+  for (int o = 0; o < NO; ++o)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      auto part = [&](int i) {
-        const f16x8_t z = {};
-        return row_in ? *reinterpret_cast<const f16x8_t *>(s_q + (AC * i + y) * RS + 64 * h + 16 * grp + 8 * e) : z;
-      };
-      qh[h][e] = part(PK ? col >> 3 : 0);
-      if constexpr (!PK) ql[h][e] = part(1);
+    for (int h = 0; h < NH; ++h) {
+      const int k = AC == 4 ? col >> 2 : AC == 8 ? (o ? 1 : col >> 3 << 1) : o;
+      qf[o][h] = row_in && k < 3 ? *reinterpret_cast<const uint4 *>(s_q + (k * AC + y) * RS + 64 * h + 16 * grp) : zero4();
     }
   auto each = [&](auto fn) {
     fn(Int<0>{}); fn(Int<1>{}); fn(Int<2>{}); fn(Int<3>{}); fn(Int<4>{}); fn(Int<5>{}); fn(Int<6>{}); fn(Int<7>{});
@@ -326,21 +341,24 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     float s[16];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      f32x4_t hi = f32x4_t{0.f, 0.f, 0.f, 0.f}, lo = hi;
+      i32x4_t d[NO];
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        f16x8_t a[2];
-        to_f16(kf[t][h], a[0], a[1]);
+      for (int o = 0; o < NO; ++o) {
+        d[o] = i32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          hi = mfma_f16(a[e], qh[h][e], hi);
-          if constexpr (!PK) lo = mfma_f16(a[e], ql[h][e], lo);
-        }
+        for (int h = 0; h < NH; ++h) d[o] = mfma_i8(kf[t][h], qf[o][h], d[o]);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (PK) s[4 * t + i] = hi[i] + dpp_f<0x128>(hi[i]);  // row_ror:8, the other part's column
-        else s[4 * t + i] = hi[i] + lo[i];
+        float x = (float)d[0][i] * weight;
+        if constexpr (AC == 16) {
+          x = (x + (float)d[2][i]) + (float)d[1][i] * 128.f;
+        } else {
+          x += dpp_f<0x128>(x);  // row_ror:8, a + c
+          if constexpr (AC == 8) x += (float)d[1][i] * 128.f;
+          else x += dpp_f<0x124>(x);  // row_ror:4
+        }
+        s[4 * t + i] = x;
       }
     }
     // lane (col, grp) holds slots s0 + 16 grp + i of its row
@@ -419,7 +437,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     }
   }
   lds_barrier();
-  if (!row_in || (PK && col >= 8)) return;
+  if (!row_in || col >= AC) return;
   float mw[kW], lw[kW], uw[kW], M = NEG_INF, U = NEG_INF, sum = 0.f;
 #pragma unroll
   for (int w = 0; w < kW; w += 4) {
@@ -512,8 +530,9 @@ template <int D>
 hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   const int R = p.t_rows * (p.nq / p.nkv);
   const dim3 grid(p.splits, p.nkv, p.batch * ((R + 15) / 16)), block(64 * kW);
-  if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, true>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((kv8_attn_kernel<D, false>), grid, block, 0, s, p);
+  if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4>), grid, block, 0, s, p);
+  else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((kv8_attn_kernel<D, 16>), grid, block, 0, s, p);
   if (p.splits > 1) {
     const int per = 256 / (D / 4);
     hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3((R + per - 1) / per, p.nkv, p.batch), dim3(256), 0, s, p);

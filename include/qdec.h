@@ -665,9 +665,10 @@ int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
  *          rounds where the reference does, five times);
  *   k and the raw v go into cache slot lens[b] + t as above;
  *   out  = softmax(q . K^T * sm_scale) . V over slots 0 .. lens[b] + t as the
- *          cache holds them, the new ones included: fp32 statistics and
- *          accumulation, q in two fp16 parts (22 bits), p * v_scale in fp16,
- *          one rounding to bf16.
+ *          cache holds them, the new ones included: q in 21 bits relative to
+ *          its row's largest channel, exact products with the held keys, fp32
+ *          statistics and accumulation, p * v_scale in fp16, one rounding to
+ *          bf16.
  * What a row does not see does not reach it, whatever its slot or scale holds.  A length
  * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
  * of sequence b become NaN.

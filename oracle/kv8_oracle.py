@@ -47,14 +47,14 @@ def attend(q, k8, ks, v8, vs, L, scale):
     """Rows q [T, nq, D] (row t at position L + t) over the cache of one
     sequence that already holds slots up to L + T - 1.  Returns (out [T, nq,
     D], mag: sum |p v| / sum p, step: 128 n max(p v_scale) / sum p [T, nq, 1],
-    reach: max sum |q k| * scale over seen slots)."""
+    reach and grid: max sum |q k| * scale and max|q| * sum |k| * scale over seen slots)."""
     T, nq, D = q.shape
     nkv = k8.shape[0]
     G = nq // nkv
     out = torch.zeros_like(q)
     mag = torch.zeros_like(q)
     step = torch.zeros_like(q[..., :1])
-    reach = 0.0
+    reach = grid = 0.0
     keys = k8[:, :L + T].double() * ks[:, :L + T, None].double()
     vals = row_major(v8.double())[:, :L + T] * vs[:, :L + T, None].double()
     for t in range(T):
@@ -65,6 +65,9 @@ def attend(q, k8, ks, v8, vs, L, scale):
             out[t, h * G:(h + 1) * G] = p @ vals[h, :n]
             mag[t, h * G:(h + 1) * G] = p @ vals[h, :n].abs()
             step[t, h * G:(h + 1) * G] = 128 * n * (p * vs[h, :n].double()).amax(-1, keepdim=True)
-            r = (qh.abs() @ keys[h, :n].abs().t()).max() * scale
-            reach = max(reach, float(r)) if math.isfinite(float(r)) else reach
-    return out, mag, step, reach
+            size = keys[h, :n].abs()
+            r = float((qh.abs() @ size.t()).max() * scale)
+            reach = max(reach, r) if math.isfinite(r) else reach
+            r = float(qh.abs().max() * size.sum(-1).max() * scale)
+            grid = max(grid, r) if math.isfinite(r) else grid
+    return out, mag, step, reach, grid

@@ -143,8 +143,8 @@ def test_oracle_attends():
     ks[0, :2], vs[0, :2] = 0.1, 2.0
     q = torch.zeros((1, 1, D), dtype=torch.float64)
     q[0, 0, 0] = 2.0
-    out, mag, step, reach = kv8_oracle.attend(q, k8, ks, v8, vs, 1, 0.5)
+    out, mag, step, reach, grid = kv8_oracle.attend(q, k8, ks, v8, vs, 1, 0.5)
     w = math.exp(-2.0)
     assert torch.allclose(out, torch.full_like(out, (6 + 10 * w) / (1 + w)), rtol=1e-6)
     assert abs(step[0, 0, 0].item() - 128 * 2 * 2 / (1 + w)) < 1e-4
-    assert torch.equal(out, mag) and abs(reach - 1.0) < 1e-6
+    assert torch.equal(out, mag) and abs(reach - 1.0) < 1e-6 and abs(grid - 1.0) < 1e-6

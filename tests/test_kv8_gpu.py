@@ -13,8 +13,9 @@ by itself.  An output may be off by
   2 d         the scores, d = reach * (2 D + 64) * 2^-24 * 2: each of at most 2 D fp32
               additions and about 64 operations of the norm, the rotation, the
               scales and the exponent's argument, relative to reach = max sum |q k| *
-              sm_scale; the two fp16 parts of q leave 2^-22 of it, less than that;
-              twice, for p and for the sum of p;
+              sm_scale; twice, for p and for the sum of p;
+  2 * 2^-20 grid  q's 21 bits: each channel is off by half a step of 2^(e - 20) with
+              2^e <= 2 max|q|, so a score by 2^-20 of grid = max|q| * max sum |k| * sm_scale;
   (n + 64) 2^-22  the sums over n slots, exponentials and rescaling factors in fp32;
 and, fp16 having no steps below 2^-24, by 2^-25 of the unit for each of n slots times
 |v| <= 128, the unit being at most 2^-14 of the largest w: 2^-39 step.
@@ -218,8 +219,8 @@ class Call:
                 keep[pos] = False
                 assert torch.equal(q8[b][:, keep], x8[b][:, keep])
             q = ko.norm_rope(x[b, :, :nq], self.qw, *tab, EPS)
-            ref, mag, step, reach = ko.attend(q, self.c["k8"][b], self.c["k_scale"][b], self.c["v8"][b], self.c["v_scale"][b], L, D ** -0.5)
-            tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + 4 * reach * (2 * D + 64) * 2 ** -24 + (L + T + 64) * 2 ** -22)
+            ref, mag, step, reach, grid = ko.attend(q, self.c["k8"][b], self.c["k_scale"][b], self.c["v8"][b], self.c["v_scale"][b], L, D ** -0.5)
+            tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + 4 * reach * (2 * D + 64) * 2 ** -24 + 2 ** -19 * grid + (L + T + 64) * 2 ** -22)
             tol += step * 2 ** -39
             bad = ~((got[b] - ref).abs() <= tol)
             assert not bool(bad.any()), (f"sequence {b} of length {L}: {int(bad.sum())} outputs off, worst "
@@ -464,8 +465,8 @@ def test_offsets_past_32_bits(lib):
     x = a.qkv.view(B, 1, 24, D)
     tab = cos[:1], sin[:1]
     qn = ko.norm_rope(x[-1, :, :8], a.qw, *tab, EPS)
-    ref, mag, step, reach = ko.attend(qn, c["k8"][-1], c["k_scale"][-1], c["v8"][-1], c["v_scale"][-1], L, D ** -0.5)
-    tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + 4 * reach * (2 * D + 64) * 2 ** -24 + (L + 65) * 2 ** -22) + step * 2 ** -39
+    ref, mag, step, reach, grid = ko.attend(qn, c["k8"][-1], c["k_scale"][-1], c["v8"][-1], c["v_scale"][-1], L, D ** -0.5)
+    tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + 4 * reach * (2 * D + 64) * 2 ** -24 + 2 ** -19 * grid + (L + 65) * 2 ** -22) + step * 2 ** -39
     assert bool(((a.rows()[-1].double() - ref).abs() <= tol).all())
     k2, v2 = torch.zeros((B, nkv, 32, D), dtype=BF, device=DEV), torch.zeros((B, nkv, 4, D, 8), dtype=BF, device=DEV)
     lib.kv8_load(capi.Kv8LoadArgs(starts=a.lens_t.data_ptr(), k_slab=k2.data_ptr(), v_slab=v2.data_ptr(), batch=B, nkv=nkv,
