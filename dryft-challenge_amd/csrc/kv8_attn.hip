@@ -66,19 +66,6 @@ __device__ __forceinline__ void to_f16(const uint4 &v, f16x8_t &a, f16x8_t &b) {
 template <int I>
 __device__ __forceinline__ float row_lane(float v) { return dpp_f<0x150 + I>(v); }
 
-// The value of lane ^ X (16 or 32).
-template <int X>
-__device__ __forceinline__ float lane_xor(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const bool low = !(threadIdx.x & X);
-  if constexpr (X == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(low ? r[1] : r[0]);
-  } else {
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __uint_as_float(low ? r[1] : r[0]);
-  }
-}
 __device__ __forceinline__ float sum_xor16_32(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -86,40 +73,82 @@ __device__ __forceinline__ float sum_xor16_32(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Head RMSNorm and RoPE of channels 2 lane, 2 lane + 1 of a row, in fp32 (lanes
-// from D / 2 on pass raw = 0).
-template <int D>
-__device__ __forceinline__ void norm_rope(uint32_t raw, uint32_t w, uint32_t cw, uint32_t sw, float eps, float &o0, float &o1) {
-  const float x0 = lo16(raw), x1 = hi16(raw);
-  const float rstd = 1.0f / sqrtf(wave_sum(x0 * x0 + x1 * x1) / (float)D + eps);
-  const float y0 = x0 * rstd * lo16(w), y1 = x1 * rstd * hi16(w);
-  // the first half's partner counts negative
-  const float sign = (threadIdx.x & (D / 4)) ? 1.f : -1.f;
-  o0 = y0 * lo16(cw) + lane_xor<D / 4>(y0) * (sign * lo16(sw));
-  o1 = y1 * hi16(cw) + lane_xor<D / 4>(y1) * (sign * hi16(sw));
+// A head row on the 16 lanes of a DPP row, N = D / 16 consecutive channels to a
+// lane, so that a wave prepares four rows at once; the rotation's partner
+// channels are the lane's 8 further round.
+template <int N>
+struct Part {
+  uint32_t v[N / 2];
+  __device__ __forceinline__ void load(const uint16_t *p) {
+    if constexpr (N == 8) {
+      const uint4 x = ld16(p);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2 *>(p);
+      v[0] = x.x; v[1] = x.y;
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return (i & 1) ? hi16(v[i >> 1]) : lo16(v[i >> 1]); }
+};
+
+// Its RMSNorm (gain w) and RoPE (tables c, s), in fp32.
+template <int N>
+__device__ __forceinline__ void norm_rope(const Part<N> &raw, const Part<N> &w, const Part<N> &c, const Part<N> &s, float eps,
+                                          float (&o)[N]) {
+  float ss = 0.f, y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) ss += raw[i] * raw[i];
+  ss += dpp_f<0xB1>(ss);
+  ss += dpp_f<0x4E>(ss);
+  ss += dpp_f<0x141>(ss);
+  ss += dpp_f<0x140>(ss);
+  const float rstd = __builtin_amdgcn_rsqf(ss * (1.f / (16 * N)) + eps);
+  Part<N> sn = s;  // the first half's partner counts negative
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) sn.v[i] ^= (threadIdx.x & 8) ? 0u : 0x80008000u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = raw[i] * (rstd * w[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) o[i] = y[i] * c[i] + dpp_f<0x128>(y[i]) * sn[i];
+}
+
+// The largest magnitude of such a row as its bits (from 0x7f800000 on: one of
+// them is not finite).
+template <int N>
+__device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  auto step = [&](auto ctrl) {
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  step(Int<0xB1>{});
+  step(Int<0x4E>{});
+  step(Int<0x141>{});
+  step(Int<0x140>{});
+  return m;
+}
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(int a, int b, int c, int d) {
+  return __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
 }
 
 // The factors 2^(20 - e) and 2^(e - 20) of a row with 2^(e-1) <= max|x| < 2^e.
-__device__ __forceinline__ void grid_of(float top, float &down, float &up) {
-  const int e = min(max((int)(__float_as_uint(top) >> 23), 47), 247) - 126;
+__device__ __forceinline__ void grid_of(uint32_t top, float &down, float &up) {
+  const int e = min(max((int)(top >> 23), 47), 247) - 126;
   down = __uint_as_float((uint32_t)(127 + 20 - e) << 23);
   up = __uint_as_float((uint32_t)(127 - 20 + e) << 23);
 }
-// A whole number of at most 2^20 as a 2^14 + b 2^7 + c, each an int8 in its low byte.
-__device__ __forceinline__ void digits(int q, int &a, int &b, int &c) {
-  a = (q + (1 << 13)) >> 14;
-  q -= a << 14;
-  b = (q + 64) >> 7;
-  c = q - (b << 7);
-}
-
-// A row held in 8 bits: this lane's two values in the low bytes of q; its scale.
-__device__ __forceinline__ float hold2(float x0, float x1, uint32_t &q) {
-  const float top = wave_max(fmaxf(fabsf(x0), fabsf(x1)));
-  const bool fin = __all(finite_f(x0) && finite_f(x1));
-  const Kv8Div div(top, fin);
-  q = __builtin_amdgcn_perm(div.one(x1), div.one(x0), 0x0c0c0400u);
-  return kv8_scale(top, fin);
+// Four numbers of at most 2^20, rounded, as a 2^14 + b 2^7 + c, 0 <= b, c < 128, each
+// digit an int8.  (1.5 * 2^23 added: the sum's low 22 bits are the whole number.)
+__device__ __forceinline__ void digits4(const float *x, float down, uint32_t &a, uint32_t &b, uint32_t &c) {
+  int q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = __float_as_int(__builtin_fmaf(x[i], down, 12582912.f));
+  a = low_bytes(q[0] >> 14, q[1] >> 14, q[2] >> 14, q[3] >> 14);
+  b = low_bytes(q[0] >> 7, q[1] >> 7, q[2] >> 7, q[3] >> 7) & 0x7f7f7f7fu;
+  c = low_bytes(q[0], q[1], q[2], q[3]) & 0x7f7f7f7fu;
 }
 
 // LDS (bytes).
@@ -187,20 +216,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   };
   // This wave's first block, and one round's step.
   const int j0 = kW * c + wave, step = kW * C;
-  // Rows to prepare: this tile's queries, then the new keys and values (for a
-  // workgroup that takes some of their blocks); row i on wave 7 - i % 8.  Waves with rows
-  // ask for their blocks behind them, the others at once: the first block's
-  // addresses do not depend on the length.
-  const int first = kW - 1 - wave;
-  const bool late = first < nr + T;
-  if (!late && j0 < p.cap / kKv8Block) {
-    load_k(j0);
-    load_v(j0);
-  }
-  const int ch = 2 * min(lane, D / 2 - 1);
-  const bool lv = lane < D / 2;
   const uint16_t *rows = p.qkv + (size_t)b * T * width;
-  auto pair = [&](const uint16_t *x) { return *reinterpret_cast<const uint32_t *>(x + ch); };
   const int L = p.lens[b];
   if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
     if (c == 0)
@@ -214,60 +230,95 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const int last = L + T - 1, nb = last / kKv8Block + 1;
   if (kW * c >= nb) return;
   const bool mine = (L / (kW * kKv8Block)) % C == c || ((nb - 1) / kW) % C == c;  // takes some of the new rows' blocks
-  const int jobs = mine ? nr + T : nr;
-  for (int i = first; i < jobs; i += kW) {
-    const bool query = i < nr;
-    const int r = r0 + i, t = query ? r / G : i - nr, head = query ? kvh * G + r - t * G : nq + kvh;
-    const uint16_t *x = rows + (size_t)t * width + (size_t)head * D;
-    const uint32_t raw = pair(x), vraw = query ? 0u : pair(x + (size_t)nkv * D), w = pair(query ? p.q_norm_w : p.k_norm_w);
-    const uint32_t cw = pair(p.cos_tab + (size_t)(L + t) * D), sw = pair(p.sin_tab + (size_t)(L + t) * D);
-    float x0, x1;
-    norm_rope<D>(lv ? raw : 0u, w, cw, sw, p.eps, x0, x1);
+  // Rows to prepare, four to a wave: this tile's queries from the last wave on, behind them
+  // the new keys and values (for a workgroup that takes some of their blocks).  Every wave's
+  // row loads leave before any wave's block loads: the rows' chain (length, tables,
+  // preparation) is what the first block waits for, and behind the blocks of a full
+  // launch each of its steps would take microseconds.
+  constexpr int N = D / 16;
+  const int quad = kW - 1 - wave, quads = (nr + 3) / 4;
+  const bool query = quad < quads, job = query || (mine && quad < quads + (T + 3) / 4);
+  const int i = 4 * (query ? quad : quad - quads) + grp, n = query ? nr : T, at = min(i, n - 1);
+  const int t = query ? (r0 + at) / G : at, head = query ? kvh * G + r0 + at - t * G : nq + kvh, ch = N * col;
+  Part<N> raw, vraw, w, cw, sw;
+  if (job) {
+    const uint16_t *x = rows + (size_t)t * width + (size_t)head * D + ch;
+    raw.load(x);
+    w.load((query ? p.q_norm_w : p.k_norm_w) + ch);
+    cw.load(p.cos_tab + (size_t)(L + t) * D + ch);
+    sw.load(p.sin_tab + (size_t)(L + t) * D + ch);
+    if (!query) vraw.load(x + (size_t)nkv * D);
+  }
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (!job && j0 < nb) {
+    load_k(j0);
+    load_v(j0);
+  }
+  if (job) {
+    float o[N];
+    norm_rope<N>(raw, w, cw, sw, p.eps, o);
+    const uint32_t top = top_bits<N>(o);
+    const bool fin = top < 0x7f800000u;
     if (query) {
       // 21 bits, relative to the row's largest, as three digits
-      if (!lv) x0 = x1 = 0.f;
-      const bool fin = __all(finite_f(x0) && finite_f(x1));
       float down, up;
-      grid_of(wave_max(fmaxf(fabsf(x0), fabsf(x1))), down, up);
-      int d0[3], d1[3];
-      digits(fin ? (int)rintf(x0 * down) : 0, d0[0], d0[1], d0[2]);
-      digits(fin ? (int)rintf(x1 * down) : 0, d1[0], d1[1], d1[2]);
-      if (lv) {
+      grid_of(top, down, up);
+      if (i < n) {  // (a row that is not finite is NaN by its factor)
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
-          *reinterpret_cast<uint16_t *>(s_q + (k * AC + i) * RS + ch) = (uint16_t)((d0[k] & 0xff) | (d1[k] << 8));
-      }
-      if (lane == 0) s_qs[i] = fin ? up * p.scale_log2 : __builtin_nanf("");
-    } else {
-      const int slot = L + t, e = slot & 15;
-      const bool put = tile == 0 && (slot / (kW * kKv8Block)) % C == c;
-      uint32_t kq, vq;
-      const float sk = hold2(lv ? x0 : 0.f, lv ? x1 : 0.f, kq), sv = hold2(lv ? lo16(vraw) : 0.f, lv ? hi16(vraw) : 0.f, vq);
-      if (lv) {
-        unsigned char *vl = s_v8 + (((slot >> 4) - (L >> 4)) * D + ch) * 16 + e;
-        *reinterpret_cast<uint16_t *>(s_k8 + t * D + ch) = (uint16_t)kq;
-        vl[0] = (unsigned char)vq;
-        vl[16] = (unsigned char)(vq >> 8);
-        if (put) {
-          int8_t *vg = v8 + ((size_t)(slot >> 4) * D + ch) * 16 + e;
-          *reinterpret_cast<uint16_t *>(k8 + (size_t)slot * D + ch) = (uint16_t)kq;
-          vg[0] = (int8_t)vq;
-          vg[16] = (int8_t)(vq >> 8);
+        for (int e = 0; e < N; e += 4) {
+          uint32_t d[3];
+          digits4(o + e, down, d[0], d[1], d[2]);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t *>(s_q + (k * AC + i) * RS + ch + e) = d[k];
         }
+        if (col == 0) s_qs[i] = fin ? up * p.scale_log2 : __builtin_nanf("");
       }
-      if (lane == 0) {
-        s_sk[t] = sk;
-        s_sv[t] = sv;
-        if (put) {
-          kscale[slot] = sk;
-          vscale[slot] = sv;
+    } else {
+      const Kv8Div kd(__uint_as_float(top), fin);
+      const float sk = kv8_scale(__uint_as_float(top), fin);
+      uint32_t kq[N / 4], vq[N / 4];
+#pragma unroll
+      for (int e = 0; e < N; e += 4) kq[e / 4] = kd.four(o[e], o[e + 1], o[e + 2], o[e + 3]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = vraw[e];
+      const uint32_t vtop = top_bits<N>(o);
+      const bool vfin = vtop < 0x7f800000u;
+      const Kv8Div vd(__uint_as_float(vtop), vfin);
+      const float sv = kv8_scale(__uint_as_float(vtop), vfin);
+#pragma unroll
+      for (int e = 0; e < N; e += 4) vq[e / 4] = vd.four(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      const int slot = L + t, byte = slot & 15;
+      if (i < n) {
+        const bool put = tile == 0 && (slot / (kW * kKv8Block)) % C == c;
+        unsigned char *vl = s_v8 + (((slot >> 4) - (L >> 4)) * D + ch) * 16 + byte;
+        int8_t *vg = v8 + ((size_t)(slot >> 4) * D + ch) * 16 + byte;
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          *reinterpret_cast<uint32_t *>(s_k8 + t * D + ch + e) = kq[e / 4];
+          if (put) *reinterpret_cast<uint32_t *>(k8 + (size_t)slot * D + ch + e) = kq[e / 4];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const uint32_t x = vq[e / 4] >> (8 * (e & 3));
+          vl[16 * e] = (unsigned char)x;
+          if (put) vg[16 * e] = (int8_t)x;
+        }
+        if (col == 0) {
+          s_sk[t] = sk;
+          s_sv[t] = sv;
+          if (put) {
+            kscale[slot] = sk;
+            vscale[slot] = sv;
+          }
         }
       }
     }
-  }
-  if (late && j0 < nb) {
-    load_k(j0);
-    load_v(j0);
+    if (j0 < nb) {
+      load_k(j0);
+      load_v(j0);
+    }
   }
   lds_barrier();
 
