@@ -183,14 +183,23 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int c = blockIdx.x, kvh = blockIdx.y, C = p.splits, z = blockIdx.z;
-  const int tile = (z >= p.batch) + (z >= 2 * p.batch) + (z >= 3 * p.batch), b = z - tile * p.batch;
-  const int T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv, R = T * G;
+  // The tiles of one (sequence, kv head, split) read the same blocks: their
+  // workgroups are numbered 8 apart, 8 XCDs, so that they share an L2.
+  const int C = p.splits, T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv, R = T * G;
+  int tile = 0, unit = blockIdx.x;  // unit = (b * nkv + kvh) * C + c
+  if constexpr (AC == 16) {
+    const int tiles = (R + 15) / 16, units = p.batch * nkv * C, whole = units & ~7, x = blockIdx.x;
+    if (tiles > 1) {
+      const int w = x < whole * tiles ? x >> 3 : x - whole * tiles, q = w / tiles;
+      tile = w - q * tiles;
+      unit = x < whole * tiles ? q * 8 + (x & 7) : whole + q;
+    }
+  }
+  const int cell = unit / C, c = unit - cell * C, b = cell / nkv, kvh = cell - b * nkv;
   const int r0 = tile * 16, nr = min(R - r0, 16);  // this workgroup's query rows
   const int width = (nq + 2 * nkv) * D;
-  const size_t cell = (size_t)b * nkv + kvh;
-  int8_t *k8 = p.k8 + cell * p.cap * D, *v8 = p.v8 + cell * p.cap * D;
-  float *kscale = p.k_scale + cell * p.cap, *vscale = p.v_scale + cell * p.cap;
+  int8_t *k8 = p.k8 + (size_t)cell * p.cap * D, *v8 = p.v8 + (size_t)cell * p.cap * D;
+  float *kscale = p.k_scale + (size_t)cell * p.cap, *vscale = p.v_scale + (size_t)cell * p.cap;
   const float NEG_INF = -__builtin_huge_valf();
 
   // One block's keys, values and scales.  MFMA row r of K's tile t is slot 16 (r
@@ -328,8 +337,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const float qs = row_in ? s_qs[y] : 0.f;
   const int lim = row_in ? L + (r0 + y) / G : -1;  // the last slot the row sees
   // Of the blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
-  // units of 2^(unit - 15).
-  float m_run = NEG_INF, l_run = 0.f, unit = NEG_INF;
+  // units of 2^(level - 15).
+  float m_run = NEG_INF, l_run = 0.f, level = NEG_INF;
   f32x4_t acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -448,17 +457,17 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     for (int i = 0; i < 16; ++i) big = fmaxf(big, s[i]);
     const float alpha = m_old == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m_old - m_run) * qs);
     l_run = l_run * alpha + psum;
-    const float u_old = unit;
-    unit = fmaxf(unit, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
-    const float up = unit == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mq - unit + 15.f);
+    const float level_old = level;
+    level = fmaxf(level, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
+    const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mq - level + 15.f);
     f16x8_t w[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       w[0][e] = (_Float16)(s[e] * up);
       w[1][e] = (_Float16)(s[8 + e] * up);
     }
-    if (__any(u_old < unit)) {
-      const float ra = u_old < unit ? __builtin_amdgcn_exp2f(u_old - unit) : 1.f;
+    if (__any(level_old < level)) {
+      const float ra = level_old < level ? __builtin_amdgcn_exp2f(level_old - level) : 1.f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) acc[dt] *= ra;
     }
@@ -480,7 +489,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     if (grp == 0) {
       s_m[col * kW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
       s_m[(16 + col) * kW + wave] = lw;
-      s_m[(32 + col) * kW + wave] = unit;
+      s_m[(32 + col) * kW + wave] = level;
     }
     if (wave < nw) {
 #pragma unroll
@@ -508,7 +517,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
   }
   const int r = r0 + y;
-  float *part = p.partial + (cell * C + c) * (size_t)(R * (D + 2));
+  float *part = p.partial + (size_t)unit * (R * (D + 2));
   const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = 1.f / sum;
   for (int dt = wave; dt < DT; dt += kW) {
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -580,7 +589,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
 template <int D>
 hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   const int R = p.t_rows * (p.nq / p.nkv);
-  const dim3 grid(p.splits, p.nkv, p.batch * ((R + 15) / 16)), block(64 * kW);
+  const dim3 grid((unsigned)(p.batch * p.nkv * p.splits * ((R + 15) / 16))), block(64 * kW);
   if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4>), grid, block, 0, s, p);
   else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((kv8_attn_kernel<D, 16>), grid, block, 0, s, p);
@@ -595,7 +604,8 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
 
 int kv8_attn_splits(int batch, int nkv, int cap) {
   const int64_t cells = (int64_t)batch * nkv;
-  const int64_t n = std::min<int64_t>(256 / cells, cap / (kW * kKv8Block));
+  if (cap <= 2 * kW * kKv8Block) return 1;
+  const int64_t n = std::min<int64_t>(256 / cells, (cap + kW * kKv8Block - 1) / (kW * kKv8Block));
   return (int)std::max<int64_t>(1, n);
 }
 
