@@ -992,6 +992,10 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
   p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
   // A launch's work items are numbered in 32 bits.
   const int64_t tiles = (a->t_rows * (a->nq / a->nkv) + 15) / 16;
+  p->by_splits = fast_div(p->splits);
+  p->by_nkv = fast_div(p->nkv);
+  p->by_g = fast_div(p->nq / p->nkv);
+  p->by_tiles = fast_div((uint32_t)tiles);
   if ((int64_t)p->batch * p->nkv * p->splits * tiles * 512 > 0xffffffffll)
     return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: batch %d x nkv %d x %d splits", p->batch, p->nkv, p->splits);
   if (!need_scratch) return QDEC_OK;

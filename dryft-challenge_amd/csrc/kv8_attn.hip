@@ -32,7 +32,9 @@ namespace qdec {
 
 namespace {
 
-constexpr int kW = 8;       // waves of a workgroup
+constexpr int kW = 8;                  // waves of a workgroup
+constexpr int kRun = kW * kKv8Block;   // slots of a run
+__device__ __forceinline__ int div_by(const FastDiv &d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4_t mfma_i8(const uint4 &a, const uint4 &b, i32x4_t c) {
@@ -185,17 +187,17 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const int col = lane & 15, grp = lane >> 4;
   // The tiles of one (sequence, kv head, split) read the same blocks: their
   // workgroups are numbered 8 apart, 8 XCDs, so that they share an L2.
-  const int C = p.splits, T = p.t_rows, nq = p.nq, nkv = p.nkv, G = nq / nkv, R = T * G;
+  const int C = p.splits, T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d, R = T * G;
   int tile = 0, unit = blockIdx.x;  // unit = (b * nkv + kvh) * C + c
   if constexpr (AC == 16) {
     const int tiles = (R + 15) / 16, units = p.batch * nkv * C, whole = units & ~7, x = blockIdx.x;
     if (tiles > 1) {
-      const int w = x < whole * tiles ? x >> 3 : x - whole * tiles, q = w / tiles;
+      const int w = x < whole * tiles ? x >> 3 : x - whole * tiles, q = div_by(p.by_tiles, w);
       tile = w - q * tiles;
       unit = x < whole * tiles ? q * 8 + (x & 7) : whole + q;
     }
   }
-  const int cell = unit / C, c = unit - cell * C, b = cell / nkv, kvh = cell - b * nkv;
+  const int cell = div_by(p.by_splits, unit), c = unit - cell * C, b = div_by(p.by_nkv, cell), kvh = cell - b * nkv;
   const int r0 = tile * 16, nr = min(R - r0, 16);  // this workgroup's query rows
   const int width = (nq + 2 * nkv) * D;
   int8_t *k8 = p.k8 + (size_t)cell * p.cap * D, *v8 = p.v8 + (size_t)cell * p.cap * D;
@@ -230,7 +232,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
     if (c == 0)
       for (int i = threadIdx.x; i < nr * (D / 4); i += blockDim.x) {
-        const int y = i / (D / 4), ch = (i - y * (D / 4)) * 4, r = r0 + y, row = b * T + r / G, k = (kvh * G + r % G) * D + ch;
+        const int y = i / (D / 4), ch = (i - y * (D / 4)) * 4, r = r0 + y, t = div_by(p.by_g, r), row = b * T + t,
+                  k = (kvh * G + r - t * G) * D + ch;
         uint16_t *o = p.out + (p.ofrag ? frag_off(row, k, p.ofrag) : (size_t)row * nq * D + k);
         *reinterpret_cast<uint2 *>(o) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
       }
@@ -238,7 +241,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   }
   const int last = L + T - 1, nb = last / kKv8Block + 1;
   if (kW * c >= nb) return;
-  const bool mine = (L / (kW * kKv8Block)) % C == c || ((nb - 1) / kW) % C == c;  // takes some of the new rows' blocks
+  auto ours = [&](int slot) { return slot / kRun - div_by(p.by_splits, slot / kRun) * C == c; };  // its run is this workgroup's
+  const bool mine = ours(L) || ours(last);
   // Rows to prepare, four to a wave: this tile's queries from the last wave on, behind them
   // the new keys and values (for a workgroup that takes some of their blocks).  Every wave's
   // row loads leave before any wave's block loads: the rows' chain (length, tables,
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const int quad = kW - 1 - wave, quads = (nr + 3) / 4;
   const bool query = quad < quads, job = query || (mine && quad < quads + (T + 3) / 4);
   const int i = 4 * (query ? quad : quad - quads) + grp, n = query ? nr : T, at = min(i, n - 1);
-  const int t = query ? (r0 + at) / G : at, head = query ? kvh * G + r0 + at - t * G : nq + kvh, ch = N * col;
+  const int t = query ? div_by(p.by_g, r0 + at) : at, head = query ? kvh * G + r0 + at - t * G : nq + kvh, ch = N * col;
   Part<N> raw, vraw, w, cw, sw;
   if (job) {
     const uint16_t *x = rows + (size_t)t * width + (size_t)head * D + ch;
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       for (int e = 0; e < N; e += 4) vq[e / 4] = vd.four(o[e], o[e + 1], o[e + 2], o[e + 3]);
       const int slot = L + t, byte = slot & 15;
       if (i < n) {
-        const bool put = tile == 0 && (slot / (kW * kKv8Block)) % C == c;
+        const bool put = tile == 0 && ours(slot);
         unsigned char *vl = s_v8 + (((slot >> 4) - (L >> 4)) * D + ch) * 16 + byte;
         int8_t *vg = v8 + ((size_t)(slot >> 4) * D + ch) * 16 + byte;
 #pragma unroll
@@ -335,7 +339,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const int y = col & (AC - 1);
   const bool row_in = y < nr;
   const float qs = row_in ? s_qs[y] : 0.f;
-  const int lim = row_in ? L + (r0 + y) / G : -1;  // the last slot the row sees
+  const int lim = row_in ? L + div_by(p.by_g, r0 + y) : -1;  // the last slot the row sees
   // Of the blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
   // units of 2^(level - 15).
   float m_run = NEG_INF, l_run = 0.f, level = NEG_INF;
@@ -483,7 +487,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 
   // ---- the waves' sums, in wave order; then the output or a partial: the
   // normalised row, its maximum and its sum.
-  const int n_active = min(C, (nb + kW - 1) / kW), nw = min(nb - kW * c, kW);  // waves that had blocks
+  const int n_active = min(C, (nb + kW - 1) / kW);
   if (col < AC) {
     const float lw = sum_xor16_32(l_run);
     if (grp == 0) {
@@ -491,10 +495,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       s_m[(16 + col) * kW + wave] = lw;
       s_m[(32 + col) * kW + wave] = level;
     }
-    if (wave < nw) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
-    }
+    for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
   }
   lds_barrier();
   if (!row_in || col >= AC) return;
@@ -518,15 +520,16 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   }
   const int r = r0 + y;
   float *part = p.partial + (size_t)unit * (R * (D + 2));
-  const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = 1.f / sum;
+  const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum);
   for (int dt = wave; dt < DT; dt += kW) {
     f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < nw; ++w) o += s_acc[((w * DT + dt) * 4 + grp) * AC + col] * uw[w];
+#pragma unroll
+    for (int w = 0; w < kW; ++w) o += s_acc[((w * DT + dt) * 4 + grp) * AC + col] * uw[w];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
     const int k = dt * 16 + grp * 4;
     if (n_active == 1) {
-      const int t = r / G, row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
+      const int t = div_by(p.by_g, r), row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
       uint16_t *dst = p.out + (p.ofrag ? frag_off(row, kk, p.ofrag) : (size_t)row * nq * D + kk);
       *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
     } else {
@@ -543,11 +546,11 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 template <int D>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   constexpr int TR = D / 4;
-  const int G = p.nq / p.nkv, R = p.t_rows * G, kvh = blockIdx.y, b = blockIdx.z;
+  const int G = p.by_g.d, R = p.t_rows * G, kvh = blockIdx.y, b = blockIdx.z;
   const int r = blockIdx.x * (256 / TR) + threadIdx.x / TR;
   const int L = p.lens[b];
   if (r >= R || L < 0 || L > p.cap - p.t_rows) return;
-  const int n = min(p.splits, (L + p.t_rows - 1) / (kKv8Block * kW) + 1);
+  const int n = min(p.splits, (L + p.t_rows - 1) / kRun + 1);
   if (n == 1) return;  // written by its workgroup
   const int ch = (int)(threadIdx.x % TR) * 4;
   const size_t stride = (size_t)R * (D + 2);
@@ -581,7 +584,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
     M = Mn;
   }
   const float inv = 1.f / l;
-  const int t = r / G, row = b * p.t_rows + t, k = (kvh * G + r - t * G) * D + ch;
+  const int t = div_by(p.by_g, r), row = b * p.t_rows + t, k = (kvh * G + r - t * G) * D + ch;
   uint16_t *dst = p.out + (p.ofrag ? frag_off(row, k, p.ofrag) : (size_t)row * p.nq * D + k);
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
 }
@@ -604,8 +607,8 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
 
 int kv8_attn_splits(int batch, int nkv, int cap) {
   const int64_t cells = (int64_t)batch * nkv;
-  if (cap <= 2 * kW * kKv8Block) return 1;
-  const int64_t n = std::min<int64_t>(256 / cells, (cap + kW * kKv8Block - 1) / (kW * kKv8Block));
+  if (cap <= 2 * kRun) return 1;
+  const int64_t n = std::min<int64_t>(256 / cells, (cap + kRun - 1) / kRun);
   return (int)std::max<int64_t>(1, n);
 }
 
