@@ -941,7 +941,7 @@ static int plan_kv8_copy(const char *fn, const A *a, Kv8CopyParams *p) {
 
 // A launch's work items are numbered in 32 bits.
 static int kv8_copy_grid(const char *fn, const Kv8CopyParams &p) {
-  if (p.cells * p.groups > (1ll << 26) - 8) return set_error(QDEC_EUNSUPPORTED, "%s: %lld (sequence, kv head) pairs x %d slots", fn, (long long)p.cells, p.n);
+  if (p.cells * p.groups > (1ll << 25) - 2) return set_error(QDEC_EUNSUPPORTED, "%s: %lld (sequence, kv head) pairs x %d slots", fn, (long long)p.cells, p.n);
   return QDEC_OK;
 }
 

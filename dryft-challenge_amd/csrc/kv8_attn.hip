@@ -131,11 +131,6 @@ __device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {
   return m;
 }
 
-// The low bytes of four words.
-__device__ __forceinline__ uint32_t low_bytes(int a, int b, int c, int d) {
-  return __builtin_amdgcn_perm((uint32_t)b, (uint32_t)a, 0x0c0c0400u) | __builtin_amdgcn_perm((uint32_t)d, (uint32_t)c, 0x04000c0cu);
-}
-
 // The factors 2^(20 - e) and 2^(e - 20) of a row with 2^(e-1) <= max|x| < 2^e.
 __device__ __forceinline__ void grid_of(uint32_t top, float &down, float &up) {
   const int e = min(max((int)(top >> 23), 47), 247) - 126;
@@ -145,9 +140,9 @@ __device__ __forceinline__ void grid_of(uint32_t top, float &down, float &up) {
 // Four numbers of at most 2^20, rounded, as a 2^14 + b 2^7 + c, 0 <= b, c < 128, each
 // digit an int8.  (1.5 * 2^23 added: the sum's low 22 bits are the whole number.)
 __device__ __forceinline__ void digits4(const float *x, float down, uint32_t &a, uint32_t &b, uint32_t &c) {
-  int q[4];
+  uint32_t q[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = __float_as_int(__builtin_fmaf(x[i], down, 12582912.f));
+  for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__builtin_fmaf(x[i], down, 12582912.f));
   a = low_bytes(q[0] >> 14, q[1] >> 14, q[2] >> 14, q[3] >> 14);
   b = low_bytes(q[0] >> 7, q[1] >> 7, q[2] >> 7, q[3] >> 7) & 0x7f7f7f7fu;
   c = low_bytes(q[0], q[1], q[2], q[3]) & 0x7f7f7f7fu;

@@ -24,12 +24,18 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float kv8_scale(float top, bool finite) {
   return finite ? (top < kKv8Tiny ? 0.f : top / 127.f) : __builtin_nanf("");
 }
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+}
+
 // Rounding of a row's values.  127 x / top as (127 / 256) x / (top / 256), which keeps
 // 127 x in range; the quotient by one step of refinement, which leaves a quotient
 // that fp32 can hold as it is; rounded by adding 1.5 * 2^23, whose sum's low bits are
 // the whole number.  A row held as zeros (and inf * 0 = NaN) has the reciprocal 0.
 struct Kv8Div {
   float div, rcp;
+  __device__ __forceinline__ Kv8Div() {}
   __device__ __forceinline__ Kv8Div(float top, bool finite) {
     const bool held = finite && top >= kKv8Tiny;
     div = held ? top * 0.00390625f : 0.f;
@@ -42,23 +48,16 @@ struct Kv8Div {
     return __float_as_uint(__builtin_fmaf(__builtin_fmaf(-q, div, a), rcp, q) + 12582912.f);
   }
   __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
-    const uint32_t a = __builtin_amdgcn_perm(one(x1), one(x0), 0x0c0c0400u), b = __builtin_amdgcn_perm(one(x3), one(x2), 0x04000c0cu);
-    return a | b;
+    return low_bytes(one(x0), one(x1), one(x2), one(x3));
+  }
+  // Lane I's of this lane's 16-lane row.
+  template <int I>
+  __device__ __forceinline__ Kv8Div at() const {
+    Kv8Div r;
+    r.div = dpp_f<0x150 + I>(div);
+    r.rcp = dpp_f<0x150 + I>(rcp);
+    return r;
   }
 };
-
-// Maximum over the 64 lanes of a wave, over 16-lane rows, of numbers >= 0.
-__device__ __forceinline__ float row16_maxf(float v) {
-  v = fmaxf(v, dpp_f<0xB1>(v));
-  v = fmaxf(v, dpp_f<0x4E>(v));
-  v = fmaxf(v, dpp_f<0x141>(v));
-  return fmaxf(v, dpp_f<0x140>(v));
-}
-__device__ __forceinline__ float wave_max(float v) {
-  v = row16_maxf(v);
-  return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
-}
-
-__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 }  // namespace qdec
