@@ -42,6 +42,11 @@ from . import capi
 
 GEMM_MAX_ROWS = 64
 KV8_BLOCK = 64  # the 8-bit cache's slots come in whole blocks (kKv8Block of qdec_kernels.h)
+# A state with an 8-bit cache holds a multiple of KV8_SLOTS slots: one (sequence, kv head)'s
+# keys then end on 16 KiB.  Strides of an odd number of 8 KiB can put every
+# workgroup's stream on the same memory banks (attention of 32 sequences at 8200
+# slots, us by capacity: 8256 111, 8320 89, 8384 92, 8448 89, 9216 91, 9280 102).
+KV8_SLOTS = 128
 GEMM_WIDE_MIN_ROWS = 9  # of qdec_gemm_wide
 ATTN_MAX_T = 16
 # Rows (sequences x positions) of one prefill chunk: activations of 32K rows
@@ -527,7 +532,7 @@ class DecodeState:
         self.model, self.lib = model, model.lib
         self.batch = batch
         self.kv8 = kv8
-        self.cap = round_up(capacity, KV8_BLOCK if kv8 else 32)
+        self.cap = round_up(capacity, KV8_SLOTS if kv8 else 32)
         if kv8 and tree_t:
             raise ValueError("tree passes read a bf16 cache (kv8 state)")
         self.max_t = max_rows_per_seq(batch, max_t, c.group)

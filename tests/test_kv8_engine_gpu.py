@@ -130,7 +130,7 @@ def test_a_longer_prompt_after_a_shorter_one(model):
 def test_memory(model):
     _, _, eng, _ = model
     from qdec.runtime import DecodeState
-    st, bf = state(eng, 2, 500), DecodeState(eng.model, 2, 500, max_t=16)
+    st, bf = state(eng, 2, 512), DecodeState(eng.model, 2, 512, max_t=16)
     held8 = sum(x.numel() * x.element_size() for x in (st.k8, st.v8, st.k_scale, st.v_scale))
     both = sum(x.numel() * x.element_size() for x in (bf.k_cache, bf.v_cache))
     assert held8 <= both * (0.5 + 2 / eng.model.cfg.head_dim)
