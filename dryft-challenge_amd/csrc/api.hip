@@ -976,7 +976,7 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
   if (rc != QDEC_OK) return rc;
   if (a->nq < a->nkv || a->nq % a->nkv)
     return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: nq %d / nkv %d (whole query heads per kv head)", a->nq, a->nkv);
-  if (a->t_rows < 1 || a->t_rows > kKv8MaxT || a->t_rows > a->cap)
+  if (a->t_rows < 1 || a->t_rows > kKv8MaxT)
     return set_error(QDEC_EINVAL, "qdec_kv8_attn: t_rows %d not in [1, %d]", a->t_rows, kKv8MaxT);
   if ((int64_t)a->t_rows * (a->nq / a->nkv) > 64)
     return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: t_rows %d x %d query heads per kv head (at most 64 rows)", a->t_rows,

@@ -131,11 +131,12 @@ __device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {
   return m;
 }
 
-// The factors 2^(20 - e) and 2^(e - 20) of a row with 2^(e-1) <= max|x| < 2^e.
+// The factors 2^(20 - e) and 2^e of a row with 2^(e-1) <= max|x| < 2^e <= 2^127 (a row
+// below 2^-108 takes those of 2^-107: steps of 2^-127).
 __device__ __forceinline__ void grid_of(uint32_t top, float &down, float &up) {
-  const int e = min(max((int)(top >> 23), 47), 247) - 126;
+  const int e = min(max((int)(top >> 23), 19), 253) - 126;
   down = __uint_as_float((uint32_t)(127 + 20 - e) << 23);
-  up = __uint_as_float((uint32_t)(127 - 20 + e) << 23);
+  up = __uint_as_float((uint32_t)(127 + e) << 23);
 }
 // Four numbers of at most 2^20, rounded, as a 2^14 + b 2^7 + c, 0 <= b, c < 128, each
 // digit an int8.  (1.5 * 2^23 added: the sum's low 22 bits are the whole number.)
@@ -268,12 +269,12 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     float o[N];
     norm_rope<N>(raw, w, cw, sw, p.eps, o);
     const uint32_t top = top_bits<N>(o);
-    const bool fin = top < 0x7f800000u;
     if (query) {
-      // 21 bits, relative to the row's largest, as three digits
+      // 21 bits, relative to the row's largest, as three digits; a row of 2^127 or more is NaN
+      const bool fin = top < 0x7f000000u;
       float down, up;
       grid_of(top, down, up);
-      if (i < n) {  // (a row that is not finite is NaN by its factor)
+      if (i < n) {
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
           uint32_t d[3];
@@ -284,6 +285,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
         if (col == 0) s_qs[i] = fin ? up * p.scale_log2 : __builtin_nanf("");
       }
     } else {
+      const bool fin = top < 0x7f800000u;
       const Kv8Div kd(__uint_as_float(top), fin);
       const float sk = kv8_scale(__uint_as_float(top), fin);
       uint32_t kq[N / 4], vq[N / 4];
@@ -342,11 +344,12 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // Query operands: 16 channels 64 h + 16 grp of the column's row, the digits so that
-  // scores are (a 2^14 + c) + b 2^7 in every form: four columns each of a, b, c and
-  // nothing; eight of a and c, and b in a second operand; or three operands.
+  // scores are (a 2^-6 + c 2^-20) + b 2^-13 in every form: four columns each of a,
+  // b, c and nothing; eight of a and c, and b in a second operand; or three operands.
   constexpr int NO = AC == 4 ? 1 : AC == 8 ? 2 : 3;
   uint4 qf[NO][NH];
-  const float weight = AC == 16 ? 16384.f : AC == 8 ? (col < 8 ? 16384.f : 1.f) : col < 4 ? 16384.f : col < 8 ? 128.f : 1.f;
+  constexpr float WA = 0x1p-6f, WB = 0x1p-13f, WC = 0x1p-20f;
+  const float weight = AC == 16 ? WA : AC == 8 ? (col < 8 ? WA : WC) : col < 4 ? WA : col < 8 ? WB : WC;
 #pragma unroll
   for (int o = 0; o < NO; ++o)
 #pragma unroll
@@ -411,10 +414,10 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       for (int i = 0; i < 4; ++i) {
         float x = (float)d[0][i] * weight;
         if constexpr (AC == 16) {
-          x = (x + (float)d[2][i]) + (float)d[1][i] * 128.f;
+          x = (x + (float)d[2][i] * WC) + (float)d[1][i] * WB;
         } else {
           x += dpp_f<0x128>(x);  // row_ror:8, a + c
-          if constexpr (AC == 8) x += (float)d[1][i] * 128.f;
+          if constexpr (AC == 8) x += (float)d[1][i] * WB;
           else x += dpp_f<0x124>(x);  // row_ror:4
         }
         s[4 * t + i] = x;

@@ -212,7 +212,9 @@ class Call:
                                      (vr, self.c["v_scale"], ko.row_major(before["v8"]), x[b, :, nq + nkv:].double())):
                 want = want.transpose(0, 1)
                 top = want.abs().amax(-1)
-                off = (q8[b, :, pos].double() - 127 * want / top[..., None]).abs().max()
+                low = top < 2 ** -100  # held as zeros
+                top = top.masked_fill(low, 0)
+                off = (q8[b, :, pos].double() - (127 * want / top[..., None]).masked_fill(low[..., None], 0)).abs().max()
                 assert off <= 0.5 + 127 * 4 * (D + 64) * 2 ** -24, f"new rows of sequence {b} off by {off} steps"
                 torch.testing.assert_close(sc[b, :, pos].double(), top / 127, rtol=2 * (D + 64) * 2 ** -24, atol=0)
                 keep = torch.ones(self.cap, dtype=torch.bool, device=DEV)
@@ -247,6 +249,9 @@ ATTN = [
     (2, 40, 8, 128, 3, [700, 129]), (2, 64, 8, 128, 8, [300, 60]), (1, 16, 8, 128, 16, [1000]), (4, 16, 8, 128, 4, [0, 2001, 511, 512]),
     (1, 16, 1, 64, 4, [200]), (1, 64, 1, 128, 1, [333]), (2, 9, 3, 64, 5, [575, 576]), (8, 32, 8, 128, 1, [900, 1535, 1, 0, 1023, 1024, 1025, 77]),
     (5, 32, 8, 128, 2, [4100, 50, 3000, 64, 4095]), (1, 64, 8, 128, 1, [20011]), (1, 8, 2, 64, 10, [5837]),
+    # several row tiles, workgroups in no whole eights; new rows on either side of a run's end
+    (3, 12, 3, 64, 16, [500, 1020, 0]), (1, 20, 5, 128, 16, [1017]), (7, 64, 1, 64, 1, [511, 512, 513, 1023, 1024, 1535, 1536]),
+    (1, 32, 8, 128, 16, [1531]), (2, 8, 8, 128, 16, [507, 2045]), (3, 7, 7, 128, 1, [63, 64, 512]), (2, 48, 4, 128, 5, [2100, 3]),
 ]
 
 
@@ -270,12 +275,28 @@ def test_fragment_order(lib, shape, splits):
     assert torch.equal(a.rows(), b.rows())
 
 
+@pytest.mark.parametrize("shape", [(3, 12, 3, 64, 16, [500, 1020, 505]), (1, 64, 8, 128, 8, [1533]), (1, 32, 8, 128, 16, [2040])])
+@pytest.mark.parametrize("splits", [2, 3])
+def test_new_rows_in_two_splits(lib, shape, splits):
+    Call(lib, *shape, splits=splits).checked()
+
+
+@pytest.mark.parametrize("q,k", [(1e30, 1e-28), (1e-28, 1e30), (3e36, 1e-34), (1e-20, 1e-20)])
+def test_norm_gains_of_any_size(lib, q, k):
+    """Queries and new keys far from 1, among cached keys as far from it."""
+    a = Call(lib, 1, 32, 8, 128, 2, [300])
+    a.qw.mul_(q), a.kw.mul_(k)
+    a.c["k_scale"].mul_(k)
+    a.checked()
+
+
 @pytest.mark.parametrize("gain", [0.01, 30.0])
 def test_flat_and_peaked_scores(lib, gain):
     Call(lib, 2, 32, 8, 128, 3, [1200, 70], gain=gain).checked()
 
 
-@pytest.mark.parametrize("shape", [(2, 32, 8, 128, [700, 61]), (1, 64, 8, 128, [1022]), (3, 8, 2, 64, [0, 63, 500])])
+@pytest.mark.parametrize("shape", [(2, 32, 8, 128, [700, 61]), (1, 64, 8, 128, [1022]), (3, 8, 2, 64, [0, 63, 500]),
+                                   (2, 16, 8, 128, [509, 1021]), (1, 30, 3, 64, [1533])])
 @pytest.mark.parametrize("splits", [0, 1, 3])
 def test_rows_do_not_depend_on_the_pass(lib, shape, splits):
     """One pass of 6 rows and 6 passes of one leave the same bits, in the rows
