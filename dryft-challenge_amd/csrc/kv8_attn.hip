@@ -461,7 +461,9 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     l_run = l_run * alpha + psum;
     const float level_old = level;
     level = fmaxf(level, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
-    const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mq - level + 15.f);
+    // (in range also where a slot with values of zero has raised mq, not level: from a factor
+    // of 2^126 on the others' p are below 2^-111)
+    const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(mq - level + 15.f, 126.f));
     f16x8_t w[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

@@ -375,6 +375,31 @@ def test_values_of_many_magnitudes(lib, splits, T):
         a.checked()
 
 
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("slot", [100, 600, 899])
+@pytest.mark.parametrize("loud", [0.04, 0.07, 1.0, 100.0])
+def test_zero_values_with_the_probability(lib, splits, slot, loud):
+    """A slot whose score is far above all others, with values of zero: before
+    and behind it in its wave are slots of 2^-80 of its probability and less."""
+    a = Call(lib, 1, 32, 8, 128, 2, [900], splits=splits)
+    x = a.qkv.view(2, -1, 128)
+    x[:, :32] = 0.0
+    x[:, :32, 63] = 1.0
+    a.qw[63] = 16.0
+    a.cos[:], a.sin[:] = 1.0, 0.0
+    a.c["k_scale"][:] = 0.002
+    a.c["k8"][0, :, slot, 63] = 127
+    a.c["k_scale"][0, :, slot] = loud
+    a.c["v_scale"][0, :, slot] = 0.0
+    x[:, 32:40, 63] = 0.0
+    a.run()
+    got = a.rows()
+    assert bool(torch.isfinite(got).all())
+    # scores are 16 times the key's channel: at most 16 * 128 * 0.002 of 901 slots, 16 * 127 * loud of one
+    vals = 128 * max(1.0, float(a.c["v_scale"][0, :, :902].max()))
+    assert float(got.abs().max()) <= 901 * vals * math.exp(-0.99 * 16 * (127 * loud - 128 * 0.002))
+
+
 def test_not_finite_where_it_is_seen(lib):
     """A NaN scale reaches the rows and heads that see its slot, no others."""
     for which in ("k_scale", "v_scale"):
