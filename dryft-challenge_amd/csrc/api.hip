@@ -993,6 +993,7 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
   // A launch's work items are numbered in 32 bits.
   const int64_t tiles = (a->t_rows * (a->nq / a->nkv) + 15) / 16;
   p->by_splits = fast_div(p->splits);
+  p->by_parts = fast_div((uint32_t)kv8_attn_parts(p->batch, p->nkv, p->splits, (int)tiles));
   p->by_nkv = fast_div(p->nkv);
   p->by_g = fast_div(p->nq / p->nkv);
   p->by_tiles = fast_div((uint32_t)tiles);

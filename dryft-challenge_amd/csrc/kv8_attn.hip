@@ -28,6 +28,10 @@
 #include "kv8_dev.h"
 #include "qdec_kernels.h"
 
+// A row has the same bits in every form of the kernel, so products and sums are fused
+// where it is written and nowhere else.
+#pragma clang fp contract(off)
+
 namespace qdec {
 
 namespace {
@@ -99,19 +103,19 @@ __device__ __forceinline__ void norm_rope(const Part<N> &raw, const Part<N> &w, 
                                           float (&o)[N]) {
   float ss = 0.f, y[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) ss += raw[i] * raw[i];
+  for (int i = 0; i < N; ++i) ss = __builtin_fmaf(raw[i], raw[i], ss);
   ss += dpp_f<0xB1>(ss);
   ss += dpp_f<0x4E>(ss);
   ss += dpp_f<0x141>(ss);
   ss += dpp_f<0x140>(ss);
-  const float rstd = __builtin_amdgcn_rsqf(ss * (1.f / (16 * N)) + eps);
+  const float rstd = __builtin_amdgcn_rsqf(__builtin_fmaf(ss, 1.f / (16 * N), eps));
   Part<N> sn = s;  // the first half's partner counts negative
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) sn.v[i] ^= (threadIdx.x & 8) ? 0u : 0x80008000u;
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = raw[i] * (rstd * w[i]);
 #pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = y[i] * c[i] + dpp_f<0x128>(y[i]) * sn[i];
+  for (int i = 0; i < N; ++i) o[i] = __builtin_fmaf(dpp_f<0x128>(y[i]), sn[i], y[i] * c[i]);
 }
 
 // The largest magnitude of such a row as its bits (from 0x7f800000 on: one of
@@ -166,7 +170,7 @@ struct Lds {
 
 // AC: 4, 8 or 16, the columns of 16 that query rows take, at most so many rows; the
 // others hold other digits of them.
-template <int D, int AC>
+template <int D, int AC, bool FOLD>
 __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p) {
   constexpr int NH = D / 64, DT = D / 16;
   using LY = Lds<D, AC>;
@@ -184,16 +188,17 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   // The tiles of one (sequence, kv head, split) read the same blocks: their
   // workgroups are numbered 8 apart, 8 XCDs, so that they share an L2.
   const int C = p.splits, T = p.t_rows, nq = p.nq, nkv = p.nkv, G = p.by_g.d, R = T * G;
-  int tile = 0, unit = blockIdx.x;  // unit = (b * nkv + kvh) * C + c
+  const int P = FOLD ? (int)p.by_parts.d : C;  // c0, c0 + P, ... are this workgroup's splits
+  int tile = 0, unit = blockIdx.x;             // unit = (b * nkv + kvh) * P + c0
   if constexpr (AC == 16) {
-    const int tiles = (R + 15) / 16, units = p.batch * nkv * C, whole = units & ~7, x = blockIdx.x;
+    const int tiles = (R + 15) / 16, units = p.batch * nkv * P, whole = units & ~7, x = blockIdx.x;
     if (tiles > 1) {
       const int w = x < whole * tiles ? x >> 3 : x - whole * tiles, q = div_by(p.by_tiles, w);
       tile = w - q * tiles;
       unit = x < whole * tiles ? q * 8 + (x & 7) : whole + q;
     }
   }
-  const int cell = div_by(p.by_splits, unit), c = unit - cell * C, b = div_by(p.by_nkv, cell), kvh = cell - b * nkv;
+  const int cell = div_by(p.by_parts, unit), c0 = unit - cell * P, b = div_by(p.by_nkv, cell), kvh = cell - b * nkv;
   const int r0 = tile * 16, nr = min(R - r0, 16);  // this workgroup's query rows
   const int width = (nq + 2 * nkv) * D;
   int8_t *k8 = p.k8 + (size_t)cell * p.cap * D, *v8 = p.v8 + (size_t)cell * p.cap * D;
@@ -222,11 +227,11 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     vs = __builtin_nontemporal_load(vscale + s0 + lane);
   };
   // This wave's first block, and one round's step.
-  const int j0 = kW * c + wave, step = kW * C;
+  const int j0 = kW * c0 + wave, step = kW * C;
   const uint16_t *rows = p.qkv + (size_t)b * T * width;
   const int L = p.lens[b];
   if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
-    if (c == 0)
+    if (c0 == 0)
       for (int i = threadIdx.x; i < nr * (D / 4); i += blockDim.x) {
         const int y = i / (D / 4), ch = (i - y * (D / 4)) * 4, r = r0 + y, t = div_by(p.by_g, r), row = b * T + t,
                   k = (kvh * G + r - t * G) * D + ch;
@@ -236,8 +241,11 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     return;
   }
   const int last = L + T - 1, nb = last / kKv8Block + 1;
-  if (kW * c >= nb) return;
-  auto ours = [&](int slot) { return slot / kRun - div_by(p.by_splits, slot / kRun) * C == c; };  // its run is this workgroup's
+  if (kW * c0 >= nb) return;
+  auto ours = [&](int slot) {  // its run is of one of this workgroup's splits
+    const int run = slot / kRun, c = run - div_by(p.by_splits, run) * C;
+    return FOLD ? c - div_by(p.by_parts, c) * P == c0 : c == c0;
+  };
   const bool mine = ours(L) || ours(last);
   // Rows to prepare, four to a wave: this tile's queries from the last wave on, behind them
   // the new keys and values (for a workgroup that takes some of their blocks).  Every wave's
@@ -337,12 +345,6 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const bool row_in = y < nr;
   const float qs = row_in ? s_qs[y] : 0.f;
   const int lim = row_in ? L + div_by(p.by_g, r0 + y) : -1;  // the last slot the row sees
-  // Of the blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
-  // units of 2^(level - 15).
-  float m_run = NEG_INF, l_run = 0.f, level = NEG_INF;
-  f32x4_t acc[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   // Query operands: 16 channels 64 h + 16 grp of the column's row, the digits so that
   // scores are (a 2^-6 + c 2^-20) + b 2^-13 in every form: four columns each of a,
   // b, c and nothing; eight of a and c, and b in a second operand; or three operands.
@@ -362,183 +364,199 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     fn(Int<8>{}); fn(Int<9>{}); fn(Int<10>{}); fn(Int<11>{}); fn(Int<12>{}); fn(Int<13>{}); fn(Int<14>{}); fn(Int<15>{});
   };
 
-  for (int j = j0; j < nb; j += step) {
-    const int s0 = j * kKv8Block;
-    const bool edge = s0 + kKv8Block > L;  // slots that not every row sees, the new rows among them
-    if (edge) {                            // which come from LDS
+  const int n_active = min(C, (nb + kW - 1) / kW);
+  for (int c = c0; c < n_active; c += P) {
+    // Of the split's blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
+    // units of 2^(level - 15).
+    float m_run = NEG_INF, l_run = 0.f, level = NEG_INF;
+    f32x4_t acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = kW * c + wave; j < nb; j += step) {
+      const int next = j + step < nb ? j + step : FOLD && c + P < n_active ? kW * (c + P) + wave : nb;
+      const int s0 = j * kKv8Block;
+      const bool edge = s0 + kKv8Block > L;  // slots that not every row sees, the new rows among them
+      if (edge) {                            // which come from LDS
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int i = s0 + 16 * (col >> 2) + 4 * t + (col & 3) - L;
+          const bool is = (unsigned)i < (unsigned)T;
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(s_k8 + min(max(i, 0), kKv8MaxT - 1) * D + 64 * h + 16 * grp);
+            if (is) kf[t][h] = x;
+          }
+        }
+        const int v0 = s0 + 16 * grp, gi = min(max((v0 >> 4) - (L >> 4), 0), 1);
+        // byte i of this lane's 16: slot v0 + i, a new row's from L to `last`
+        auto from = [&](int s, int d) {  // dword d's bytes from slot s on
+          const int n = min(max(s - v0 - 4 * d, 0), 4);
+          return (uint32_t)(0xffffffffull << (8 * n));
+        };
+        uint32_t take[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) take[d] = from(L, d) & ~from(last + 1, d);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint4 x = *reinterpret_cast<const uint4 *>(s_v8 + (gi * D + dt * 16 + col) * 16);
+          uint4 &v = vf[dt];
+          v.x = (v.x & ~take[0]) | (x.x & take[0]);
+          v.y = (v.y & ~take[1]) | (x.y & take[1]);
+          v.z = (v.z & ~take[2]) | (x.z & take[2]);
+          v.w = (v.w & ~take[3]) | (x.w & take[3]);
+        }
+        const int i = s0 + lane - L;
+        if ((unsigned)i < (unsigned)T) {
+          ks = s_sk[i];
+          vs = s_sv[i];
+        }
+      }
+      float s[16];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int i = s0 + 16 * (col >> 2) + 4 * t + (col & 3) - L;
-        const bool is = (unsigned)i < (unsigned)T;
+        i32x4_t d[NO];
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(s_k8 + min(max(i, 0), kKv8MaxT - 1) * D + 64 * h + 16 * grp);
-          if (is) kf[t][h] = x;
+        for (int o = 0; o < NO; ++o) {
+          d[o] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int h = 0; h < NH; ++h) d[o] = mfma_i8(kf[t][h], qf[o][h], d[o]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x = (float)d[0][i] * weight;
+          if constexpr (AC == 16) {
+            x = __builtin_fmaf((float)d[1][i], WB, __builtin_fmaf((float)d[2][i], WC, x));
+          } else {
+            x += dpp_f<0x128>(x);  // row_ror:8, a + c
+            if constexpr (AC == 8) x = __builtin_fmaf((float)d[1][i], WB, x);
+            else x += dpp_f<0x124>(x);  // row_ror:4
+          }
+          s[4 * t + i] = x;
         }
       }
-      const int v0 = s0 + 16 * grp, gi = min(max((v0 >> 4) - (L >> 4), 0), 1);
-      // byte i of this lane's 16: slot v0 + i, a new row's from L to `last`
-      auto from = [&](int s, int d) {  // dword d's bytes from slot s on
-        const int n = min(max(s - v0 - 4 * d, 0), 4);
-        return (uint32_t)(0xffffffffull << (8 * n));
-      };
-      uint32_t take[4];
+      // lane (col, grp) holds slots s0 + 16 grp + i of its row
+      each([&](auto n) {
+        constexpr int i = decltype(n)::value;
+        s[i] *= row_lane<i>(ks);
+        pin(s[i]);
+      });
+      if (next < nb) load_k(next);
+      // of them, those up to `seen` (pins: a branch around the selects, not sixteen in every block)
+      int seen = lim - s0 - 16 * grp;
+      if (edge) {
+        pin(seen);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) take[d] = from(L, d) & ~from(last + 1, d);
+        for (int i = 0; i < 16; ++i) s[i] = i > seen ? NEG_INF : s[i];
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      const float m_old = m_run;
+      m_run = fmaxf(m_run, max_xor16_32(top));
+      const float mq = m_run == NEG_INF ? 0.f : m_run * qs;
+      float psum = 0.f, big = 0.f;
+      each([&](auto n) {
+        constexpr int i = decltype(n)::value;
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, -mq));
+        psum += e;
+        s[i] = e * row_lane<i>(vs);
+      });
+      if (edge) {
+        pin(seen);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = i > seen ? 0.f : s[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) big = fmaxf(big, s[i]);
+      const float alpha = m_old == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m_old - m_run) * qs);
+      l_run = __builtin_fmaf(l_run, alpha, psum);
+      const float level_old = level;
+      level = fmaxf(level, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
+      // (in range also where a slot with values of zero has raised mq, not level: from a factor
+      // of 2^126 on the others' p are below 2^-111)
+      const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(mq - level + 15.f, 126.f));
+      f16x8_t w[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        w[0][e] = (_Float16)(s[e] * up);
+        w[1][e] = (_Float16)(s[8 + e] * up);
+      }
+      if (__any(level_old < level)) {
+        const float ra = level_old < level ? __builtin_amdgcn_exp2f(level_old - level) : 1.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) acc[dt] *= ra;
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(s_v8 + (gi * D + dt * 16 + col) * 16);
-        uint4 &v = vf[dt];
-        v.x = (v.x & ~take[0]) | (x.x & take[0]);
-        v.y = (v.y & ~take[1]) | (x.y & take[1]);
-        v.z = (v.z & ~take[2]) | (x.z & take[2]);
-        v.w = (v.w & ~take[3]) | (x.w & take[3]);
+        f16x8_t a[2];
+        to_f16(vf[dt], a[0], a[1]);
+        acc[dt] = mfma_f16(a[0], w[0], acc[dt]);
+        acc[dt] = mfma_f16(a[1], w[1], acc[dt]);
       }
-      const int i = s0 + lane - L;
-      if ((unsigned)i < (unsigned)T) {
-        ks = s_sk[i];
-        vs = s_sv[i];
-      }
+      if (next < nb) load_v(next);
     }
-    float s[16];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      i32x4_t d[NO];
-#pragma unroll
-      for (int o = 0; o < NO; ++o) {
-        d[o] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int h = 0; h < NH; ++h) d[o] = mfma_i8(kf[t][h], qf[o][h], d[o]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = (float)d[0][i] * weight;
-        if constexpr (AC == 16) {
-          x = (x + (float)d[2][i] * WC) + (float)d[1][i] * WB;
-        } else {
-          x += dpp_f<0x128>(x);  // row_ror:8, a + c
-          if constexpr (AC == 8) x += (float)d[1][i] * WB;
-          else x += dpp_f<0x124>(x);  // row_ror:4
-        }
-        s[4 * t + i] = x;
-      }
-    }
-    // lane (col, grp) holds slots s0 + 16 grp + i of its row
-    each([&](auto n) {
-      constexpr int i = decltype(n)::value;
-      s[i] *= row_lane<i>(ks);
-      pin(s[i]);
-    });
-    if (j + step < nb) load_k(j + step);
-    // of them, those up to `seen` (pins: a branch around the selects, not sixteen in every block)
-    int seen = lim - s0 - 16 * grp;
-    if (edge) {
-      pin(seen);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = i > seen ? NEG_INF : s[i];
-    }
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    const float m_old = m_run;
-    m_run = fmaxf(m_run, max_xor16_32(top));
-    const float mq = m_run == NEG_INF ? 0.f : m_run * qs;
-    float psum = 0.f, big = 0.f;
-    each([&](auto n) {
-      constexpr int i = decltype(n)::value;
-      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, -mq));
-      psum += e;
-      s[i] = e * row_lane<i>(vs);
-    });
-    if (edge) {
-      pin(seen);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = i > seen ? 0.f : s[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) big = fmaxf(big, s[i]);
-    const float alpha = m_old == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m_old - m_run) * qs);
-    l_run = l_run * alpha + psum;
-    const float level_old = level;
-    level = fmaxf(level, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
-    // (in range also where a slot with values of zero has raised mq, not level: from a factor
-    // of 2^126 on the others' p are below 2^-111)
-    const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(mq - level + 15.f, 126.f));
-    f16x8_t w[2];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[0][e] = (_Float16)(s[e] * up);
-      w[1][e] = (_Float16)(s[8 + e] * up);
-    }
-    if (__any(level_old < level)) {
-      const float ra = level_old < level ? __builtin_amdgcn_exp2f(level_old - level) : 1.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] *= ra;
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      f16x8_t a[2];
-      to_f16(vf[dt], a[0], a[1]);
-      acc[dt] = mfma_f16(a[0], w[0], acc[dt]);
-      acc[dt] = mfma_f16(a[1], w[1], acc[dt]);
-    }
-    if (j + step < nb) load_v(j + step);
-  }
 
-  // ---- the waves' sums, in wave order; then the output or a partial: the
-  // normalised row, its maximum and its sum.
-  const int n_active = min(C, (nb + kW - 1) / kW);
-  if (col < AC) {
-    const float lw = sum_xor16_32(l_run);
-    if (grp == 0) {
-      s_m[col * kW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
-      s_m[(16 + col) * kW + wave] = lw;
-      s_m[(32 + col) * kW + wave] = level;
+    // ---- the waves' sums, in wave order; then the output or a partial: the
+    // normalised row, its maximum and its sum.
+    if (FOLD && c > c0) lds_barrier();  // the last split's are read
+    if (col < AC) {
+      const float lw = sum_xor16_32(l_run);
+      if (grp == 0) {
+        s_m[col * kW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
+        s_m[(16 + col) * kW + wave] = lw;
+        s_m[(32 + col) * kW + wave] = level;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
     }
+    lds_barrier();
+    if (row_in && col < AC) {
+      float mw[kW], lw[kW], uw[kW], M = NEG_INF, U = NEG_INF, sum = 0.f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
-  }
-  lds_barrier();
-  if (!row_in || col >= AC) return;
-  float mw[kW], lw[kW], uw[kW], M = NEG_INF, U = NEG_INF, sum = 0.f;
+      for (int w = 0; w < kW; w += 4) {
+        *reinterpret_cast<f32x4_t *>(mw + w) = *reinterpret_cast<const f32x4_t *>(s_m + col * kW + w);
+        *reinterpret_cast<f32x4_t *>(lw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (16 + col) * kW + w);
+        *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * kW + w);
+      }
 #pragma unroll
-  for (int w = 0; w < kW; w += 4) {
-    *reinterpret_cast<f32x4_t *>(mw + w) = *reinterpret_cast<const f32x4_t *>(s_m + col * kW + w);
-    *reinterpret_cast<f32x4_t *>(lw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (16 + col) * kW + w);
-    *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * kW + w);
-  }
+      for (int w = 0; w < kW; ++w) {
+        M = fmaxf(M, mw[w]);
+        U = fmaxf(U, uw[w]);
+      }
 #pragma unroll
-  for (int w = 0; w < kW; ++w) {
-    M = fmaxf(M, mw[w]);
-    U = fmaxf(U, uw[w]);
-  }
+      for (int w = 0; w < kW; ++w) {
+        // (a NaN among a wave's scores stays, also where it saw nothing else)
+        sum = __builtin_fmaf(lw[w], mw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M), sum);
+        uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
+      }
+      const int r = r0 + y;
+      float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
+      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum);
+      for (int dt = wave; dt < DT; dt += kW) {
+        f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kW; ++w) {
-    // (a NaN among a wave's scores stays, also where it saw nothing else)
-    sum += lw[w] * (mw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M));
-    uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
-  }
-  const int r = r0 + y;
-  float *part = p.partial + (size_t)unit * (R * (D + 2));
-  const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum);
-  for (int dt = wave; dt < DT; dt += kW) {
-    f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < kW; ++w) {
+          const f32x4_t a = s_acc[((w * DT + dt) * 4 + grp) * AC + col];
 #pragma unroll
-    for (int w = 0; w < kW; ++w) o += s_acc[((w * DT + dt) * 4 + grp) * AC + col] * uw[w];
+          for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(a[i], uw[w], o[i]);
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
-    const int k = dt * 16 + grp * 4;
-    if (n_active == 1) {
-      const int t = div_by(p.by_g, r), row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
-      uint16_t *dst = p.out + (p.ofrag ? frag_off(row, kk, p.ofrag) : (size_t)row * nq * D + kk);
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
-    } else {
-      *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + k) = sum == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : o;
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
+        const int k = dt * 16 + grp * 4;
+        if (n_active == 1) {
+          const int t = div_by(p.by_g, r), row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
+          uint16_t *dst = p.out + (p.ofrag ? frag_off(row, kk, p.ofrag) : (size_t)row * nq * D + kk);
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
+        } else {
+          *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + k) = sum == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : o;
+        }
+      }
+      if (n_active > 1 && wave == 0 && grp == 0) {
+        part[(size_t)R * D + r] = M;
+        part[(size_t)R * D + R + r] = sum;
+      }
     }
-  }
-  if (n_active > 1 && wave == 0 && grp == 0) {
-    part[(size_t)R * D + r] = M;
-    part[(size_t)R * D + R + r] = sum;
+    if constexpr (!FOLD) break;
   }
 }
 
@@ -592,10 +610,11 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
 template <int D>
 hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   const int R = p.t_rows * (p.nq / p.nkv);
-  const dim3 grid((unsigned)(p.batch * p.nkv * p.splits * ((R + 15) / 16))), block(64 * kW);
-  if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4>), grid, block, 0, s, p);
-  else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((kv8_attn_kernel<D, 16>), grid, block, 0, s, p);
+  const dim3 grid((unsigned)(p.batch * p.nkv * (int)p.by_parts.d * ((R + 15) / 16))), block(64 * kW);
+  if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4, false>), grid, block, 0, s, p);
+  else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8, false>), grid, block, 0, s, p);
+  else if ((int)p.by_parts.d == p.splits) hipLaunchKernelGGL((kv8_attn_kernel<D, 16, false>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((kv8_attn_kernel<D, 16, true>), grid, block, 0, s, p);
   if (p.splits > 1) {
     const int per = 256 / (D / 4);
     hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3((R + per - 1) / per, p.nkv, p.batch), dim3(256), 0, s, p);
@@ -610,6 +629,12 @@ int kv8_attn_splits(int batch, int nkv, int cap) {
   if (cap <= 2 * kRun) return 1;
   const int64_t n = std::min<int64_t>(256 / cells, (cap + kRun - 1) / kRun);
   return (int)std::max<int64_t>(1, n);
+}
+
+int kv8_attn_parts(int batch, int nkv, int splits, int tiles) {
+  if (tiles == 1) return splits;
+  const int64_t n = 256 / ((int64_t)batch * nkv * tiles);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(splits, n));
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnParams &p, hipStream_t s) {

@@ -324,11 +324,13 @@ struct Kv8AttnParams {
   float eps;
   float scale_log2;  // log2(e) / sqrt(head_dim)
   int batch, t_rows, nq, nkv, head_dim, cap;
-  int splits;  // workgroups per (sequence, kv head): run j of 8 blocks goes to workgroup j % splits
-  FastDiv by_splits, by_nkv, by_g, by_tiles;  // g: query heads per kv head; tiles: of 16 query rows
+  int splits;  // of a (sequence, kv head): run j of 8 blocks goes to split j % splits
+  FastDiv by_splits, by_parts, by_nkv, by_g, by_tiles;  // parts: workgroups that share the splits; g: query heads
+                                                        // per kv head; tiles: of 16 query rows
   int ofrag;   // > 0: out is written in fragment order with this many M tiles
 };
 int kv8_attn_splits(int batch, int nkv, int cap);
+int kv8_attn_parts(int batch, int nkv, int splits, int tiles);
 hipError_t launch_kv8_attn(const Kv8AttnParams &p, hipStream_t s);
 
 }  // namespace qdec
