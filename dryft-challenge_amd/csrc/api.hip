@@ -73,6 +73,38 @@ static bool wide_offsets(const qdec_gemm_args *a) { return (uint64_t)a->n * a->k
 enum class PlanFor { kCall, kWide, kLayer };
 
 // Derive the launch plan of a GEMM call; returns QDEC_OK or an error code.
+// The partials that an attention call with out_partials leaves (x_attn, x_kv8); false:
+// not of a shape that a GEMM merges.
+struct Partials {
+  const float *partial;
+  const int32_t *lens;
+  int batch, t_rows, nkv, cap;
+  int chunk, nchunks, strided;  // slots of a chunk, chunks of a (sequence, kv head), every how many blocks
+  int norm;                     // acc is divided by its sum
+};
+template <class A>
+static bool partials_shape(const A &a, Partials *p) {
+  *p = Partials{};
+  p->partial = a.partial;
+  p->lens = a.lens;
+  p->batch = a.batch; p->t_rows = a.t_rows; p->nkv = a.nkv; p->cap = a.cap;
+  return a.head_dim == 128 && a.nkv >= 1 && a.nkv < (1 << 20) && a.nq == 4 * a.nkv && a.t_rows >= 1 && a.batch >= 1;
+}
+static bool partials_of(const qdec_attn_args &a, Partials *p) {
+  if (!partials_shape(a, p) || a.chunk < 32 || a.cap < 32) return false;
+  p->chunk = a.chunk;
+  p->nchunks = (a.cap + a.chunk - 1) / a.chunk;
+  p->strided = a.strided;
+  return true;
+}
+static bool partials_of(const qdec_kv8_attn_args &a, Partials *p) {
+  if (!partials_shape(a, p) || a.cap < kKv8Block || a.splits < 0 || a.splits > 256) return false;
+  p->chunk = kKv8Run;
+  p->nchunks = a.splits ? a.splits : kv8_attn_splits(a.batch, a.nkv, a.cap);
+  p->norm = 1;
+  return true;
+}
+
 static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, PlanFor what = PlanFor::kCall) {
   const bool wide = what == PlanFor::kWide;
   if (!a) return set_error(QDEC_EINVAL, "qdec_gemm: null args");
@@ -115,16 +147,18 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     if ((reinterpret_cast<uintptr_t>(a->x_parts) & 15u) || (a->x_merged && !aligned16(a->x_merged)))
       return set_error(QDEC_EALIGN, "qdec_gemm: x_parts and x_merged must be 16-byte aligned");
   }
-  const qdec_attn_args *xa = a->x_attn;
+  Partials xp = {};
+  const bool xa = a->x_attn || a->x_kv8;
   if (xa) {
     if (f & QDEC_NORM_IN) return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_attn with NORM_IN");
-    if (!xa->out_partials) return set_error(QDEC_EINVAL, "qdec_gemm: x_attn call was not made with out_partials");
-    if (xa->head_dim != 128 || xa->nkv < 1 || xa->nq != 4 * xa->nkv || xa->chunk < 32 || xa->cap < 32 ||
-        xa->t_rows < 1 || xa->batch < 1)
+    if (a->x_attn && a->x_kv8) return set_error(QDEC_EINVAL, "qdec_gemm: both x_attn and x_kv8");
+    if (!(a->x_attn ? a->x_attn->out_partials : a->x_kv8->out_partials))
+      return set_error(QDEC_EINVAL, "qdec_gemm: x_attn call was not made with out_partials");
+    if (!(a->x_attn ? partials_of(*a->x_attn, &xp) : partials_of(*a->x_kv8, &xp)))
       return set_error(QDEC_EINVAL, "qdec_gemm: x_attn shape");
-    if (a->rows != xa->batch * xa->t_rows || a->k != xa->nq * xa->head_dim)
+    if (a->rows != (int64_t)xp.batch * xp.t_rows || a->k != xp.nkv * 4 * 128)
       return set_error(QDEC_EINVAL, "qdec_gemm: x_attn rows %d / k %d do not match the attention call", a->rows, a->k);
-    if (need_scratch && (!xa->partial || !xa->lens)) return set_error(QDEC_EINVAL, "qdec_gemm: x_attn needs partial and lens");
+    if (need_scratch && (!xp.partial || !xp.lens)) return set_error(QDEC_EINVAL, "qdec_gemm: x_attn needs partial and lens");
   }
   if (need_scratch && ((!a->x && !xa) || !a->w)) return set_error(QDEC_EINVAL, "qdec_gemm: null x or w");
   if (need_scratch && (f & QDEC_NORM_IN) && !a->norm_w) return set_error(QDEC_EINVAL, "qdec_gemm: NORM_IN needs norm_w");
@@ -355,14 +389,15 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     if (!p->xfast || p->xd || a->ksplit != 1)
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_attn needs activations staged from registers (rows %d)", a->rows);
     p->amerge = 1;
-    p->apart = xa->partial;
-    p->alens = xa->lens;
-    p->a_t_rows = xa->t_rows;
-    p->a_nkv = xa->nkv;
-    p->a_chunk = xa->chunk;
-    p->a_nchunks = (xa->cap + xa->chunk - 1) / xa->chunk;
-    p->a_cap = xa->cap;
-    p->a_strided = xa->strided;
+    p->apart = xp.partial;
+    p->alens = xp.lens;
+    p->a_t_rows = xp.t_rows;
+    p->a_nkv = xp.nkv;
+    p->a_chunk = xp.chunk;
+    p->a_nchunks = xp.nchunks;
+    p->a_cap = xp.cap;
+    p->a_strided = xp.strided;
+    p->a_norm = xp.norm;
   }
   size_t pb = 0, cb = 0, xn_off = 0;
   gemm_scratch(a, *p, &pb, &cb, &xn_off);
@@ -983,13 +1018,16 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
                      a->nq / a->nkv);
   if (a->splits < 0 || a->splits > 256) return set_error(QDEC_EINVAL, "qdec_kv8_attn: splits %d not in [0, 256]", a->splits);
   if (a->out_frag != 0 && a->out_frag != 1) return set_error(QDEC_EINVAL, "qdec_kv8_attn: out_frag %d not 0 or 1", a->out_frag);
+  if (a->out_partials != 0 && a->out_partials != 1)
+    return set_error(QDEC_EINVAL, "qdec_kv8_attn: out_partials %d not 0 or 1", a->out_partials);
   *p = Kv8AttnParams{};
   p->eps = a->eps;
   p->scale_log2 = a->sm_scale * 1.4426950408889634f;
   p->batch = a->batch; p->t_rows = a->t_rows; p->nq = a->nq; p->nkv = a->nkv;
   p->head_dim = a->head_dim; p->cap = a->cap;
   p->splits = a->splits ? a->splits : kv8_attn_splits(a->batch, a->nkv, a->cap);
-  p->ofrag = a->out_frag ? (a->batch * a->t_rows + 15) / 16 : 0;
+  p->out_partials = a->out_partials;
+  p->ofrag = a->out_frag && !a->out_partials ? (a->batch * a->t_rows + 15) / 16 : 0;
   // A launch's work items are numbered in 32 bits.
   const int64_t tiles = (a->t_rows * (a->nq / a->nkv) + 15) / 16;
   p->by_splits = fast_div(p->splits);
@@ -1001,11 +1039,12 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
     return set_error(QDEC_EUNSUPPORTED, "qdec_kv8_attn: batch %d x nkv %d x %d splits", p->batch, p->nkv, p->splits);
   if (!need_scratch) return QDEC_OK;
   if (!a->qkv || !a->q_norm_w || !a->k_norm_w || !a->cos_tab || !a->sin_tab || !a->lens || !a->k8 || !a->v8 || !a->k_scale ||
-      !a->v_scale || !a->out)
+      !a->v_scale || (!a->out && !a->out_partials))
     return set_error(QDEC_EINVAL, "qdec_kv8_attn: null pointer argument");
   if (!(p->scale_log2 > 0.f) || !std::isfinite(p->scale_log2))
     return set_error(QDEC_EINVAL, "qdec_kv8_attn: sm_scale %g is not positive and finite", (double)a->sm_scale);
-  if (p->splits > 1 && !a->partial) return set_error(QDEC_EINVAL, "qdec_kv8_attn: more than one split needs partial");
+  if ((p->splits > 1 || a->out_partials) && !a->partial)
+    return set_error(QDEC_EINVAL, "qdec_kv8_attn: out_partials and more than one split need partial");
   if (!aligned16(a->qkv) || !aligned16(a->q_norm_w) || !aligned16(a->k_norm_w) || !aligned16(a->cos_tab) ||
       !aligned16(a->sin_tab) || !aligned16(a->k8) || !aligned16(a->v8) || !aligned16(a->k_scale) || !aligned16(a->v_scale) ||
       !aligned16(a->out) || !aligned16(a->partial))
@@ -1028,7 +1067,7 @@ int qdec_kv8_attn_workspace(const qdec_kv8_attn_args *a, size_t *partial_bytes, 
   const int rc = plan_kv8_attn(a, &p, false);
   if (rc != QDEC_OK) return rc;
   const size_t rows = (size_t)p.batch * p.t_rows * p.nq;
-  if (partial_bytes) *partial_bytes = p.splits > 1 ? sizeof(float) * rows * p.splits * (p.head_dim + 2) : 0;
+  if (partial_bytes) *partial_bytes = p.splits > 1 || p.out_partials ? sizeof(float) * rows * p.splits * (p.head_dim + 2) : 0;
   if (counter_bytes) *counter_bytes = 0;
   return QDEC_OK;
 }

@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kW = 8;                  // waves of a workgroup
 constexpr int kRun = kW * kKv8Block;   // slots of a run
+static_assert(kRun == kKv8Run);
 __device__ __forceinline__ int div_by(const FastDiv &d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   const uint16_t *rows = p.qkv + (size_t)b * T * width;
   const int L = p.lens[b];
   if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
-    if (c0 == 0)
+    if (c0 == 0 && !p.out_partials)
       for (int i = threadIdx.x; i < nr * (D / 4); i += blockDim.x) {
         const int y = i / (D / 4), ch = (i - y * (D / 4)) * 4, r = r0 + y, t = div_by(p.by_g, r), row = b * T + t,
                   k = (kvh * G + r - t * G) * D + ch;
@@ -497,7 +498,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     }
 
     // ---- the waves' sums, in wave order; then the output or a partial: the
-    // normalised row, its maximum and its sum.
+    // normalised row, its maximum and its sum's 2^-20, a weight that no value
+    // overflows with.
     if (FOLD && c > c0) lds_barrier();  // the last split's are read
     if (col < AC) {
       const float lw = sum_xor16_32(l_run);
@@ -531,7 +533,9 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       }
       const int r = r0 + y;
       float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
-      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum);
+      const bool direct = n_active == 1 && !p.out_partials;
+      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum),
+                  wt = sum * 0x1p-20f;
       for (int dt = wave; dt < DT; dt += kW) {
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -543,25 +547,29 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
         const int k = dt * 16 + grp * 4;
-        if (n_active == 1) {
+        if (direct) {  // (as the merge has it of one partial)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = (o[i] * wt) / wt;
           const int t = div_by(p.by_g, r), row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
           uint16_t *dst = p.out + (p.ofrag ? frag_off(row, kk, p.ofrag) : (size_t)row * nq * D + kk);
           *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
         } else {
-          *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + k) = sum == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : o;
+          *reinterpret_cast<f32x4_t *>(part + (size_t)r * D + k) = o;
         }
       }
-      if (n_active > 1 && wave == 0 && grp == 0) {
-        part[(size_t)R * D + r] = M;
-        part[(size_t)R * D + R + r] = sum;
+      if (!direct && wave == 0 && grp == 0) {  // (a maximum of -inf: nothing seen)
+        part[(size_t)R * D + r] = M == NEG_INF && sum != 0.f ? 0.f : M;
+        part[(size_t)R * D + R + r] = wt;
       }
     }
     if constexpr (!FOLD) break;
   }
 }
 
-// Merge of the splits' partials, in order: D / 4 threads per query row.
-template <int D>
+// Merge of the splits' partials, in order: D / 4 threads per query row.  The operations
+// are those of attn_merge8 (gemm_dev.h), so a GEMM that merges has the same bits.
+// CB partials are loaded at a time, 8 or (from 9 splits on) 16.
+template <int D, int CB>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   constexpr int TR = D / 4;
   const int G = p.by_g.d, R = p.t_rows * G, kvh = blockIdx.y, b = blockIdx.z;
@@ -574,37 +582,43 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   const size_t stride = (size_t)R * (D + 2);
   const float *part = p.partial + ((size_t)b * p.nkv + kvh) * p.splits * stride;
   const float NEG_INF = -__builtin_huge_valf();
-  float M = NEG_INF, l = 0.f;
-  f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float mi[8], li[8];
-    f32x4_t a[8];
+  float m[CB], l[CB];
+  f32x4_t a[CB];
+  auto load_group = [&](int i0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < CB; ++i) {
       const float *pr = part + (size_t)min(i0 + i, n - 1) * stride;
-      mi[i] = pr[(size_t)R * D + r];
-      li[i] = pr[(size_t)R * D + R + r];
+      m[i] = pr[(size_t)R * D + r];
+      l[i] = pr[(size_t)R * D + R + r];
       a[i] = *reinterpret_cast<const f32x4_t *>(pr + (size_t)r * D + ch);
     }
-    float Mn = M;
+  };
+  load_group(0);
+  float M = NEG_INF, sum = 0.f;
+  f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) Mn = fmaxf(Mn, mi[i]);  // (the last partial repeats)
-    const float w0 = M == NEG_INF ? l * 0.f : __builtin_amdgcn_exp2f(M - Mn);
-    l *= w0;
-    o *= w0;
+  for (int i = 0; i < CB; ++i) M = fmaxf(M, m[i]);  // (the last partial repeats)
+  for (int i0 = CB; i0 < n; i0 += CB) {
+    float x[CB];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= n) continue;
-      const float w = li[i] * (mi[i] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mi[i] - Mn));
-      l += w;
-      o += a[i] * w;
-    }
-    M = Mn;
+    for (int i = 0; i < CB; ++i) x[i] = part[(size_t)min(i0 + i, n - 1) * stride + (size_t)R * D + r];
+#pragma unroll
+    for (int i = 0; i < CB; ++i) M = fmaxf(M, x[i]);
   }
-  const float inv = 1.f / l;
+  for (int i0 = 0; i0 < n; i0 += CB) {
+    if (i0 > 0) load_group(i0);
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+      if (i0 + i >= n || m[i] == NEG_INF) continue;
+      const float e = exp2f(m[i] - M), w = l[i] * e;
+      sum = __builtin_fmaf(l[i], e, sum);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = __builtin_fmaf(a[i][d], w, o[d]);
+    }
+  }
   const int t = div_by(p.by_g, r), row = b * p.t_rows + t, k = (kvh * G + r - t * G) * D + ch;
   uint16_t *dst = p.out + (p.ofrag ? frag_off(row, k, p.ofrag) : (size_t)row * p.nq * D + k);
-  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] * inv, o[1] * inv), pack2(o[2] * inv, o[3] * inv));
+  *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] / sum, o[1] / sum), pack2(o[2] / sum, o[3] / sum));
 }
 
 template <int D>
@@ -615,9 +629,10 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8, false>), grid, block, 0, s, p);
   else if ((int)p.by_parts.d == p.splits) hipLaunchKernelGGL((kv8_attn_kernel<D, 16, false>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((kv8_attn_kernel<D, 16, true>), grid, block, 0, s, p);
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.out_partials) {
     const int per = 256 / (D / 4);
-    hipLaunchKernelGGL((kv8_merge_kernel<D>), dim3((R + per - 1) / per, p.nkv, p.batch), dim3(256), 0, s, p);
+    const auto merge = p.splits > 8 ? kv8_merge_kernel<D, 16> : kv8_merge_kernel<D, 8>;
+    hipLaunchKernelGGL(merge, dim3((R + per - 1) / per, p.nkv, p.batch), dim3(256), 0, s, p);
   }
   return hipSuccess;
 }

@@ -52,7 +52,7 @@ class GemmArgs(ctypes.Structure):
                 ("tiles_per_wg", I32), ("x_attn", P), ("x_frag", I32), ("out_frag", I32),
                 ("parts_out", P), ("x_parts", P), ("x_nparts", I32), ("x_merged", P),
                 ("next_norm_w", P), ("next_xn", P), ("next_merged", P), ("next_threads", I32),
-                ("resident", I32)]
+                ("resident", I32), ("x_kv8", P)]
 
 
 class AttnArgs(ctypes.Structure):
@@ -141,7 +141,7 @@ class Kv8AttnArgs(ctypes.Structure):
     _fields_ = [("qkv", P), ("q_norm_w", P), ("k_norm_w", P), ("cos_tab", P), ("sin_tab", P), ("lens", P),
                 ("k8", P), ("v8", P), ("k_scale", P), ("v_scale", P), ("out", P), ("partial", P), ("eps", F32),
                 ("sm_scale", F32), ("batch", I32), ("t_rows", I32), ("nq", I32), ("nkv", I32), ("head_dim", I32),
-                ("cap", I32), ("splits", I32), ("out_frag", I32)]
+                ("cap", I32), ("splits", I32), ("out_frag", I32), ("out_partials", I32)]
 
 
 def declared_functions(header=HEADER):

@@ -47,6 +47,13 @@ KV8_BLOCK = 64  # the 8-bit cache's slots come in whole blocks (kKv8Block of qde
 # workgroup's stream on the same memory banks (attention of 32 sequences at 8200
 # slots, us by capacity: 8256 111, 8320 89, 8384 92, 8448 89, 9216 91, 9280 102).
 KV8_SLOTS = 128
+# Up to so many splits of the 8-bit cache's attention the O projection merges their
+# partials, for one sequence.  Every workgroup of O reads all of them, so a launch
+# that merges them once is ahead from there on and for two sequences (Qwen3-4B, ms
+# per step, merged by a launch / in O: one sequence, 3 splits 2.145 / 2.117, 5 2.153 /
+# 2.125, 7 2.167 / 2.140, 9 2.193 / 2.200, 17 2.238 / 2.302; two, 3 splits 2.178 /
+# 2.202).
+KV8_MERGE_IN_O_MAX_SPLITS = 8
 GEMM_WIDE_MIN_ROWS = 9  # of qdec_gemm_wide
 ATTN_MAX_T = 16
 # Rows (sequences x positions) of one prefill chunk: activations of 32K rows
@@ -640,10 +647,15 @@ class DecodeState:
         attention leaves its chunk partials and the O projection merges them
         while staging its activations (no arrival pass); bit-identical to
         the merged output.  The O-side merge takes 4 query heads per kv
-        head; other shapes merge in the attention."""
+        head; other shapes merge in the attention.  With an 8-bit cache:
+        one sequence of 2 to KV8_MERGE_IN_O_MAX_SPLITS splits."""
         c = self.model.cfg
-        return (t_rows == 1 and self.batch <= MERGE_IN_O_MAX_BATCH and c.group == 4 and c.head_dim == 128
-                and not self.kv8)
+        if t_rows != 1 or c.group != 4 or c.head_dim != 128:
+            return False
+        if not self.kv8:
+            return self.batch <= MERGE_IN_O_MAX_BATCH
+        part = self.lib.kv8_attn_workspace(self._kv8_args(0, 1))[0]  # 0: one split
+        return self.batch == 1 and 0 < part <= KV8_MERGE_IN_O_MAX_SPLITS * 4 * c.nq * (c.head_dim + 2)
 
     def _resident(self, a, role):
         """Whether the call ``a`` of ``role`` (resident still 0) runs
@@ -651,7 +663,7 @@ class DecodeState:
         plans (gate/up at RESIDENT_ROWS, RESIDENT_RES_ROLES at
         RESIDENT_RES_ROWS), and a plan the library accepts for this shape
         (asked once per role and row count)."""
-        if not self.resident or a.x_attn or a.next_norm_w:
+        if not self.resident or a.x_attn or a.x_kv8 or a.next_norm_w:
             return False
         if role == "gate_up":
             ok = not a.x_frag and any(lo <= a.rows <= hi for lo, hi in RESIDENT_ROWS)
@@ -749,7 +761,10 @@ class DecodeState:
             a.x, a.w, a.res = self.attn_out.data_ptr(), m.w_o[layer].data_ptr(), h.data_ptr()
             a.n, a.k, a.flags = c.hidden, c.nq * c.head_dim, capi.RES_OUT
             if x_attn is not None:
-                a.x_attn = ctypes.addressof(x_attn)
+                if self.kv8:
+                    a.x_kv8 = ctypes.addressof(x_attn)
+                else:
+                    a.x_attn = ctypes.addressof(x_attn)
                 a._x_attn = x_attn  # keeps the referenced struct alive
             else:
                 a.x_frag = 1 if rows >= FRAG_ROWS else 0
@@ -829,7 +844,7 @@ class DecodeState:
                     v_scale=self.v_scale[layer].data_ptr(), batch=self.batch, nkv=c.nkv, head_dim=c.head_dim,
                     cap=self.cap)
 
-    def _kv8_args(self, layer, t_rows):
+    def _kv8_args(self, layer, t_rows, partials=False):
         m, c = self.model, self.model.cfg
         a = capi.Kv8AttnArgs(**self.kv8_held(layer))
         a.qkv, a.q_norm_w, a.k_norm_w = self.qkv.data_ptr(), m.q_norm[layer].data_ptr(), m.k_norm[layer].data_ptr()
@@ -838,7 +853,8 @@ class DecodeState:
         if hasattr(self, "attn_partial"):
             a.partial = self.attn_partial.data_ptr()
         a.eps, a.sm_scale, a.t_rows, a.nq, a.splits = c.eps, c.head_dim ** -0.5, t_rows, c.nq, 0
-        a.out_frag = 1 if self.batch * t_rows >= FRAG_ROWS else 0
+        a.out_partials = 1 if partials else 0
+        a.out_frag = 1 if (not partials and self.batch * t_rows >= FRAG_ROWS) else 0
         return a
 
     def _tree_args(self, layer):
@@ -908,11 +924,14 @@ class DecodeState:
             lib.gemm(self._cached_gemm("qkv", i, rows), s)
             if tree:
                 lib.tree_attn(self._cached_tree(i), s)
+                at = None
             elif self.kv8:
-                lib.kv8_attn(self._cached_kv8(i, t_rows), s)
+                at = self._cached_kv8(i, t_rows, pm)
+                lib.kv8_attn(at, s)
             else:
-                lib.attn(self._cached_attn(i, t_rows, pm), s)
-            lib.gemm(self._cached_gemm("o", i, rows, self._cached_attn(i, t_rows, pm) if pm else None), s)
+                at = self._cached_attn(i, t_rows, pm)
+                lib.attn(at, s)
+            lib.gemm(self._cached_gemm("o", i, rows, at if pm else None), s)
             lib.gemm(self._cached_gemm("gate_up", i, rows), s)
             lib.gemm(self._cached_gemm("down", i, rows), s)
         if lm_head:
@@ -936,10 +955,11 @@ class DecodeState:
             self._attn_cache[key] = a
         return a
 
-    def _cached_kv8(self, layer, t_rows):
-        a = self._attn_cache.get(("kv8", layer, t_rows))
+    def _cached_kv8(self, layer, t_rows, partials=False):
+        key = ("kv8", layer, t_rows, partials)
+        a = self._attn_cache.get(key)
         if a is None:
-            a = self._attn_cache[("kv8", layer, t_rows)] = self._kv8_args(layer, t_rows)
+            a = self._attn_cache[key] = self._kv8_args(layer, t_rows, partials)
         return a
 
     def _cached_tree(self, layer):

@@ -368,6 +368,23 @@ def _shape_gemms(state, t):
         _fail("lm_head", f"{R} rows: cache lengths not advanced by one")
 
 
+def _merged_in_o(state, a, want, s, what):
+    """The O projection of the partials that the attention call ``a`` left must equal O
+    over the known rows ``want`` fed the ordinary way."""
+    lib, c, R = state.lib, state.model.cfg, want.shape[0]
+    res0 = torch.linspace(-2, 2, c.hidden, device=want.device).to(torch.bfloat16)[None].expand(R, -1)
+    state.attn_out.fill_(7.0)
+    state._hb(0)[:R].copy_(res0)
+    lib.gemm(state._gemm_args("o", 0, R, x_attn=a), s)
+    got = state._hb(0)[:R].clone()
+    o = state._gemm_args("o", 0, R)
+    _put_rows(state.attn_out, want, o.x_frag)
+    state._hb(0)[:R].copy_(res0)
+    lib.gemm(o, s)
+    if not torch.equal(got.view(torch.int16), state._hb(0)[:R].view(torch.int16)):
+        _fail(what, f"{R} rows: the O projection's merge of the chunk partials differs from the known attention output")
+
+
 def _shape_attention(state, t):
     """The attention of a step over t rows per sequence, through the state's
     chunking, wave count, output order (or the O projection's merge of its
@@ -423,21 +440,8 @@ def _shape_attention(state, t):
     pm = state._merge_in_o(t)
     a = state._attn_args(0, t, partials=pm)
     if pm:
-        # partials merged by the O projection: its output must equal O over
-        # the known rows fed the ordinary way
-        state.attn_out.fill_(7.0)
         lib.attn(a, s)
-        res0 = torch.linspace(-2, 2, c.hidden, device=dev).to(torch.bfloat16)[None].expand(R, -1)
-        state._hb(0)[:R].copy_(res0)
-        lib.gemm(state._gemm_args("o", 0, R, x_attn=a), s)
-        got = state._hb(0)[:R].clone()
-        o = state._gemm_args("o", 0, R)
-        _put_rows(state.attn_out, want, o.x_frag)
-        state._hb(0)[:R].copy_(res0)
-        lib.gemm(o, s)
-        if not torch.equal(got.view(torch.int16), state._hb(0)[:R].view(torch.int16)):
-            _fail("attention", f"{R} rows: the O projection's merge of the chunk partials differs from the "
-                               "known attention output")
+        _merged_in_o(state, a, want, s, "attention")
     else:
         lib.attn(a, s)
         got = _get_rows(state.attn_out, R, nq * D, a.out_frag)
@@ -516,6 +520,10 @@ def _shape_kv8(state, t):
     state.lens.copy_(torch.tensor(lens, dtype=torch.int32, device=dev))
     hv = rows[bi, hi, hs].view(B, nkv, D)
     want = hv.repeat_interleave(G, 1).reshape(B, 1, nq * D).expand(B, t, nq * D).reshape(R, nq * D).to(torch.bfloat16)
+    if state._merge_in_o(t):
+        a = state._kv8_args(0, t, partials=True)
+        lib.kv8_attn(a, s)
+        _merged_in_o(state, a, want, s, "8-bit attention")
     a = state._kv8_args(0, t)
     lib.kv8_attn(a, s)
     got = _get_rows(state.attn_out, R, nq * D, a.out_frag)

@@ -118,7 +118,8 @@ int qdec_embed(const qdec_embed_args *a, qdec_stream_t stream);
 
 /* ------------------------------------------------------------ skinny GEMM */
 
-struct qdec_attn_args;  /* below: the attention call a GEMM may take its x from */
+struct qdec_attn_args;  /* below: the attention calls a GEMM may take its x from */
+struct qdec_kv8_attn_args;
 
 /* y[m, n] = sum_k x'[m, k] * W[n, k] over the tiled weight, for m < rows
  * (1 <= rows <= 64), fp32 accumulation, one rounding to bf16, then:
@@ -256,6 +257,10 @@ typedef struct {
    * per output block, each normalising the rows itself
    * (engine/kernels/fused.py:33-172). */
   int32_t resident;
+  /* NULL, or a qdec_kv8_attn call made with out_partials = 1, in place of
+   * x_attn and on the same terms (head_dim 128, nq = 4 nkv).  No counterpart in
+   * the reference. */
+  const struct qdec_kv8_attn_args *x_kv8;
 } qdec_gemm_args;
 int qdec_gemm(const qdec_gemm_args *a, qdec_stream_t stream);
 /* Scratch sizes (bytes) a qdec_gemm call with these arguments needs. */
@@ -672,13 +677,13 @@ int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
  * What a row does not see does not reach it, whatever its slot or scale holds.  A length
  * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
  * of sequence b become NaN.
- * Slots are dealt in runs of 512, run j to workgroup j % splits of its
- * (sequence, kv head); with splits > 1 a second launch merges the workgroups'
- * partials, in order.  So a row's bits follow from what it sees and from splits,
+ * Slots are dealt in runs of 512, run j to split j % splits of its (sequence,
+ * kv head); with splits > 1 a second launch merges the splits' partials, in
+ * order, or a qdec_gemm that reads them (out_partials).  So a row's bits follow from what it sees and from splits,
  * never from t_rows, the other sequences or timing; 0 splits takes a number that
  * follows from batch, nkv and cap.  partial is scratch: calls that overlap in
  * time must not share it. */
-typedef struct {
+typedef struct qdec_kv8_attn_args {
   const void *qkv;      /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
   const void *q_norm_w; /* [head_dim] bf16 */
   const void *k_norm_w; /* [head_dim] bf16 */
@@ -701,6 +706,10 @@ typedef struct {
   int32_t cap;          /* slots per sequence, multiple of 64 */
   int32_t splits;       /* 1..256, or 0: chosen from the shape */
   int32_t out_frag;     /* 1: out in the fragment order of qdec_gemm_args */
+  int32_t out_partials; /* 0: rows to out.  1: every split leaves its unnormalised
+                           (acc, max, sum) in partial, out is not written, and a
+                           qdec_gemm with x_kv8 = these arguments merges them:
+                           the same bits without the merge's launch */
 } qdec_kv8_attn_args;
 int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream);
 /* Bytes of `partial`; counter_bytes, as in the other queries, is 0. */

@@ -16,7 +16,7 @@ def test_structs_match_header_fields():
     text = re.sub(r"/\*.*?\*/", "", open(capi.HEADER).read(), flags=re.S)
     for cname, st in (("qdec_kv8_store_args", capi.Kv8StoreArgs), ("qdec_kv8_load_args", capi.Kv8LoadArgs),
                       ("qdec_kv8_attn_args", capi.Kv8AttnArgs)):
-        body = re.search(r"typedef struct \{([^{}]*)\}\s*" + cname + ";", text).group(1)
+        body = re.search(r"typedef struct(?: \w+)? \{([^{}]*)\}\s*" + cname + ";", text).group(1)
         assert re.findall(r"\*?\s*(\w+)\s*;", body) == [f[0] for f in st._fields_], cname
 
 
@@ -39,7 +39,7 @@ def load(**kw):
 
 def attn(**kw):
     return fill(capi.Kv8AttnArgs, **{**dict(batch=2, t_rows=4, nq=32, nkv=8, head_dim=128, cap=1024, splits=0,
-                                            out_frag=0), **kw})
+                                            out_frag=0, out_partials=0), **kw})
 
 
 def shared(name, make):
@@ -89,6 +89,8 @@ CASES = shared("kv8_store", store) + shared("kv8_load", load) + shared("kv8_attn
     ("kv8_attn", attn, dict(splits=-1), -1, "splits"),
     ("kv8_attn", attn, dict(splits=257), -1, "splits"),
     ("kv8_attn", attn, dict(out_frag=2), -1, "out_frag"),
+    ("kv8_attn", attn, dict(out_partials=2), -1, "out_partials"),
+    ("kv8_attn", attn, dict(out_partials=1, splits=1, partial=None), -1, "partial"),
     ("kv8_attn", attn, dict(batch=16383, nkv=1000, nq=4000, splits=2), -3, "splits"),
     ("kv8_attn", attn, dict(splits=2, partial=None), -1, "partial"),
     ("kv8_attn", attn, dict(splits=2, partial=8), -2, "aligned"),
@@ -112,8 +114,53 @@ def test_null_args(qlib, name):
     assert getattr(qlib.so, "qdec_" + name)(None, None) == -1
 
 
+def merging(at, **kw):
+    """An O projection that merges the attention call's partials."""
+    g = fill(capi.GemmArgs, **{**dict(rows=1, n=2560, k=4096, flags=capi.RES_OUT, waves=8, x=None, x_attn=None, parts_out=None,
+                                      x_parts=None, x_frag=0, out_frag=0, next_norm_w=None, resident=0), **kw})
+    g.x_kv8 = ctypes.addressof(at)
+    return g
+
+
+def one(**kw):
+    return attn(**{**dict(batch=1, t_rows=1, out_partials=1), **kw})
+
+
+def test_merge_in_a_gemm(qlib):
+    for at, kw in ((one(), {}), (one(splits=1), {}), (one(cap=1 << 20), {}), (one(batch=2), dict(rows=2)),
+                   (one(t_rows=3), dict(rows=3)), (one(nq=16, nkv=4), dict(k=2048))):
+        qlib.gemm_workspace(merging(at, **kw))
+
+
+@pytest.mark.parametrize("at,kw,code,needle", [
+    (dict(out_partials=0), {}, -1, "out_partials"),
+    (dict(nq=64), dict(k=8192), -1, "shape"),
+    (dict(nq=16), dict(k=2048), -1, "shape"),
+    (dict(head_dim=64, nq=32), dict(k=2048), -1, "shape"),
+    (dict(cap=0), {}, -1, "shape"),
+    (dict(splits=-1), {}, -1, "shape"),
+    (dict(splits=257), {}, -1, "shape"),
+    (dict(batch=0), {}, -1, "shape"),
+    (dict(t_rows=2), {}, -1, "rows 1"),
+    ({}, dict(k=2048), -1, "rows 1"),
+    ({}, dict(flags=capi.NORM_IN), -3, "NORM_IN"),
+    ({}, dict(x_attn=16), -1, "both"),
+    ({}, dict(resident=1), -3, "x_attn"),
+    ({}, dict(ksplit=2, k=4096), -3, "x_attn"),
+    (dict(batch=5), dict(rows=5), -3, "x_attn"),
+    (dict(partial=None), {}, -1, "partial"),
+    (dict(lens=None), {}, -1, "lens"),
+])
+def test_merge_refusals(qlib, at, kw, code, needle):
+    a = one(**at)
+    g = merging(a, **kw)
+    assert qlib.so.qdec_gemm(ctypes.byref(g), None) == code
+    assert needle in qlib.last_error()
+
+
 def test_workspace(qlib):
     assert qlib.kv8_attn_workspace(attn(splits=1)) == (0, 0)
+    assert qlib.kv8_attn_workspace(attn(splits=1, out_partials=1)) == (4 * 2 * 4 * 32 * 130, 0)
     for nq, t, d, s in ((32, 4, 128, 2), (8, 16, 64, 7), (64, 8, 128, 256)):
         assert qlib.kv8_attn_workspace(attn(splits=s, nq=nq, t_rows=t, head_dim=d)) == (4 * 2 * t * nq * s * (d + 2), 0)
     # splits = 0 follows from batch, nkv and cap alone

@@ -127,6 +127,45 @@ def test_a_longer_prompt_after_a_shorter_one(model):
     assert torch.equal(st.logits[:2], want.logits[:2]) and torch.equal(st.k8, want.k8)
 
 
+@pytest.mark.parametrize("S", [500, 700, 1500])
+def test_attention_merged_in_o(model, monkeypatch, S):
+    """The steps whose O projection merges the attention's partials have the bits of
+    those whose attention does, and so do verify passes."""
+    name, cfg, eng, _ = model
+    if eng.model.cfg.group != 4 or eng.model.cfg.head_dim != 128:
+        pytest.skip("O merges 4 query heads of 128 channels per kv head")
+    B = 1
+    prompt = prompts(cfg["vocab_size"], B, S, S).to(eng.device)
+    got = []
+    for merge in (True, False):
+        st = state(eng, B, 1700, keep_logits=True)
+        assert st._merge_in_o(1) and not st._merge_in_o(2)
+        if not merge:
+            monkeypatch.setattr(st, "_merge_in_o", lambda t: False)
+        st.prefill(prompt)
+        rows = []
+        for _ in range(3):
+            st.run_step()
+            rows.append((st.logits[:B].clone(), st.ids[:B].clone()))
+        got.append(rows)
+    for x, y in zip(*got):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+    # one workgroup takes a sequence; many partials; two sequences
+    assert not any(state(eng, b, cap)._merge_in_o(1) for b, cap in ((1, 1000), (1, 4200), (2, 1700)))
+
+
+def test_long_speculation_gives_the_plain_tokens(model):
+    name, cfg, eng, _ = model
+    for B, S in ((1, 1100), (2, 1030)):
+        prompt = prompts(cfg["vocab_size"], B, S, 5 + B, motif=9).tolist()
+        plain = list(eng.generate(prompt, 30))
+        eng.speculate, eng.spec_gate = True, False
+        try:
+            assert list(eng.generate(prompt, 30)) == plain, (name, B)
+        finally:
+            eng.speculate, eng.spec_gate = False, True
+
+
 def test_memory(model):
     _, _, eng, _ = model
     from qdec.runtime import DecodeState

@@ -23,6 +23,7 @@ A new key before its rounding may be off by (D + 64) 2^-24 of the row's
 largest (norm and rotation in fp32), so |q - 127 k / top| <= 0.5 + 127 * 4 * (D
 + 64) * 2^-24: 0.506."""
 
+import ctypes
 import math
 import random
 
@@ -418,6 +419,52 @@ def test_not_finite_where_it_is_seen(lib):
     nan = torch.isnan(a.rows())
     assert not bool(nan[0, 0].any()) and bool(nan[0, 1:, :4].all()) and not bool(nan[0, 1:, 4:].any())
     assert bool(torch.isnan(a.c["v_scale"][0, 0, 71])) and int(torch.isnan(a.c["v_scale"][0, :, :73]).sum()) == 1
+
+
+@pytest.mark.parametrize("B,nkv,T,lens,splits", [
+    (1, 8, 1, [700], 0), (1, 8, 1, [1500], 0), (1, 8, 1, [9000], 0), (1, 8, 1, [511], 3), (1, 8, 1, [512], 3), (1, 8, 1, [40], 1),
+    (2, 8, 1, [3000, 90], 0), (2, 4, 1, [1023, 2600], 5), (1, 8, 3, [1022], 2), (1, 4, 4, [6000], 12), (1, 4, 1, [17000], 33)])
+@pytest.mark.parametrize("kind", ["plain", "loud", "nan"])
+def test_merge_in_the_next_gemm(lib, B, nkv, T, lens, splits, kind):
+    """A product that merges the partials (weights one on the diagonal, so that it
+    gives its rows) has the bits of the call that merges them itself."""
+    rows = []
+    k = nkv * 4 * 128
+    eye = torch.eye(k, device=DEV).to(BF)
+    w = torch.empty_like(eye)
+    lib.pack_tiles(eye.data_ptr(), w.data_ptr(), k, k, stream())
+    for partials in (0, 1):
+        a = Call(lib, B, 4 * nkv, nkv, 128, T, lens, splits=splits)
+        if kind == "loud":
+            a.c["v_scale"].mul_(1e33)
+        if kind == "nan":
+            a.c["k_scale"][B - 1, 1, 7] = NAN
+            a.qkv[B * T - 1, 2 * 128 + 5] = math.inf
+        a.a.out_partials = partials
+        pb, _ = lib.kv8_attn_workspace(a.a)
+        a.partial = torch.full((pb // 4 + 4,), NAN, device=DEV)
+        a.a.partial = a.partial.data_ptr()
+        a.run()
+        res = torch.zeros((B * T, k), dtype=BF, device=DEV)
+        o = capi.GemmArgs(x=a.out.data_ptr(), w=w.data_ptr(), res=res.data_ptr(), eps=EPS, rows=B * T, n=k, k=k,
+                          flags=capi.RES_OUT, ksplit=1, waves=8, tiles_per_wg=1)
+        if partials:
+            o.x_kv8 = ctypes.addressof(a.a)
+            assert bool((a.out == 9.0).all())
+        lib.gemm(o, stream())
+        rows.append(res)
+        if not partials and kind != "nan":
+            assert torch.equal(res, a.out) and bool(torch.isfinite(res).all())
+    torch.testing.assert_close(rows[1], rows[0], rtol=0, atol=0, equal_nan=True)
+    if kind == "nan":
+        assert bool(torch.isnan(rows[0]).any())
+    # a length that the attention refuses
+    a.lens_t.copy_(i32([a.cap - T + 1] + lens[1:]))
+    a.run()
+    res = torch.zeros((B * T, k), dtype=BF, device=DEV)
+    o.res = res.data_ptr()
+    lib.gemm(o, stream())
+    assert bool(torch.isnan(res[:T]).all())
 
 
 def test_run_of_the_operators(lib):
