@@ -2,26 +2,36 @@
 // quantised write of the new rows folded in: t_rows query rows per sequence,
 // row t at position lens[b] + t over slots 0 .. lens[b] + t.
 //
-// A workgroup of 8 waves takes up to 16 query rows of one (sequence, kv head) and
-// the runs c, c + splits, ... of 8 consecutive 64-slot blocks, its wave w one block
-// of each.  Blocks are dealt by
-// absolute slot numbers and a row is rescaled by its own scores alone, so a
-// row's bits do not depend on t_rows.  Per block
+// A workgroup of 8 waves takes up to 16 query rows of one (sequence, kv head) and,
+// for split c, the runs c, c + splits, ... of 8 consecutive 64-slot blocks, its
+// wave w one block of each.  Blocks are dealt by absolute slot numbers and a row is
+// rescaled by its own scores alone, so a row's bits do not depend on t_rows.  Per
+// block
 //   S^T = K . Q^T (v_mfma_i32_16x16x64_i8), exact: K as it is held, q in 21 bits,
 //     relative to its row's largest, as three digits of 7 bits.  The columns that few
 //     query rows leave hold their other digits: up to 4 rows take one matrix instruction
-//     where fp16 parts of q took two, and K no conversion (5 of every 20 vector
-//     instructions of a block).
+//     where fp16 parts of q took two, and K no conversion, a quarter of a block's
+//     vector instructions (32 x 4160 slots: 52.6 us with fp16 parts, 49.9 so).
 //   p = 2^(S scale_k scale_q - m), fp32 statistics.
 //   O^T += V^T . W^T (v_mfma_f32_16x16x32_f16) with w = p scale_v in fp16: 2^-11
 //     relative, an eighth of the output's rounding.  V's 8 bits are fp16 integers: a byte under
 //     the exponent byte 0x64 is 1024 + byte, so one byte permute makes two of them
-//     and one packed subtraction takes 1152 off.  fp16 reaches down to 2^-24 only, so a row's w are
-//     held in units of 2^(u - 15), 2^u above the largest |w| so far.
+//     and one packed subtraction takes 1152 off.  fp16 reaches down to 2^-24 only, so
+//     a row's w are held in units of 2^(level - 15), 2^level the largest |w| so far.
 // K's rows are dealt to MFMA rows so that a lane's 16 scores are the 16 slots of
 // one V group, the operand of the second product; slot l's scales sit in lane
-// l and reach the row by DPP.  K and V hold integers whatever lies behind the last slot, so
-// only scores and scales are masked.
+// l and reach the row by DPP.  K and V hold integers whatever lies behind the last
+// slot, so only scores and scales are masked.
+//
+// What bounds it, 32 query heads on 8 kv heads of 128 (MI355X, replayed graphs whose
+// caches take turns): where a launch fills the GPU, the cache's bytes, which arithmetic
+// lengthens by 1 to 2 us.  32 sequences of 4096 to 4220 slots: 281 MB in 49.4 us, 5.7
+// TB/s (47.3 with no arithmetic; a read of as much takes 40); the last of 9 rounds
+// occupies one or two of 8 waves.  131000 slots, 64 heads: 53 us, 7 of them the
+// merge.  A small launch is a chain: length, then rows and tables, then their
+// preparation, then the blocks that were loaded meanwhile: one sequence of 640 slots
+// 9.7 us (8.3 with no arithmetic; an empty launch takes 1.8), of 4100 slots in 9
+// splits 12.2 with the merge's 3.3.
 #include <algorithm>
 
 #include "dma_dev.h"
@@ -165,12 +175,13 @@ struct Lds {
   static constexpr int v8 = k8 + kKv8MaxT * D;                   // [2][D][16]
   static constexpr int sk = v8 + 2 * D * 16;                     // [kKv8MaxT]
   static constexpr int sv = sk + kKv8MaxT * 4;
-  static constexpr int m = sv + kKv8MaxT * 4;                    // [3][16][kW] wave statistics: maximum, sum, unit
+  static constexpr int m = sv + kKv8MaxT * 4;                    // [3][16][kW] the waves' maximum, sum and level
   static constexpr int bytes = m + 3 * kW * 16 * 4;
 };
 
 // AC: 4, 8 or 16, the columns of 16 that query rows take, at most so many rows; the
-// others hold other digits of them.
+// others hold other digits of them (one, two or three matrix instructions for 64
+// channels).  FOLD: several splits to a workgroup.
 template <int D, int AC, bool FOLD>
 __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p) {
   constexpr int NH = D / 64, DT = D / 16;
@@ -639,6 +650,12 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
 
 }  // namespace
 
+// At most one workgroup of few rows to a CU (registers hold one: a second would run
+// behind it), and runs of 512 slots to deal.  us, 32 heads on 8, with 1 / 2 / 4 splits: one
+// sequence of 640 slots 9.7 / 11.2 / -, of 1500 16.7 / - / 12.2; 8 of 1100 slots -
+// / 13.5 / 12.9; 13 of 1100 15.2 / 14.1 / 21.3; 20 of 1100 16.2 / 23.4 / -; 16 of
+// 4200 41.6 / 30.9 / 35.6.  Up to 1024 slots a merge costs what the second
+// round of blocks does.  The rule must not look at t_rows: a row keeps its bits.
 int kv8_attn_splits(int batch, int nkv, int cap) {
   const int64_t cells = (int64_t)batch * nkv;
   if (cap <= 2 * kRun) return 1;
@@ -646,6 +663,10 @@ int kv8_attn_splits(int batch, int nkv, int cap) {
   return (int)std::max<int64_t>(1, n);
 }
 
+// Workgroups that share the splits of a (sequence, kv head, row tile): with several
+// tiles of rows, so many that all run at once.  us for 8 sequences of 2000 slots and
+// 8 rows, 4 splits, a workgroup each / shared: 32 heads on 8 23.9 / 20.7, 64 on 8 41.0 /
+// 31.7; 500 slots in 4 splits 20.9 / 12.3.
 int kv8_attn_parts(int batch, int nkv, int splits, int tiles) {
   if (tiles == 1) return splits;
   const int64_t n = 256 / ((int64_t)batch * nkv * tiles);
