@@ -80,7 +80,6 @@ struct Partials {
   const int32_t *lens;
   int batch, t_rows, nkv, cap;
   int chunk, nchunks, strided;  // slots of a chunk, chunks of a (sequence, kv head), every how many blocks
-  int norm;                     // acc is divided by its sum
 };
 template <class A>
 static bool partials_shape(const A &a, Partials *p) {
@@ -98,10 +97,9 @@ static bool partials_of(const qdec_attn_args &a, Partials *p) {
   return true;
 }
 static bool partials_of(const qdec_kv8_attn_args &a, Partials *p) {
-  if (!partials_shape(a, p) || a.cap < kKv8Block || a.splits < 0 || a.splits > 256) return false;
+  if (!partials_shape(a, p) || a.t_rows != 1 || a.cap < kKv8Block || a.splits < 0 || a.splits > 256) return false;
   p->chunk = kKv8Run;
   p->nchunks = a.splits ? a.splits : kv8_attn_splits(a.batch, a.nkv, a.cap);
-  p->norm = 1;
   return true;
 }
 
@@ -397,7 +395,6 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     p->a_nchunks = xp.nchunks;
     p->a_cap = xp.cap;
     p->a_strided = xp.strided;
-    p->a_norm = xp.norm;
   }
   size_t pb = 0, cb = 0, xn_off = 0;
   gemm_scratch(a, *p, &pb, &cb, &xn_off);

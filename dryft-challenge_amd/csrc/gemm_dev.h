@@ -113,8 +113,7 @@ __device__ __forceinline__ void argmax_finish(uint64_t *keys, int rows, int nw, 
 // Activation vector (8 consecutive elements from k index kk) of row m,
 // merged from the attention chunk partials the previous launch left with
 // out_partials (attn_dev.h: per (sequence, kv head, chunk) acc [R][128],
-// max [R], sum [R], R = t_rows * 4; a_norm, kv8_attn.hip: acc divided by the
-// sum).  The same operations in the same order
+// max [R], sum [R], R = t_rows * 4; kv8_attn.hip with one row).  The same operations in the same order
 // as the attention's own chunk merge, so the bf16 result is bit-identical
 // to the output that call would have written.
 template <bool COH>
@@ -131,7 +130,7 @@ __device__ __forceinline__ uint4 attn_merge8(const GemmParams &p, int m, int kk)
   // A length the attention rejected (it wrote no partials) gives NaN, never
   // a merge of stale partials; the NaN reaches the argmax, whose pick is
   // then an out-of-vocabulary id the host refuses.
-  if (L < 0 || L > p.a_cap - T) return make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+  if (L < 0 || L + T - 1 >= p.a_cap) return make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
   const int n_active = min((p.a_strided ? (L + T - 1) >> 5 : (L + T - 1) / p.a_chunk) + 1, p.a_nchunks);
   const float NEG_INF = -__builtin_huge_valf();
   float mc[CB], lc[CB];
@@ -181,9 +180,8 @@ __device__ __forceinline__ uint4 attn_merge8(const GemmParams &p, int m, int kk)
       if (cc + j >= n_active || mc[j] == NEG_INF) continue;
       const float w = exp2f(mc[j] - mmax);
       lsum += lc[j] * w;
-      const float wa = p.a_norm ? lc[j] * w : w;
-      o0 += a0[j] * wa;
-      o1 += a1[j] * wa;
+      o0 += a0[j] * w;
+      o1 += a1[j] * w;
     }
   }
   uint4 v;

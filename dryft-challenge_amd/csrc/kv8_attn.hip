@@ -509,8 +509,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     }
 
     // ---- the waves' sums, in wave order; then the output or a partial: the
-    // normalised row, its maximum and its sum's 2^-20, a weight that no value
-    // overflows with.
+    // row's sum of values and of probabilities, both times 2^-20 (no value overflows
+    // with so many slots), and its maximum.
     if (FOLD && c > c0) lds_barrier();  // the last split's are read
     if (col < AC) {
       const float lw = sum_xor16_32(l_run);
@@ -545,8 +545,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       const int r = r0 + y;
       float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
       const bool direct = n_active == 1 && !p.out_partials;
-      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 15.f), inv = __builtin_amdgcn_rcpf(sum),
-                  wt = sum * 0x1p-20f;
+      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 35.f), wt = sum * 0x1p-20f;
       for (int dt = wave; dt < DT; dt += kW) {
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -556,11 +555,11 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
           for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(a[i], uw[w], o[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * inv * scale;
+        for (int i = 0; i < 4; ++i) o[i] *= scale;
         const int k = dt * 16 + grp * 4;
         if (direct) {  // (as the merge has it of one partial)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = (o[i] * wt) / wt;
+          for (int i = 0; i < 4; ++i) o[i] /= wt;
           const int t = div_by(p.by_g, r), row = b * T + t, kk = (kvh * G + r - t * G) * D + k;
           uint16_t *dst = p.out + (p.ofrag ? frag_off(row, kk, p.ofrag) : (size_t)row * nq * D + kk);
           *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
@@ -621,8 +620,8 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
 #pragma unroll
     for (int i = 0; i < CB; ++i) {
       if (i0 + i >= n || m[i] == NEG_INF) continue;
-      const float e = exp2f(m[i] - M), w = l[i] * e;
-      sum = __builtin_fmaf(l[i], e, sum);
+      const float w = exp2f(m[i] - M);
+      sum = __builtin_fmaf(l[i], w, sum);
 #pragma unroll
       for (int d = 0; d < 4; ++d) o[d] = __builtin_fmaf(a[i][d], w, o[d]);
     }

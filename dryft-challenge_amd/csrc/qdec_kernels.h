@@ -92,7 +92,7 @@ struct GemmParams {
   int amerge;
   const float *apart;
   const int32_t *alens;
-  int a_t_rows, a_nkv, a_chunk, a_nchunks, a_cap, a_strided, a_norm;
+  int a_t_rows, a_nkv, a_chunk, a_nchunks, a_cap, a_strided;
   // Split residual updates: a RES_OUT producer writes its k-split partials
   // (parts_out); a NORM_IN consumer merges xnparts of them into x first
   // (xparts) and writes the merged residual rows to xmerged.

@@ -258,8 +258,8 @@ typedef struct {
    * (engine/kernels/fused.py:33-172). */
   int32_t resident;
   /* NULL, or a qdec_kv8_attn call made with out_partials = 1, in place of
-   * x_attn and on the same terms (head_dim 128, nq = 4 nkv).  No counterpart in
-   * the reference. */
+   * x_attn and on the same terms, with t_rows 1 (head_dim 128, nq = 4 nkv).  No
+   * counterpart in the reference. */
   const struct qdec_kv8_attn_args *x_kv8;
 } qdec_gemm_args;
 int qdec_gemm(const qdec_gemm_args *a, qdec_stream_t stream);
@@ -709,7 +709,8 @@ typedef struct qdec_kv8_attn_args {
   int32_t out_partials; /* 0: rows to out.  1: every split leaves its unnormalised
                            (acc, max, sum) in partial, out is not written, and a
                            qdec_gemm with x_kv8 = these arguments merges them:
-                           the same bits without the merge's launch */
+                           the same bits without the merge's launch (both sums
+                           are held times 2^-20, so that none overflows) */
 } qdec_kv8_attn_args;
 int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream);
 /* Bytes of `partial`; counter_bytes, as in the other queries, is 0. */

@@ -128,7 +128,7 @@ def one(**kw):
 
 def test_merge_in_a_gemm(qlib):
     for at, kw in ((one(), {}), (one(splits=1), {}), (one(cap=1 << 20), {}), (one(batch=2), dict(rows=2)),
-                   (one(t_rows=3), dict(rows=3)), (one(nq=16, nkv=4), dict(k=2048))):
+                   (one(nq=16, nkv=4), dict(k=2048))):
         qlib.gemm_workspace(merging(at, **kw))
 
 
@@ -141,7 +141,8 @@ def test_merge_in_a_gemm(qlib):
     (dict(splits=-1), {}, -1, "shape"),
     (dict(splits=257), {}, -1, "shape"),
     (dict(batch=0), {}, -1, "shape"),
-    (dict(t_rows=2), {}, -1, "rows 1"),
+    (dict(t_rows=2), dict(rows=2), -1, "shape"),
+    (dict(batch=2), {}, -1, "rows 1"),
     ({}, dict(k=2048), -1, "rows 1"),
     ({}, dict(flags=capi.NORM_IN), -3, "NORM_IN"),
     ({}, dict(x_attn=16), -1, "both"),

@@ -423,7 +423,7 @@ def test_not_finite_where_it_is_seen(lib):
 
 @pytest.mark.parametrize("B,nkv,T,lens,splits", [
     (1, 8, 1, [700], 0), (1, 8, 1, [1500], 0), (1, 8, 1, [9000], 0), (1, 8, 1, [511], 3), (1, 8, 1, [512], 3), (1, 8, 1, [40], 1),
-    (2, 8, 1, [3000, 90], 0), (2, 4, 1, [1023, 2600], 5), (1, 8, 3, [1022], 2), (1, 4, 4, [6000], 12), (1, 4, 1, [17000], 33)])
+    (2, 8, 1, [3000, 90], 0), (2, 4, 1, [1023, 2600], 5), (4, 8, 1, [1022, 0, 511, 40], 2), (1, 4, 1, [17000], 33)])
 @pytest.mark.parametrize("kind", ["plain", "loud", "nan"])
 def test_merge_in_the_next_gemm(lib, B, nkv, T, lens, splits, kind):
     """A product that merges the partials (weights one on the diagonal, so that it
