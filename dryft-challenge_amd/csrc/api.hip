@@ -98,8 +98,8 @@ static bool partials_of(const qdec_attn_args &a, Partials *p) {
 }
 static bool partials_of(const qdec_kv8_attn_args &a, Partials *p) {
   if (!partials_shape(a, p) || a.t_rows != 1 || a.cap < kKv8Block || a.splits < 0 || a.splits > 256) return false;
-  p->chunk = kKv8Run;
   p->nchunks = a.splits ? a.splits : kv8_attn_splits(a.batch, a.nkv, a.cap);
+  p->chunk = kv8_attn_run(a.batch, a.nkv, a.cap, p->nchunks);
   return true;
 }
 
@@ -1023,6 +1023,7 @@ static int plan_kv8_attn(const qdec_kv8_attn_args *a, Kv8AttnParams *p, bool nee
   p->batch = a->batch; p->t_rows = a->t_rows; p->nq = a->nq; p->nkv = a->nkv;
   p->head_dim = a->head_dim; p->cap = a->cap;
   p->splits = a->splits ? a->splits : kv8_attn_splits(a->batch, a->nkv, a->cap);
+  p->run_log2 = kv8_attn_run(a->batch, a->nkv, a->cap, p->splits) == 256 ? 8 : 9;
   p->out_partials = a->out_partials;
   p->ofrag = a->out_frag && !a->out_partials ? (a->batch * a->t_rows + 15) / 16 : 0;
   // A launch's work items are numbered in 32 bits.

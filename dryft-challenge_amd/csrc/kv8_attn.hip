@@ -2,9 +2,9 @@
 // quantised write of the new rows folded in: t_rows query rows per sequence,
 // row t at position lens[b] + t over slots 0 .. lens[b] + t.
 //
-// A workgroup of 8 waves takes up to 16 query rows of one (sequence, kv head) and,
-// for split c, the runs c, c + splits, ... of 8 consecutive 64-slot blocks, its
-// wave w one block of each.  Blocks are dealt by absolute slot numbers and a row is
+// A workgroup takes up to 16 query rows of one (sequence, kv head) and, for split c,
+// the runs c, c + splits, ... of 4 or 8 consecutive 64-slot blocks, one block of
+// each to a wave.  Blocks are dealt by absolute slot numbers and a row is
 // rescaled by its own scores alone, so a row's bits do not depend on t_rows.  Per
 // block
 //   S^T = K . Q^T (v_mfma_i32_16x16x64_i8), exact: K as it is held, q in 21 bits,
@@ -30,8 +30,8 @@
 // occupies one or two of 8 waves.  131000 slots, 64 heads: 53 us, 7 of them the
 // merge.  A small launch is a chain: length, then rows and tables, then their
 // preparation, then the blocks that were loaded meanwhile: one sequence of 640 slots
-// 9.7 us (8.3 with no arithmetic; an empty launch takes 1.8), of 4100 slots in 9
-// splits 12.2 with the merge's 3.3.
+// 6.8 us before its partials are merged (an empty launch takes 1.8) and 9.3 with the
+// merge's launch, of 4100 slots in 9 splits 12.1.
 #include <algorithm>
 
 #include "dma_dev.h"
@@ -46,9 +46,6 @@ namespace qdec {
 
 namespace {
 
-constexpr int kW = 8;                  // waves of a workgroup
-constexpr int kRun = kW * kKv8Block;   // slots of a run
-static_assert(kRun == kKv8Run);
 __device__ __forceinline__ int div_by(const FastDiv &d, int n) { return (int)(((uint64_t)(uint32_t)n * d.mul) >> d.shift); }
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
@@ -165,27 +162,28 @@ __device__ __forceinline__ void digits4(const float *x, float down, uint32_t &a,
 }
 
 // LDS (bytes).
-template <int D, int AC>
+template <int D, int AC, int BW>
 struct Lds {
   static constexpr int RS = D + 16;                              // bytes per query row (bank spread)
   static constexpr int q = 0;                                    // [3][AC][RS] digits of the queries
-  static constexpr int acc = q + 3 * AC * RS;                    // [kW][D / 16][4][AC] f32x4
-  static constexpr int qs = acc + kW * (D / 16) * 4 * AC * 16;   // [16] query rows' factors
+  static constexpr int acc = q + 3 * AC * RS;                    // [BW][D / 16][4][AC] f32x4
+  static constexpr int qs = acc + BW * (D / 16) * 4 * AC * 16;   // [16] query rows' factors
   static constexpr int k8 = qs + 16 * 4;                         // [kKv8MaxT][D]
   static constexpr int v8 = k8 + kKv8MaxT * D;                   // [2][D][16]
   static constexpr int sk = v8 + 2 * D * 16;                     // [kKv8MaxT]
   static constexpr int sv = sk + kKv8MaxT * 4;
-  static constexpr int m = sv + kKv8MaxT * 4;                    // [3][16][kW] the waves' maximum, sum and level
-  static constexpr int bytes = m + 3 * kW * 16 * 4;
+  static constexpr int m = sv + kKv8MaxT * 4;                    // [3][16][BW] the waves' maximum, sum and level
+  static constexpr int bytes = m + 3 * BW * 16 * 4;
 };
 
 // AC: 4, 8 or 16, the columns of 16 that query rows take, at most so many rows; the
 // others hold other digits of them (one, two or three matrix instructions for 64
-// channels).  FOLD: several splits to a workgroup.
-template <int D, int AC, bool FOLD>
-__global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p) {
-  constexpr int NH = D / 64, DT = D / 16;
-  using LY = Lds<D, AC>;
+// channels).  BW: waves that take blocks, a run's; NW waves in all, 4 rows to prepare for
+// each.  FOLD: several splits to a workgroup.
+template <int D, int AC, int BW, bool FOLD>
+__global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(const Kv8AttnParams p) {
+  constexpr int NH = D / 64, DT = D / 16, NW = AC == 16 ? 8 : BW, RUN = BW * kKv8Block;
+  using LY = Lds<D, AC, BW>;
   constexpr int RS = LY::RS;
   __shared__ __attribute__((aligned(16))) unsigned char smem[LY::bytes];
   unsigned char *s_q = smem + LY::q;
@@ -239,7 +237,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     vs = __builtin_nontemporal_load(vscale + s0 + lane);
   };
   // This wave's first block, and one round's step.
-  const int j0 = kW * c0 + wave, step = kW * C;
+  const bool takes = BW == NW || wave < BW;
+  const int j0 = takes ? BW * c0 + wave : 0x7fffffff, step = BW * C;
   const uint16_t *rows = p.qkv + (size_t)b * T * width;
   const int L = p.lens[b];
   if (L < 0 || L > p.cap - T) {  // no cache access that counts; the rows become NaN
@@ -253,9 +252,9 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     return;
   }
   const int last = L + T - 1, nb = last / kKv8Block + 1;
-  if (kW * c0 >= nb) return;
+  if (BW * c0 >= nb) return;
   auto ours = [&](int slot) {  // its run is of one of this workgroup's splits
-    const int run = slot / kRun, c = run - div_by(p.by_splits, run) * C;
+    const int run = slot / RUN, c = run - div_by(p.by_splits, run) * C;
     return FOLD ? c - div_by(p.by_parts, c) * P == c0 : c == c0;
   };
   const bool mine = ours(L) || ours(last);
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
   // preparation) is what the first block waits for, and behind the blocks of a full
   // launch each of its steps would take microseconds.
   constexpr int N = D / 16;
-  const int quad = kW - 1 - wave, quads = (nr + 3) / 4;
+  const int quad = NW - 1 - wave, quads = (nr + 3) / 4;
   const bool query = quad < quads, job = query || (mine && quad < quads + (T + 3) / 4);
   const int i = 4 * (query ? quad : quad - quads) + grp, n = query ? nr : T, at = min(i, n - 1);
   const int t = query ? div_by(p.by_g, r0 + at) : at, head = query ? kvh * G + r0 + at - t * G : nq + kvh, ch = N * col;
@@ -376,7 +375,7 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     fn(Int<8>{}); fn(Int<9>{}); fn(Int<10>{}); fn(Int<11>{}); fn(Int<12>{}); fn(Int<13>{}); fn(Int<14>{}); fn(Int<15>{});
   };
 
-  const int n_active = min(C, (nb + kW - 1) / kW);
+  const int n_active = min(C, (nb + BW - 1) / BW);
   for (int c = c0; c < n_active; c += P) {
     // Of the split's blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
     // units of 2^(level - 15).
@@ -384,8 +383,8 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     f32x4_t acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int j = kW * c + wave; j < nb; j += step) {
-      const int next = j + step < nb ? j + step : FOLD && c + P < n_active ? kW * (c + P) + wave : nb;
+    for (int j = takes ? BW * c + wave : nb; j < nb; j += step) {
+      const int next = j + step < nb ? j + step : FOLD && c + P < n_active ? BW * (c + P) + wave : nb;
       const int s0 = j * kKv8Block;
       const bool edge = s0 + kKv8Block > L;  // slots that not every row sees, the new rows among them
       if (edge) {                            // which come from LDS
@@ -512,32 +511,32 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
     // row's sum of values and of probabilities, both times 2^-20 (no value overflows
     // with so many slots), and its maximum.
     if (FOLD && c > c0) lds_barrier();  // the last split's are read
-    if (col < AC) {
+    if (takes && col < AC) {
       const float lw = sum_xor16_32(l_run);
       if (grp == 0) {
-        s_m[col * kW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
-        s_m[(16 + col) * kW + wave] = lw;
-        s_m[(32 + col) * kW + wave] = level;
+        s_m[col * BW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
+        s_m[(16 + col) * BW + wave] = lw;
+        s_m[(32 + col) * BW + wave] = level;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) s_acc[((wave * DT + dt) * 4 + grp) * AC + col] = acc[dt];
     }
     lds_barrier();
     if (row_in && col < AC) {
-      float mw[kW], lw[kW], uw[kW], M = NEG_INF, U = NEG_INF, sum = 0.f;
+      float mw[BW], lw[BW], uw[BW], M = NEG_INF, U = NEG_INF, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kW; w += 4) {
-        *reinterpret_cast<f32x4_t *>(mw + w) = *reinterpret_cast<const f32x4_t *>(s_m + col * kW + w);
-        *reinterpret_cast<f32x4_t *>(lw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (16 + col) * kW + w);
-        *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * kW + w);
+      for (int w = 0; w < BW; w += 4) {
+        *reinterpret_cast<f32x4_t *>(mw + w) = *reinterpret_cast<const f32x4_t *>(s_m + col * BW + w);
+        *reinterpret_cast<f32x4_t *>(lw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (16 + col) * BW + w);
+        *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * BW + w);
       }
 #pragma unroll
-      for (int w = 0; w < kW; ++w) {
+      for (int w = 0; w < BW; ++w) {
         M = fmaxf(M, mw[w]);
         U = fmaxf(U, uw[w]);
       }
 #pragma unroll
-      for (int w = 0; w < kW; ++w) {
+      for (int w = 0; w < BW; ++w) {
         // (a NaN among a wave's scores stays, also where it saw nothing else)
         sum = __builtin_fmaf(lw[w], mw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M), sum);
         uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
@@ -546,10 +545,10 @@ __global__ void __launch_bounds__(64 * kW) kv8_attn_kernel(const Kv8AttnParams p
       float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
       const bool direct = n_active == 1 && !p.out_partials;
       const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 35.f), wt = sum * 0x1p-20f;
-      for (int dt = wave; dt < DT; dt += kW) {
+      for (int dt = wave; dt < DT; dt += NW) {
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kW; ++w) {
+        for (int w = 0; w < BW; ++w) {
           const f32x4_t a = s_acc[((w * DT + dt) * 4 + grp) * AC + col];
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(a[i], uw[w], o[i]);
@@ -586,7 +585,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   const int r = blockIdx.x * (256 / TR) + threadIdx.x / TR;
   const int L = p.lens[b];
   if (r >= R || L < 0 || L > p.cap - p.t_rows) return;
-  const int n = min(p.splits, (L + p.t_rows - 1) / kRun + 1);
+  const int n = min(p.splits, ((L + p.t_rows - 1) >> p.run_log2) + 1);
   if (n == 1) return;  // written by its workgroup
   const int ch = (int)(threadIdx.x % TR) * 4;
   const size_t stride = (size_t)R * (D + 2);
@@ -631,14 +630,15 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] / sum, o[1] / sum), pack2(o[2] / sum, o[3] / sum));
 }
 
-template <int D>
+template <int D, int BW>
 hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   const int R = p.t_rows * (p.nq / p.nkv);
-  const dim3 grid((unsigned)(p.batch * p.nkv * (int)p.by_parts.d * ((R + 15) / 16))), block(64 * kW);
-  if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4, false>), grid, block, 0, s, p);
-  else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8, false>), grid, block, 0, s, p);
-  else if ((int)p.by_parts.d == p.splits) hipLaunchKernelGGL((kv8_attn_kernel<D, 16, false>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((kv8_attn_kernel<D, 16, true>), grid, block, 0, s, p);
+  const dim3 grid((unsigned)(p.batch * p.nkv * (int)p.by_parts.d * ((R + 15) / 16)));
+  const dim3 block(64 * (R <= 8 ? BW : 8));
+  if (R <= 4) hipLaunchKernelGGL((kv8_attn_kernel<D, 4, BW, false>), grid, block, 0, s, p);
+  else if (R <= 8) hipLaunchKernelGGL((kv8_attn_kernel<D, 8, BW, false>), grid, block, 0, s, p);
+  else if ((int)p.by_parts.d == p.splits) hipLaunchKernelGGL((kv8_attn_kernel<D, 16, BW, false>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((kv8_attn_kernel<D, 16, BW, true>), grid, block, 0, s, p);
   if (p.splits > 1 && !p.out_partials) {
     const int per = 256 / (D / 4);
     const auto merge = p.splits > 8 ? kv8_merge_kernel<D, 16> : kv8_merge_kernel<D, 8>;
@@ -649,17 +649,29 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
 
 }  // namespace
 
-// At most one workgroup of few rows to a CU (registers hold one: a second would run
-// behind it), and runs of 512 slots to deal.  us, 32 heads on 8, with 1 / 2 / 4 splits: one
-// sequence of 640 slots 9.7 / 11.2 / -, of 1500 16.7 / - / 12.2; 8 of 1100 slots -
-// / 13.5 / 12.9; 13 of 1100 15.2 / 14.1 / 21.3; 20 of 1100 16.2 / 23.4 / -; 16 of
-// 4200 41.6 / 30.9 / 35.6.  Up to 1024 slots a merge costs what the second
-// round of blocks does.  The rule must not look at t_rows: a row keeps its bits.
+// Slots of a run: 8 blocks, or 4 where a workgroup for each of those finds a CU of its own.  A CU
+// has about 64 KB in flight, half of what 8 waves ask for at once, so more CUs take
+// less time until their partials cost more than that.  us with runs of 512 / 256, each in
+// its splits and with the merge, 32 heads on 8: one sequence of 1500 slots 11.1 / 9.4, of
+// 4000 12.1 / 12.0 and with 9 rows 13.1 / 14.9, of 6100 12.5 / 12.9; two of 1100 11.1 /
+// 9.2, four 11.4 / 9.7.  Up to 512 slots a run of 8 blocks needs no merge.  The rules must not
+// look at t_rows: a row keeps its bits.
+static bool short_runs(int batch, int nkv, int cap) {
+  return cap > 512 && cap <= 2048 && (int64_t)batch * nkv * ((cap + 255) / 256) <= 256;
+}
+int kv8_attn_run(int batch, int nkv, int cap, int splits) { return splits > 1 && short_runs(batch, nkv, cap) ? 256 : 512; }
+
+// At most one workgroup of few rows to a CU (registers hold one of 8 waves: a second
+// would run behind it).  us for runs of 512 in 1 / 2 / 4 splits: 8 sequences of 1100
+// slots 13.8 / 12.8 / 12.1; 13 of 1100 15.2 / 14.1 / 21.3; 20 of 1100 16.2 / 23.4 / -; 16
+// of 4200 41.6 / 30.9 / 35.6.  Up to 1024 slots a merge costs as much as it gives: one
+// sequence of 640 slots in 1 split 9.7, in 3 of short runs 9.3 in a replayed graph, but 11.5
+// and 12.9 launch by launch.  A caller that has the merge done elsewhere asks for 3.
 int kv8_attn_splits(int batch, int nkv, int cap) {
   const int64_t cells = (int64_t)batch * nkv;
-  if (cap <= 2 * kRun) return 1;
-  const int64_t n = std::min<int64_t>(256 / cells, (cap + kRun - 1) / kRun);
-  return (int)std::max<int64_t>(1, n);
+  if (cap <= 1024) return 1;
+  if (short_runs(batch, nkv, cap)) return (cap + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(256 / cells, (cap + 511) / 512));
 }
 
 // Workgroups that share the splits of a (sequence, kv head, row tile): with several
@@ -673,7 +685,8 @@ int kv8_attn_parts(int batch, int nkv, int splits, int tiles) {
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnParams &p, hipStream_t s) {
-  return p.head_dim == 128 ? launch_d<128>(p, s) : launch_d<64>(p, s);
+  if (p.run_log2 == 8) return p.head_dim == 128 ? launch_d<128, 4>(p, s) : launch_d<64, 4>(p, s);
+  return p.head_dim == 128 ? launch_d<128, 8>(p, s) : launch_d<64, 8>(p, s);
 }
 
 }  // namespace qdec

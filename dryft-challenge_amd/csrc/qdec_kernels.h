@@ -325,12 +325,13 @@ struct Kv8AttnParams {
   float scale_log2;  // log2(e) / sqrt(head_dim)
   int batch, t_rows, nq, nkv, head_dim, cap;
   int out_partials;  // partials of every split, no merge
-  int splits;  // of a (sequence, kv head): run j of 8 blocks goes to split j % splits
+  int splits;  // of a (sequence, kv head): run j goes to split j % splits
+  int run_log2;  // slots of a run: 256 or 512
   FastDiv by_splits, by_parts, by_nkv, by_g, by_tiles;  // parts: workgroups that share the splits; g: query heads
                                                         // per kv head; tiles: of 16 query rows
   int ofrag;   // > 0: out is written in fragment order with this many M tiles
 };
-constexpr int kKv8Run = 512;  // slots of a run: 8 blocks
+int kv8_attn_run(int batch, int nkv, int cap, int splits);
 int kv8_attn_splits(int batch, int nkv, int cap);
 int kv8_attn_parts(int batch, int nkv, int splits, int tiles);
 hipError_t launch_kv8_attn(const Kv8AttnParams &p, hipStream_t s);

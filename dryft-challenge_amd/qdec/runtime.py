@@ -50,9 +50,8 @@ KV8_SLOTS = 128
 # Up to so many splits of the 8-bit cache's attention the O projection merges their
 # partials, for one sequence.  Every workgroup of O reads all of them, so a launch
 # that merges them once is ahead from there on and for two sequences (Qwen3-4B, ms
-# per step, merged by a launch / in O: one sequence, 3 splits 2.145 / 2.117, 5 2.153 /
-# 2.125, 7 2.167 / 2.140, 9 2.193 / 2.200, 17 2.238 / 2.302; two, 3 splits 2.178 /
-# 2.202).
+# per step, merged by a launch / in O: one sequence, 3 splits 2.094 / 2.054, 7 2.092 /
+# 2.056, 9 2.193 / 2.200, 17 2.238 / 2.302; two, 3 splits 2.178 / 2.202).
 KV8_MERGE_IN_O_MAX_SPLITS = 8
 GEMM_WIDE_MIN_ROWS = 9  # of qdec_gemm_wide
 ATTN_MAX_T = 16
@@ -369,6 +368,16 @@ def attn_waves(batch):
     batch alone: plain and speculative states of one batch agree.  8 waves
     take at most ATTN8_MAX_T rows per sequence (max_rows_per_seq)."""
     return 8 if batch >= ATTN8_MIN_BATCH else 4
+
+
+def kv8_splits(batch, nkv, cap):
+    """Splits of the 8-bit cache's attention in replayed steps (0: the library's
+    choice).  From 513 to 1024 slots, where a call by itself is as fast in one:
+    runs of 256, whose merge O does or a replayed launch (Qwen3-4B, ms per step of 640
+    slots in 1 split / in 3: one sequence 2.099 / 2.054, and us per call of two 9.8 /
+    9.3, four 10.0 / 9.6)."""
+    n = -(-cap // 256)
+    return n if 512 < cap <= 1024 and batch * nkv * n <= 256 else 0
 
 
 def state_attn_waves(batch, nkv, head_dim, cap):
@@ -852,7 +861,8 @@ class DecodeState:
         a.out = self.attn_out.data_ptr()
         if hasattr(self, "attn_partial"):
             a.partial = self.attn_partial.data_ptr()
-        a.eps, a.sm_scale, a.t_rows, a.nq, a.splits = c.eps, c.head_dim ** -0.5, t_rows, c.nq, 0
+        a.eps, a.sm_scale, a.t_rows, a.nq = c.eps, c.head_dim ** -0.5, t_rows, c.nq
+        a.splits = kv8_splits(self.batch, c.nkv, self.cap)
         a.out_partials = 1 if partials else 0
         a.out_frag = 1 if (not partials and self.batch * t_rows >= FRAG_ROWS) else 0
         return a

@@ -677,12 +677,12 @@ int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
  * What a row does not see does not reach it, whatever its slot or scale holds.  A length
  * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
  * of sequence b become NaN.
- * Slots are dealt in runs of 512, run j to split j % splits of its (sequence,
+ * Slots are dealt in runs of 256 or 512, run j to split j % splits of its (sequence,
  * kv head); with splits > 1 a second launch merges the splits' partials, in
- * order, or a qdec_gemm that reads them (out_partials).  So a row's bits follow from what it sees and from splits,
- * never from t_rows, the other sequences or timing; 0 splits takes a number that
- * follows from batch, nkv and cap.  partial is scratch: calls that overlap in
- * time must not share it. */
+ * order, or a qdec_gemm that reads them (out_partials).  The run follows from batch,
+ * nkv, cap and splits, and 0 splits takes a number that follows from the first
+ * three, so a row's bits follow from these and from what it sees, never from
+ * t_rows, the other sequences or timing.  partial is scratch: calls that overlap in time must not share it. */
 typedef struct qdec_kv8_attn_args {
   const void *qkv;      /* [batch*t_rows, (nq + 2*nkv)*head_dim] bf16 */
   const void *q_norm_w; /* [head_dim] bf16 */

@@ -151,7 +151,7 @@ def test_attention_merged_in_o(model, monkeypatch, S):
     for x, y in zip(*got):
         assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
     # one workgroup takes a sequence; many partials; two sequences
-    assert not any(state(eng, b, cap)._merge_in_o(1) for b, cap in ((1, 1000), (1, 4200), (2, 1700)))
+    assert not any(state(eng, b, cap)._merge_in_o(1) for b, cap in ((1, 500), (1, 4200), (2, 1700)))
 
 
 def test_long_speculation_gives_the_plain_tokens(model):

@@ -21,3 +21,10 @@ def test_modes_that_go_together():
         engine.check_modes(kv, True, False)
     engine.check_modes("bf16", "tree", None)
     engine.check_modes("bf16", False, True)
+
+
+def test_splits_of_a_state():
+    from qdec.runtime import kv8_splits
+    for shape, n in (((1, 8, 512), 0), ((1, 8, 640), 3), ((1, 8, 1024), 4), ((1, 8, 1152), 0), ((8, 8, 1024), 4), ((9, 8, 1024), 0),
+                     ((32, 2, 640), 3), ((32, 8, 640), 0)):
+        assert kv8_splits(*shape) == n, shape
