@@ -468,6 +468,43 @@ def test_merge_in_the_next_gemm(lib, B, nkv, T, lens, splits, kind):
     assert bool(torch.isnan(res[:T]).all())
 
 
+class Banded:
+    """A tensor's copy in the middle of a larger buffer."""
+
+    def __init__(self, x, band=4096):
+        n = x.numel() * x.element_size()
+        self.buf = torch.full((n + 2 * band,), 0x5a, dtype=torch.uint8, device=DEV)
+        self.t = self.buf[band:band + n].view(x.dtype).view(x.shape)
+        self.t.copy_(x)
+        self.band = band
+
+    def whole(self):
+        return bool((self.buf[:self.band] == 0x5a).all()) and bool((self.buf[-self.band:] == 0x5a).all())
+
+
+@pytest.mark.parametrize("shape", [(2, 32, 8, 128, 1, [1087, 0]), (1, 64, 8, 128, 8, [2040]), (3, 9, 3, 64, 5, [59, 123, 0]), (5, 40, 8, 128, 1, [639] * 5)])
+@pytest.mark.parametrize("splits", [0, 1, 7])
+def test_guard_bands(lib, shape, splits):
+    """Nothing is written outside the tensors, with the last slots of the cache taken."""
+    a = Call(lib, *shape, splits=splits, frag=shape[0] * shape[4] >= 5)
+    pb, _ = lib.kv8_attn_workspace(a.a)
+    held = {k: Banded(v) for k, v in a.c.items()}
+    out, part = Banded(a.out), Banded(torch.zeros(max(pb, 16) // 4, device=DEV))
+    for k, v in held.items():
+        setattr(a.a, k, v.t.data_ptr())
+    a.a.out, a.a.partial = out.t.data_ptr(), part.t.data_ptr()
+    a.run()
+    n, slots, st = a.cap - 7, (a.cap + 31) // 32 * 32, i32([7] * a.B)
+    rows = [randn(gen(4), a.B, a.nkv, a.cap, a.D).to(BF) for _ in range(2)]
+    ks, vs = (Banded(x) for x in slab(rows, slots))
+    both = dict(k_slab=ks.t.data_ptr(), v_slab=vs.t.data_ptr(), batch=a.B, nkv=a.nkv, head_dim=a.D, cap=a.cap, slab_cap=slots, n=n,
+                **{k: v.t.data_ptr() for k, v in held.items()})
+    lib.kv8_store(capi.Kv8StoreArgs(pos0=7, **both), stream())
+    lib.kv8_load(capi.Kv8LoadArgs(starts=st.data_ptr(), **both), stream())
+    torch.cuda.synchronize()
+    assert all(x.whole() for x in (*held.values(), out, part, ks, vs))
+
+
 def test_run_of_the_operators(lib):
     """A prompt's slots stored, steps over them, and a read back of all of it
     into slabs that are stored again.  A row held from bf16 numbers comes back
