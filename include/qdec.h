@@ -709,8 +709,11 @@ typedef struct qdec_kv8_attn_args {
   int32_t out_partials; /* 0: rows to out.  1: every split leaves its unnormalised
                            (acc, max, sum) in partial, out is not written, and a
                            qdec_gemm with x_kv8 = these arguments merges them:
-                           the same bits without the merge's launch (both sums
-                           are held times 2^-20, so that none overflows) */
+                           the same bits without the merge's launch.  partial:
+                           [batch][nkv][splits] x (acc [R][head_dim], max [R] of
+                           the scores in powers of 2, sum [R]), R = t_rows * nq /
+                           nkv, acc and sum times 2^-20, so that none overflows;
+                           splits that hold no slot are not written */
 } qdec_kv8_attn_args;
 int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream);
 /* Bytes of `partial`; counter_bytes, as in the other queries, is 0. */

@@ -468,6 +468,34 @@ def test_merge_in_the_next_gemm(lib, B, nkv, T, lens, splits, kind):
     assert bool(torch.isnan(res[:T]).all())
 
 
+@pytest.mark.parametrize("shape", [(2, 32, 8, 128, 1, [1500, 300]), (4, 32, 8, 128, 9, [1100, 255, 768, 1143]), (1, 8, 2, 64, 10, [3000]),
+                                   (5, 64, 8, 128, 8, [1800, 40, 511, 1000, 1543]), (3, 16, 8, 128, 4, [20, 0, 500])])
+@pytest.mark.parametrize("splits", [0, 3])
+def test_partials(lib, shape, splits):
+    """What out_partials leaves, merged in 64 bits, against the call's own rows: both
+    round once to bf16, the call's with a merge in fp32."""
+    B, nq, nkv, D, T, lens = shape
+    a = Call(lib, *shape, splits=splits).run()
+    b = Call(lib, *shape, splits=splits)
+    b.a.out_partials = 1
+    R, pb = T * nq // nkv, lib.kv8_attn_workspace(b.a)[0]
+    C = pb // (4 * B * nkv * R * (D + 2))
+    b.partial = torch.full((pb // 4 + 4,), NAN, device=DEV)
+    b.a.partial = b.partial.data_ptr()
+    b.run()
+    assert bool((b.out == 9.0).all()) and bool(torch.isnan(b.partial[pb // 4:]).all())
+    part = b.partial[:pb // 4].view(B, nkv, C, R * (D + 2)).double()
+    acc, m, l = part[..., :R * D].reshape(B, nkv, C, R, D), part[..., R * D:R * (D + 1)], part[..., R * (D + 1):]
+    left = ~torch.isnan(m)  # the splits that hold slots left theirs: as many of the first for every row
+    n = left.sum(2, keepdim=True)
+    assert bool((left == (torch.arange(C, device=DEV)[:, None] < n)).all()) and bool((n == n[:, :1, :, :1]).all())
+    top = m.masked_fill(~left, -math.inf).amax(2, keepdim=True)
+    w = torch.where(left & (m > -math.inf), torch.exp2(m - top), 0.0)
+    want = (torch.where(w[..., None] > 0, acc, 0.0) * w[..., None]).sum(2) / (torch.where(w > 0, l, 0.0) * w).sum(2)[..., None]
+    want = want.view(B, nkv, T, nq // nkv, D).transpose(1, 2).reshape(B, T, nq, D)
+    torch.testing.assert_close(a.rows().double(), want, rtol=2 ** -8, atol=float(want.abs().max()) * 2 ** -18)
+
+
 class Banded:
     """A tensor's copy in the middle of a larger buffer."""
 
