@@ -577,12 +577,14 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
 
 // Merge of the splits' partials, in order: D / 4 threads per query row.  The operations
 // are those of attn_merge8 (gemm_dev.h), so a GEMM that merges has the same bits.
-// CB partials are loaded at a time, 8 or (from 9 splits on) 16.
+// CB partials are loaded at a time, 8 or (from 9 splits on) 16.  Workgroups of one wave
+// reach more CUs than those of four (call and merge, us, 256 / 64 threads: 13 sequences of
+// 1100 slots 13.8 / 13.5, one of 131000 in 32 splits 54.1 / 53.2).
 template <int D, int CB>
-__global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
+__global__ void __launch_bounds__(64) kv8_merge_kernel(const Kv8AttnParams p) {
   constexpr int TR = D / 4;
   const int G = p.by_g.d, R = p.t_rows * G, kvh = blockIdx.y, b = blockIdx.z;
-  const int r = blockIdx.x * (256 / TR) + threadIdx.x / TR;
+  const int r = blockIdx.x * (64 / TR) + threadIdx.x / TR;
   const int L = p.lens[b];
   if (r >= R || L < 0 || L > p.cap - p.t_rows) return;
   const int n = min(p.splits, ((L + p.t_rows - 1) >> p.run_log2) + 1);
@@ -640,9 +642,9 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
   else if ((int)p.by_parts.d == p.splits) hipLaunchKernelGGL((kv8_attn_kernel<D, 16, BW, false>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((kv8_attn_kernel<D, 16, BW, true>), grid, block, 0, s, p);
   if (p.splits > 1 && !p.out_partials) {
-    const int per = 256 / (D / 4);
+    const int per = 64 / (D / 4);
     const auto merge = p.splits > 8 ? kv8_merge_kernel<D, 16> : kv8_merge_kernel<D, 8>;
-    hipLaunchKernelGGL(merge, dim3((R + per - 1) / per, p.nkv, p.batch), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(merge, dim3((R + per - 1) / per, p.nkv, p.batch), dim3(64), 0, s, p);
   }
   return hipSuccess;
 }
