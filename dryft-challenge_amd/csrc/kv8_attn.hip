@@ -661,7 +661,16 @@ hipError_t launch_d(const Kv8AttnParams &p, hipStream_t s) {
 static bool short_runs(int batch, int nkv, int cap) {
   return cap > 512 && cap <= 2048 && (int64_t)batch * nkv * ((cap + 255) / 256) <= 256;
 }
-int kv8_attn_run(int batch, int nkv, int cap, int splits) { return splits > 1 && short_runs(batch, nkv, cap) ? 256 : 512; }
+// In one split: also where there are more workgroups than CUs, since registers hold two of 4
+// waves, which start and end beside each other (us, 64 sequences of 300 slots 18.0 /
+// 13.4, of 500 21.4 / 17.7, of 1100 33.6 / 30.5, of 2100 53.6 / 50.6, 40 of 500 18.9 / 15.5; but
+// 32 of 1100 18.4 / 19.3), and for short caches of more than a few sequences (32 of 200 8.7 /
+// 8.3; one of 60 6.2 / 6.6).
+int kv8_attn_run(int batch, int nkv, int cap, int splits) {
+  const int64_t cells = (int64_t)batch * nkv;
+  if (splits > 1) return short_runs(batch, nkv, cap) ? 256 : 512;
+  return cells > 256 || (cells > 64 && cap <= 512) ? 256 : 512;
+}
 
 // At most one workgroup of few rows to a CU (registers hold one of 8 waves: a second
 // would run behind it).  us for runs of 512 in 1 / 2 / 4 splits: 8 sequences of 1100

@@ -252,6 +252,8 @@ ATTN = [
     (5, 32, 8, 128, 2, [4100, 50, 3000, 64, 4095]), (1, 64, 8, 128, 1, [20011]), (1, 8, 2, 64, 10, [5837]),
     # several row tiles, workgroups in no whole eights; new rows on either side of a run's end
     (3, 12, 3, 64, 16, [500, 1020, 0]), (1, 20, 5, 128, 16, [1017]), (7, 64, 1, 64, 1, [511, 512, 513, 1023, 1024, 1535, 1536]),
+    # one split of runs of 256 slots
+    (33, 32, 8, 128, 1, [97 * i % 700 for i in range(33)]), (9, 16, 8, 128, 6, [63 * i for i in range(9)]), (65, 8, 4, 64, 3, [11 * i for i in range(65)]),
     # splits that share a workgroup, runs of 512 slots and of 256
     (4, 32, 8, 128, 9, [1100, 255, 768, 1143]), (3, 48, 6, 64, 8, [2040, 256, 1023]),
     (5, 64, 8, 128, 8, [2600, 511, 0, 1537, 2048]), (11, 24, 4, 64, 10, [3000, 90, 1024, 1526, 600, 5, 1018, 2999, 64, 512, 1800]),
@@ -301,7 +303,8 @@ def test_flat_and_peaked_scores(lib, gain):
 
 @pytest.mark.parametrize("shape", [(2, 32, 8, 128, [700, 61]), (1, 64, 8, 128, [1022]), (3, 8, 2, 64, [0, 63, 500]),
                                    (2, 16, 8, 128, [509, 1021]), (1, 30, 3, 64, [1533]),
-                                   (5, 64, 8, 128, [1500, 1021, 3, 1533, 700]), (4, 64, 8, 128, [1100, 253, 766, 1])])
+                                   (5, 64, 8, 128, [1500, 1021, 3, 1533, 700]), (4, 64, 8, 128, [1100, 253, 766, 1]),
+                                   (33, 32, 8, 128, [53 * i for i in range(33)]), (9, 40, 8, 128, [55 * i for i in range(9)])])
 @pytest.mark.parametrize("splits", [0, 1, 3])
 def test_rows_do_not_depend_on_the_pass(lib, shape, splits):
     """One pass of 6 rows and 6 passes of one leave the same bits, in the rows
