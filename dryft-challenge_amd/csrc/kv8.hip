@@ -153,10 +153,11 @@ __global__ void __launch_bounds__(64 * kWaves) kv8_store_kernel(const Kv8CopyPar
   else store_values<D>(p, at.cell, s0, s1);
 }
 
-// Byte i of w as an int8, times s: the byte with its sign bit turned is 128 more, and
-// 128 s is exact, so the product is rounded once.
+// Byte i of w, whose sign bits are turned, as an int8 times s: the byte is 128 more and
+// the difference exact, so the product is rounded once.  (Taking 128 s off the product
+// instead would leave fp32's range from s = 2^121 on, rows of the two largest bf16 numbers.)
 __device__ __forceinline__ float byte_times(uint32_t w, int i, float s) {
-  return __builtin_fmaf((float)((w >> (8 * i)) & 0xffu), s, -128.f * s);
+  return ((float)((w >> (8 * i)) & 0xffu) - 128.f) * s;
 }
 
 template <int D>

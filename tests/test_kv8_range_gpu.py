@@ -1,0 +1,68 @@
+"""The 8-bit cache over the whole range of its numbers: what is finite stays finite, at the
+largest and the smallest scales, scores, queries and values that fp32 holds.
+
+Where scores are large, their rounding is too, so the cases are those whose result does not
+depend on it: scores that are the same number for every slot (weights exactly equal),
+or so far apart that one slot has all the weight (the next one less than e^-100).  What is left
+of the tolerance of test_kv8_gpu.py is then its part without scores:
+  2^-8 |ref|  the rounding to bf16, and of mag = sum |p v| / sum p
+  2^-11       w = p * v_scale in fp16
+  (n + 64) 2^-22  sums over n slots, exponentials, rescaling factors in fp32
+and 2^-39 step for fp16's smallest steps."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv8_oracle as ko
+from qdec import capi
+from test_kv8_gpu import BF, DEV, EPS, NAN, Call, cache, gen, lib, ptrs, randn, slab, stream  # noqa: F401  (lib: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def read_back(lib, c, B, nkv, D, cap, n):
+    """Slots 0 .. n - 1 of a cache as rows of bf16."""
+    slots = (n + 31) // 32 * 32
+    k, v = torch.zeros((B, nkv, slots, D), dtype=BF, device=DEV), torch.zeros((B, nkv, slots // 8, D, 8), dtype=BF, device=DEV)
+    lib.kv8_load(capi.Kv8LoadArgs(k_slab=k.data_ptr(), v_slab=v.data_ptr(), batch=B, nkv=nkv, head_dim=D, cap=cap, slab_cap=slots,
+                                  n=n, **ptrs(c)), stream())
+    return k[:, :, :n], ko.slab_rows(v)[:, :, :n]
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_load_of_any_scale(lib, D):
+    B, nkv, cap = 2, 3, 192
+    c = cache(gen(3), B, nkv, cap, D)
+    c["k8"].clamp_(min=-127), c["v8"].clamp_(min=-127)  # what a store writes
+    big = torch.tensor([0x7f7f, 0x7f7e, 0x7f7d, 0x7f00], dtype=torch.int16).view(BF).double()
+    scales = torch.cat(((big / 127).float(), torch.tensor([2.0 ** 120, 2.0 ** -100 / 127, 2.0 ** -100, 0.0, NAN, 1e-20, 1.0])))
+    for name in ("k_scale", "v_scale"):
+        c[name].copy_(scales.to(DEV)[torch.randint(len(scales), (B, nkv, cap), generator=gen(4), device=DEV)])
+    for got, q8, sc in zip(read_back(lib, c, B, nkv, D, cap, cap), (c["k8"], ko.row_major(c["v8"])), (c["k_scale"], c["v_scale"])):
+        want = (q8.float() * sc[..., None]).to(BF)
+        torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+        assert torch.equal(torch.isfinite(got), torch.isfinite(sc)[..., None].expand_as(got))
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_extreme_rows_there_and_back(lib, D):
+    """Rows whose largest is a bf16 number at either end of what is held."""
+    tops = torch.tensor([0x7f7f, 0x7f7e, 0x7f7d, 0x7f01, 0x7f00, 0x7e80, 0x3f80, 0x0e01, 0x0d80, 0x0d7f, 0x0001, 0x0000],
+                        dtype=torch.int16, device=DEV).view(BF)  # 0x0d80: 2^-100
+    g, n = gen(6), len(tops)
+    rows = []
+    for _ in range(2):
+        x = (torch.rand((1, 2, n, D), generator=g, device=DEV) * 2 - 1) * tops.float()[:, None]
+        x[..., 7], x[..., 20] = tops.float(), 0.0
+        rows.append(x.to(BF))
+    ks, vs = slab(rows, 32)
+    c = cache(g, 1, 2, 64, D)
+    lib.kv8_store(capi.Kv8StoreArgs(k_slab=ks.data_ptr(), v_slab=vs.data_ptr(), batch=1, nkv=2, head_dim=D, cap=64, slab_cap=32, pos0=0,
+                                    n=n, **ptrs(c)), stream())
+    for got, x in zip(read_back(lib, c, 1, 2, D, 64, n), rows):
+        q, s = ko.hold(x)
+        want = (q.float() * s.float()[..., None]).to(BF)
+        assert bool(torch.isfinite(got).all()) and bool((got[..., 20] == 0).all())
+        assert torch.equal(got, want)
