@@ -12,12 +12,15 @@
 //     query rows leave hold their other digits: up to 4 rows take one matrix instruction
 //     where fp16 parts of q took two, and K no conversion, a quarter of a block's
 //     vector instructions (32 x 4160 slots: 52.6 us with fp16 parts, 49.9 so).
-//   p = 2^(S scale_k scale_q - m), fp32 statistics.
+//   p = 2^((S scale_k - m) scale_q), fp32 statistics.  The difference comes first: it is as
+//     exact as the scores, where m scale_q, rounded by itself, is off by whole powers of 2 from
+//     2^24 on and takes p and w out of range.
 //   O^T += V^T . W^T (v_mfma_f32_16x16x32_f16) with w = p scale_v in fp16: 2^-11
 //     relative, an eighth of the output's rounding.  V's 8 bits are fp16 integers: a byte under
 //     the exponent byte 0x64 is 1024 + byte, so one byte permute makes two of them
 //     and one packed subtraction takes 1152 off.  fp16 reaches down to 2^-24 only, so
-//     a row's w are held in units of 2^(level - 15), 2^level the largest |w| so far.
+//     a row's w are held in units of 2^(level - 15), 2^level the largest |w| so far, like p
+//     relative to the maximum so far, so that level is a small number whatever the scores.
 // K's rows are dealt to MFMA rows so that a lane's 16 scores are the 16 slots of
 // one V group, the operand of the second product; slot l's scales sit in lane
 // l and reach the row by DPP.  K and V hold integers whatever lies behind the last
@@ -377,8 +380,8 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
 
   const int n_active = min(C, (nb + BW - 1) / BW);
   for (int c = c0; c < n_active; c += P) {
-    // Of the split's blocks so far: the largest score and, in powers of 2, the largest |w|; acc is in
-    // units of 2^(level - 15).
+    // Of the split's blocks so far: the largest score (before scale_q) and, in powers of 2, the largest
+    // |w| beside it; acc is in units of 2^(level - 15).
     float m_run = NEG_INF, l_run = 0.f, level = NEG_INF;
     f32x4_t acc[DT];
 #pragma unroll
@@ -464,11 +467,11 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
       for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
       const float m_old = m_run;
       m_run = fmaxf(m_run, max_xor16_32(top));
-      const float mq = m_run == NEG_INF ? 0.f : m_run * qs;
+      const float base = m_run == NEG_INF ? 0.f : m_run;
       float psum = 0.f, big = 0.f;
       each([&](auto n) {
         constexpr int i = decltype(n)::value;
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], qs, -mq));
+        const float e = __builtin_amdgcn_exp2f((s[i] - base) * qs);
         psum += e;
         s[i] = e * row_lane<i>(vs);
       });
@@ -479,13 +482,13 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) big = fmaxf(big, s[i]);
-      const float alpha = m_old == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m_old - m_run) * qs);
-      l_run = __builtin_fmaf(l_run, alpha, psum);
-      const float level_old = level;
-      level = fmaxf(level, mq + __builtin_amdgcn_logf(max_xor16_32(big)));
-      // (in range also where a slot with values of zero has raised mq, not level: from a factor
-      // of 2^126 on the others' p are below 2^-111)
-      const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(mq - level + 15.f, 126.f));
+      const float fall = (m_old - base) * qs;  // of what is there, in powers of 2
+      l_run = __builtin_fmaf(l_run, __builtin_amdgcn_exp2f(fall), psum);
+      const float level_old = level + fall;
+      level = fmaxf(level_old, __builtin_amdgcn_logf(max_xor16_32(big)));
+      // (in range also where a slot with values of zero has raised the maximum, not level: from a
+      // factor of 2^126 on the others' p are below 2^-111)
+      const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(15.f - level, 126.f));
       f16x8_t w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
     if (takes && col < AC) {
       const float lw = sum_xor16_32(l_run);
       if (grp == 0) {
-        s_m[col * BW + wave] = m_run * (m_run == NEG_INF ? 1.f : qs);
+        s_m[col * BW + wave] = m_run;
         s_m[(16 + col) * BW + wave] = lw;
         s_m[(32 + col) * BW + wave] = level;
       }
@@ -531,20 +534,21 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
         *reinterpret_cast<f32x4_t *>(uw + w) = *reinterpret_cast<const f32x4_t *>(s_m + (32 + col) * BW + w);
       }
 #pragma unroll
+      for (int w = 0; w < BW; ++w) M = fmaxf(M, mw[w]);
+#pragma unroll
       for (int w = 0; w < BW; ++w) {
-        M = fmaxf(M, mw[w]);
+        const float fall = mw[w] == NEG_INF ? NEG_INF : (mw[w] - M) * qs;
+        // (a NaN among a wave's scores stays, also where it saw nothing else)
+        sum = __builtin_fmaf(lw[w], __builtin_amdgcn_exp2f(fall), sum);
+        uw[w] += fall;
         U = fmaxf(U, uw[w]);
       }
 #pragma unroll
-      for (int w = 0; w < BW; ++w) {
-        // (a NaN among a wave's scores stays, also where it saw nothing else)
-        sum = __builtin_fmaf(lw[w], mw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(mw[w] - M), sum);
-        uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
-      }
+      for (int w = 0; w < BW; ++w) uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
       const int r = r0 + y;
       float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
       const bool direct = n_active == 1 && !p.out_partials;
-      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - M - 35.f), wt = sum * 0x1p-20f;
+      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - 35.f), wt = sum * 0x1p-20f;
       for (int dt = wave; dt < DT; dt += NW) {
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
         }
       }
       if (!direct && wave == 0 && grp == 0) {  // (a maximum of -inf: nothing seen)
-        part[(size_t)R * D + r] = M == NEG_INF && sum != 0.f ? 0.f : M;
+        part[(size_t)R * D + r] = M != NEG_INF ? M * qs : sum != 0.f ? 0.f : M;
         part[(size_t)R * D + R + r] = wt;
       }
     }

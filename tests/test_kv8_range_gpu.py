@@ -66,3 +66,66 @@ def test_extreme_rows_there_and_back(lib, D):
         want = (q.float() * s.float()[..., None]).to(BF)
         assert bool(torch.isfinite(got).all()) and bool((got[..., 20] == 0).all())
         assert torch.equal(got, want)
+
+
+def along_one_channel(lib, shape, splits, gain, key):
+    """A call whose queries lie on channel 63 alone, so that a slot's score is gain times
+    its key there: 100 * key(slot), and 0 for the new slots."""
+    B, nq, nkv, D, T, lens = shape
+    a = Call(lib, *shape, splits=splits)
+    x = a.qkv.view(B * T, -1, D)
+    x[:, :nq] = 0.0
+    x[:, :nq, D // 2 - 1] = 1.0
+    x[:, nq:nq + nkv, D // 2 - 1] = 0.0
+    a.cos[:], a.sin[:] = 1.0, 0.0
+    a.qw[D // 2 - 1] = gain
+    a.c["k8"][..., D // 2 - 1] = 100
+    for b, L in enumerate(lens):
+        a.c["k_scale"][b, :, :L] = key(torch.arange(L, device=DEV, dtype=torch.float32), L)
+    return a
+
+
+def check_no_score_error(a):
+    a.run()
+    got, tab = a.rows().double(), (a.cos[:a.T], a.sin[:a.T])
+    assert bool(torch.isfinite(got).all())
+    for b, L in enumerate(a.lens):
+        q = ko.norm_rope(a.qkv.view(a.B, a.T, a.nq + 2 * a.nkv, a.D)[b, :, :a.nq], a.qw, *tab, EPS)
+        ref, mag, step, _, _ = ko.attend(q, a.c["k8"][b], a.c["k_scale"][b], a.c["v8"][b], a.c["v_scale"][b], L, a.D ** -0.5)
+        tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + (L + a.T + 64) * 2 ** -22) + step * 2 ** -39
+        worst = ((got[b] - ref).abs() / tol).max().item()
+        assert worst <= 1, f"sequence {b} of length {L}: {worst:.3g} of the tolerance"
+
+
+SHAPES = [(1, 32, 8, 128, 1, [900]), (2, 32, 8, 128, 2, [700, 61]), (1, 32, 8, 128, 9, [1500]), (2, 8, 2, 64, 3, [64, 1100]),
+          (9, 16, 8, 128, 4, [55 * i + 1 for i in range(9)]), (3, 64, 8, 128, 8, [2000, 511, 5])]
+ORDERS = {
+    "equal": lambda i, L: torch.full_like(i, 0.01),
+    "rising": lambda i, L: 0.001 * (i + 1),
+    "falling": lambda i, L: 0.001 * (L - i),
+    "mixed": lambda i, L: 0.001 * (1 + (i * 641) % L if math.gcd(641, L) == 1 else 1 + i),
+}
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("order", sorted(ORDERS))
+def test_scores_of_any_size(lib, shape, splits, order):
+    """gain times 1 for every slot, or gain / 10 from one to the next."""
+    for log2 in (10, 20, 24, 25, 26, 27, 30, 31, 33, 40, 60, 100):
+        check_no_score_error(along_one_channel(lib, shape, splits, 2.0 ** log2, ORDERS[order]))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("log2", [20, 24, 28, 32, 50, 90])
+def test_large_random_scores_stay_among_the_values(lib, shape, log2):
+    """An output is a mean of values: never beyond the largest of them, by more than the
+    rounding of the weights (2^-11) and its own (2^-8)."""
+    a = Call(lib, *shape, gain=2.0 ** log2).run()
+    got = a.rows()
+    assert bool(torch.isfinite(got).all())
+    for b, L in enumerate(a.lens):
+        end = L + a.T
+        top = (ko.row_major(a.c["v8"])[b, :, :end].float().abs() * a.c["v_scale"][b, :, :end, None]).amax((1, 2))  # per kv head
+        most = got[b].float().abs().view(a.T, a.nkv, -1).amax((0, 2))
+        assert bool((most <= top * (1 + 2 ** -7)).all())
