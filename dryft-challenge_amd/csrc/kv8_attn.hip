@@ -548,7 +548,9 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
       const int r = r0 + y;
       float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
       const bool direct = n_active == 1 && !p.out_partials;
-      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - 35.f), wt = sum * 0x1p-20f;
+      // (2^(U - 15), a normal number for every row that is held, and 2^-20 by itself: together they
+      // would be 0 for values below 2^-84)
+      const float scale = U == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(U - 15.f), wt = sum * 0x1p-20f;
       for (int dt = wave; dt < DT; dt += NW) {
         f32x4_t o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
           for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(a[i], uw[w], o[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= scale;
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * 0x1p-20f * scale;
         const int k = dt * 16 + grp * 4;
         if (direct) {  // (as the merge has it of one partial)
 #pragma unroll

@@ -129,3 +129,16 @@ def test_large_random_scores_stay_among_the_values(lib, shape, log2):
         top = (ko.row_major(a.c["v8"])[b, :, :end].float().abs() * a.c["v_scale"][b, :, :end, None]).amax((1, 2))  # per kv head
         most = got[b].float().abs().view(a.T, a.nkv, -1).amax((0, 2))
         assert bool((most <= top * (1 + 2 ** -7)).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("log2", [-60, -80, -86, -92, 110, 120])
+def test_values_of_one_size(lib, shape, splits, log2):
+    """All values, the new ones too, about 2^log2: from near 2^-100, where rows are held as
+    zeros, to near the largest bf16 number."""
+    a = Call(lib, *shape, splits=splits)
+    a.c["v_scale"].copy_((torch.rand(a.c["v_scale"].shape, generator=gen(8), device=DEV) * 0.01 + 0.002) * 2.0 ** log2)
+    a.qkv.view(a.B * a.T, -1, a.D)[:, -a.nkv:] *= 2.0 ** log2
+    a.checked()
+    assert bool((a.rows().float().abs().amax(-1) > 2.0 ** (log2 - 12)).all())
