@@ -485,10 +485,10 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
       const float fall = (m_old - base) * qs;  // of what is there, in powers of 2
       l_run = __builtin_fmaf(l_run, __builtin_amdgcn_exp2f(fall), psum);
       const float level_old = level + fall;
-      level = fmaxf(level_old, __builtin_amdgcn_logf(max_xor16_32(big)));
-      // (in range also where a slot with values of zero has raised the maximum, not level: from a
-      // factor of 2^126 on the others' p are below 2^-111)
-      const float up = level == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(fminf(15.f - level, 126.f));
+      // (Not below -111, so that w's factor stays in range also where a slot with values of zero has
+      // raised the maximum, not level: a normal w is 1 or more then, which fp16 rounds as ever.)
+      level = fmaxf(fmaxf(level_old, __builtin_amdgcn_logf(max_xor16_32(big))), -111.f);
+      const float up = __builtin_amdgcn_exp2f(15.f - level);
       f16x8_t w[2];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {

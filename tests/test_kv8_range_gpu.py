@@ -85,14 +85,15 @@ def along_one_channel(lib, shape, splits, gain, key):
     return a
 
 
-def check_no_score_error(a):
+def check_no_score_error(a, score=0.0, least=0.0):
+    """`score`: what is known of the weights' error all the same, `least`: an error of any output."""
     a.run()
     got, tab = a.rows().double(), (a.cos[:a.T], a.sin[:a.T])
     assert bool(torch.isfinite(got).all())
     for b, L in enumerate(a.lens):
         q = ko.norm_rope(a.qkv.view(a.B, a.T, a.nq + 2 * a.nkv, a.D)[b, :, :a.nq], a.qw, *tab, EPS)
         ref, mag, step, _, _ = ko.attend(q, a.c["k8"][b], a.c["k_scale"][b], a.c["v8"][b], a.c["v_scale"][b], L, a.D ** -0.5)
-        tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + (L + a.T + 64) * 2 ** -22) + step * 2 ** -39
+        tol = 2 ** -8 * ref.abs() + mag * (2 ** -11 + score + (L + a.T + 64) * 2 ** -22) + step * 2 ** -39 + least
         worst = ((got[b] - ref).abs() / tol).max().item()
         assert worst <= 1, f"sequence {b} of length {L}: {worst:.3g} of the tolerance"
 
@@ -142,3 +143,20 @@ def test_values_of_one_size(lib, shape, splits, log2):
     a.qkv.view(a.B * a.T, -1, a.D)[:, -a.nkv:] *= 2.0 ** log2
     a.checked()
     assert bool((a.rows().float().abs().amax(-1) > 2.0 ** (log2 - 12)).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("gap", [60.0, 75.0, 80.0, 84.0])
+def test_small_weights_beside_values_of_zero(lib, shape, splits, gap):
+    """The last cached slot has values of zero and a score `gap` above all others, so an output
+    is their values times e^-gap, down to 2^-121.  The one score is off by its query's 21
+    bits (2^-20 of it) and by 64 roundings at most, which scales every other weight; an output
+    is held times 2^-20 (in up to 3 partials), so in steps of 2^-129, rounded once each and
+    once where it is joined."""
+    a = along_one_channel(lib, shape, splits, 1.0, lambda i, L: torch.where(i == L - 1, gap / 100, 0.0))
+    a.c["v_scale"].copy_(torch.rand(a.c["v_scale"].shape, generator=gen(8), device=DEV) * 5 + 1)
+    for b, L in enumerate(a.lens):
+        a.c["v_scale"][b, :, L - 1] = 0.0
+    check_no_score_error(a, score=2 * gap * (2 ** -20 + 64 * 2 ** -24), least=6 * 2.0 ** -130)
+    assert bool((a.rows().float().abs().amax(-1) > 2.0 ** -126).all())
