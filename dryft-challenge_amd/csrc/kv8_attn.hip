@@ -146,12 +146,12 @@ __device__ __forceinline__ uint32_t top_bits(const float (&x)[N]) {
   return m;
 }
 
-// The factors 2^(20 - e) and 2^e of a row with 2^(e-1) <= max|x| < 2^e <= 2^127 (a row
+// The factors 2^(20 - e) and 2^(e - 1) of a row with 2^(e-1) <= max|x| < 2^e <= 2^128 (a row
 // below 2^-108 takes those of 2^-107: steps of 2^-127).
-__device__ __forceinline__ void grid_of(uint32_t top, float &down, float &up) {
-  const int e = min(max((int)(top >> 23), 19), 253) - 126;
+__device__ __forceinline__ void grid_of(uint32_t top, float &down, float &half_up) {
+  const int e = min(max((int)(top >> 23), 19), 254) - 126;
   down = __uint_as_float((uint32_t)(127 + 20 - e) << 23);
-  up = __uint_as_float((uint32_t)(127 + e) << 23);
+  half_up = __uint_as_float((uint32_t)(126 + e) << 23);
 }
 // Four numbers of at most 2^20, rounded, as a 2^14 + b 2^7 + c, 0 <= b, c < 128, each
 // digit an int8.  (1.5 * 2^23 added: the sum's low 22 bits are the whole number.)
@@ -292,10 +292,10 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
     norm_rope<N>(raw, w, cw, sw, p.eps, o);
     const uint32_t top = top_bits<N>(o);
     if (query) {
-      // 21 bits, relative to the row's largest, as three digits; a row of 2^127 or more is NaN
-      const bool fin = top < 0x7f000000u;
-      float down, up;
-      grid_of(top, down, up);
+      // 21 bits, relative to the row's largest, as three digits
+      const bool fin = top < 0x7f800000u;
+      float down, half_up;
+      grid_of(top, down, half_up);
       if (i < n) {
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
 #pragma unroll
           for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t *>(s_q + (k * AC + i) * RS + ch + e) = d[k];
         }
-        if (col == 0) s_qs[i] = fin ? up * p.scale_log2 : __builtin_nanf("");
+        if (col == 0) s_qs[i] = fin ? half_up * p.scale_log2 * 2.f : __builtin_nanf("");
       }
     } else {
       const bool fin = top < 0x7f800000u;

@@ -160,3 +160,12 @@ def test_small_weights_beside_values_of_zero(lib, shape, splits, gap):
         a.c["v_scale"][b, :, L - 1] = 0.0
     check_no_score_error(a, score=2 * gap * (2 ** -20 + 64 * 2 ** -24), least=6 * 2.0 ** -130)
     assert bool((a.rows().float().abs().amax(-1) > 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("order", sorted(ORDERS))
+def test_queries_up_to_the_largest_number(lib, shape, order):
+    """Queries whose one channel is gain sqrt(D), from just below 2^127 to just below 2^128 (eps
+    takes it below), beside keys of 2^-100."""
+    for gain in {128: [1.0, 1.375], 64: [1.0, 2.0]}[shape[3]]:
+        check_no_score_error(along_one_channel(lib, shape, 1, gain * 2.0 ** 124, lambda i, L: ORDERS[order](i, L) * 2.0 ** -100))
