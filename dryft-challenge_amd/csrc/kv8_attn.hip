@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
 #pragma unroll
           for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t *>(s_q + (k * AC + i) * RS + ch + e) = d[k];
         }
-        if (col == 0) s_qs[i] = fin ? half_up * p.scale_log2 * 2.f : __builtin_nanf("");
+        // (never 0, so that it leaves -inf, a slot not seen, as it is)
+        if (col == 0) s_qs[i] = fin ? fmaxf(half_up * p.scale_log2 * 2.f, 0x1p-149f) : __builtin_nanf("");
       }
     } else {
       const bool fin = top < 0x7f800000u;

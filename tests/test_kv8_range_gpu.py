@@ -169,3 +169,13 @@ def test_queries_up_to_the_largest_number(lib, shape, order):
     takes it below), beside keys of 2^-100."""
     for gain in {128: [1.0, 1.375], 64: [1.0, 2.0]}[shape[3]]:
         check_no_score_error(along_one_channel(lib, shape, 1, gain * 2.0 ** 124, lambda i, L: ORDERS[order](i, L) * 2.0 ** -100))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=[f"{s[0]}x{s[1]}/{s[2]}x{s[3]}-t{s[4]}" for s in SHAPES])
+@pytest.mark.parametrize("sm_scale", [1e-10, 1e-20, 1e-38])
+def test_zero_queries_under_a_tiny_scale(lib, shape, sm_scale):
+    """Scores of 0 for every slot: the values' mean."""
+    a = along_one_channel(lib, shape, 1, 1.0, ORDERS["mixed"])
+    a.qkv.view(a.B * a.T, -1, a.D)[:, :a.nq] = 0.0
+    a.a.sm_scale = sm_scale
+    check_no_score_error(a)
