@@ -1064,8 +1064,8 @@ int qdec_kv8_attn_workspace(const qdec_kv8_attn_args *a, size_t *partial_bytes, 
   Kv8AttnParams p;
   const int rc = plan_kv8_attn(a, &p, false);
   if (rc != QDEC_OK) return rc;
-  const size_t rows = (size_t)p.batch * p.t_rows * p.nq;
-  if (partial_bytes) *partial_bytes = p.splits > 1 || p.out_partials ? sizeof(float) * rows * p.splits * (p.head_dim + 2) : 0;
+  const size_t one = sizeof(float) * kv8_partial_floats(p.t_rows * (p.nq / p.nkv), p.head_dim);
+  if (partial_bytes) *partial_bytes = p.splits > 1 || p.out_partials ? one * p.batch * p.nkv * p.splits : 0;
   if (counter_bytes) *counter_bytes = 0;
   return QDEC_OK;
 }

@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(64 * (AC == 16 ? 8 : BW)) kv8_attn_kernel(cons
 #pragma unroll
       for (int w = 0; w < BW; ++w) uw[w] = uw[w] == NEG_INF ? 0.f : __builtin_amdgcn_exp2f(uw[w] - U);
       const int r = r0 + y;
-      float *part = p.partial + ((size_t)cell * C + c) * (R * (D + 2));
+      float *part = p.partial + ((size_t)cell * C + c) * kv8_partial_floats(R, D);
       const bool direct = n_active == 1 && !p.out_partials;
       // (2^(U - 15), a normal number for every row that is held, and 2^-20 by itself: together they
       // would be 0 for values below 2^-84)
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(64) kv8_merge_kernel(const Kv8AttnParams p) {
   const int n = min(p.splits, ((L + p.t_rows - 1) >> p.run_log2) + 1);
   if (n == 1) return;  // written by its workgroup
   const int ch = (int)(threadIdx.x % TR) * 4;
-  const size_t stride = (size_t)R * (D + 2);
+  const size_t stride = kv8_partial_floats(R, D);
   const float *part = p.partial + ((size_t)b * p.nkv + kvh) * p.splits * stride;
   const float NEG_INF = -__builtin_huge_valf();
   float m[CB], l[CB];

@@ -331,6 +331,9 @@ struct Kv8AttnParams {
                                                         // per kv head; tiles: of 16 query rows
   int ofrag;   // > 0: out is written in fragment order with this many M tiles
 };
+// Floats of one split's partial, R rows of D channels: sums, maxima, sums of probabilities.  In whole 16
+// bytes, the vectors that hold them: an odd R leaves 2 floats unused.
+__host__ __device__ constexpr int kv8_partial_floats(int R, int D) { return (R * (D + 2) + 3) & ~3; }
 int kv8_attn_run(int batch, int nkv, int cap, int splits);
 int kv8_attn_splits(int batch, int nkv, int cap);
 int kv8_attn_parts(int batch, int nkv, int splits, int tiles);

@@ -711,9 +711,10 @@ typedef struct qdec_kv8_attn_args {
                            qdec_gemm with x_kv8 = these arguments merges them:
                            the same bits without the merge's launch.  partial:
                            [batch][nkv][splits] x (acc [R][head_dim], max [R] of
-                           the scores in powers of 2, sum [R]), R = t_rows * nq /
-                           nkv, acc and sum times 2^-20, so that none overflows;
-                           splits that hold no slot are not written */
+                           the scores in powers of 2, sum [R], 2 floats unused
+                           where R is odd), R = t_rows * nq / nkv, acc and sum
+                           times 2^-20, so that none overflows; splits that hold
+                           no slot are not written */
 } qdec_kv8_attn_args;
 int qdec_kv8_attn(const qdec_kv8_attn_args *a, qdec_stream_t stream);
 /* Bytes of `partial`; counter_bytes, as in the other queries, is 0. */

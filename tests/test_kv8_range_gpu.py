@@ -179,3 +179,29 @@ def test_zero_queries_under_a_tiny_scale(lib, shape, sm_scale):
     a.qkv.view(a.B * a.T, -1, a.D)[:, :a.nq] = 0.0
     a.a.sm_scale = sm_scale
     check_no_score_error(a)
+
+
+@pytest.mark.parametrize("shape", [(5, 40, 8, 128, 1, [639, 0, 1500, 64, 512]), (3, 9, 3, 64, 5, [59, 1123, 0]),
+                                   (2, 1, 1, 64, 1, [700, 300]), (2, 7, 7, 128, 1, [900, 3])])
+@pytest.mark.parametrize("splits", [2, 3])
+def test_partials_of_an_odd_number_of_rows(lib, shape, splits):
+    """Every split's partial begins at a multiple of 16 bytes; what out_partials leaves, merged
+    in 64 bits, against the call's own rows: both round once to bf16."""
+    B, nq, nkv, D, T, lens = shape
+    R = T * nq // nkv
+    assert R % 2
+    a, b = Call(lib, *shape, splits=splits).run(), Call(lib, *shape, splits=splits)
+    b.a.out_partials = 1
+    b.partial.fill_(NAN)
+    b.run()
+    pb, stride = lib.kv8_attn_workspace(b.a)[0], R * (D + 2) + 2
+    assert pb == 4 * B * nkv * splits * stride and stride % 4 == 0
+    part = b.partial[:pb // 4].view(B, nkv, splits, stride).double()
+    acc, m, l, pad = part[..., :R * D].reshape(B, nkv, splits, R, D), part[..., R * D:R * (D + 1)], part[..., R * (D + 1):-2], part[..., -2:]
+    assert bool(torch.isnan(pad).all()) and bool(torch.isnan(b.partial[pb // 4:]).all())
+    left = ~torch.isnan(m)
+    top = m.masked_fill(~left, -math.inf).amax(2, keepdim=True)
+    w = torch.where(left, torch.exp2(m - top), 0.0)
+    want = (torch.where(w[..., None] > 0, acc, 0.0) * w[..., None]).sum(2) / (torch.where(w > 0, l, 0.0) * w).sum(2)[..., None]
+    want = want.view(B, nkv, T, nq // nkv, D).transpose(1, 2).reshape(B, T, nq, D)
+    torch.testing.assert_close(a.rows().double(), want, rtol=2 ** -8, atol=float(want.abs().max()) * 2 ** -18)
