@@ -72,7 +72,6 @@ static bool wide_offsets(const qdec_gemm_args *a) { return (uint64_t)a->n * a->k
 // for).
 enum class PlanFor { kCall, kWide, kLayer };
 
-// Derive the launch plan of a GEMM call; returns QDEC_OK or an error code.
 // The partials that an attention call with out_partials leaves (x_attn, x_kv8); false:
 // not of a shape that a GEMM merges.
 struct Partials {
@@ -103,6 +102,7 @@ static bool partials_of(const qdec_kv8_attn_args &a, Partials *p) {
   return true;
 }
 
+// Derive the launch plan of a GEMM call; returns QDEC_OK or an error code.
 static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, PlanFor what = PlanFor::kCall) {
   const bool wide = what == PlanFor::kWide;
   if (!a) return set_error(QDEC_EINVAL, "qdec_gemm: null args");
@@ -130,15 +130,16 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     return set_error(QDEC_EINVAL, "qdec_gemm: x_frag %d / out_frag %d not 0 or 1", a->x_frag, a->out_frag);
   if (a->out_frag && (f & (QDEC_RES_OUT | QDEC_ARGMAX)))
     return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: out_frag with RES_OUT or ARGMAX");
-  if (a->x_frag && ((f & QDEC_NORM_IN) || a->x_attn))
-    return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_frag needs no NORM_IN and no x_attn");
+  const bool xa = a->x_attn || a->x_kv8;
+  if (a->x_frag && ((f & QDEC_NORM_IN) || xa))
+    return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_frag needs no NORM_IN and no x_attn or x_kv8");
   if ((f == QDEC_GLU || f == QDEC_ARGMAX) && !a->x_frag)
     return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: GLU or ARGMAX without NORM_IN needs x_frag = 1");
   if (a->parts_out && (f != QDEC_RES_OUT || a->ksplit < 2))
     return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: parts_out needs RES_OUT alone and ksplit > 1");
   if (a->x_parts) {
-    if (!(f & QDEC_NORM_IN) || a->ksplit != 1 || a->x_attn)
-      return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_parts needs NORM_IN, ksplit 1 and no x_attn");
+    if (!(f & QDEC_NORM_IN) || a->ksplit != 1 || xa)
+      return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_parts needs NORM_IN, ksplit 1 and no x_attn or x_kv8");
     if (a->x_nparts < 1 || a->x_nparts > 8) return set_error(QDEC_EINVAL, "qdec_gemm: x_nparts %d not in [1, 8]", a->x_nparts);
     if (need_scratch && (!a->x_merged || a->x_merged == a->x))
       return set_error(QDEC_EINVAL, "qdec_gemm: x_parts needs x_merged, a buffer other than x");
@@ -146,17 +147,17 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
       return set_error(QDEC_EALIGN, "qdec_gemm: x_parts and x_merged must be 16-byte aligned");
   }
   Partials xp = {};
-  const bool xa = a->x_attn || a->x_kv8;
   if (xa) {
-    if (f & QDEC_NORM_IN) return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_attn with NORM_IN");
     if (a->x_attn && a->x_kv8) return set_error(QDEC_EINVAL, "qdec_gemm: both x_attn and x_kv8");
+    const char *from = a->x_attn ? "x_attn" : "x_kv8";
+    if (f & QDEC_NORM_IN) return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: %s with NORM_IN", from);
     if (!(a->x_attn ? a->x_attn->out_partials : a->x_kv8->out_partials))
-      return set_error(QDEC_EINVAL, "qdec_gemm: x_attn call was not made with out_partials");
+      return set_error(QDEC_EINVAL, "qdec_gemm: %s call was not made with out_partials", from);
     if (!(a->x_attn ? partials_of(*a->x_attn, &xp) : partials_of(*a->x_kv8, &xp)))
-      return set_error(QDEC_EINVAL, "qdec_gemm: x_attn shape");
+      return set_error(QDEC_EINVAL, "qdec_gemm: %s shape", from);
     if (a->rows != (int64_t)xp.batch * xp.t_rows || a->k != xp.nkv * 4 * 128)
-      return set_error(QDEC_EINVAL, "qdec_gemm: x_attn rows %d / k %d do not match the attention call", a->rows, a->k);
-    if (need_scratch && (!xp.partial || !xp.lens)) return set_error(QDEC_EINVAL, "qdec_gemm: x_attn needs partial and lens");
+      return set_error(QDEC_EINVAL, "qdec_gemm: %s rows %d / k %d do not match the attention call", from, a->rows, a->k);
+    if (need_scratch && (!xp.partial || !xp.lens)) return set_error(QDEC_EINVAL, "qdec_gemm: %s needs partial and lens", from);
   }
   if (need_scratch && ((!a->x && !xa) || !a->w)) return set_error(QDEC_EINVAL, "qdec_gemm: null x or w");
   if (need_scratch && (f & QDEC_NORM_IN) && !a->norm_w) return set_error(QDEC_EINVAL, "qdec_gemm: NORM_IN needs norm_w");
@@ -194,7 +195,7 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     if (a->ksplit < 2 || a->waves != 4 || !a->x_frag || xa || a->next_norm_w || a->rows < 17 || a->rows > 32 ||
         kp > kResSplitKSteps)
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: resident RES_OUT with parts_out needs ksplit > 1, 4 waves, "
-                       "x_frag = 1, 17..32 rows and at most %d k steps per split (no x_attn or next_norm_w)",
+                       "x_frag = 1, 17..32 rows and at most %d k steps per split (no x_attn, x_kv8 or next_norm_w)",
                        kResSplitKSteps);
     p->resident = 3;
     p->rw = kResSplitRing;
@@ -209,7 +210,7 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     if (a->resident != 1) return set_error(QDEC_EINVAL, "qdec_gemm: resident %d not 0 or 1", a->resident);
     if (a->ksplit != 1 || a->tiles_per_wg != 1 || a->x_frag || xa || a->parts_out || a->next_norm_w)
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: resident RES_OUT needs ksplit 1, one tile per workgroup and "
-                       "row-major x (no x_frag, x_attn, parts_out or next_norm_w)");
+                       "row-major x (no x_frag, x_attn, x_kv8, parts_out or next_norm_w)");
     if (a->rows > kResLdsRows)
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: resident RES_OUT takes 1..%d rows, not %d", kResLdsRows, a->rows);
     if (KS > kResLdsKSteps || (KS & 15))
@@ -227,7 +228,7 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
     if ((f != (QDEC_NORM_IN | QDEC_GLU) && f != QDEC_NORM_IN) || a->ksplit != 1 || a->waves != 4 ||
         a->tiles_per_wg != 1 || a->x_frag || xa || a->next_norm_w)
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: resident needs NORM_IN (with or without GLU), ksplit 1, 4 waves, "
-                       "one tile per workgroup and row-major x (no x_frag, x_attn or next_norm_w)");
+                       "one tile per workgroup and row-major x (no x_frag, x_attn, x_kv8 or next_norm_w)");
     const bool two = a->rows >= kResMinRows2 && a->rows <= kResMaxRows2;
     if (!two && (a->rows < kResMinRows || a->rows > kResMaxRows))
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: resident takes %d..%d or %d..%d rows, not %d", kResMinRows,
@@ -319,7 +320,7 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
   if (wide) {
     if (!many || arg || xa || a->resident || (!a->x_frag && !(f & QDEC_NORM_IN)))
       return set_error(QDEC_EUNSUPPORTED, "qdec_gemm_wide: needs 4 waves, one tile per workgroup, x_frag = 1 or NORM_IN, "
-                       "ksplit 1 or parts_out, no ARGMAX, x_attn, next_norm_w or resident");
+                       "ksplit 1 or parts_out, no ARGMAX, x_attn, x_kv8, next_norm_w or resident");
     if (!ring_d) ring_d = 1;  // its own ring
   }
   // Past its register-staged rows a NORM_IN call does better on the direct
@@ -385,7 +386,7 @@ static int plan_gemm(const qdec_gemm_args *a, GemmParams *p, bool need_scratch, 
   p->alens = nullptr;
   if (xa) {
     if (!p->xfast || p->xd || a->ksplit != 1)
-      return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_attn needs activations staged from registers (rows %d)", a->rows);
+      return set_error(QDEC_EUNSUPPORTED, "qdec_gemm: x_attn or x_kv8 needs activations staged from registers (rows %d)", a->rows);
     p->amerge = 1;
     p->apart = xp.partial;
     p->alens = xp.lens;

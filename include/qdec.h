@@ -174,7 +174,7 @@ typedef struct {
    * last M tile are ignored.
    * x_frag = 1: x is in fragment order (as a call with out_frag = 1 or an
    * attention call with out_frag = 1 over the same rows wrote it).  Not with
-   * NORM_IN or x_attn (the call takes the direct path).
+   * NORM_IN, x_attn or x_kv8 (the call takes the direct path).
    * out_frag = 1: out is written in fragment order (plain or GLU only). */
   int32_t x_frag;
   int32_t out_frag;
@@ -225,7 +225,7 @@ typedef struct {
   int32_t next_threads;
   /* 1: gate/up with its rows resident in LDS.  For NORM_IN | GLU with
    * ksplit 1, 4 waves, one tile per workgroup, row-major x (no x_frag,
-   * x_attn, x_parts or next_norm_w), 1..8 or 17..32 rows, k <= 2560 and
+   * x_attn, x_kv8, x_parts or next_norm_w), 1..8 or 17..32 rows, k <= 2560 and
    * k / 128 a multiple of 10: one workgroup per compute unit takes a
    * contiguous run of (gate, up) tile pairs and reads its MFMA operands
    * from one copy of the normalised rows in LDS, so no workgroup re-reads
@@ -240,7 +240,7 @@ typedef struct {
    * place of the pairs (one or two per workgroup); the same bits as
    * resident = 0.
    * For RES_OUT with ksplit 1, one tile per workgroup, row-major x (no
-   * x_frag, x_attn, parts_out or next_norm_w), 1..8 rows and k / 32 a
+   * x_frag, x_attn, x_kv8, parts_out or next_norm_w), 1..8 rows and k / 32 a
    * multiple of 16 and at most 304: every workgroup first copies the rows
    * into LDS (LDS DMA, up to 8 rows x 64 bytes per k step) and its weight
    * ring then holds
@@ -278,7 +278,7 @@ int qdec_gemm_prepass(const qdec_gemm_args *a, int32_t *threads);
  * flags 0, NORM_IN, RES_OUT, GLU or NORM_IN | GLU, waves 4, tiles_per_wg 1, k / 32
  * / ksplit a multiple of 4, x_frag = 1 or NORM_IN (whose pre-pass writes the
  * normalised rows to the partial workspace), ksplit > 1 only with parts_out,
- * and no x_attn, next_norm_w or resident; n x k (with GLU of either half)
+ * and no x_attn, x_kv8, next_norm_w or resident; n x k (with GLU of either half)
  * below 2 Gi elements.  QDEC_EUNSUPPORTED otherwise.  For the products of a short prompt,
  * whose weights are read once for all rows.
  * Replaces F.linear as the prefill forward uses it (engine/engine.py:448-461). */

@@ -1,8 +1,11 @@
 """What the header promises of the 8-bit cache's calls beside their shapes, without a GPU."""
 
+import ctypes
+
 import pytest
 
-from test_kv8_capi import attn
+from qdec import capi
+from test_kv8_capi import attn, merging, one
 
 
 @pytest.mark.parametrize("nq,nkv,t,d", [(40, 8, 1, 128), (40, 8, 3, 128), (9, 3, 5, 64), (8, 8, 1, 128), (30, 10, 1, 64), (32, 8, 1, 128)])
@@ -13,3 +16,33 @@ def test_partials_begin_on_16_bytes(qlib, nq, nkv, t, d):
     assert one % 16 == 0
     for splits in (2, 3, 7):
         assert qlib.kv8_attn_workspace(attn(nq=nq, nkv=nkv, t_rows=t, head_dim=d, splits=splits)) == (2 * nkv * splits * one, 0)
+
+
+@pytest.mark.parametrize("at,kw,code,needle", [
+    ({}, dict(x_frag=1), -3, "x_frag needs no"),
+    (dict(batch=4), dict(rows=4, x_frag=1), -3, "x_frag needs no"),
+    (dict(batch=17), dict(rows=17, waves=4, x_frag=1), -3, "x_frag needs no"),
+    ({}, dict(flags=capi.GLU, x_frag=1), -3, "x_frag needs no"),
+    ({}, dict(flags=capi.ARGMAX, x_frag=1), -3, "x_frag needs no"),
+    ({}, dict(x_parts=16, x_nparts=2, x_merged=32), -3, "x_parts needs"),
+    ({}, dict(x_parts=16, x_nparts=2, x_merged=32, flags=capi.NORM_IN), -3, "x_parts needs"),
+    ({}, dict(flags=capi.NORM_IN), -3, "NORM_IN"),
+    (dict(out_partials=0), {}, -1, "out_partials"),
+    (dict(nq=64), dict(k=8192), -1, "shape"),
+    (dict(batch=2), {}, -1, "rows 1"),
+    (dict(lens=None), {}, -1, "lens"),
+    ({}, dict(resident=1), -3, "resident"),
+    ({}, dict(ksplit=2), -3, "registers"),
+])
+def test_a_product_names_the_partials_it_refuses(qlib, at, kw, code, needle):
+    """The partials of an 8-bit call are refused where those of a bf16 call are, by their own name."""
+    a = one(**at)
+    g = merging(a, **kw)
+    assert qlib.so.qdec_gemm(ctypes.byref(g), None) == code
+    assert needle in qlib.last_error() and "x_kv8" in qlib.last_error()
+
+
+def test_a_many_row_product_takes_no_partials(qlib):
+    a = one(batch=16)
+    g = merging(a, rows=16, waves=4)
+    assert qlib.so.qdec_gemm_wide_workspace(ctypes.byref(g), None) == -3 and "x_kv8" in qlib.last_error()
