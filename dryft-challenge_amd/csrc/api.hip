@@ -647,6 +647,22 @@ extern "C" {
 
 int qdec_version(void) { return QDEC_ABI_VERSION; }
 
+int qdec_args_size(const char *name) {
+#define ARGS(t) {#t, (int)sizeof(t)}
+  static const struct {
+    const char *name;
+    int size;
+  } all[] = {ARGS(qdec_embed_args),      ARGS(qdec_gemm_args),       ARGS(qdec_attn_args),       ARGS(qdec_layer_args),
+             ARGS(qdec_draft_args),      ARGS(qdec_accept_args),     ARGS(qdec_tree_draft_args), ARGS(qdec_tree_attn_args),
+             ARGS(qdec_tree_accept_args), ARGS(qdec_tree_commit_args), ARGS(qdec_kv8_store_args), ARGS(qdec_kv8_load_args),
+             ARGS(qdec_kv8_attn_args),   ARGS(qdec_rownorm_args),    ARGS(qdec_pgemm_args),      ARGS(qdec_prefill_qk_args),
+             ARGS(qdec_prefill_attn_args)};
+#undef ARGS
+  for (const auto &a : all)
+    if (name && !strcmp(name, a.name)) return a.size;
+  return set_error(QDEC_EINVAL, "qdec_args_size: no struct of this name");
+}
+
 const char *qdec_last_error(void) { return g_err; }
 
 int qdec_device_count(void) {

@@ -144,6 +144,15 @@ class Kv8AttnArgs(ctypes.Structure):
                 ("cap", I32), ("splits", I32), ("out_frag", I32), ("out_partials", I32)]
 
 
+# The C structs that these mirror.
+ARGS = {"qdec_embed_args": EmbedArgs, "qdec_gemm_args": GemmArgs, "qdec_attn_args": AttnArgs, "qdec_layer_args": LayerArgs,
+        "qdec_draft_args": DraftArgs, "qdec_accept_args": AcceptArgs, "qdec_tree_draft_args": TreeDraftArgs,
+        "qdec_tree_attn_args": TreeAttnArgs, "qdec_tree_accept_args": TreeAcceptArgs,
+        "qdec_tree_commit_args": TreeCommitArgs, "qdec_kv8_store_args": Kv8StoreArgs, "qdec_kv8_load_args": Kv8LoadArgs,
+        "qdec_kv8_attn_args": Kv8AttnArgs, "qdec_rownorm_args": RownormArgs, "qdec_pgemm_args": PgemmArgs,
+        "qdec_prefill_qk_args": PrefillQkArgs, "qdec_prefill_attn_args": PrefillAttnArgs}
+
+
 def declared_functions(header=HEADER):
     """Names of every function declared in include/qdec.h."""
     with open(header) as f:
@@ -164,6 +173,11 @@ class Lib:
         self.so = ctypes.CDLL(path)
         so = self.so
         so.qdec_version.restype = ctypes.c_int
+        so.qdec_args_size.argtypes, so.qdec_args_size.restype = [ctypes.c_char_p], ctypes.c_int
+        for name, st in ARGS.items():
+            if so.qdec_args_size(name.encode()) != ctypes.sizeof(st):
+                raise RuntimeError(f"{path} is of another build: {name} has {so.qdec_args_size(name.encode())} bytes there, "
+                                   f"{ctypes.sizeof(st)} here; build it again")
         so.qdec_last_error.restype = ctypes.c_char_p
         so.qdec_device_count.restype = ctypes.c_int
         so.qdec_tiled_offset.restype = ctypes.c_int64

@@ -70,8 +70,16 @@ extern "C" {
 
 typedef void *qdec_stream_t;
 
-/* Library ABI version (QDEC_ABI_VERSION). */
+/* Library ABI version (QDEC_ABI_VERSION).  It stays where an argument struct only grows at
+ * its end; qdec_args_size tells such libraries apart. */
 int qdec_version(void);
+
+/* sizeof the argument struct of that name ("qdec_gemm_args") in this library,
+ * QDEC_EINVAL for a name it does not have.  An entry point reads its whole
+ * struct, so a caller that may have been built with another release's header
+ * compares this with its own sizeof before the first call: a shorter struct would be read
+ * past its end. */
+int qdec_args_size(const char *name);
 
 /* Text of the last error returned on this thread ("" if none). */
 const char *qdec_last_error(void);

@@ -1,6 +1,7 @@
 """What the header promises of the 8-bit cache's calls beside their shapes, without a GPU."""
 
 import ctypes
+import re
 
 import pytest
 
@@ -46,3 +47,24 @@ def test_a_many_row_product_takes_no_partials(qlib):
     a = one(batch=16)
     g = merging(a, rows=16, waves=4)
     assert qlib.so.qdec_gemm_wide_workspace(ctypes.byref(g), None) == -3 and "x_kv8" in qlib.last_error()
+
+
+def test_a_library_tells_its_structs_sizes(qlib):
+    """Every argument struct of the header is mirrored and has the library's size, and a
+    caller with another one can tell before it calls."""
+    text = re.sub(r"/\*.*?\*/", "", open(capi.HEADER).read(), flags=re.S)
+    assert sorted(re.findall(r"\}\s*(qdec_\w+_args);", text)) == sorted(capi.ARGS)
+    for name, st in capi.ARGS.items():
+        assert qlib.so.qdec_args_size(name.encode()) == ctypes.sizeof(st), name
+    for name in (b"qdec_gem_args", b"", None):
+        assert qlib.so.qdec_args_size(name) == -1 and "struct" in qlib.last_error()
+
+
+def test_a_binding_of_another_header_is_refused(monkeypatch):
+    class Shorter(ctypes.Structure):  # the product's arguments before x_kv8
+        _fields_ = [f for f in capi.GemmArgs._fields_ if f[0] != "x_kv8"]
+
+    assert ctypes.sizeof(Shorter) < ctypes.sizeof(capi.GemmArgs)
+    monkeypatch.setitem(capi.ARGS, "qdec_gemm_args", Shorter)
+    with pytest.raises(RuntimeError, match="qdec_gemm_args"):
+        capi.Lib()
