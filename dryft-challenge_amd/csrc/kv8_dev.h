@@ -7,9 +7,10 @@
 // a row's bits would depend on how many rows its pass had.)  127 x of a bf16 x has 15
 // bits, so in fp32 it is exact and only the division rounds: quotients that
 // are halves, as of x = top / 2, come out as such, and no other quotient of two
-// bf16 numbers is within 2^-9 of one.  A row with an infinity or a NaN gets the
-// scale NaN, one with top below 2^-100, whose reciprocals would leave fp32's
-// range, the scale 0.
+// bf16 numbers is nearer to one than 2^-16 of itself (127 * 254 / 255 = 126.502), 2^7
+// times what the refined quotient below can be off by.  A row with an infinity or
+// a NaN gets the scale NaN, one with top below 2^-100, whose reciprocals would
+// leave fp32's range, the scale 0.
 #pragma once
 
 #include "qdec_common.h"
@@ -30,8 +31,8 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 }
 
 // Rounding of a row's values.  127 x / top as (127 / 256) x / (top / 256), which keeps
-// 127 x in range; the quotient by one step of refinement, which leaves a quotient
-// that fp32 can hold as it is; rounded by adding 1.5 * 2^23, whose sum's low bits are
+// 127 x in range; the quotient by one step of refinement, within 2^-23 of itself, which leaves a
+// quotient that fp32 can hold as it is; rounded by adding 1.5 * 2^23, whose sum's low bits are
 // the whole number.  A row held as zeros (and inf * 0 = NaN) has the reciprocal 0.
 struct Kv8Div {
   float div, rcp;

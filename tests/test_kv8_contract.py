@@ -3,6 +3,7 @@
 import ctypes
 import re
 
+import numpy as np
 import pytest
 
 from qdec import capi
@@ -68,3 +69,19 @@ def test_a_binding_of_another_header_is_refused(monkeypatch):
     monkeypatch.setitem(capi.ARGS, "qdec_gemm_args", Shorter)
     with pytest.raises(RuntimeError, match="qdec_gemm_args"):
         capi.Lib()
+
+
+def test_quotients_near_a_half():
+    """127 x / top of bf16 numbers 2^7 <= X, T < 2^8, x / top = X / T 2^-k: a half, or further
+    from one than 2^-16 of itself, which the kernels' fp32 quotient (within 2^-23) tells
+    apart.  From k = 9 on it is below 0.495."""
+    X, T = np.meshgrid(np.arange(128, 256), np.arange(128, 256))
+    least = 1.0
+    for k in range(9):
+        num, den = 254 * X, (T << k)  # twice the quotient, which is odd where it is a half
+        held = X <= den
+        off = np.abs(num - (num // (2 * den) * 2 + 1) * den)  # to the half above the whole number below
+        held &= off > 0
+        least = min(least, (off[held] / num[held]).min())
+    assert 2.0 ** -16 < least < 2.0 ** -15.9
+    assert 127 * 255 / (128 * 2 ** 9) < 0.495

@@ -2,7 +2,7 @@
 (oracle/kv8_oracle.py), through the C ABI.
 
 store and load have to be right bit for bit: 127 x is exact in fp32, a quotient
-of two bf16 numbers is either a half or at least 2^-9 from one, scale = top / 127
+of two bf16 numbers is either a half or at least 2^-16 of itself from one, scale = top / 127
 and q * scale are one fp32 operation each and the result is rounded to bf16 once.
 
 Attention: the cache after the call is what the oracle attends over, so a new
