@@ -689,7 +689,7 @@ int kv8_attn_splits(int batch, int nkv, int cap) {
   const int64_t cells = (int64_t)batch * nkv;
   if (cap <= 1024) return 1;
   if (short_runs(batch, nkv, cap)) return (cap + 255) / 256;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(256 / cells, (cap + 511) / 512));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(256 / cells, (cap + 511ll) / 512));
 }
 
 // Workgroups that share the splits of a (sequence, kv head, row tile): with several

@@ -85,3 +85,10 @@ def test_quotients_near_a_half():
         least = min(least, (off[held] / num[held]).min())
     assert 2.0 ** -16 < least < 2.0 ** -15.9
     assert 127 * 255 / (128 * 2 ** 9) < 0.495
+
+
+def test_splits_of_the_longest_cache(qlib):
+    """The chosen number follows the cap up to the largest there is."""
+    got = [qlib.kv8_attn_workspace(attn(batch=2, nkv=1, nq=4, t_rows=1, cap=cap))[0] // (2 * 4 * 4 * 130)
+           for cap in (1 << 20, (1 << 31) - 1024, (1 << 31) - 512, (1 << 31) - 256, (1 << 31) - 64)]
+    assert got == [128] * 5
