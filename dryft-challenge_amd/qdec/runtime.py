@@ -1121,8 +1121,9 @@ class Prefill:
     With an 8-bit cache the layer's keys and values go to a pair of bf16 slabs
     of one layer, from there into the cache (qdec_kv8_store), and the slots so
     far come back from it (qdec_kv8_load) before the attention: every row
-    attends over what the cache holds, as the steps after it do, in whatever
-    chunks the prompt ran.
+    attends over the cached numbers rounded to bf16, in whatever chunks the
+    prompt ran.  (A step attends over q * scale itself, and holds its key from
+    fp32 where a prompt's was rounded to bf16 first.)
 
     Replaces engine/engine.py:448-490 (``_layers_forward`` over the whole
     prompt, ``_attend_prefill``, ``_prefill``)."""

@@ -682,7 +682,10 @@ int qdec_kv8_load(const qdec_kv8_load_args *a, qdec_stream_t stream);
  *          its row's largest channel, exact products with the held keys, fp32
  *          statistics and accumulation, p * v_scale in fp16, one rounding to
  *          bf16.
- * What a row does not see does not reach it, whatever its slot or scale holds.  A length
+ * What a row does not see does not reach it, whatever its slot or scale holds.
+ * All this holds as long as fp32 does what lies between: a raw head's sum of squares,
+ * a gain times its row's 1 / rms, key rows below 2^120, scores times log2(e) below
+ * 2^128.  Outputs below 2^-104 lose bits with the partials' 2^-20.  A length
  * with lens[b] < 0 or lens[b] + t_rows > cap touches no cache memory; the rows
  * of sequence b become NaN.
  * Slots are dealt in runs of 256 or 512, run j to split j % splits of its (sequence,
@@ -712,7 +715,10 @@ typedef struct qdec_kv8_attn_args {
   int32_t nkv;
   int32_t head_dim;     /* 128 or 64 */
   int32_t cap;          /* slots per sequence, multiple of 64 */
-  int32_t splits;       /* 1..256, or 0: chosen from the shape */
+  int32_t splits;       /* 1..256, or 0: chosen from the shape, for a call that is
+                           launched by itself.  In replayed graphs, whose launches cost
+                           less, caps of 513 to 1024 are faster in (cap + 255) / 256
+                           splits if batch * nkv times that is at most 256 */
   int32_t out_frag;     /* 1: out in the fragment order of qdec_gemm_args */
   int32_t out_partials; /* 0: rows to out.  1: every split leaves its unnormalised
                            (acc, max, sum) in partial, out is not written, and a
