@@ -30,7 +30,7 @@
 // caches take turns): where a launch fills the GPU, the cache's bytes, which arithmetic
 // lengthens by 1 to 2 us.  32 sequences of 4096 to 4220 slots: 281 MB in 49.4 us, 5.7
 // TB/s (47.3 with no arithmetic; a read of as much takes 40): 6.8 from round to round
-// by the cycle counter, the rest launch, first loads and merge.  131000 slots, 64 heads: 53 us, 7 of them the
+// by the cycle counter, the rest launch, first loads and merge.  131000 slots, 64 heads: 53.5 us, 7 of them the
 // merge.  A small launch is a chain: length, then rows and tables, then their
 // preparation, then the blocks that were loaded meanwhile: one sequence of 640 slots
 // 6.8 us before its partials are merged (an empty launch takes 1.8) and 9.3 with the
